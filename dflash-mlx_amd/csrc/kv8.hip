@@ -1,0 +1,531 @@
+// The 8-bit key/value cache: append (with the query / key norm and rotary in
+// front of it), load and read back (include/dflash_kv8.h).
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+#include <stdint.h>
+
+#include "kv8_common.h"
+
+namespace dflash {
+namespace {
+
+constexpr int kRow = kHD + 8;  // bf16 of a token's row in LDS (16 bytes of pad)
+
+// Quantise block j of head bh from the tail: a thread holds 32 neighbouring
+// values of the block in its stored order (keys [64][128], values [128][64]).
+template <int TYPE>
+__device__ __forceinline__ void quantise_tail_block(const Kv8& c, int64_t bh, int j, bool values, uint32_t* red) {
+  const int t = threadIdx.x;
+  const int at = (j & 1) * kBlk;
+  const uint16_t* src = values ? c.tail_values(bh) + (t >> 1) * kSlots + at + (t & 1) * 32
+                               : c.tail_keys(bh) + (at + (t >> 2)) * kHD + (t & 3) * 32;
+  u32x4 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = ld16(src + 8 * i);
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a = max(a, abs_bits16(w[i]));
+  const f32x2 sm = block_scale<TYPE>(group_max_u32(a, red));
+  uint8_t* dst = (values ? c.values(bh, j) : c.keys(bh, j)) + 32 * t;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x2 lo = quantise8<TYPE>(w[2 * i], sm.y), hi = quantise8<TYPE>(w[2 * i + 1], sm.y);
+    *reinterpret_cast<u32x4*>(dst + 16 * i) = u32x4{lo.x, lo.y, hi.x, hi.y};
+  }
+  if (t == 0) (values ? c.vs : c.ks)[bh * c.nblk + j] = sm.x;
+}
+
+// Block L / 64 - 1 may have become complete since the last append.
+__device__ __forceinline__ bool may_wait(int L, int Smax) { return L >= kBlk && L <= Smax && (L & 63) <= kMaxDraft; }
+
+struct AppendParams {
+  Kv8 c;
+  const uint16_t* proj;  // [B*T, row_stride]: Hq x (q | gate), Hkv x k, Hkv x v
+  int64_t row_stride;
+  const uint16_t* q_norm_w;
+  const uint16_t* k_norm_w;
+  const int32_t* lens;
+  uint16_t* q_out;
+  int32_t* overflow;
+  int T, Hq, rot;
+  int nb;      // prompt: block tasks of a head
+  int qtiles;  // prompt: 16-token query tiles of a sequence
+  double log2_base;
+  float eps;
+};
+
+// ------------------------------------------------------------ draft append
+// Workgroups 0 .. 2 B Hkv - 1: the waiting block of one head, keys or values, if
+// any (4096 tokens of the tail's 16 KB in, 8 KB of codes out).  The others: a wave
+// a (token, head), as the bf16 cache's append; keys and values go to the tail.
+// The tail's slots that a waiting block is read from are not written by the same
+// call: it waits only where L % 64 <= 16, and the at most 16 new tokens then stay in
+// block L / 64, the other half of the slots.
+template <int TYPE>
+__global__ __launch_bounds__(256) void kv8_append_draft_kernel(const AppendParams p) {
+  __shared__ uint32_t red[4];
+  const Kv8& c = p.c;
+  const int nquant = 2 * c.B * c.Hkv;
+  if ((int)blockIdx.x < nquant) {
+    const int64_t bh = blockIdx.x >> 1;
+    const int L = p.lens[bh / c.Hkv];
+    if (may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, (L >> 6) - 1, blockIdx.x & 1, red);
+    return;
+  }
+  const int slots = p.Hq + 2 * c.Hkv, groups = (slots + 3) >> 2;
+  const int wg = blockIdx.x - nquant;
+  const int bt = wg / groups;
+  const int slot = (wg - bt * groups) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (slot >= slots) return;
+  const int b = bt / p.T;
+  const int L = p.lens[b];
+  const int pos = L + (bt - b * p.T);
+  const bool in_cache = L >= 0 && L <= c.Smax && pos < c.Smax;
+  if (!in_cache && slot == 0 && lane == 0 && p.overflow != nullptr) p.overflow[b] = 1;
+  const int d0 = 2 * lane;
+  const uint16_t* row = p.proj + (int64_t)bt * p.row_stride + d0;
+  const int at = pos & (kSlots - 1);
+  if (slot >= p.Hq + c.Hkv) {
+    if (!in_cache) return;
+    const int h = slot - p.Hq - c.Hkv;
+    const uint32_t vv = *reinterpret_cast<const uint32_t*>(row + (2 * p.Hq + c.Hkv + h) * kHD);
+    uint16_t* col = c.tail_values((int64_t)b * c.Hkv + h) + d0 * kSlots + at;
+    col[0] = (uint16_t)vv;
+    col[kSlots] = (uint16_t)(vv >> 16);
+    return;
+  }
+  const bool is_q = slot < p.Hq;
+  const int h = is_q ? slot : slot - p.Hq;
+  const uint32_t xv = *reinterpret_cast<const uint32_t*>(row + (is_q ? 2 * h : 2 * p.Hq + h) * kHD);
+  const uint32_t wv = *reinterpret_cast<const uint32_t*>((is_q ? p.q_norm_w : p.k_norm_w) + d0);
+  const uint32_t packed = norm_rotate(
+      xv, wv, [&] { return rotation_of(pos, d0, p.rot, p.log2_base); }, d0, p.rot, p.eps);
+  if (is_q) {
+    *reinterpret_cast<uint32_t*>(p.q_out + ((int64_t)bt * p.Hq + h) * kHD + d0) = packed;
+  } else if (in_cache) {
+    *reinterpret_cast<uint32_t*>(c.tail_keys((int64_t)b * c.Hkv + h) + at * kHD + d0) = packed;
+  }
+}
+
+// ----------------------------------------------------------- prompt append
+// Cosines and sines of N positions pos0 .. and the rot / 2 frequencies, to LDS
+// [N][rot / 2].  A thread keeps one frequency (256 is a multiple of rot / 2), so
+// its fp64 exponential is taken once; the angles are those of rotation_of.
+template <int N>
+__device__ __forceinline__ void rotation_table(f32x2* table, int pos0, int rot, double log2_base) {
+  if (rot == 0) return;
+  const int half = rot >> 1, shift = __builtin_ctz(half);
+  const int i = threadIdx.x & (half - 1);
+  for (int t = threadIdx.x >> shift; t < N; t += 256 >> shift) {
+    float sn, cs;
+    sincosf(rope_angle(pos0 + t, i, rot, log2_base), &sn, &cs);
+    table[t * half + i] = f32x2{cs, sn};
+  }
+}
+
+__device__ __forceinline__ Rotation table_rotation(const f32x2* table, int t, int d0, int rot) {
+  const int half = rot >> 1;
+  const int i0 = d0 < half ? d0 : d0 - half;
+  const f32x2 a = table[t * half + i0], b = table[t * half + i0 + 1];
+  return Rotation{a.y, a.x, b.y, b.x};
+}
+
+// Block j's 64 token rows of head h to LDS: positions of this call from proj (keys
+// normalized and rotated), earlier ones from the tail, others zero.  Ends with a
+// barrier.
+__device__ __forceinline__ void prompt_block_rows(const AppendParams& p, int b, int h, int L, int j, bool values,
+                                                  uint16_t (*rows)[kRow], f32x2* table) {
+  const Kv8& c = p.c;
+  const int64_t bh = (int64_t)b * c.Hkv + h;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, d0 = 2 * lane;
+  const int end = min(L + p.T, c.Smax);
+  const uint16_t* proj = p.proj + (int64_t)b * p.T * p.row_stride + (2 * p.Hq + h + (values ? c.Hkv : 0)) * kHD;
+  __syncthreads();  // the rows and the table may still be read
+  if (!values) rotation_table<kBlk>(table, kBlk * j, p.rot, p.log2_base);
+  if (values) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // 16-byte pieces: token e / 16, features 8 (e % 16)
+      const int e = tid + 256 * i, pos = kBlk * j + (e >> 4);
+      u32x4 w = {0u, 0u, 0u, 0u};
+      if (pos >= L && pos < end) w = ld16(proj + (int64_t)(pos - L) * p.row_stride + (e & 15) * 8);
+      if (pos >= L) *reinterpret_cast<u32x4*>(&rows[e >> 4][(e & 15) * 8]) = w;
+    }
+    if (kBlk * j < L) {  // the tail's values are transposed: thread (feature, 32 slots)
+      const uint16_t* src = c.tail_values(bh) + (tid >> 1) * kSlots + (j & 1) * kBlk + (tid & 1) * 32;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 w = ld16(src + 8 * i);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int tk = (tid & 1) * 32 + 8 * i + u;
+          if (kBlk * j + tk < L) rows[tk][tid >> 1] = (uint16_t)(w[u >> 1] >> (16 * (u & 1)));
+        }
+      }
+    }
+    __syncthreads();
+    return;
+  }
+  uint32_t xv[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int pos = kBlk * j + 16 * wave + i;
+    xv[i] = 0u;
+    if (pos >= L && pos < end)
+      xv[i] = *reinterpret_cast<const uint32_t*>(proj + (int64_t)(pos - L) * p.row_stride + d0);
+    else if (pos < L)
+      xv[i] = *reinterpret_cast<const uint32_t*>(c.tail_keys(bh) + (pos & (kSlots - 1)) * kHD + d0);
+  }
+  const uint32_t wv = *reinterpret_cast<const uint32_t*>(p.k_norm_w + d0);
+  __syncthreads();  // the table is whole
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int tk = 16 * wave + i, pos = kBlk * j + tk;
+    if (pos >= L && pos < end)
+      xv[i] = norm_rotate(xv[i], wv, [&] { return table_rotation(table, tk, d0, p.rot); }, d0, p.rot, p.eps);
+    *reinterpret_cast<uint32_t*>(&rows[tk][d0]) = xv[i];
+  }
+  __syncthreads();
+}
+
+// The codes of the block in LDS rows.
+template <int TYPE>
+__device__ __forceinline__ void quantise_rows(const Kv8& c, int64_t bh, int j, bool values,
+                                              const uint16_t (*rows)[kRow], uint32_t* red) {
+  const int t = threadIdx.x;
+  u32x4 w[4];
+  if (values) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int tk = (t & 1) * 32 + 2 * i;
+      w[i >> 2][i & 3] = (uint32_t)rows[tk][t >> 1] | ((uint32_t)rows[tk + 1][t >> 1] << 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const u32x4*>(&rows[t >> 2][(t & 3) * 32 + 8 * i]);
+  }
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a = max(a, abs_bits16(w[i]));
+  const f32x2 sm = block_scale<TYPE>(group_max_u32(a, red));
+  uint8_t* dst = (values ? c.values(bh, j) : c.keys(bh, j)) + 32 * t;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x2 lo = quantise8<TYPE>(w[2 * i], sm.y), hi = quantise8<TYPE>(w[2 * i + 1], sm.y);
+    *reinterpret_cast<u32x4*>(dst + 16 * i) = u32x4{lo.x, lo.y, hi.x, hi.y};
+  }
+  if (t == 0) (values ? c.vs : c.ks)[bh * c.nblk + j] = sm.x;
+}
+
+// The rows of block j at positions [from, to) into the tail.
+__device__ __forceinline__ void rows_to_tail(const Kv8& c, int64_t bh, int j, bool values, int from, int to,
+                                             const uint16_t (*rows)[kRow]) {
+  const int t = threadIdx.x;
+  if (values) {
+    uint16_t* dst = c.tail_values(bh) + (t >> 1) * kSlots + (j & 1) * kBlk;
+    for (int i = 0; i < 32; ++i) {
+      const int tk = (t & 1) * 32 + i, pos = kBlk * j + tk;
+      if (pos >= from && pos < to) dst[tk] = rows[tk][t >> 1];
+    }
+  } else {
+    const int pos = kBlk * j + (t >> 2);
+    if (pos < from || pos >= to) return;
+    uint16_t* dst = c.tail_keys(bh) + (pos & (kSlots - 1)) * kHD + (t & 3) * 32;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<u32x4*>(dst + 8 * i) = *reinterpret_cast<const u32x4*>(&rows[t >> 2][(t & 3) * 32 + 8 * i]);
+  }
+}
+
+// Workgroups: nb block tasks for the keys and nb for the values of every head, then
+// 16 tokens x 4 query heads each.  Task i quantises block L / 64 + i if the prompt
+// completes it.  Task 0 alone touches the tail: it reads the waiting block and the
+// first block's earlier positions, and only then stores the last two blocks' rows
+// (they take the same slots).
+template <int TYPE>
+__global__ __launch_bounds__(256) void kv8_append_prompt_kernel(const AppendParams p) {
+  __shared__ __attribute__((aligned(16))) uint16_t rows[kBlk][kRow];
+  __shared__ f32x2 table[kBlk * kHD / 2];
+  __shared__ uint32_t red[4];
+  const Kv8& c = p.c;
+  const int64_t ntask = (int64_t)c.B * c.Hkv * 2 * p.nb;
+  int64_t id = blockIdx.x;
+  if (id < ntask) {
+    const int i = (int)(id % p.nb);
+    id /= p.nb;
+    const bool values = id & 1;
+    const int64_t bh = id >> 1;
+    const int b = (int)(bh / c.Hkv), h = (int)(bh % c.Hkv);
+    const int L = p.lens[b];
+    if (L < 0 || L > c.Smax) return;
+    const int first = L >> 6, end = min(L + p.T, c.Smax), done = end >> 6, j = first + i;
+    if (i == 0 && may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, first - 1, values, red);
+    if (j < done) {
+      prompt_block_rows(p, b, h, L, j, values, rows, table);
+      quantise_rows<TYPE>(c, bh, j, values, rows, red);
+    }
+    if (i != 0) return;
+    for (int jj = max(done - 1, first); jj <= done && kBlk * jj < end; ++jj) {
+      prompt_block_rows(p, b, h, L, jj, values, rows, table);
+      rows_to_tail(c, bh, jj, values, L, end, rows);
+    }
+    return;
+  }
+  // queries: a wave 4 tokens x 4 heads
+  id -= ntask;
+  const int hgroups = (p.Hq + 3) >> 2;
+  const int h0 = 4 * (int)(id % hgroups);
+  id /= hgroups;
+  const int tile = (int)(id % p.qtiles), b = (int)(id / p.qtiles);
+  const int L = p.lens[b], t0 = 16 * tile;
+  if (h0 == 0 && tile == 0 && threadIdx.x == 0 && (L < 0 || L > c.Smax - p.T) && p.overflow != nullptr)
+    p.overflow[b] = 1;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = 2 * lane;
+  uint32_t xv[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int t = min(t0 + 4 * wave + (i >> 2), p.T - 1), h = min(h0 + (i & 3), p.Hq - 1);
+    xv[i] = *reinterpret_cast<const uint32_t*>(p.proj + ((int64_t)b * p.T + t) * p.row_stride + 2 * h * kHD + d0);
+  }
+  const uint32_t wv = *reinterpret_cast<const uint32_t*>(p.q_norm_w + d0);
+  rotation_table<16>(table, L + t0, p.rot, p.log2_base);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int tk = 4 * wave + (i >> 2), t = t0 + tk, h = h0 + (i & 3);
+    if (t >= p.T || h >= p.Hq) continue;
+    *reinterpret_cast<uint32_t*>(p.q_out + (((int64_t)b * p.T + t) * p.Hq + h) * kHD + d0) =
+        norm_rotate(xv[i], wv, [&] { return table_rotation(table, tk, d0, p.rot); }, d0, p.rot, p.eps);
+  }
+}
+
+// -------------------------------------------------------------------- load
+struct LoadParams {
+  Kv8 c;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t ks[3], vs[3];  // strides: b, h, position
+  const int32_t* lens;
+  int S, nb;
+};
+
+// Workgroup (block j, keys or values, head): 64 rows to LDS, codes if the block is
+// complete, the tail if it is one of the last two.
+template <int TYPE>
+__global__ __launch_bounds__(256) void kv8_load_kernel(const LoadParams p) {
+  __shared__ __attribute__((aligned(16))) uint16_t rows[kBlk][kRow];
+  __shared__ uint32_t red[4];
+  const Kv8& c = p.c;
+  const int j = (int)(blockIdx.x % p.nb);
+  const int64_t id = blockIdx.x / p.nb;
+  const bool values = id & 1;
+  const int64_t bh = id >> 1;
+  const int b = (int)(bh / c.Hkv), h = (int)(bh % c.Hkv);
+  const int n = min(p.lens[b], min(p.S, c.Smax));
+  if (kBlk * j >= n) return;
+  const int64_t* st = values ? p.vs : p.ks;
+  const uint16_t* src = (values ? p.v : p.k) + b * st[0] + h * st[1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int e = threadIdx.x + 256 * i, pos = min(kBlk * j + (e >> 4), n - 1);
+    *reinterpret_cast<u32x4*>(&rows[e >> 4][(e & 15) * 8]) = ld16(src + pos * st[2] + (e & 15) * 8);
+  }
+  __syncthreads();
+  if (j < n >> 6) quantise_rows<TYPE>(c, bh, j, values, rows, red);
+  if (j >= (n >> 6) - 1) rows_to_tail(c, bh, j, values, 0, n, rows);
+}
+
+// -------------------------------------------------------------------- read
+struct ReadParams {
+  Kv8 c;
+  const int32_t* lens;
+  const int32_t* starts;
+  int start, count, nb;
+  uint16_t* k;
+  uint16_t* v;
+};
+
+// Workgroup (block of positions, keys or values, head): a thread takes 32
+// neighbouring values in stored order, codes or tail, as bf16; the values' rows
+// turn through LDS.
+template <int TYPE>
+__global__ __launch_bounds__(256) void kv8_read_kernel(const ReadParams p) {
+  __shared__ __attribute__((aligned(16))) uint16_t rows[kBlk][kRow];
+  __shared__ uint32_t red[4];
+  const Kv8& c = p.c;
+  const int i = (int)(blockIdx.x % p.nb);
+  const int64_t id = blockIdx.x / p.nb;
+  const bool values = id & 1;
+  const int64_t bh = id >> 1;
+  uint16_t* out = values ? p.v : p.k;
+  if (out == nullptr) return;
+  const int b = (int)(bh / c.Hkv), t = threadIdx.x;
+  const int L = p.lens[b];
+  const int held = min(max(L, 0), c.Smax);
+  const int64_t start = (int64_t)p.start + (p.starts ? p.starts[b] : 0);
+  // block j = floor(start / 64) + i covers the outputs 64 j - start ..
+  const int64_t j = (start >> 6) + i;
+  if (kBlk * j >= start + p.count) return;
+  u32x4 w[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) w[u] = u32x4{0u, 0u, 0u, 0u};
+  if (j >= 0 && kBlk * j < held) {
+    const bool waits = j == (held >> 6) - 1 && may_wait(L, c.Smax);
+    if (j < held >> 6 && !waits) {
+      const uint8_t* src = (values ? c.values(bh, (int)j) : c.keys(bh, (int)j)) + 32 * t;
+      const float s = (values ? c.vs : c.ks)[bh * c.nblk + j];
+      const u32x4 q[2] = {ld16(src), ld16(src + 16)};
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const f32x4 f = codes_f32<TYPE>(q[u >> 2][u & 3]) * s;
+        w[u >> 1][2 * (u & 1)] = pack2(f.x, f.y);
+        w[u >> 1][2 * (u & 1) + 1] = pack2(f.z, f.w);
+      }
+    } else {
+      const int at = ((int)j & 1) * kBlk;
+      const uint16_t* src = values ? c.tail_values(bh) + (t >> 1) * kSlots + at + (t & 1) * 32
+                                   : c.tail_keys(bh) + (at + (t >> 2)) * kHD + (t & 3) * 32;
+      uint32_t a = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        w[u] = ld16(src + 8 * u);
+        a = max(a, abs_bits16(w[u]));
+      }
+      if (waits) {
+        const f32x2 sm = block_scale<TYPE>(group_max_u32(a, red));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const u32x2 q = quantise8<TYPE>(w[u], sm.y);
+          const f32x4 lo = codes_f32<TYPE>(q.x) * sm.x, hi = codes_f32<TYPE>(q.y) * sm.x;
+          w[u] = u32x4{pack2(lo.x, lo.y), pack2(lo.z, lo.w), pack2(hi.x, hi.y), pack2(hi.z, hi.w)};
+        }
+      }
+    }
+  }
+  if (values) {
+#pragma unroll
+    for (int u = 0; u < 32; ++u)
+      rows[(t & 1) * 32 + u][t >> 1] = (uint16_t)(w[u >> 3][(u >> 1) & 3] >> (16 * (u & 1)));
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const u32x4*>(&rows[t >> 2][(t & 3) * 32 + 8 * u]);
+  }
+  const int64_t pos = kBlk * j + (t >> 2), o = pos - start;
+  if (o < 0 || o >= p.count) return;
+  if (pos >= held) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = u32x4{0u, 0u, 0u, 0u};
+  }
+  uint16_t* dst = out + (bh * p.count + o) * kHD + (t & 3) * 32;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) *reinterpret_cast<u32x4*>(dst + 8 * u) = w[u];
+}
+
+bool fits_grid(int64_t wgs) { return wgs <= INT32_MAX; }
+
+}  // namespace
+}  // namespace dflash
+
+using namespace dflash;
+
+#define DFLASH_KV8_LAUNCH(kernel, type, grid, stream, p)                                         \
+  do {                                                                                           \
+    if ((type) == DFLASH_KV_INT8)                                                                \
+      hipLaunchKernelGGL((kernel<DFLASH_KV_INT8>), dim3((unsigned)(grid)), dim3(256), 0,         \
+                         static_cast<hipStream_t>(stream), p);                                   \
+    else                                                                                         \
+      hipLaunchKernelGGL((kernel<DFLASH_KV_E4M3>), dim3((unsigned)(grid)), dim3(256), 0,         \
+                         static_cast<hipStream_t>(stream), p);                                   \
+  } while (0)
+
+extern "C" int dflash_kv8_append(const dflash_kv8_cache* cache, const void* proj, int64_t proj_row_stride,
+                                 const void* q_norm_w, const void* k_norm_w, const int32_t* lens,
+                                 void* q_out, int32_t* overflow, int T, int Hq, int rot_dims,
+                                 float rope_base, float eps, int prompt, void* stream) {
+  AppendParams p{};
+  if (const int rc = check_cache(cache, &p.c)) return rc;
+  const int B = p.c.B, Hkv = p.c.Hkv;
+  if (T < 0 || Hq <= 0 || Hq % Hkv != 0 || (!prompt && T > kMaxDraft)) return DFLASH_ERR_SHAPE;
+  if (!(rot_dims == 0 || rot_dims == 16 || rot_dims == 32 || rot_dims == 64 || rot_dims == 128))
+    return DFLASH_ERR_UNSUPPORTED;
+  if (proj_row_stride < (int64_t)(2 * (int64_t)Hq + 2 * Hkv) * kHD) return DFLASH_ERR_SHAPE;
+  if (T > INT32_MAX - p.c.Smax) return DFLASH_ERR_SHAPE;  // positions are 32-bit
+  if (B == 0 || T == 0) return DFLASH_OK;
+  if (proj == nullptr || q_norm_w == nullptr || k_norm_w == nullptr || lens == nullptr || q_out == nullptr)
+    return DFLASH_ERR_NULL;
+  if (((uintptr_t)proj & 15) || proj_row_stride % 8 || ((uintptr_t)q_norm_w & 3) || ((uintptr_t)k_norm_w & 3) ||
+      ((uintptr_t)q_out & 3))
+    return DFLASH_ERR_ALIGN;
+  p.proj = static_cast<const uint16_t*>(proj);
+  p.row_stride = proj_row_stride;
+  p.q_norm_w = static_cast<const uint16_t*>(q_norm_w);
+  p.k_norm_w = static_cast<const uint16_t*>(k_norm_w);
+  p.lens = lens;
+  p.q_out = static_cast<uint16_t*>(q_out);
+  p.overflow = overflow;
+  p.T = T; p.Hq = Hq; p.rot = rot_dims;
+  p.log2_base = log2((double)rope_base);
+  p.eps = eps;
+  if (!prompt) {
+    const int64_t grid = (int64_t)2 * B * Hkv + (int64_t)B * T * ceil_div(Hq + 2 * Hkv, 4);
+    if (!fits_grid(grid)) return DFLASH_ERR_SHAPE;
+    DFLASH_KV8_LAUNCH(kv8_append_draft_kernel, cache->type, grid, stream, p);
+  } else {
+    p.nb = (int)std::min<int64_t>(T / kBlk + 2, p.c.nblk);
+    p.qtiles = (int)ceil_div(T, 16);
+    const int64_t grid = (int64_t)2 * B * Hkv * p.nb + (int64_t)B * p.qtiles * ceil_div(Hq, 4);
+    if (!fits_grid(grid)) return DFLASH_ERR_SHAPE;
+    DFLASH_KV8_LAUNCH(kv8_append_prompt_kernel, cache->type, grid, stream, p);
+  }
+  return to_status(hipGetLastError());
+}
+
+extern "C" int dflash_kv8_load(const dflash_kv8_cache* cache, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, const int32_t* lens, int S,
+                               void* stream) {
+  LoadParams p{};
+  if (const int rc = check_cache(cache, &p.c)) return rc;
+  if (S < 0) return DFLASH_ERR_SHAPE;
+  if (p.c.B == 0 || S == 0) return DFLASH_OK;
+  if (k == nullptr || v == nullptr || lens == nullptr || k_strides == nullptr || v_strides == nullptr)
+    return DFLASH_ERR_NULL;
+  if (((uintptr_t)k & 15) || ((uintptr_t)v & 15)) return DFLASH_ERR_ALIGN;
+  for (int i = 0; i < 3; ++i) {
+    if (k_strides[i] < 0 || v_strides[i] < 0) return DFLASH_ERR_SHAPE;
+    if (k_strides[i] % 8 || v_strides[i] % 8) return DFLASH_ERR_ALIGN;
+    p.ks[i] = k_strides[i];
+    p.vs[i] = v_strides[i];
+  }
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.lens = lens;
+  p.S = S;
+  p.nb = (int)ceil_div(std::min(S, p.c.Smax), kBlk);
+  const int64_t grid = (int64_t)2 * p.c.B * p.c.Hkv * p.nb;
+  if (!fits_grid(grid)) return DFLASH_ERR_SHAPE;
+  DFLASH_KV8_LAUNCH(kv8_load_kernel, cache->type, grid, stream, p);
+  return to_status(hipGetLastError());
+}
+
+extern "C" int dflash_kv8_read(const dflash_kv8_cache* cache, const int32_t* lens, const int32_t* starts,
+                               int start, int count, void* k_out, void* v_out, void* stream) {
+  ReadParams p{};
+  if (const int rc = check_cache(cache, &p.c)) return rc;
+  if (count < 0) return DFLASH_ERR_SHAPE;
+  if (p.c.B == 0 || count == 0) return DFLASH_OK;
+  if (lens == nullptr || (k_out == nullptr && v_out == nullptr)) return DFLASH_ERR_NULL;
+  if (((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15)) return DFLASH_ERR_ALIGN;
+  p.lens = lens;
+  p.starts = starts;
+  p.start = start;
+  p.count = count;
+  p.nb = (int)(((int64_t)count + 62) / kBlk + 1);  // blocks that count positions can touch
+  p.k = static_cast<uint16_t*>(k_out);
+  p.v = static_cast<uint16_t*>(v_out);
+  const int64_t grid = (int64_t)2 * p.c.B * p.c.Hkv * p.nb;
+  if (!fits_grid(grid)) return DFLASH_ERR_SHAPE;
+  DFLASH_KV8_LAUNCH(kv8_read_kernel, cache->type, grid, stream, p);
+  return to_status(hipGetLastError());
+}

@@ -27,6 +27,15 @@ from .gated_delta import (
     gated_delta_verify_rollback,
     tape_select,
 )
+from .kv8 import (
+    QuantizedKVCache,
+    attn_prefill_q8,
+    attn_prep_q8,
+    attn_verify_q8,
+    attn_verify_q8_workspace_bytes,
+    kv_load_q8,
+    kv_read_q8,
+)
 from .runtime import (
     DFlashRuntimeEvent,
     dflash_generate,
@@ -59,9 +68,14 @@ __all__ = [
     "verify_block_parallel_lazy_logits",
     "verify_block_stream",
     "KVCache",
+    "QuantizedKVCache",
     "Qwen35TargetAdapter",
     "adapter_for_model_type",
     "advance_gated_delta_states",
+    "attn_prefill_q8",
+    "attn_prep_q8",
+    "attn_verify_q8",
+    "attn_verify_q8_workspace_bytes",
     "chunked_prefill_workspace_bytes",
     "conv_rollback",
     "gated_delta_kernel",
@@ -69,6 +83,8 @@ __all__ = [
     "gated_delta_verify",
     "gated_delta_verify_rollback",
     "greedy_accept",
+    "kv_load_q8",
+    "kv_read_q8",
     "lm_head_argmax",
     "lm_head_greedy_accept",
     "longest_prefix_match",

@@ -1,4 +1,5 @@
-"""ctypes binding of libdflash_gfx950.so (declared in include/dflash_gdn.h).
+"""ctypes binding of libdflash_gfx950.so (declared in include/dflash_gdn.h and
+include/dflash_kv8.h).
 
 The library is loaded after ``import torch`` so that it binds to the HIP
 runtime torch already loaded (both use the soname libamdhip64.so.7); loading
@@ -21,7 +22,7 @@ DFLASH_DTYPE_F32 = 0
 DFLASH_DTYPE_BF16 = 1
 DFLASH_DTYPE_F16 = 2
 
-# Every entry point of include/dflash_gdn.h, with its ctypes signature.
+# Every entry point of both headers, with its ctypes signature.
 _VP = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -110,6 +111,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I,
         [_VP, _VP, _VP, _VP, _VP, _I64, _VP, _I, _I, _I, _I, _I, ctypes.c_float, _VP],
     ),
+    "dflash_kv8_append": (
+        _I,
+        [_VP, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, ctypes.c_float, ctypes.c_float, _I, _VP],
+    ),
+    "dflash_kv8_load": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _VP]),
+    "dflash_kv8_read": (_I, [_VP, _VP, _VP, _I, _I, _VP, _VP, _VP]),
+    "dflash_attn_verify_q8_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "dflash_attn_verify_q8": (
+        _I, [_VP, _VP, _VP, _VP, _I64, _VP, _I, _I, ctypes.c_float, _VP, _SZ, _VP]),
+    "dflash_attn_prefill_q8": (
+        _I, [_VP, _VP, _VP, _VP, _I64, _VP, _I, _I, ctypes.c_float, _VP]),
     "dflash_commit_accept": (_I, [_VP, _VP, _VP, _I, _I, _VP]),
     "dflash_greedy_accept_workspace_bytes": (_SZ, [_I, _I, _I]),
     "dflash_greedy_accept_noalloc_max_bytes": (_SZ, []),

@@ -1,0 +1,191 @@
+"""Attention over the 8-bit key/value cache against the same cache in 64 bits.
+
+The bound on an output's error is derived in tests/kv8_util.attention_error:
+the weights' and the output's rounding to bf16."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.kv8_util import BLOCK, D, DTYPES, SLOTS, attention_error, loaded, proj_rows, random_kv, raw
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(device, dtype, T, Hq, Hkv, lens, Smax, seed, prompt, qstd=1.5, pad=16):
+    """A cache holding lens + T positions, as after the rows' append."""
+    B = len(lens)
+    k, v = random_kv(B, Hkv, Smax, seed, spread=False)
+    g = torch.Generator().manual_seed(seed + 1)
+    k = (k.float() * (0.3 + torch.rand(B, Hkv, Smax // BLOCK, generator=g).repeat_interleave(BLOCK, 2)[..., None])).bfloat16()
+    held = [min(max(L, 0) + (T if L >= 0 else 0), Smax) for L in lens]
+    # complete blocks are quantised up to the committed length only
+    cache, _ = loaded(device, k, v, held if prompt else [min(L, Smax) for L in lens], Smax, dtype, fill=0xFF)
+    if not prompt:
+        for b, L in enumerate(lens):
+            if L >= 0:
+                p = torch.arange(min(L, Smax), held[b])
+                cache.tail_k[b, :, p % SLOTS] = k[b, :, p].to(device)
+                cache.tail_vt[b, :, :, p % SLOTS] = v[b, :, p].transpose(1, 2).to(device)
+    q = (qstd * torch.randn(B, T, Hq, D, generator=g)).bfloat16()
+    proj = proj_rows(B, T, Hq, Hkv, seed + 2, pad)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=device)
+    ends = [(n, (n if prompt else min(max(L, 0), Smax)) // BLOCK) for n, L in zip(held, lens)]
+    return cache, lens_d, k, v, q, proj, ends
+
+
+def _check(device, dtype, T, Hq, Hkv, lens, Smax, seed, prompt, scale=None, qstd=1.5):
+    import dflash_mlx as dm
+
+    cache, lens_d, k, v, q, proj, ends = _case(device, dtype, T, Hq, Hkv, lens, Smax, seed, prompt, qstd)
+    before = raw(cache)
+    attend = dm.attn_prefill_q8 if prompt else dm.attn_verify_q8
+    got = attend(q.to(device), cache, lens_d, proj.to(device), scale=scale).cpu()
+    assert all(torch.equal(a, b) for a, b in zip(before, raw(cache)))
+    live = [b for b, L in enumerate(lens) if L >= 0]
+    assert all((got[b] == 0).all() for b in range(len(lens)) if b not in live)
+    pick = lambda x: [x[b] for b in live]  # noqa: E731
+    worst = attention_error(got[live], q[live], pick(k), pick(v), proj[live], [min(L, Smax) for L in pick(lens)], pick(ends),
+                            dtype, D ** -0.5 if scale is None else scale)
+    print(f"[attn q8] {dtype} T={T} {Hq}:{Hkv} lens={lens} prompt={prompt}: {worst:.3f} of the bound", flush=True)
+    assert worst <= 1.0
+
+
+VERIFY = [
+    # T, Hq, Hkv, lens, Smax
+    (1, 4, 1, [0], 64),
+    (1, 16, 4, [500], 576),
+    (16, 16, 4, [0], 64),
+    (16, 16, 4, [1000], 1024),
+    (16, 4, 4, [63, 64, 65, 127, 128, 129], 192),
+    (5, 8, 8, [300, 0, 1, 767], 832),
+    (3, 12, 4, [200, 5000, 64], 5056),
+    (16, 8, 4, [77, 129], 256),
+    (4, 16, 1, [129, 40], 192),     # sixteen query heads on one key/value head
+    (1, 64, 1, [200], 256),         # sixty-four
+    (2, 5, 1, [90], 128),
+    (1, 8, 2, list(range(0, 140)), 192),  # more sequences than lanes
+    (7, 4, 2, [-1, 100, -5, 60], 128),    # two take no part
+    (16, 4, 1, [56, 64], 64),             # the rows run over the cache's end
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Hq,Hkv,lens,Smax", VERIFY)
+def test_verify(device, dtype, T, Hq, Hkv, lens, Smax):
+    _check(device, dtype, T, Hq, Hkv, lens, Smax, seed=T + Hq + len(lens), prompt=False)
+
+
+PROMPT = [
+    (1, 4, 1, [0], 64),
+    (17, 16, 4, [0], 64),
+    (37, 8, 4, [5], 128),
+    (300, 16, 4, [130], 448),
+    (200, 3, 1, [0, 60], 320),
+    (64, 16, 4, [448], 512),
+    (130, 4, 4, [70, 0, 1], 256),
+    (100, 8, 1, [33], 192),     # eight query heads a key/value head: two groups of four
+    (70, 5, 1, [10], 128),      # five: one by one
+    (90, 6, 1, [64], 192),      # six: two groups of three
+    (40, 4, 2, [-1, 30], 128),
+    (80, 4, 2, [20, 64], 64),   # rows past the cache's end see all of it
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Hq,Hkv,lens,Smax", PROMPT)
+def test_prompt(device, dtype, T, Hq, Hkv, lens, Smax):
+    _check(device, dtype, T, Hq, Hkv, lens, Smax, seed=T + Hq + len(lens), prompt=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("scale", [0.5, -0.1, 0.0])
+def test_scales(device, dtype, prompt, scale):
+    _check(device, dtype, 9, 8, 2, [150, 64], 256, seed=4, prompt=prompt, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("prompt", [False, True])
+def test_peaked_scores(device, dtype, prompt):
+    """Queries of std 8: a row's weight sits on a few keys, the maximum moves often."""
+    _check(device, dtype, 16, 4, 2, [700], 768, seed=6, prompt=prompt, qstd=8.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_value_scales_of_every_size(device, dtype):
+    """Blocks whose values differ by 2^60: the output follows the largest, the
+    sum of weights counts all."""
+    import dflash_mlx as dm
+
+    cache, lens_d, k, v, q, proj, ends = _case(device, dtype, 4, 4, 2, [400], 448, 8, False)
+    mag = torch.tensor([1.0, 2.0 ** -60, 2.0 ** 20, 1.0, 2.0 ** 40, 2.0 ** -30, 1.0]).repeat_interleave(BLOCK)
+    v = (v.float() * mag[:, None]).bfloat16()
+    dm.kv_load_q8(k.to(device), v.to(device), lens_d, cache)
+    p = torch.arange(400, 404)
+    cache.tail_k[0, :, p % SLOTS] = k[0, :, p].to(device)
+    cache.tail_vt[0, :, :, p % SLOTS] = v[0, :, p].transpose(1, 2).to(device)
+    got = dm.attn_verify_q8(q.to(device), cache, lens_d, proj.to(device)).cpu()
+    assert attention_error(got, q, k, v, proj, [400], ends, dtype, D ** -0.5) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_that_are_not_finite(device, dtype, bad):
+    """A draft token's value that is not finite is seen by its own row and the
+    later ones, in its feature alone; key NaNs by all features of those rows."""
+    import dflash_mlx as dm
+
+    T, Hq, Hkv, L = 6, 4, 2, 130
+    cache, lens_d, k, v, q, proj, ends = _case(device, dtype, T, Hq, Hkv, [L], 192, 3, False)
+    clean = dm.attn_verify_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(T, Hq, D)
+    cache.tail_vt[0, 1, 17, (L + 3) % SLOTS] = bad
+    got = dm.attn_verify_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(T, Hq, D)
+    hit = torch.zeros(T, Hq, D, dtype=torch.bool)
+    hit[3:, 2:, 17] = True  # key/value head 1: query heads 2 and 3
+    assert not torch.isfinite(got[hit].float()).any()
+    assert torch.equal(got[~hit], clean[~hit])
+    cache.tail_vt[0, 1, 17, (L + 3) % SLOTS] = 0.5
+    cache.tail_k[0, 0, (L + 4) % SLOTS, 5] = float("nan")
+    got = dm.attn_verify_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(T, Hq, D)
+    assert got[4:, :2].isnan().all() and torch.isfinite(got[:4].float()).all() and torch.isfinite(got[4:, 2:].float()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompt_values_that_are_not_finite(device, dtype):
+    """In a prompt: the last partial block's by feature, a quantised block's as NaN
+    of the whole block, and neither by earlier rows."""
+    import dflash_mlx as dm
+
+    T, Hq, Hkv, L = 150, 4, 2, 0
+    cache, lens_d, k, v, q, proj, ends = _case(device, dtype, T, Hq, Hkv, [L], 192, 3, True)
+    clean = dm.attn_prefill_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(T, Hq, D)
+    cache.tail_vt[0, 1, 17, 140 % SLOTS] = float("inf")
+    got = dm.attn_prefill_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(T, Hq, D)
+    hit = torch.zeros(T, Hq, D, dtype=torch.bool)
+    hit[140:, 2:, 17] = True
+    assert not torch.isfinite(got[hit].float()).any()
+    assert torch.equal(got[~hit], clean[~hit])
+    cache.tail_vt[0, 1, 17, 140 % SLOTS] = 0.5
+    for scales in (cache.k_scale, cache.v_scale):
+        good = scales[0, 0, 1].clone()
+        scales[0, 0, 1] = float("nan")  # positions 64 .. 127 of key/value head 0
+        got = dm.attn_prefill_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(T, Hq, D)
+        scales[0, 0, 1] = good
+        assert got[64:, :2].isnan().all()
+        assert torch.equal(got[:64], clean[:64])
+        assert torch.isfinite(got[64:, 2:].float()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_verify_blocks_that_read_as_nan(device, dtype):
+    import dflash_mlx as dm
+
+    cache, lens_d, k, v, q, proj, _ = _case(device, dtype, 2, 4, 2, [200, 200], 256, 3, False)
+    for scales in (cache.k_scale, cache.v_scale):
+        good = scales[1, 0, 2].clone()
+        scales[1, 0, 2] = float("nan")
+        got = dm.attn_verify_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(2, 2, 4, D)
+        scales[1, 0, 2] = good
+        assert got[1, :, :2].isnan().all()
+        assert torch.isfinite(got[0].float()).all() and torch.isfinite(got[1, :, 2:].float()).all()
