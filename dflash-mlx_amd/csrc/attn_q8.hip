@@ -14,25 +14,18 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // ------------------------------------------------------------------ verify
-// The T * Hq / Hkv query rows of a (sequence, key/value head) are packed into RT
-// tiles of 16 (row t * rep + r is query head r of the group, token t).  Work is
+// The T * Hq / Hkv query rows of a (sequence, key/value head), row t * rep + r being
+// query head r of the group at token t, against the positions that they see.  Work is
 // counted in blocks of 64 positions over all heads and sequences; every workgroup
-// takes an equal run of them, whatever the sequences' lengths, its four waves
-// block by block in turn.  A wave keeps running maximum, sum and output of all rows
-// in registers:
-//   - S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16.  A lane (r = lane
-//     % 16, g = lane / 16) holds row r's scores of 16 positions: result row 4 g + e
-//     of tile n is position 16 g + 8 (n / 2) + 4 (n % 2) + e (the tile's operand row
-//     i is loaded from position 16 (i / 4) + ..), so tiles 2 s and 2 s + 1 are
-//     the operand of P V's step s as they stand, with the 8 values 16 g + 8 s .. of
-//     V^T, and P never leaves the lane.
-//   - a block's key scale is one factor of its scores; its value scale goes into
+// takes an equal run of them, whatever the sequences' lengths (found from lens in
+// the kernel).  The runs' ends cut heads into parts: those go to the workspace and a
+// second launch merges them; a head that one workgroup has to itself is finished there.
+//   - Products on MFMA in transposed form, S^T = K Q^T and O^T = V^T P^T: a lane
+//     holds one row's scores and outputs, and P stays in its registers.
+//   - A block's key scale is one factor of its scores; its value scale goes into
 //     the exponent (weights 2^(x + log2 scale - m), m the running maximum of that),
 //     and the sum takes the weights times 1 / scale.
-// The runs' ends cut heads into parts: those go to the workspace and a second
-// launch merges them; a head that one workgroup has to itself is finished there.
-constexpr int kMinRun = 4;  // blocks of a run: one for each wave
-
+//   - Weights are rounded to bf16 for P V; the maximum's is 1 exactly.
 struct VerifyParams {
   Kv8 c;
   const uint16_t* q;  // [B, T, Hq, D]
@@ -40,10 +33,14 @@ struct VerifyParams {
   const uint16_t* gate;
   int64_t gate_stride;
   uint16_t* out;    // [B, T, Hq * D]
-  float* part_o;    // [2 * runs][16 RT][D]
-  float* part_ml;   // [2 * runs][16 RT][2]
-  int T, Hq, rep, runs, rows;  // rows: 16 RT
+  float* part_o;    // [2 * runs][part_rows][D], in the order that the kernel's lanes hold them
+  float* part_ml;   // [2 * runs][part_rows][2]
+  int T, Hq, rep, runs, min_run;
+  int part_rows;  // rows of a part in the workspace
+  uint32_t rep_inv;
   float scale;
+
+  __device__ int token_of(int row) const { return (int)((uint32_t)row * rep_inv >> 16); }  // row / rep, row < 64
 };
 
 __device__ __forceinline__ int wave_sum_i32(int x) {
@@ -70,8 +67,8 @@ __device__ __forceinline__ int all_blocks(const VerifyParams& p, int b, int* bef
     n += v;
     pre += i < b ? v : 0;
   }
-  if (before != nullptr) *before = wave_sum_i32(pre);
-  return wave_sum_i32(n);
+  if (before != nullptr) *before = __builtin_amdgcn_readfirstlane(wave_sum_i32(pre));
+  return __builtin_amdgcn_readfirstlane(wave_sum_i32(n));
 }
 
 // The sequence that unit u falls in, and the units before it.
@@ -100,7 +97,7 @@ __device__ __forceinline__ int sequence_of(const VerifyParams& p, int u, int* be
 }
 
 __device__ __forceinline__ int run_length(const VerifyParams& p, int units) {
-  return max(kMinRun, (units + p.runs - 1) / p.runs);
+  return max(p.min_run, (units + p.runs - 1) / p.runs);
 }
 
 __device__ __forceinline__ float max_over_groups(float x) {  // lanes r, r + 16, r + 32, r + 48
@@ -110,63 +107,23 @@ __device__ __forceinline__ float max_over_groups(float x) {  // lanes r, r + 16,
   return fmaxf(b.x, b.y);
 }
 
-__device__ __forceinline__ bool has_nonfinite(uint32_t w) {
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-}
-__device__ __forceinline__ uint32_t drop_nonfinite(uint32_t w) {
-  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
-  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
-  return w;
+// The halves of packed bf16 that are NaN or infinite, as their bits 15 and 31 (an
+// exponent of all ones carries into them).  Arithmetic, not compares: a mask a value
+// would take a pair of scalar registers each.
+__device__ __forceinline__ uint32_t nonfinite_bits(uint32_t w) {
+  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
 }
 
-// Eight bf16 with those from n on zero.
-__device__ __forceinline__ u32x4 keep_first(u32x4 w, int n) {
+// Eight values' bf16 with those from n on, and those that are not finite, zero.
+__device__ __forceinline__ u32x4 clean_values(u32x4 w, int n, uint32_t& bad) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] &= n >= 2 * i + 2 ? 0xffffffffu : n == 2 * i + 1 ? 0x0000ffffu : 0u;
-  return w;
-}
-
-template <int RT>
-struct Rows {  // a wave's running state: lane (r, g) has row 16 rt + r, features 16 dt + 4 g + e
-  float m[RT], l[RT];
-  f32x4 o[RT][8];
-};
-
-// One block's scores to weights: s[rt][n] in, the operand of P V out.
-template <int RT>
-__device__ __forceinline__ void softmax_block(Rows<RT>& a, f32x4 (&s)[RT][4], float sl, float lv, float iv,
-                                              u32x4 (&pb)[RT][2]) {
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    float mx = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[rt][n][e]);
-    mx = fmaf(max_over_groups(mx), sl, lv);
-    if (__any(mx > a.m[rt])) {
-      const float mn = fmaxf(a.m[rt], mx);
-      const float alpha = a.m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.m[rt] - mn);
-      a.l[rt] *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) a.o[rt][dt] *= alpha;
-      a.m[rt] = mn;
-    }
-    const float off = lv - (a.m[rt] == -INFINITY ? 0.f : a.m[rt]);
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float pe[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        pe[i] = __builtin_amdgcn_exp2f(fmaf(s[rt][2 * k + (i >> 2)][i & 3], sl, off));
-        sum += pe[i];
-      }
-      pb[rt][k] = cvt8_bf16(pe);
-    }
-    a.l[rt] = fmaf(sum, iv, a.l[rt]);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t held = ((uint32_t)((2 * i - n) >> 31) & 0xffffu) | ((uint32_t)((2 * i + 1 - n) >> 31) & 0xffff0000u);
+    const uint32_t x = w[i] & held, y = nonfinite_bits(x);
+    bad |= y;
+    w[i] = x & ~((y >> 15) * 0xffffu);
   }
+  return w;
 }
 
 __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
@@ -174,294 +131,627 @@ __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
                                                  0, 0);
 }
 
-template <int TYPE, int RT>
-__global__ __launch_bounds__(256, RT <= 2 ? 2 : 1) void attn_verify_q8_kernel(const VerifyParams p) {
-  __shared__ __attribute__((aligned(16))) float so[4][16 * RT][kHD + 4];
-  __shared__ float sml[4][16 * RT][2];
+// Four normalized features of a row, times the sigmoid of their gates.
+__device__ __forceinline__ void store_gated(const VerifyParams& p, int64_t bt, int qh, int d, f32x4 v) {
+  const u32x2 g = *reinterpret_cast<const u32x2*>(p.gate + bt * p.gate_stride + qh * 2 * kHD + kHD + d);
+  const float ga[4] = {bf16_lo(g.x), bf16_hi(g.x), bf16_lo(g.y), bf16_hi(g.y)};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] *= 1.f / (1.f + __expf(-ga[e]));
+  *reinterpret_cast<u32x2*>(p.out + (bt * p.Hq + qh) * kHD + d) = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
+}
+
+// The sum of feature d's values at tail positions from .. to that are not finite.  The
+// kernels drop those before P V, where the weight 0 of a row that does not see them
+// would not leave 0, and add them to the rows that do: a NaN or an infinity as in the
+// plain sum.
+__device__ __forceinline__ float dropped_values(const Kv8& c, int64_t bh, int d, int from, int to) {
+  const uint16_t* row = c.tail_values(bh) + d * kSlots;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int pos = from; pos <= to; ++pos) {
+    const uint32_t x = row[pos & (kSlots - 1)];
+    if ((x & 0x7f80u) == 0x7f80u) sum += bf16_bits_to_f32(x);
+  }
+  return sum;
+}
+
+// Where a run starts: the sequence, head and block of unit run0.
+struct Place {
+  int b, h, blk;
+};
+__device__ __forceinline__ Place place_of(const VerifyParams& p, int unit) {
+  int before;
+  const int b = __builtin_amdgcn_readfirstlane(sequence_of(p, unit, &before));
+  const int rem = __builtin_amdgcn_readfirstlane(unit - before);
+  const int nb = max(seen_blocks(__builtin_amdgcn_readfirstlane(p.lens[b]), p.T, p.c.Smax), 1);
+  const int h = rem / nb;
+  return Place{b, h, rem - h * nb};
+}
+
+// Scores are scaled by a positive factor: the scale's sign goes to q, a zero to q itself.
+struct QuerySign {
+  uint32_t keep, flip;
+  __device__ explicit QuerySign(float scale)
+      : keep(scale == 0.f ? 0u : 0xffffffffu), flip(scale < 0.f ? 0x80008000u : 0u) {}
+  __device__ u32x4 operator()(u32x4 q) const { return (q & keep) ^ flip; }
+};
+__device__ __forceinline__ float positive_scale(float scale) { return (scale == 0.f ? 1.f : fabsf(scale)) * kLog2e; }
+
+// N scores of one row and block to weights w[], the running maximum m, sum l and the
+// outputs' factor (1 if the maximum stays).
+template <int N>
+__device__ __forceinline__ float weights(const float (&s)[N], float mx, float sl, float lv, float iv, float& m, float& l,
+                                         float (&w)[N]) {
+  mx = fmaf(mx, sl, lv);
+  float alpha = 1.f;
+  if (__any(mx > m)) {
+    const float mn = fmaxf(m, mx);
+    alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    l *= alpha;
+    m = mn;
+  }
+  const float off = lv - (m == -INFINITY ? 0.f : m);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sl, off));
+    sum += w[i];
+  }
+  l = fmaf(sum, iv, l);
+  return alpha;
+}
+
+// ------------------------------------------------- up to 16 rows (single tokens)
+// Four waves, block by block in turn, straight from memory to registers: nothing is
+// shared.  v_mfma_f32_16x16x32_bf16; lane (r, g) = (lane % 16, lane / 16) has row r.
+// Operand row i of K's tile n is position 16 (i / 4) + 8 (n / 2) + 4 (n % 2) + i % 4,
+// so that result rows 4 g + e of tiles 2 s and 2 s + 1 are positions 16 g + 8 s .. + 7,
+// the ones whose values lie side by side in a row of V^T.  The next block's keys
+// are loaded once these are consumed, its values likewise.
+template <int TYPE>
+__global__ __launch_bounds__(256, 2) void attn_verify_q8_rows16_kernel(const VerifyParams p) {
+  __shared__ __attribute__((aligned(16))) float so[4][16][kHD + 4];
+  __shared__ float sml[4][16][2];
+  __shared__ int dropped;  // the tail's values hold a NaN or an infinity
   const Kv8& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
+  if (tid == 0) dropped = 0;
+  __syncthreads();
   const int units = c.Hkv * all_blocks(p, 0, nullptr);
   const int per = run_length(p, units);
   const int run0 = blockIdx.x * per;
   int left = min(per, units - run0);
   if (left <= 0) return;
-  int before;
-  int b = __builtin_amdgcn_readfirstlane(sequence_of(p, run0, &before));
-  int rem = __builtin_amdgcn_readfirstlane(run0 - before);
-  const float sl0 = (p.scale == 0.f ? 1.f : fabsf(p.scale)) * kLog2e;
+  Place at = place_of(p, run0);
+  const float sl0 = positive_scale(p.scale);
+  const QuerySign sign(p.scale);
+  const int nrows = p.T * p.rep;
+  const int t = min(p.token_of(r), p.T - 1), rr = r - p.token_of(r) * p.rep;
+  const int key0 = 16 * (r >> 2) + (r & 3);  // operand row r of tile n: + 8 (n / 2) + 4 (n % 2)
   bool first_part = true;
-  int h = -1, blk = 0;
   while (left > 0) {
-    const int L = __builtin_amdgcn_readfirstlane(p.lens[b]);
+    const int L = __builtin_amdgcn_readfirstlane(p.lens[at.b]);
     const int seen = seen_positions(L, p.T, c.Smax);
     const int nb = (seen + kBlk - 1) >> 6;
     if (nb == 0) {
-      ++b;
+      ++at.b;
       continue;
     }
-    if (h < 0) {
-      h = rem / nb;
-      blk = rem - h * nb;
-    }
-    const int b1 = min(nb, blk + left);
+    const int b1 = min(nb, at.blk + left);
     const int base = min(L, c.Smax), done = base >> 6;
-    const int64_t bh = (int64_t)b * c.Hkv + h;
-    // the rows' queries: operand (c2, hh) holds features 64 c2 + 16 g + 8 hh ..
-    u32x4 qf[RT][4];
-    int last[RT];  // the last position the lane's row sees
+    const int64_t bh = (int64_t)at.b * c.Hkv + at.h;
+    const int last = min(base + t, seen - 1);  // the last position the lane's row sees
+    u32x4 qf[4];  // operand (k / 2, k % 2): features 64 (k / 2) + 16 g + 8 (k % 2) ..
+    const uint16_t* qsrc = p.q + (((int64_t)at.b * p.T + t) * p.Hq + at.h * p.rep + rr) * kHD + 16 * g;
+    u32x4 kc[4][2], vc[8];
+    float ks = 0.f, vs = 0.f;
+    const uint8_t* kb = c.keys(bh, 0) + key0 * kHD + 16 * g;
+    const uint8_t* vb = c.values(bh, 0) + r * kBlk + 16 * g;
+    const float* ksp = c.ks + bh * c.nblk;
+    const float* vsp = c.vs + bh * c.nblk;
+    auto load_keys = [&](int j) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int row = 16 * rt + r, t = min(row / p.rep, p.T - 1), rr = row % p.rep;
-      last[rt] = min(base + t, seen - 1);
-      const uint16_t* src = p.q + (((int64_t)b * p.T + t) * p.Hq + h * p.rep + rr) * kHD + 16 * g;
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        qf[rt][k] = ld16(src + 64 * (k >> 1) + 8 * (k & 1));
-        // scores are scaled by a positive factor: the sign goes to q, a zero to q itself
-        if (!(p.scale > 0.f))
-          qf[rt][k] = p.scale < 0.f ? qf[rt][k] ^ 0x80008000u : p.scale == 0.f ? u32x4{0u, 0u, 0u, 0u} : qf[rt][k];
+        for (int k = 0; k < 2; ++k)
+          kc[n][k] = ld16(kb + (int64_t)j * kBlkBytes + (8 * (n >> 1) + 4 * (n & 1)) * kHD + 64 * k);
+    };
+    auto load_values = [&](int j) {
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) vc[dt] = ld16(vb + (int64_t)j * kBlkBytes + 16 * dt * kBlk);
+    };
+    const int coded = min(b1, done);
+    int j = at.blk + wave;
+    if (j < coded) {
+      load_keys(j);
+      load_values(j);
+      ks = ksp[j];
+      vs = vsp[j];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) qf[k] = sign(ld16(qsrc + 64 * (k >> 1) + 8 * (k & 1)));
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[8];
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float s[16], w[16];
+    u32x4 pb[2];
+    auto softmax = [&](float sl, float lv, float iv) {
+      float mx = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      const float alpha = weights<16>(s, max_over_groups(mx), sl, lv, iv, m, l, w);
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[dt] *= alpha;
       }
-    }
-    Rows<RT> a;
+      pb[0] = cvt8_bf16(w);
+      pb[1] = cvt8_bf16(w + 8);
+    };
+    for (; j < coded; j += 4) {  // every row sees the whole block
+      const int next = min(j + 4, coded - 1);  // (past the last: loaded again, not used)
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      a.m[rt] = -INFINITY;
-      a.l[rt] = 0.f;
+      for (int n = 0; n < 4; ++n) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt) a.o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int j = blk + wave; j < b1; j += 4) {
-      f32x4 s[RT][4];
-      u32x4 pb[RT][2];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) s[rt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (j < done) {  // codes; every row sees the whole block
-        const uint8_t* kb = c.keys(bh, j) + 16 * g;
-        const uint8_t* vb = c.values(bh, j) + r * kBlk + 16 * g;
-        u32x4 kc[4][2], vc[8];
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            kc[n][k] = ld16(kb + (16 * (r >> 2) + 8 * (n >> 1) + 4 * (n & 1) + (r & 3)) * kHD + 64 * k);
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) vc[dt] = ld16(vb + 16 * dt * kBlk);
-        const float ks = c.ks[bh * c.nblk + j], vs = c.vs[bh * c.nblk + j];
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const u32x2 lo = codes_bf16<TYPE>(kc[n][k >> 1][2 * (k & 1)]);
-            const u32x2 hi = codes_bf16<TYPE>(kc[n][k >> 1][2 * (k & 1) + 1]);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[rt][n] = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, qf[rt][k], s[rt][n]);
-          }
-        softmax_block<RT>(a, s, sl0 * ks, __log2f(vs), 1.f / vs, pb);
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const u32x2 lo = codes_bf16<TYPE>(vc[dt][2 * k]), hi = codes_bf16<TYPE>(vc[dt][2 * k + 1]);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              a.o[rt][dt] = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[rt][k], a.o[rt][dt]);
-          }
-      } else {  // the tail, in bf16
-        const int at = (j & 1) * kBlk, p0 = kBlk * j;
-        const uint16_t* kb = c.tail_keys(bh) + at * kHD + 16 * g;
-        const uint16_t* vb = c.tail_values(bh) + r * kSlots + at + 16 * g;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const u32x4 kf = ld16(kb + (16 * (r >> 2) + 8 * (n >> 1) + 4 * (n & 1) + (r & 3)) * kHD + 64 * (k >> 1) +
-                                  8 * (k & 1));
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[rt][n] = mfma_bf16(kf, qf[rt][k], s[rt][n]);
-          }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (p0 + 16 * g + 8 * (n >> 1) + 4 * (n & 1) + e > last[rt]) s[rt][n][e] = -INFINITY;
-        softmax_block<RT>(a, s, sl0, 0.f, 1.f, pb);
-        // slots past the held positions hold anything; a row's weight for a
-        // token it does not see is 0, which a NaN or an infinity would not leave 0
-        bool bad = false;
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            u32x4 vf = keep_first(ld16(vb + 16 * dt * kSlots + 8 * k), seen - (p0 + 16 * g + 8 * k));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              bad |= has_nonfinite(vf[i]);
-              vf[i] = drop_nonfinite(vf[i]);
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) a.o[rt][dt] = mfma_bf16(vf, pb[rt][k], a.o[rt][dt]);
-          }
-        if (__any(bad)) {  // what was dropped, for the rows that see it
-          const int n = min(kBlk, seen - p0);
-          for (int i = 0; i < n; ++i)
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t x = c.tail_values(bh)[(16 * dt + 4 * g + e) * kSlots + at + i];
-                if ((x & 0x7f80u) != 0x7f80u) continue;
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                  if (p0 + i <= last[rt]) a.o[rt][dt][e] += bf16_bits_to_f32(x);
-              }
+        for (int k = 0; k < 4; ++k) {
+          const u32x2 lo = codes_bf16<TYPE>(kc[n][k >> 1][2 * (k & 1)]);
+          const u32x2 hi = codes_bf16<TYPE>(kc[n][k >> 1][2 * (k & 1) + 1]);
+          acc = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, qf[k], acc);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * n + e] = acc[e];
       }
+      const float sl = sl0 * ks, lv = __log2f(vs), iv = 1.f / vs;
+      load_keys(next);
+      ks = ksp[next];
+      vs = vsp[next];
+      softmax(sl, lv, iv);
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const u32x2 lo = codes_bf16<TYPE>(vc[dt][2 * k]), hi = codes_bf16<TYPE>(vc[dt][2 * k + 1]);
+          o[dt] = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[k], o[dt]);
+        }
+      load_values(next);
+    }
+    for (; j < b1; j += 4) {  // the tail, in bf16
+      const int slot = (j & 1) * kBlk, p0 = kBlk * j;
+      const uint16_t* tk = c.tail_keys(bh) + (slot + key0) * kHD + 16 * g;
+      const uint16_t* tv = c.tail_values(bh) + r * kSlots + slot + 16 * g;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          acc = mfma_bf16(ld16(tk + (8 * (n >> 1) + 4 * (n & 1)) * kHD + 64 * (k >> 1) + 8 * (k & 1)), qf[k], acc);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[4 * n + e] = p0 + 16 * g + 8 * (n >> 1) + 4 * (n & 1) + e > last ? -INFINITY : acc[e];
+      }
+      softmax(sl0, 0.f, 1.f);
+      // slots past the held positions hold anything; a row's weight for a token
+      // that it does not see is 0, which a NaN or an infinity would not leave 0
+      uint32_t bad = 0;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          o[dt] = mfma_bf16(clean_values(ld16(tv + 16 * dt * kSlots + 8 * k), seen - (p0 + 16 * g + 8 * k), bad), pb[k],
+                            o[dt]);
+      if (bad) dropped = 1;
     }
     // the four waves' states through LDS
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float l = a.l[rt];
-      l += __shfl_xor(l, 16, 64);
-      l += __shfl_xor(l, 32, 64);
-      const int row = 16 * rt + r;
-      if (g == 0) {
-        sml[wave][row][0] = a.m[rt];
-        sml[wave][row][1] = l;
-      }
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(&so[wave][row][16 * dt + 4 * g]) = a.o[rt][dt];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g == 0) {
+      sml[wave][r][0] = m;
+      sml[wave][r][1] = l;
     }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(&so[wave][r][16 * dt + 4 * g]) = o[dt];
     __syncthreads();
-    const bool whole = blk == 0 && b1 == nb;
+    const bool whole = at.blk == 0 && b1 == nb;
     const int64_t part = 2 * (int64_t)blockIdx.x + (first_part ? 0 : 1);
-    for (int i = tid; i < 16 * RT * 32; i += 256) {
+    for (int i = tid; i < nrows * 32; i += 256) {
       const int row = i >> 5, d = (i & 31) * 4;
-      if (row >= p.T * p.rep) break;
-      float m = -INFINITY, l = 0.f;
+      float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) m = fmaxf(m, sml[w][row][0]);
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < 4; ++x) mm = fmaxf(mm, sml[x][row][0]);
+      f32x4 oo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float mw = sml[w][row][0];
-        const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
-        l = fmaf(sml[w][row][1], f, l);
-        o += *reinterpret_cast<const f32x4*>(&so[w][row][d]) * f;
+      for (int x = 0; x < 4; ++x) {
+        const float mw = sml[x][row][0];
+        const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
+        ll = fmaf(sml[x][row][1], f, ll);
+        oo += *reinterpret_cast<const f32x4*>(&so[x][row][d]) * f;
       }
+      const int tt = p.token_of(row);
+      if (dropped)
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+          const float x = dropped_values(c, bh, d + e, kBlk * max(done, at.blk), min(min(base + tt, seen - 1), kBlk * b1 - 1));
+          oo.x += e == 0 ? x : 0.f;
+          oo.y += e == 1 ? x : 0.f;
+          oo.z += e == 2 ? x : 0.f;
+          oo.w += e == 3 ? x : 0.f;
+        }
       if (whole) {
-        const int t = row / p.rep, qh = h * p.rep + row % p.rep;
-        const int64_t bt = (int64_t)b * p.T + t;
-        const u32x2 gv = *reinterpret_cast<const u32x2*>(p.gate + bt * p.gate_stride + qh * 2 * kHD + kHD + d);
-        const float inv = 1.f / l;
-        const float ga[4] = {bf16_lo(gv.x), bf16_hi(gv.x), bf16_lo(gv.y), bf16_hi(gv.y)};
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = o[e] * inv * (1.f / (1.f + __expf(-ga[e])));
-        *reinterpret_cast<u32x2*>(p.out + (bt * p.Hq + qh) * kHD + d) = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
+        const int qh = at.h * p.rep + row - tt * p.rep;
+        store_gated(p, (int64_t)at.b * p.T + tt, qh, d, oo * (1.f / ll));
       } else {
-        *reinterpret_cast<f32x4*>(p.part_o + (part * p.rows + row) * kHD + d) = o;
-        if (d == 0) *reinterpret_cast<f32x2*>(p.part_ml + (part * p.rows + row) * 2) = f32x2{m, l};
+        *reinterpret_cast<f32x4*>(p.part_o + (part * p.part_rows + row) * kHD + d) = oo;
+        if (d == 0) *reinterpret_cast<f32x2*>(p.part_ml + (part * p.part_rows + row) * 2) = f32x2{mm, ll};
       }
     }
     __syncthreads();
+    if (tid == 0) dropped = 0;
     first_part = false;
-    left -= b1 - blk;
-    blk = 0;
-    if (b1 == nb && ++h == c.Hkv) {
-      h = 0;
-      ++b;
+    left -= b1 - at.blk;
+    at.blk = 0;
+    if (b1 == nb && ++at.h == c.Hkv) {
+      at.h = 0;
+      ++at.b;
     }
   }
 }
 
-// One workgroup per (token, query head): merges the parts of a head that several
-// runs share, wave w the parts w, w + 4, ..; lane l has features 2 l, 2 l + 1.
-__global__ __launch_bounds__(256) void attn_verify_q8_merge_kernel(const VerifyParams p) {
+// ------------------------------------------------- up to 64 rows (draft blocks)
+// RT tiles of 32 rows, two waves each: wave half hf takes 32 of a block's 64
+// positions, on v_mfma_f32_32x32x16_bf16 (lane: row lane % 32, positions 8 (i / 4) + 4
+// (lane / 32) + i % 4 of its half in result element i).  All waves read the same
+// block: its codes are loaded once, a block ahead, and become bf16 on their way
+// to the other of two LDS buffers, as the prompt kernel's.
+template <int TYPE, int RT>
+__global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(const VerifyParams p) {
+  constexpr int NT = 128 * RT, PER = kBlk * kHD / 16 / NT;
+  constexpr int BUF = 2 * kBlk * kHD * 2;  // bytes of a block's K and V^T in bf16
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
+  __shared__ f32x2 sml[RT][2][32];
+  __shared__ int dropped;  // the tail's values hold a NaN or an infinity
+  const Kv8& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, hl = lane >> 5;
+  const int hf = wave / RT, rt = wave % RT;
+  if (tid == 0) dropped = 0;
+  __syncthreads();
+  const int units = c.Hkv * all_blocks(p, 0, nullptr);
+  const int per = run_length(p, units);
+  const int run0 = blockIdx.x * per;
+  int left = min(per, units - run0);
+  if (left <= 0) return;
+  Place at = place_of(p, run0);
+  const float sl0 = positive_scale(p.scale);
+  const QuerySign sign(p.scale);
+  const int nrows = p.T * p.rep;
+  const int row = 32 * rt + r32;
+  const int t = min(p.token_of(row), p.T - 1), rr = row - p.token_of(row) * p.rep;
+  bool first_part = true;
+  while (left > 0) {
+    const int L = __builtin_amdgcn_readfirstlane(p.lens[at.b]);
+    const int seen = seen_positions(L, p.T, c.Smax);
+    const int nb = (seen + kBlk - 1) >> 6;
+    if (nb == 0) {
+      ++at.b;
+      continue;
+    }
+    const int b1 = min(nb, at.blk + left);
+    const int base = min(L, c.Smax), done = base >> 6;
+    const int64_t bh = (int64_t)at.b * c.Hkv + at.h;
+    const int last = min(base + t, seen - 1);
+    u32x4 kv[PER], vv[PER];
+    // Unit i of a thread: K's key kkey + NT / 8 i, features 16 (tid % 8) ..; V^T's feature
+    // vrow + NT / 4 i, keys 16 (tid % 4) ..  (both steps multiples of 8: one swizzle).
+    const int kkey = tid >> 3, vrow = tid >> 2;
+    auto load_block = [&](int j) {
+      if (j >= done) return;
+      const uint8_t* ksrc = c.keys(bh, j) + 16 * tid;
+      const uint8_t* vsrc = c.values(bh, j) + 16 * tid;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        kv[i] = ld16(ksrc + 16 * NT * i);
+        vv[i] = ld16(vsrc + 16 * NT * i);
+      }
+    };
+    auto store_pair = [&](unsigned char* row, int piece, int swizzle, u32x4 x, u32x4 y) {
+      *reinterpret_cast<u32x4*>(row + ((piece ^ swizzle) << 4)) = x;
+      *reinterpret_cast<u32x4*>(row + (((piece + 1) ^ swizzle) << 4)) = y;
+    };
+    auto store_block = [&](unsigned char* buf, int j) {
+      unsigned char* kdst = buf + kkey * 256;
+      unsigned char* vdst = buf + BUF / 2 + vrow * 128;
+      if (j < done) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          u32x2 x[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) x[u] = codes_bf16<TYPE>(kv[i][u]);
+          store_pair(kdst + 32 * NT * i, 2 * (tid & 7), kkey & 7, u32x4{x[0].x, x[0].y, x[1].x, x[1].y},
+                     u32x4{x[2].x, x[2].y, x[3].x, x[3].y});
+          __builtin_amdgcn_sched_barrier(0);
+          // 16 keys: the first piece keeps 0-3 and 8-11 (lane / 32 = 0), the second 4-7 and 12-15
+#pragma unroll
+          for (int u = 0; u < 4; ++u) x[u] = codes_bf16<TYPE>(vv[i][u]);
+          store_pair(vdst + 32 * NT * i, 2 * (tid & 3), vrow & 7, u32x4{x[0].x, x[0].y, x[2].x, x[2].y},
+                     u32x4{x[1].x, x[1].y, x[3].x, x[3].y});
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        const int slot = (j & 1) * kBlk;
+        const uint16_t* ksrc = c.tail_keys(bh) + (slot + kkey) * kHD + (tid & 7) * 16;
+        const uint16_t* vsrc = c.tail_values(bh) + vrow * kSlots + slot + (tid & 3) * 16;
+        const int n = seen - (kBlk * j + 16 * (tid & 3));
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          store_pair(kdst + 32 * NT * i, 2 * (tid & 7), kkey & 7, ld16(ksrc + 16 * NT * i), ld16(ksrc + 16 * NT * i + 8));
+          const u32x4 x = clean_values(ld16(vsrc + 32 * NT * i), n, bad);
+          const u32x4 y = clean_values(ld16(vsrc + 32 * NT * i + 8), n - 8, bad);
+          store_pair(vdst + 32 * NT * i, 2 * (tid & 3), vrow & 7, u32x4{x.x, x.y, y.x, y.y}, u32x4{x.z, x.w, y.z, y.w});
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (bad) dropped = 1;
+      }
+    };
+    load_block(at.blk);
+    const uint16_t* qsrc = p.q + (((int64_t)at.b * p.T + t) * p.Hq + at.h * p.rep + rr) * kHD + 8 * hl;
+    u32x4 qb[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) qb[k] = sign(ld16(qsrc + 16 * k));
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[4];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) o[dt] = f32x16{};
+#pragma unroll 1
+    for (int j = at.blk; j < b1; ++j) {
+      // one barrier a block: the buffer that block j + 1 goes to was read before this one
+      unsigned char* buf = lds + (j & 1) * BUF;
+      store_block(buf, j);
+      float ks = 1.f, vs = 1.f;
+      if (j < done) {
+        ks = c.ks[bh * c.nblk + j];
+        vs = c.vs[bh * c.nblk + j];
+      }
+      if (j + 1 < b1) load_block(j + 1);
+      __syncthreads();
+      const unsigned char* sk = buf + (32 * hf + r32) * 256;
+      const unsigned char* sv = buf + BUF / 2 + r32 * 128;
+      f32x16 st = {};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(sk + (((2 * k + hl) ^ (r32 & 7)) << 4))),
+            __builtin_bit_cast(bf16x8, qb[k]), st, 0, 0, 0);
+      const int k0 = kBlk * j + 32 * hf;
+      if (j >= done) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (k0 + 8 * (i >> 2) + 4 * hl + (i & 3) > last) st[i] = -INFINITY;
+      }
+      float s[16], w[16];
+      float mx = st[0];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = st[i];
+        mx = fmaxf(mx, st[i]);
+      }
+      const f32x2 mb = both_halves(mx);
+      const float alpha = weights<16>(s, fmaxf(mb.x, mb.y), sl0 * ks, __log2f(vs), 1.f / vs, m, l, w);
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const u32x4 pb = cvt8_bf16(w + 8 * x);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
+                                             sv + 32 * dt * 128 + (((2 * (2 * hf + x) + hl) ^ (r32 & 7)) << 4))),
+              __builtin_bit_cast(bf16x8, pb), o[dt], 0, 0, 0);
+      }
+    }
+    __syncthreads();
+    // Both halves' states through LDS: the waves of a tile finish eight sixteenths of its
+    // outputs each, sixteenth q (features 32 (q / 4) + 8 (q % 4) + 4 hl ..) as the lanes
+    // hold it.
+    f32x4* so = reinterpret_cast<f32x4*>(lds) + rt * (2 * 16 * 64) + lane;
+#pragma unroll
+    for (int q = 0; q < 16; ++q)
+      so[(hf * 16 + q) * 64] = f32x4{o[q >> 2][4 * (q & 3)], o[q >> 2][4 * (q & 3) + 1], o[q >> 2][4 * (q & 3) + 2],
+                                     o[q >> 2][4 * (q & 3) + 3]};
+    const f32x2 lb = both_halves(l);
+    sml[rt][hf][r32] = f32x2{m, lb.x + lb.y};
+    __syncthreads();
+    const f32x2 ml0 = sml[rt][0][r32], ml1 = sml[rt][1][r32];
+    const float mn = fmaxf(ml0.x, ml1.x);
+    float c0 = ml0.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml0.x - mn);
+    float c1 = ml1.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml1.x - mn);
+    const float ls = ml0.y * c0 + ml1.y * c1;
+    const bool whole = at.blk == 0 && b1 == nb;
+    const int64_t part = (2 * (int64_t)blockIdx.x + (first_part ? 0 : 1)) * RT + rt;
+    const float inv = whole ? 1.f / ls : 1.f;
+    c0 *= inv;
+    c1 *= inv;
+#pragma unroll 2
+    for (int q = 8 * hf; q < 8 * hf + 8; ++q) {
+      f32x4 v = so[q * 64] * c0 + so[(16 + q) * 64] * c1;
+      const int d = 32 * (q >> 2) + 8 * (q & 3) + 4 * hl;
+      if (dropped)
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+          const float x = dropped_values(c, bh, d + e, kBlk * max(done, at.blk), min(last, kBlk * b1 - 1));
+          v.x += e == 0 ? x : 0.f;
+          v.y += e == 1 ? x : 0.f;
+          v.z += e == 2 ? x : 0.f;
+          v.w += e == 3 ? x : 0.f;
+        }
+      if (!whole) {
+        *reinterpret_cast<f32x4*>(p.part_o + part * (32 * kHD) + 256 * q + 4 * lane) = v;
+      } else if (row < nrows) {
+        store_gated(p, (int64_t)at.b * p.T + t, at.h * p.rep + rr, d, v);
+      }
+    }
+    if (!whole && hf == 0 && hl == 0) *reinterpret_cast<f32x2*>(p.part_ml + (part * 32 + r32) * 2) = f32x2{mn, ls};
+    __syncthreads();
+    if (tid == 0) dropped = 0;
+    first_part = false;
+    left -= b1 - at.blk;
+    at.blk = 0;
+    if (b1 == nb && ++at.h == c.Hkv) {
+      at.h = 0;
+      ++at.b;
+    }
+  }
+}
+
+// ------------------------------------------------------------------- merge
+// The parts of head bh: part of its first run, 2 w of the others up to run w1.
+struct Parts {
+  int w0, w1, head;
+  __device__ int at(int w) const { return w == w0 ? head : 2 * w; }
+};
+__device__ __forceinline__ Parts parts_of(const VerifyParams& p, int b, int h, int nb) {
+  int before;
+  const int per = run_length(p, p.c.Hkv * all_blocks(p, b, &before));
+  const int u0 = p.c.Hkv * before + h * nb;
+  const int w0 = u0 / per;
+  return Parts{w0, (u0 + nb - 1) / per, 2 * w0 + (u0 > w0 * per ? 1 : 0)};
+}
+
+// Running merge of parts that one lane walks, in turn with three other waves: V is
+// the vector of outputs that the lane holds.
+template <class V>
+struct Merged {
+  float m = -INFINITY, l = 0.f;
+  V o = V{};
+  __device__ void add(float pm, float pl, V po) {
+    const float mn = fmaxf(m, pm);
+    const float ca = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    const float cb = pm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm - mn);
+    l = l * ca + pl * cb;
+    o = o * ca + po * cb;
+    m = mn;
+  }
+};
+
+// Up to 16 rows: a workgroup per (token, query head); lane l has features 2 l, 2 l + 1,
+// the waves take the parts in turn.
+__global__ __launch_bounds__(256) void attn_verify_q8_merge16_kernel(const VerifyParams p) {
   __shared__ float sm[4], sl[4];
   __shared__ f32x2 so[4][64];
   const int bt = blockIdx.x, qh = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int b = bt / p.T, t = bt - b * p.T, h = qh / p.rep, row = t * p.rep + qh % p.rep;
+  const int b = bt / p.T, t = bt - b * p.T, h = qh / p.rep, row = t * p.rep + qh - h * p.rep;
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + ((int64_t)bt * p.Hq + qh) * kHD + 2 * lane);
   const int nb = seen_blocks(p.lens[b], p.T, p.c.Smax);
   if (nb == 0) {  // takes no part
     if (wave == 0) *dst = 0u;
     return;
   }
-  int before;
-  const int per = run_length(p, p.c.Hkv * all_blocks(p, b, &before));
-  const int u0 = p.c.Hkv * before + h * nb;
-  const int w0 = u0 / per, w1 = (u0 + nb - 1) / per;
-  if (w0 == w1) return;  // finished by its one run
-  const int head = 2 * w0 + (u0 > w0 * per ? 1 : 0);  // part of the first run; 2 w of the others
-  float m = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
-  for (int s0 = w0 + wave; s0 <= w1; s0 += 16) {
+  const Parts parts = parts_of(p, b, h, nb);
+  if (parts.w0 == parts.w1) return;  // finished by its one run
+  Merged<f32x2> a;
+  for (int w = parts.w0 + wave; w <= parts.w1; w += 16) {
     f32x2 ml[4], os[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int s = min(s0 + 4 * u, w1);
-      const int64_t i = (int64_t)(s == w0 ? head : 2 * s) * p.rows + row;
+      const int64_t i = (int64_t)parts.at(min(w + 4 * u, parts.w1)) * p.part_rows + row;
       ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * i);
       os[u] = *reinterpret_cast<const f32x2*>(p.part_o + i * kHD + 2 * lane);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (s0 + 4 * u > w1) continue;
-      const float mn = fmaxf(m, ml[u].x);
-      const float ca = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-      const float cb = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mn);
-      l = l * ca + ml[u].y * cb;
-      a0 = a0 * ca + os[u].x * cb;
-      a1 = a1 * ca + os[u].y * cb;
-      m = mn;
-    }
+    for (int u = 0; u < 4; ++u)
+      if (w + 4 * u <= parts.w1) a.add(ml[u].x, ml[u].y, os[u]);
   }
   if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
+    sm[wave] = a.m;
+    sl[wave] = a.l;
   }
-  so[wave][lane] = f32x2{a0, a1};
+  so[wave][lane] = a.o;
   __syncthreads();
   if (wave != 0) return;
-  float mm = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) mm = fmaxf(mm, sm[k]);
-  float lsum = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float f = sm[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[k] - mm);
-    lsum = fmaf(sl[k], f, lsum);
-    o0 = fmaf(so[k][lane].x, f, o0);
-    o1 = fmaf(so[k][lane].y, f, o1);
-  }
-  const float inv = 1.f / lsum;
+  for (int k = 1; k < 4; ++k) a.add(sm[k], sl[k], so[k][lane]);
+  const float inv = 1.f / a.l;
   const uint32_t gv =
       *reinterpret_cast<const uint32_t*>(p.gate + (int64_t)bt * p.gate_stride + qh * 2 * kHD + kHD + 2 * lane);
   const float g0 = 1.f / (1.f + __expf(-bf16_lo(gv))), g1 = 1.f / (1.f + __expf(-bf16_hi(gv)));
-  *dst = pack2(o0 * inv * g0, o1 * inv * g1);
+  *dst = pack2(a.o.x * inv * g0, a.o.y * inv * g1);
 }
 
-int verify_runs(int64_t B, int Hkv, int Smax, int rt) {
+// Up to 64 rows: a workgroup per (sequence, key/value head, tile, sixteenth q of its
+// outputs), a part's outputs as the lanes stored them; the waves take the parts in turn.
+__global__ __launch_bounds__(256) void attn_verify_q8_merge64_kernel(const VerifyParams p) {
+  __shared__ float sm[4][64], sl[4][64];
+  __shared__ f32x4 so[4][64];
+  const int tiles = p.part_rows >> 5;
+  const int q = blockIdx.x & 15, rt = (blockIdx.x >> 4) % tiles, h = (blockIdx.x >> 4) / tiles, b = blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r32 = lane & 31, hl = lane >> 5, row = 32 * rt + r32;
+  const int t = p.token_of(row), qh = h * p.rep + row - t * p.rep, d = 32 * (q >> 2) + 8 * (q & 3) + 4 * hl;
+  const bool live = row < p.T * p.rep;
+  const int nb = seen_blocks(p.lens[b], p.T, p.c.Smax);
+  if (nb == 0) {  // takes no part
+    if (wave == 0 && live)
+      *reinterpret_cast<u32x2*>(p.out + (((int64_t)b * p.T + t) * p.Hq + qh) * kHD + d) = u32x2{0u, 0u};
+    return;
+  }
+  const Parts parts = parts_of(p, b, h, nb);
+  if (parts.w0 == parts.w1) return;  // finished by its one run
+  Merged<f32x4> a;
+  for (int w = parts.w0 + wave; w <= parts.w1; w += 16) {
+    f32x2 ml[4];
+    f32x4 os[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = (int64_t)parts.at(min(w + 4 * u, parts.w1)) * tiles + rt;
+      ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + (i * 32 + r32) * 2);
+      os[u] = *reinterpret_cast<const f32x4*>(p.part_o + i * (32 * kHD) + 256 * q + 4 * lane);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (w + 4 * u <= parts.w1) a.add(ml[u].x, ml[u].y, os[u]);
+  }
+  sm[wave][lane] = a.m;
+  sl[wave][lane] = a.l;
+  so[wave][lane] = a.o;
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int k = 1; k < 4; ++k) a.add(sm[k][lane], sl[k][lane], so[k][lane]);
+  if (live) store_gated(p, (int64_t)b * p.T + t, qh, d, a.o * (1.f / a.l));
+}
+
+// Rows of a part, blocks of a run at least (a short run's own work should cost more
+// than its part's way through the workspace), and the runs: what the device holds
+// at a time, or fewer for a small cache.
+struct VerifyShape {
+  int part_rows, min_run, runs;
+};
+VerifyShape verify_shape(int64_t B, int rows, int Hkv, int Smax) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  const int64_t most = (int64_t)cus * (rt <= 2 ? 2 : 1);  // workgroups that fit at a time
-  return (int)std::max<int64_t>(1, std::min(most, ceil_div(B * Hkv * (Smax / kBlk), kMinRun)));
+  VerifyShape v;
+  v.part_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  v.min_run = rows <= 16 ? 4 : 2;
+  v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus, ceil_div(B * Hkv * (Smax / kBlk), v.min_run)));
+  return v;
 }
 
 template <int TYPE>
-void launch_verify(const VerifyParams& p, int rt, hipStream_t s) {
+void launch_verify(const VerifyParams& p, hipStream_t s) {
   const dim3 grid((unsigned)p.runs);
-  switch (rt) {
-    case 1: hipLaunchKernelGGL((attn_verify_q8_kernel<TYPE, 1>), grid, dim3(256), 0, s, p); break;
-    case 2: hipLaunchKernelGGL((attn_verify_q8_kernel<TYPE, 2>), grid, dim3(256), 0, s, p); break;
-    case 3: hipLaunchKernelGGL((attn_verify_q8_kernel<TYPE, 3>), grid, dim3(256), 0, s, p); break;
-    default: hipLaunchKernelGGL((attn_verify_q8_kernel<TYPE, 4>), grid, dim3(256), 0, s, p); break;
-  }
+  if (p.part_rows == 16)
+    hipLaunchKernelGGL((attn_verify_q8_rows16_kernel<TYPE>), grid, dim3(256), 0, s, p);
+  else if (p.part_rows == 32)
+    hipLaunchKernelGGL((attn_verify_q8_rows64_kernel<TYPE, 1>), grid, dim3(128), 0, s, p);
+  else
+    hipLaunchKernelGGL((attn_verify_q8_rows64_kernel<TYPE, 2>), grid, dim3(256), 0, s, p);
 }
 
 // ------------------------------------------------------------------ prompt
@@ -575,16 +865,11 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
           vw[u >> 1][2 * (u & 1) + 1] = y.y;
         }
       } else {
-        bool bad = false;
+        uint32_t bad = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           kw[u] = kv[i][u];
-          vw[u] = keep_first(vv[i][u], seen - (kBlk * j + 16 * (e & 3) + 8 * u));
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            bad |= has_nonfinite(vw[u][x]);
-            vw[u][x] = drop_nonfinite(vw[u][x]);
-          }
+          vw[u] = clean_values(vv[i][u], seen - (kBlk * j + 16 * (e & 3) + 8 * u), bad);
         }
         if (bad) dropped = 1;
       }
@@ -600,15 +885,11 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     }
   };
   load_turn(0);
+  const QuerySign sign(p.scale);
   const uint16_t* qr = p.q + (((int64_t)b * p.P + min(tw + r32, p.P - 1)) * p.Hq + qh) * kHD + hl * 8;
   u32x4 qb[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) qb[k] = ld16(qr + 16 * k);
-  if (!(p.scale > 0.f)) {  // as in the verify kernel
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      qb[k] = p.scale < 0.f ? qb[k] ^ 0x80008000u : p.scale == 0.f ? u32x4{0u, 0u, 0u, 0u} : qb[k];
-  }
+  for (int k = 0; k < 8; ++k) qb[k] = sign(ld16(qr + 16 * k));
   __syncthreads();  // dropped is 0
   store_turn(lds, 0);
   if (turns > 1) load_turn(1);
@@ -616,7 +897,7 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
   f32x16 o[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) o[dt] = f32x16{};
-  const float sl0 = (p.scale == 0.f ? 1.f : fabsf(p.scale)) * kLog2e;
+  const float sl0 = positive_scale(p.scale);
   const int last = min(base + tw + r32, Lw - 1);  // the last key this lane's row sees
   __syncthreads();
   for (int j = 0; j < turns; ++j) {
@@ -705,16 +986,6 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     }
     __syncthreads();
   }
-  if (dropped && hf == 0) {  // the tail's dropped values, for the rows that see them
-    for (int pos = kBlk * done; pos < seen; ++pos)
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t x = c.tail_values(bh)[(32 * dt + 8 * (i >> 2) + 4 * hl + (i & 3)) * kSlots + (pos & (kSlots - 1))];
-          if ((x & 0x7f80u) == 0x7f80u && pos <= last) o[dt][i] += bf16_bits_to_f32(x);
-        }
-  }
   // The second key half's sums go to the first through LDS, which leaves the
   // normalized rows there; every wave then gates and stores whole rows.
   float* red = reinterpret_cast<float*>(lds) + pair * kPMerge + lane;
@@ -764,8 +1035,13 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
   for (int i = 0; i < OUT; ++i) {
     const int e = tid + NT * i, t = row_of(e);
     if (t >= p.P) continue;
-    const float* row = rows + (e >> 4) * kPPitch + (e & 15) * 8;
+    float* row = rows + (e >> 4) * kPPitch + (e & 15) * 8;
     float g[8], v[8];
+    if (dropped) {
+#pragma unroll 1
+      for (int u = 0; u < 8; ++u)
+        row[u] += dropped_values(c, bh, (e & 15) * 8 + u, kBlk * done, min(base + t, seen - 1));
+    }
     unpack8(gt[i], g);
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = row[u] * (1.f / (1.f + __expf(-g[u])));
@@ -802,8 +1078,8 @@ extern "C" size_t dflash_attn_verify_q8_workspace_bytes(int B, int T, int Hq, in
   if (B <= 0 || T <= 0 || T > kMaxDraft || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || (int64_t)T * (Hq / Hkv) > 64 ||
       Smax <= 0 || Smax % kBlk != 0)
     return 0;
-  const int rt = (int)ceil_div((int64_t)T * (Hq / Hkv), 16);
-  return (size_t)2 * verify_runs(B, Hkv, Smax, rt) * 16 * rt * (kHD + 2) * sizeof(float);
+  const VerifyShape v = verify_shape(B, T * (Hq / Hkv), Hkv, Smax);
+  return (size_t)2 * v.runs * v.part_rows * (kHD + 2) * sizeof(float);
 }
 
 extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* q, const int32_t* lens,
@@ -814,7 +1090,7 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   const int B = p.c.B, Hkv = p.c.Hkv;
   if (T < 0 || T > kMaxDraft || Hq <= 0 || Hq % Hkv != 0 || (int64_t)T * (Hq / Hkv) > 64) return DFLASH_ERR_SHAPE;
   if (gate_row_stride < (int64_t)2 * Hq * kHD) return DFLASH_ERR_SHAPE;
-  if ((int64_t)B * T > INT32_MAX || Hq > 65535 || (int64_t)B * Hkv * p.c.nblk > INT32_MAX / 2) return DFLASH_ERR_SHAPE;
+  if ((int64_t)B * T > INT32_MAX || B > 65535 || Hq > 65535 || (int64_t)B * Hkv * p.c.nblk > INT32_MAX / 2) return DFLASH_ERR_SHAPE;
   if (B == 0 || T == 0) return DFLASH_OK;
   if (q == nullptr || lens == nullptr || gate_src == nullptr || out == nullptr || workspace == nullptr)
     return DFLASH_ERR_NULL;
@@ -829,17 +1105,23 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   p.out = static_cast<uint16_t*>(out);
   p.T = T; p.Hq = Hq; p.rep = Hq / Hkv;
   p.scale = scale;
-  const int rt = (int)ceil_div((int64_t)T * p.rep, 16);
-  p.rows = 16 * rt;
-  p.runs = verify_runs(B, Hkv, p.c.Smax, rt);
+  p.rep_inv = 65536u / p.rep + 1;
+  const VerifyShape v = verify_shape(B, T * p.rep, Hkv, p.c.Smax);
+  p.part_rows = v.part_rows;
+  p.min_run = v.min_run;
+  p.runs = v.runs;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + (int64_t)2 * p.runs * p.rows * kHD;
+  p.part_ml = p.part_o + (int64_t)2 * p.runs * p.part_rows * kHD;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (cache->type == DFLASH_KV_INT8) launch_verify<DFLASH_KV_INT8>(p, rt, s);
-  else launch_verify<DFLASH_KV_E4M3>(p, rt, s);
+  if (cache->type == DFLASH_KV_INT8) launch_verify<DFLASH_KV_INT8>(p, s);
+  else launch_verify<DFLASH_KV_E4M3>(p, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL(attn_verify_q8_merge_kernel, dim3((unsigned)(B * T), (unsigned)Hq), dim3(256), 0, s, p);
+  if (p.part_rows == 16)
+    hipLaunchKernelGGL(attn_verify_q8_merge16_kernel, dim3((unsigned)(B * T), (unsigned)Hq), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL(attn_verify_q8_merge64_kernel, dim3((unsigned)(Hkv * p.part_rows / 2), (unsigned)B), dim3(256),
+                       0, s, p);
   return to_status(hipGetLastError());
 }
 

@@ -95,14 +95,29 @@ __device__ __forceinline__ f32x4 codes_f32(uint32_t c) {
   return f32x4{a.x, a.y, b.x, b.y};
 }
 
+// Byte N of c, signed, as fp32, in one instruction.  (Written out: from plain C the
+// compiler takes a loaded word apart byte by byte where it is loaded and carries 16
+// registers where 4 do, and converts in two.)
+template <int N>
+__device__ __forceinline__ uint32_t signed_byte_f32(uint32_t c) {
+  uint32_t f;
+  if (N == 0)
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(c));
+  if (N == 1)
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(c));
+  if (N == 2)
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(c));
+  if (N == 3)
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(c));
+  return f;
+}
+
 // Four codes as two packed bf16 pairs: exact, both types have at most 8 significant bits.
 template <int TYPE>
 __device__ __forceinline__ u32x2 codes_bf16(uint32_t c) {
-  if (TYPE == DFLASH_KV_INT8) {
-    const f32x4 f = codes_f32<TYPE>(c);  // integers: the low half of the fp32 bits is zero
-    return u32x2{__builtin_amdgcn_perm(__float_as_uint(f.y), __float_as_uint(f.x), 0x07060302u),
-                 __builtin_amdgcn_perm(__float_as_uint(f.w), __float_as_uint(f.z), 0x07060302u)};
-  }
+  if (TYPE == DFLASH_KV_INT8)  // integers: the low half of the fp32 bits is zero
+    return u32x2{__builtin_amdgcn_perm(signed_byte_f32<1>(c), signed_byte_f32<0>(c), 0x07060302u),
+                 __builtin_amdgcn_perm(signed_byte_f32<3>(c), signed_byte_f32<2>(c), 0x07060302u)};
   return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true))};
 }
