@@ -43,12 +43,6 @@ struct VerifyParams {
   __device__ int token_of(int row) const { return (int)((uint32_t)row * rep_inv >> 16); }  // row / rep, row < 64
 };
 
-__device__ __forceinline__ int wave_sum_i32(int x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
-}
-
 // Positions that sequence b's rows attend to, and their blocks (0: takes no part).
 __device__ __forceinline__ int seen_positions(int L, int T, int Smax) {
   return L < 0 ? 0 : min(min(L, Smax) + T, Smax);
@@ -57,44 +51,70 @@ __device__ __forceinline__ int seen_blocks(int L, int T, int Smax) {
   return (seen_positions(L, T, Smax) + kBlk - 1) >> 6;
 }
 
-// Blocks of one head of all sequences; *before: of the sequences before b.
-__device__ __forceinline__ int all_blocks(const VerifyParams& p, int b, int* before) {
-  const int lane = threadIdx.x & 63;
-  int n = 0, pre = 0;
-  for (int b0 = 0; b0 < p.c.B; b0 += 64) {
-    const int i = b0 + lane;
-    const int v = i < p.c.B ? seen_blocks(p.lens[i], p.T, p.c.Smax) : 0;
-    n += v;
-    pre += i < b ? v : 0;
-  }
-  if (before != nullptr) *before = __builtin_amdgcn_readfirstlane(wave_sum_i32(pre));
-  return __builtin_amdgcn_readfirstlane(wave_sum_i32(n));
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1, 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2, 3
+  return x;
 }
 
-// The sequence that unit u falls in, and the units before it.
-__device__ __forceinline__ int sequence_of(const VerifyParams& p, int u, int* before) {
-  const int lane = threadIdx.x & 63;
-  int carry = 0;
-  for (int b0 = 0; b0 < p.c.B; b0 += 64) {
-    const int i = b0 + lane;
-    const int v = i < p.c.B ? p.c.Hkv * seen_blocks(p.lens[i], p.T, p.c.Smax) : 0;
-    int incl = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int x = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += x;
+// The batch's lengths and blocks: lane i of chunk c has sequence 64 c + i.  Up to 64
+// sequences are loaded once and stay in the lanes.
+struct Batch {
+  const VerifyParams& p;
+  int len, incl;  // of the first chunk
+  int total;      // blocks of one head over all sequences
+
+  __device__ __forceinline__ explicit Batch(const VerifyParams& params) : p(params) {
+    int carry = 0;
+    for (int c = chunks() - 1; c >= 0; --c) {
+      load(c);
+      carry += __builtin_amdgcn_readlane(incl, 63);
     }
-    const uint64_t past = __ballot(carry + incl > u);
-    if (past != 0) {
-      const int l = __builtin_ctzll(past);
-      *before = carry + __shfl(incl - v, l, 64);
-      return b0 + l;
-    }
-    carry += __shfl(incl, 63, 64);
+    total = carry;
   }
-  *before = carry;
-  return p.c.B;
-}
+  __device__ __forceinline__ int chunks() const { return (p.c.B + 63) >> 6; }
+  __device__ __forceinline__ void load(int c) {
+    const int i = 64 * c + (int)(threadIdx.x & 63);
+    len = i < p.c.B ? p.lens[i] : -1;
+    incl = wave_scan(seen_blocks(len, p.T, p.c.Smax));
+  }
+  __device__ __forceinline__ int length(int b) const {
+    return p.c.B <= 64 ? __builtin_amdgcn_readlane(len, b) : __builtin_amdgcn_readfirstlane(p.lens[b]);
+  }
+  // Blocks of one head of the sequences before b.
+  __device__ __forceinline__ int before(int b) {
+    int carry = 0;
+    if (p.c.B > 64)
+      for (int c = 0; c < b >> 6; ++c) {
+        load(c);
+        carry += __builtin_amdgcn_readlane(incl, 63);
+      }
+    if (p.c.B > 64) load(b >> 6);
+    const int i = b & 63;
+    return carry + (i == 0 ? 0 : __builtin_amdgcn_readlane(incl, i - 1));
+  }
+  // The sequence that unit u (a block of some head) falls in; *rest: u's place in it.
+  __device__ __forceinline__ int sequence_of(int u, int* rest) {
+    int carry = 0;
+    for (int c = 0; c < chunks(); ++c) {
+      if (p.c.B > 64) load(c);
+      const uint64_t past = __ballot(p.c.Hkv * (carry + incl) > u);
+      if (past != 0) {
+        const int i = __builtin_ctzll(past);
+        *rest = u - p.c.Hkv * (carry + (i == 0 ? 0 : __builtin_amdgcn_readlane(incl, i - 1)));
+        return 64 * c + i;
+      }
+      carry += __builtin_amdgcn_readlane(incl, 63);
+    }
+    *rest = 0;
+    return p.c.B;  // (u past the last unit: no caller asks)
+  }
+};
 
 __device__ __forceinline__ int run_length(const VerifyParams& p, int units) {
   return max(p.min_run, (units + p.runs - 1) / p.runs);
@@ -155,17 +175,16 @@ __device__ __forceinline__ float dropped_values(const Kv8& c, int64_t bh, int d,
   return sum;
 }
 
-// Where a run starts: the sequence, head and block of unit run0.
+// Where a run starts: the sequence, head and block of a unit.
 struct Place {
   int b, h, blk;
 };
-__device__ __forceinline__ Place place_of(const VerifyParams& p, int unit) {
-  int before;
-  const int b = __builtin_amdgcn_readfirstlane(sequence_of(p, unit, &before));
-  const int rem = __builtin_amdgcn_readfirstlane(unit - before);
-  const int nb = max(seen_blocks(__builtin_amdgcn_readfirstlane(p.lens[b]), p.T, p.c.Smax), 1);
-  const int h = rem / nb;
-  return Place{b, h, rem - h * nb};
+__device__ __forceinline__ Place place_of(const VerifyParams& p, Batch& batch, int unit) {
+  int rest;
+  const int b = batch.sequence_of(unit, &rest);
+  const int nb = seen_blocks(batch.length(b), p.T, p.c.Smax);
+  const int h = rest / nb;
+  return Place{b, h, rest - h * nb};
 }
 
 // Scores are scaled by a positive factor: the scale's sign goes to q, a zero to q itself.
@@ -202,16 +221,18 @@ __device__ __forceinline__ float weights(const float (&s)[N], float mx, float sl
 }
 
 // ------------------------------------------------- up to 16 rows (single tokens)
-// Four waves, block by block in turn, straight from memory to registers: nothing is
+// Eight waves, block by block in turn, straight from memory to registers: nothing is
 // shared.  v_mfma_f32_16x16x32_bf16; lane (r, g) = (lane % 16, lane / 16) has row r.
 // Operand row i of K's tile n is position 16 (i / 4) + 8 (n / 2) + 4 (n % 2) + i % 4,
 // so that result rows 4 g + e of tiles 2 s and 2 s + 1 are positions 16 g + 8 s .. + 7,
 // the ones whose values lie side by side in a row of V^T.  The next block's keys
 // are loaded once these are consumed, its values likewise.
+constexpr int kWaves16 = 8;
+
 template <int TYPE>
-__global__ __launch_bounds__(256, 2) void attn_verify_q8_rows16_kernel(const VerifyParams p) {
-  __shared__ __attribute__((aligned(16))) float so[4][16][kHD + 4];
-  __shared__ float sml[4][16][2];
+__global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel(const VerifyParams p) {
+  __shared__ __attribute__((aligned(16))) float so[kWaves16][16][kHD + 4];
+  __shared__ float sml[kWaves16][16][2];
   __shared__ int dropped;  // the tail's values hold a NaN or an infinity
   const Kv8& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -219,12 +240,13 @@ __global__ __launch_bounds__(256, 2) void attn_verify_q8_rows16_kernel(const Ver
   const int r = lane & 15, g = lane >> 4;
   if (tid == 0) dropped = 0;
   __syncthreads();
-  const int units = c.Hkv * all_blocks(p, 0, nullptr);
+  Batch batch(p);
+  const int units = c.Hkv * batch.total;
   const int per = run_length(p, units);
   const int run0 = blockIdx.x * per;
   int left = min(per, units - run0);
   if (left <= 0) return;
-  Place at = place_of(p, run0);
+  Place at = place_of(p, batch, run0);
   const float sl0 = positive_scale(p.scale);
   const QuerySign sign(p.scale);
   const int nrows = p.T * p.rep;
@@ -232,7 +254,7 @@ __global__ __launch_bounds__(256, 2) void attn_verify_q8_rows16_kernel(const Ver
   const int key0 = 16 * (r >> 2) + (r & 3);  // operand row r of tile n: + 8 (n / 2) + 4 (n % 2)
   bool first_part = true;
   while (left > 0) {
-    const int L = __builtin_amdgcn_readfirstlane(p.lens[at.b]);
+    const int L = batch.length(at.b);
     const int seen = seen_positions(L, p.T, c.Smax);
     const int nb = (seen + kBlk - 1) >> 6;
     if (nb == 0) {
@@ -290,8 +312,8 @@ __global__ __launch_bounds__(256, 2) void attn_verify_q8_rows16_kernel(const Ver
       pb[0] = cvt8_bf16(w);
       pb[1] = cvt8_bf16(w + 8);
     };
-    for (; j < coded; j += 4) {  // every row sees the whole block
-      const int next = min(j + 4, coded - 1);  // (past the last: loaded again, not used)
+    for (; j < coded; j += kWaves16) {  // every row sees the whole block
+      const int next = min(j + kWaves16, coded - 1);  // (past the last: loaded again, not used)
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -318,7 +340,7 @@ __global__ __launch_bounds__(256, 2) void attn_verify_q8_rows16_kernel(const Ver
         }
       load_values(next);
     }
-    for (; j < b1; j += 4) {  // the tail, in bf16
+    for (; j < b1; j += kWaves16) {  // the tail, in bf16
       const int slot = (j & 1) * kBlk, p0 = kBlk * j;
       const uint16_t* tk = c.tail_keys(bh) + (slot + key0) * kHD + 16 * g;
       const uint16_t* tv = c.tail_values(bh) + r * kSlots + slot + 16 * g;
@@ -344,7 +366,7 @@ __global__ __launch_bounds__(256, 2) void attn_verify_q8_rows16_kernel(const Ver
                             o[dt]);
       if (bad) dropped = 1;
     }
-    // the four waves' states through LDS
+    // the waves' states through LDS
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     if (g == 0) {
@@ -356,14 +378,14 @@ __global__ __launch_bounds__(256, 2) void attn_verify_q8_rows16_kernel(const Ver
     __syncthreads();
     const bool whole = at.blk == 0 && b1 == nb;
     const int64_t part = 2 * (int64_t)blockIdx.x + (first_part ? 0 : 1);
-    for (int i = tid; i < nrows * 32; i += 256) {
+    for (int i = tid; i < nrows * 32; i += 64 * kWaves16) {
       const int row = i >> 5, d = (i & 31) * 4;
       float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) mm = fmaxf(mm, sml[x][row][0]);
+      for (int x = 0; x < kWaves16; ++x) mm = fmaxf(mm, sml[x][row][0]);
       f32x4 oo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
+      for (int x = 0; x < kWaves16; ++x) {
         const float mw = sml[x][row][0];
         const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
         ll = fmaf(sml[x][row][1], f, ll);
@@ -419,12 +441,13 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
   const int hf = wave / RT, rt = wave % RT;
   if (tid == 0) dropped = 0;
   __syncthreads();
-  const int units = c.Hkv * all_blocks(p, 0, nullptr);
+  Batch batch(p);
+  const int units = c.Hkv * batch.total;
   const int per = run_length(p, units);
   const int run0 = blockIdx.x * per;
   int left = min(per, units - run0);
   if (left <= 0) return;
-  Place at = place_of(p, run0);
+  Place at = place_of(p, batch, run0);
   const float sl0 = positive_scale(p.scale);
   const QuerySign sign(p.scale);
   const int nrows = p.T * p.rep;
@@ -432,7 +455,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
   const int t = min(p.token_of(row), p.T - 1), rr = row - p.token_of(row) * p.rep;
   bool first_part = true;
   while (left > 0) {
-    const int L = __builtin_amdgcn_readfirstlane(p.lens[at.b]);
+    const int L = batch.length(at.b);
     const int seen = seen_positions(L, p.T, c.Smax);
     const int nb = (seen + kBlk - 1) >> 6;
     if (nb == 0) {
@@ -616,16 +639,14 @@ struct Parts {
   int w0, w1, head;
   __device__ int at(int w) const { return w == w0 ? head : 2 * w; }
 };
-__device__ __forceinline__ Parts parts_of(const VerifyParams& p, int b, int h, int nb) {
-  int before;
-  const int per = run_length(p, p.c.Hkv * all_blocks(p, b, &before));
-  const int u0 = p.c.Hkv * before + h * nb;
+__device__ __forceinline__ Parts parts_of(const VerifyParams& p, Batch& batch, int b, int h, int nb) {
+  const int per = run_length(p, p.c.Hkv * batch.total);
+  const int u0 = p.c.Hkv * batch.before(b) + h * nb;
   const int w0 = u0 / per;
   return Parts{w0, (u0 + nb - 1) / per, 2 * w0 + (u0 > w0 * per ? 1 : 0)};
 }
 
-// Running merge of parts that one lane walks, in turn with three other waves: V is
-// the vector of outputs that the lane holds.
+// Running merge of the parts that one lane walks; V is the vector of outputs that it holds.
 template <class V>
 struct Merged {
   float m = -INFINITY, l = 0.f;
@@ -640,34 +661,40 @@ struct Merged {
   }
 };
 
-// Up to 16 rows: a workgroup per (token, query head); lane l has features 2 l, 2 l + 1,
-// the waves take the parts in turn.
-__global__ __launch_bounds__(256) void attn_verify_q8_merge16_kernel(const VerifyParams p) {
-  __shared__ float sm[4], sl[4];
-  __shared__ f32x2 so[4][64];
+// Up to 16 rows: a workgroup per (token, query head); lane l has features 2 l, 2 l + 1.
+// The waves take the parts in turn, kMergeAhead loads in flight: up to 128 parts (one
+// sequence, two key/value heads on 256 runs) cost one trip to memory.
+constexpr int kMergeWaves = 16, kMergeAhead = 8;
+
+__global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge16_kernel(const VerifyParams p) {
+  __shared__ float sm[kMergeWaves], sl[kMergeWaves];
+  __shared__ f32x2 so[kMergeWaves][64];
   const int bt = blockIdx.x, qh = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = bt / p.T, t = bt - b * p.T, h = qh / p.rep, row = t * p.rep + qh - h * p.rep;
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + ((int64_t)bt * p.Hq + qh) * kHD + 2 * lane);
-  const int nb = seen_blocks(p.lens[b], p.T, p.c.Smax);
+  Batch batch(p);
+  const int nb = seen_blocks(__builtin_amdgcn_readfirstlane(p.lens[b]), p.T, p.c.Smax);
   if (nb == 0) {  // takes no part
     if (wave == 0) *dst = 0u;
     return;
   }
-  const Parts parts = parts_of(p, b, h, nb);
+  const Parts parts = parts_of(p, batch, b, h, nb);
   if (parts.w0 == parts.w1) return;  // finished by its one run
+  const uint32_t gv =
+      *reinterpret_cast<const uint32_t*>(p.gate + (int64_t)bt * p.gate_stride + qh * 2 * kHD + kHD + 2 * lane);
   Merged<f32x2> a;
-  for (int w = parts.w0 + wave; w <= parts.w1; w += 16) {
-    f32x2 ml[4], os[4];
+  for (int w = parts.w0 + wave; w <= parts.w1; w += kMergeWaves * kMergeAhead) {
+    f32x2 ml[kMergeAhead], os[kMergeAhead];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t i = (int64_t)parts.at(min(w + 4 * u, parts.w1)) * p.part_rows + row;
+    for (int u = 0; u < kMergeAhead; ++u) {
+      const int64_t i = (int64_t)parts.at(min(w + kMergeWaves * u, parts.w1)) * p.part_rows + row;
       ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * i);
       os[u] = *reinterpret_cast<const f32x2*>(p.part_o + i * kHD + 2 * lane);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (w + 4 * u <= parts.w1) a.add(ml[u].x, ml[u].y, os[u]);
+    for (int u = 0; u < kMergeAhead; ++u)
+      if (w + kMergeWaves * u <= parts.w1) a.add(ml[u].x, ml[u].y, os[u]);
   }
   if (lane == 0) {
     sm[wave] = a.m;
@@ -676,55 +703,56 @@ __global__ __launch_bounds__(256) void attn_verify_q8_merge16_kernel(const Verif
   so[wave][lane] = a.o;
   __syncthreads();
   if (wave != 0) return;
-#pragma unroll
-  for (int k = 1; k < 4; ++k) a.add(sm[k], sl[k], so[k][lane]);
+  const int n = min(kMergeWaves, parts.w1 - parts.w0 + 1);
+  for (int k = 1; k < n; ++k) a.add(sm[k], sl[k], so[k][lane]);
   const float inv = 1.f / a.l;
-  const uint32_t gv =
-      *reinterpret_cast<const uint32_t*>(p.gate + (int64_t)bt * p.gate_stride + qh * 2 * kHD + kHD + 2 * lane);
   const float g0 = 1.f / (1.f + __expf(-bf16_lo(gv))), g1 = 1.f / (1.f + __expf(-bf16_hi(gv)));
   *dst = pack2(a.o.x * inv * g0, a.o.y * inv * g1);
 }
 
 // Up to 64 rows: a workgroup per (sequence, key/value head, tile, sixteenth q of its
 // outputs), a part's outputs as the lanes stored them; the waves take the parts in turn.
-__global__ __launch_bounds__(256) void attn_verify_q8_merge64_kernel(const VerifyParams p) {
-  __shared__ float sm[4][64], sl[4][64];
-  __shared__ f32x4 so[4][64];
+__global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kernel(const VerifyParams p) {
+  __shared__ float sm[kMergeWaves][32], sl[kMergeWaves][32];
+  __shared__ f32x4 so[kMergeWaves][64];
   const int tiles = p.part_rows >> 5;
   const int q = blockIdx.x & 15, rt = (blockIdx.x >> 4) % tiles, h = (blockIdx.x >> 4) / tiles, b = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r32 = lane & 31, hl = lane >> 5, row = 32 * rt + r32;
   const int t = p.token_of(row), qh = h * p.rep + row - t * p.rep, d = 32 * (q >> 2) + 8 * (q & 3) + 4 * hl;
   const bool live = row < p.T * p.rep;
-  const int nb = seen_blocks(p.lens[b], p.T, p.c.Smax);
+  Batch batch(p);
+  const int nb = seen_blocks(__builtin_amdgcn_readfirstlane(p.lens[b]), p.T, p.c.Smax);
   if (nb == 0) {  // takes no part
     if (wave == 0 && live)
       *reinterpret_cast<u32x2*>(p.out + (((int64_t)b * p.T + t) * p.Hq + qh) * kHD + d) = u32x2{0u, 0u};
     return;
   }
-  const Parts parts = parts_of(p, b, h, nb);
+  const Parts parts = parts_of(p, batch, b, h, nb);
   if (parts.w0 == parts.w1) return;  // finished by its one run
   Merged<f32x4> a;
-  for (int w = parts.w0 + wave; w <= parts.w1; w += 16) {
-    f32x2 ml[4];
-    f32x4 os[4];
+  for (int w = parts.w0 + wave; w <= parts.w1; w += kMergeWaves * kMergeAhead) {
+    f32x2 ml[kMergeAhead];
+    f32x4 os[kMergeAhead];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t i = (int64_t)parts.at(min(w + 4 * u, parts.w1)) * tiles + rt;
+    for (int u = 0; u < kMergeAhead; ++u) {
+      const int64_t i = (int64_t)parts.at(min(w + kMergeWaves * u, parts.w1)) * tiles + rt;
       ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + (i * 32 + r32) * 2);
       os[u] = *reinterpret_cast<const f32x4*>(p.part_o + i * (32 * kHD) + 256 * q + 4 * lane);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (w + 4 * u <= parts.w1) a.add(ml[u].x, ml[u].y, os[u]);
+    for (int u = 0; u < kMergeAhead; ++u)
+      if (w + kMergeWaves * u <= parts.w1) a.add(ml[u].x, ml[u].y, os[u]);
   }
-  sm[wave][lane] = a.m;
-  sl[wave][lane] = a.l;
+  if (hl == 0) {
+    sm[wave][r32] = a.m;
+    sl[wave][r32] = a.l;
+  }
   so[wave][lane] = a.o;
   __syncthreads();
   if (wave != 0) return;
-#pragma unroll
-  for (int k = 1; k < 4; ++k) a.add(sm[k][lane], sl[k][lane], so[k][lane]);
+  const int n = min(kMergeWaves, parts.w1 - parts.w0 + 1);
+  for (int k = 1; k < n; ++k) a.add(sm[k][r32], sl[k][r32], so[k][lane]);
   if (live) store_gated(p, (int64_t)b * p.T + t, qh, d, a.o * (1.f / a.l));
 }
 
@@ -738,8 +766,8 @@ VerifyShape verify_shape(int64_t B, int rows, int Hkv, int Smax) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
   VerifyShape v;
   v.part_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  v.min_run = rows <= 16 ? 4 : 2;
-  v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus, ceil_div(B * Hkv * (Smax / kBlk), v.min_run)));
+  v.min_run = rows <= 16 ? kWaves16 : 2;
+  v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(rows <= 16 ? cus : 2 * cus, ceil_div(B * Hkv * (Smax / kBlk), v.min_run)));
   return v;
 }
 
@@ -747,7 +775,7 @@ template <int TYPE>
 void launch_verify(const VerifyParams& p, hipStream_t s) {
   const dim3 grid((unsigned)p.runs);
   if (p.part_rows == 16)
-    hipLaunchKernelGGL((attn_verify_q8_rows16_kernel<TYPE>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((attn_verify_q8_rows16_kernel<TYPE>), grid, dim3(64 * kWaves16), 0, s, p);
   else if (p.part_rows == 32)
     hipLaunchKernelGGL((attn_verify_q8_rows64_kernel<TYPE, 1>), grid, dim3(128), 0, s, p);
   else
@@ -1118,10 +1146,11 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (p.part_rows == 16)
-    hipLaunchKernelGGL(attn_verify_q8_merge16_kernel, dim3((unsigned)(B * T), (unsigned)Hq), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(attn_verify_q8_merge16_kernel, dim3((unsigned)(B * T), (unsigned)Hq),
+                       dim3(64 * kMergeWaves), 0, s, p);
   else
-    hipLaunchKernelGGL(attn_verify_q8_merge64_kernel, dim3((unsigned)(Hkv * p.part_rows / 2), (unsigned)B), dim3(256),
-                       0, s, p);
+    hipLaunchKernelGGL(attn_verify_q8_merge64_kernel, dim3((unsigned)(Hkv * p.part_rows / 2), (unsigned)B),
+                       dim3(64 * kMergeWaves), 0, s, p);
   return to_status(hipGetLastError());
 }
 
