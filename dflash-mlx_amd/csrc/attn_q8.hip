@@ -16,10 +16,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // ------------------------------------------------------------------ verify
 // The T * Hq / Hkv query rows of a (sequence, key/value head), row t * rep + r being
 // query head r of the group at token t, against the positions that they see.  Work is
-// counted in blocks of 64 positions over all heads and sequences; every workgroup
-// takes an equal run of them, whatever the sequences' lengths (found from lens in
-// the kernel).  The runs' ends cut heads into parts: those go to the workspace and a
-// second launch merges them; a head that one workgroup has to itself is finished there.
+// counted in blocks of 64 positions over all heads and sequences and shared by the
+// launch's workgroups whatever the sequences' lengths (Batch).  That cuts heads into
+// parts, which go to the workspace for a second launch to merge; a head that one
+// workgroup has to itself is finished there.
 //   - Products on MFMA in transposed form, S^T = K Q^T and O^T = V^T P^T: a lane
 //     holds one row's scores and outputs, and P stays in its registers.
 //   - A block's key scale is one factor of its scores; its value scale goes into
@@ -35,7 +35,7 @@ struct VerifyParams {
   uint16_t* out;    // [B, T, Hq * D]
   float* part_o;    // [2 * runs][part_rows][D], in the order that the kernel's lanes hold them
   float* part_ml;   // [2 * runs][part_rows][2]
-  int T, Hq, rep, runs, min_run;
+  int T, Hq, rep, runs, min_cut;
   int part_rows;  // rows of a part in the workspace
   uint32_t rep_inv;
   float scale;
@@ -62,47 +62,69 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// The batch's lengths and blocks: lane i of chunk c has sequence 64 c + i.  Up to 64
-// sequences are loaded once and stay in the lanes.
+// How the launch's workgroups share the blocks, from the lengths: `cut` blocks are a
+// workgroup's even share, at least min_cut.  Where every head cut into pieces of at most
+// that gives no more pieces than workgroups, a workgroup takes one piece of one head
+// (`pieces`); otherwise all blocks, in order of sequence and head, are cut into runs of
+// the even share, which cross from head to head.  Units: pieces, or blocks.  Lane i of chunk c has sequence 64 c + i; up to
+// 64 sequences are loaded once and stay in the lanes.
 struct Batch {
   const VerifyParams& p;
-  int len, incl;  // of the first chunk
-  int total;      // blocks of one head over all sequences
+  int len, incl;  // of the first chunk: lengths, and units of one head up to and with the lane's
+  bool pieces;
+  int cut;
+  int per;        // units of a workgroup
+  int units;      // of the launch
 
   __device__ __forceinline__ explicit Batch(const VerifyParams& params) : p(params) {
-    int carry = 0;
+    int nblk = 0, n = 0;
     for (int c = chunks() - 1; c >= 0; --c) {
       load(c);
-      carry += __builtin_amdgcn_readlane(incl, 63);
+      nblk += __builtin_amdgcn_readlane(wave_scan(seen_blocks(len, p.T, p.c.Smax)), 63);
     }
-    total = carry;
+    nblk *= p.c.Hkv;
+    cut = max(p.min_cut, (nblk + p.runs - 1) / p.runs);
+    pieces = true;
+    for (int c = chunks() - 1; c >= 0; --c) {
+      if (p.c.B > 64) load(c);
+      scan();
+      n += __builtin_amdgcn_readlane(incl, 63);
+    }
+    pieces = n * p.c.Hkv <= p.runs;
+    units = pieces ? n * p.c.Hkv : nblk;
+    per = pieces ? 1 : cut;
+    if (!pieces) scan();
   }
   __device__ __forceinline__ int chunks() const { return (p.c.B + 63) >> 6; }
   __device__ __forceinline__ void load(int c) {
     const int i = 64 * c + (int)(threadIdx.x & 63);
     len = i < p.c.B ? p.lens[i] : -1;
-    incl = wave_scan(seen_blocks(len, p.T, p.c.Smax));
   }
+  __device__ __forceinline__ void scan() { incl = wave_scan(units_of(seen_blocks(len, p.T, p.c.Smax))); }
+  __device__ __forceinline__ int units_of(int nb) const { return pieces ? (nb + cut - 1) / cut : nb; }
   __device__ __forceinline__ int length(int b) const {
     return p.c.B <= 64 ? __builtin_amdgcn_readlane(len, b) : __builtin_amdgcn_readfirstlane(p.lens[b]);
   }
-  // Blocks of one head of the sequences before b.
+  // Units of one head of the sequences before b.
   __device__ __forceinline__ int before(int b) {
     int carry = 0;
     if (p.c.B > 64)
-      for (int c = 0; c < b >> 6; ++c) {
+      for (int c = 0; c <= b >> 6; ++c) {
         load(c);
-        carry += __builtin_amdgcn_readlane(incl, 63);
+        scan();
+        if (c < b >> 6) carry += __builtin_amdgcn_readlane(incl, 63);
       }
-    if (p.c.B > 64) load(b >> 6);
     const int i = b & 63;
     return carry + (i == 0 ? 0 : __builtin_amdgcn_readlane(incl, i - 1));
   }
-  // The sequence that unit u (a block of some head) falls in; *rest: u's place in it.
+  // The sequence that unit u falls in; *rest: u's place in it.
   __device__ __forceinline__ int sequence_of(int u, int* rest) {
     int carry = 0;
     for (int c = 0; c < chunks(); ++c) {
-      if (p.c.B > 64) load(c);
+      if (p.c.B > 64) {
+        load(c);
+        scan();
+      }
       const uint64_t past = __ballot(p.c.Hkv * (carry + incl) > u);
       if (past != 0) {
         const int i = __builtin_ctzll(past);
@@ -116,8 +138,25 @@ struct Batch {
   }
 };
 
-__device__ __forceinline__ int run_length(const VerifyParams& p, int units) {
-  return max(p.min_run, (units + p.runs - 1) / p.runs);
+// A workgroup's share: from block blk of (b, h) on, `left` blocks.
+struct Share {
+  int b, h, blk, left;
+};
+__device__ __forceinline__ Share share_of(const VerifyParams& p, Batch& batch, int wg) {
+  const int u = wg * batch.per;
+  Share s{0, 0, 0, min(batch.per, batch.units - u)};
+  if (s.left <= 0) return s;
+  int rest;
+  s.b = batch.sequence_of(u, &rest);
+  const int nb = seen_blocks(batch.length(s.b), p.T, p.c.Smax), n = batch.units_of(nb);
+  s.h = rest / n;
+  s.blk = rest - s.h * n;
+  if (batch.pieces) {
+    const int size = (nb + n - 1) / n;
+    s.blk *= size;
+    s.left = min(size, nb - s.blk);  // (0 where even pieces leave the last one nothing)
+  }
+  return s;
 }
 
 __device__ __forceinline__ float max_over_groups(float x) {  // lanes r, r + 16, r + 32, r + 48
@@ -127,21 +166,21 @@ __device__ __forceinline__ float max_over_groups(float x) {  // lanes r, r + 16,
   return fmaxf(b.x, b.y);
 }
 
-// The halves of packed bf16 that are NaN or infinite, as their bits 15 and 31 (an
-// exponent of all ones carries into them).  Arithmetic, not compares: a mask a value
-// would take a pair of scalar registers each.
-__device__ __forceinline__ uint32_t nonfinite_bits(uint32_t w) {
-  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+// Values that are not finite are dropped before P V, where the weight 0 of a row that
+// does not see their token would not leave 0, and added to the rows that do see it
+// afterwards (dropped_values).  That takes care of the tail's slots past the held
+// positions too, which hold anything.  In packed bf16 an exponent of all ones carries
+// into bits 15 and 31.
+__device__ __forceinline__ uint32_t nonfinite_bits(uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
+__device__ __forceinline__ uint32_t nonfinite_bits(u32x4 w) {
+  return nonfinite_bits(w.x) | nonfinite_bits(w.y) | nonfinite_bits(w.z) | nonfinite_bits(w.w);
 }
-
-// Eight values' bf16 with those from n on, and those that are not finite, zero.
-__device__ __forceinline__ u32x4 clean_values(u32x4 w, int n, uint32_t& bad) {
+__device__ __forceinline__ bool any_nonfinite(uint32_t bits) { return (bits & 0x80008000u) != 0; }
+__device__ __forceinline__ u32x4 drop_nonfinite(u32x4 w) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t held = ((uint32_t)((2 * i - n) >> 31) & 0xffffu) | ((uint32_t)((2 * i + 1 - n) >> 31) & 0xffff0000u);
-    const uint32_t x = w[i] & held, y = nonfinite_bits(x);
-    bad |= y;
-    w[i] = x & ~((y >> 15) * 0xffffu);
+    const uint32_t y = nonfinite_bits(w[i]) & 0x80008000u;
+    w[i] &= ~(y | (y - (y >> 15)));
   }
   return w;
 }
@@ -160,10 +199,8 @@ __device__ __forceinline__ void store_gated(const VerifyParams& p, int64_t bt, i
   *reinterpret_cast<u32x2*>(p.out + (bt * p.Hq + qh) * kHD + d) = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
 }
 
-// The sum of feature d's values at tail positions from .. to that are not finite.  The
-// kernels drop those before P V, where the weight 0 of a row that does not see them
-// would not leave 0, and add them to the rows that do: a NaN or an infinity as in the
-// plain sum.
+// The sum of feature d's values at tail positions from .. to that are not finite: what a
+// row that sees them gets instead, a NaN or an infinity as in the plain sum.
 __device__ __forceinline__ float dropped_values(const Kv8& c, int64_t bh, int d, int from, int to) {
   const uint16_t* row = c.tail_values(bh) + d * kSlots;
   float sum = 0.f;
@@ -173,18 +210,6 @@ __device__ __forceinline__ float dropped_values(const Kv8& c, int64_t bh, int d,
     if ((x & 0x7f80u) == 0x7f80u) sum += bf16_bits_to_f32(x);
   }
   return sum;
-}
-
-// Where a run starts: the sequence, head and block of a unit.
-struct Place {
-  int b, h, blk;
-};
-__device__ __forceinline__ Place place_of(const VerifyParams& p, Batch& batch, int unit) {
-  int rest;
-  const int b = batch.sequence_of(unit, &rest);
-  const int nb = seen_blocks(batch.length(b), p.T, p.c.Smax);
-  const int h = rest / nb;
-  return Place{b, h, rest - h * nb};
 }
 
 // Scores are scaled by a positive factor: the scale's sign goes to q, a zero to q itself.
@@ -241,19 +266,14 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
   if (tid == 0) dropped = 0;
   __syncthreads();
   Batch batch(p);
-  const int units = c.Hkv * batch.total;
-  const int per = run_length(p, units);
-  const int run0 = blockIdx.x * per;
-  int left = min(per, units - run0);
-  if (left <= 0) return;
-  Place at = place_of(p, batch, run0);
+  Share at = share_of(p, batch, blockIdx.x);
   const float sl0 = positive_scale(p.scale);
   const QuerySign sign(p.scale);
   const int nrows = p.T * p.rep;
   const int t = min(p.token_of(r), p.T - 1), rr = r - p.token_of(r) * p.rep;
   const int key0 = 16 * (r >> 2) + (r & 3);  // operand row r of tile n: + 8 (n / 2) + 4 (n % 2)
   bool first_part = true;
-  while (left > 0) {
+  while (at.left > 0) {
     const int L = batch.length(at.b);
     const int seen = seen_positions(L, p.T, c.Smax);
     const int nb = (seen + kBlk - 1) >> 6;
@@ -261,37 +281,14 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
       ++at.b;
       continue;
     }
-    const int b1 = min(nb, at.blk + left);
+    const int b1 = min(nb, at.blk + at.left);
     const int base = min(L, c.Smax), done = base >> 6;
     const int64_t bh = (int64_t)at.b * c.Hkv + at.h;
     const int last = min(base + t, seen - 1);  // the last position the lane's row sees
     u32x4 qf[4];  // operand (k / 2, k % 2): features 64 (k / 2) + 16 g + 8 (k % 2) ..
     const uint16_t* qsrc = p.q + (((int64_t)at.b * p.T + t) * p.Hq + at.h * p.rep + rr) * kHD + 16 * g;
-    u32x4 kc[4][2], vc[8];
-    float ks = 0.f, vs = 0.f;
-    const uint8_t* kb = c.keys(bh, 0) + key0 * kHD + 16 * g;
-    const uint8_t* vb = c.values(bh, 0) + r * kBlk + 16 * g;
-    const float* ksp = c.ks + bh * c.nblk;
-    const float* vsp = c.vs + bh * c.nblk;
-    auto load_keys = [&](int j) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          kc[n][k] = ld16(kb + (int64_t)j * kBlkBytes + (8 * (n >> 1) + 4 * (n & 1)) * kHD + 64 * k);
-    };
-    auto load_values = [&](int j) {
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) vc[dt] = ld16(vb + (int64_t)j * kBlkBytes + 16 * dt * kBlk);
-    };
     const int coded = min(b1, done);
     int j = at.blk + wave;
-    if (j < coded) {
-      load_keys(j);
-      load_values(j);
-      ks = ksp[j];
-      vs = vsp[j];
-    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) qf[k] = sign(ld16(qsrc + 64 * (k >> 1) + 8 * (k & 1)));
     float m = -INFINITY, l = 0.f;
@@ -312,59 +309,99 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
       pb[0] = cvt8_bf16(w);
       pb[1] = cvt8_bf16(w + 8);
     };
-    for (; j < coded; j += kWaves16) {  // every row sees the whole block
-      const int next = min(j + kWaves16, coded - 1);  // (past the last: loaded again, not used)
+    if (j < coded) {  // codes: every row sees the whole block
+      u32x4 kc[4][2], vc[8];
+      float ks = 0.f, vs = 0.f;
+      const uint8_t* kb = c.keys(bh, 0) + key0 * kHD + 16 * g;
+      const uint8_t* vb = c.values(bh, 0) + r * kBlk + 16 * g;
+      const float* ksp = c.ks + bh * c.nblk;
+      const float* vsp = c.vs + bh * c.nblk;
+      auto load_keys = [&](int j) {
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const u32x2 lo = codes_bf16<TYPE>(kc[n][k >> 1][2 * (k & 1)]);
-          const u32x2 hi = codes_bf16<TYPE>(kc[n][k >> 1][2 * (k & 1) + 1]);
-          acc = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, qf[k], acc);
+          for (int k = 0; k < 2; ++k)
+            kc[n][k] = ld16(kb + (int64_t)j * kBlkBytes + (8 * (n >> 1) + 4 * (n & 1)) * kHD + 64 * k);
+      };
+      auto load_values = [&](int j) {
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) vc[dt] = ld16(vb + (int64_t)j * kBlkBytes + 16 * dt * kBlk);
+      };
+      load_keys(j);
+      load_values(j);
+      ks = ksp[j];
+      vs = vsp[j];
+      do {
+        const int next = min(j + kWaves16, coded - 1);  // (past the last: loaded again, not used)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const u32x2 lo = codes_bf16<TYPE>(kc[n][k >> 1][2 * (k & 1)]);
+            const u32x2 hi = codes_bf16<TYPE>(kc[n][k >> 1][2 * (k & 1) + 1]);
+            acc = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, qf[k], acc);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * n + e] = acc[e];
         }
+        const float sl = sl0 * ks, lv = __log2f(vs), iv = 1.f / vs;
+        load_keys(next);
+        ks = ksp[next];
+        vs = vsp[next];
+        softmax(sl, lv, iv);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[4 * n + e] = acc[e];
-      }
-      const float sl = sl0 * ks, lv = __log2f(vs), iv = 1.f / vs;
-      load_keys(next);
-      ks = ksp[next];
-      vs = vsp[next];
-      softmax(sl, lv, iv);
+        for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const u32x2 lo = codes_bf16<TYPE>(vc[dt][2 * k]), hi = codes_bf16<TYPE>(vc[dt][2 * k + 1]);
-          o[dt] = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[k], o[dt]);
-        }
-      load_values(next);
+          for (int k = 0; k < 2; ++k) {
+            const u32x2 lo = codes_bf16<TYPE>(vc[dt][2 * k]), hi = codes_bf16<TYPE>(vc[dt][2 * k + 1]);
+            o[dt] = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[k], o[dt]);
+          }
+        load_values(next);
+        j += kWaves16;
+      } while (j < coded);
     }
     for (; j < b1; j += kWaves16) {  // the tail, in bf16
       const int slot = (j & 1) * kBlk, p0 = kBlk * j;
       const uint16_t* tk = c.tail_keys(bh) + (slot + key0) * kHD + 16 * g;
       const uint16_t* tv = c.tail_values(bh) + r * kSlots + slot + 16 * g;
+      u32x4 kt[4][4], vt[8][2];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          kt[n][k] = ld16(tk + (8 * (n >> 1) + 4 * (n & 1)) * kHD + 64 * (k >> 1) + 8 * (k & 1));
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) vt[dt][0] = ld16(tv + 16 * dt * kSlots);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          acc = mfma_bf16(ld16(tk + (8 * (n >> 1) + 4 * (n & 1)) * kHD + 64 * (k >> 1) + 8 * (k & 1)), qf[k], acc);
+        for (int k = 0; k < 4; ++k) acc = mfma_bf16(kt[n][k], qf[k], acc);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           s[4 * n + e] = p0 + 16 * g + 8 * (n >> 1) + 4 * (n & 1) + e > last ? -INFINITY : acc[e];
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) vt[dt][1] = ld16(tv + 16 * dt * kSlots + 8);
       softmax(sl0, 0.f, 1.f);
-      // slots past the held positions hold anything; a row's weight for a token
-      // that it does not see is 0, which a NaN or an infinity would not leave 0
-      uint32_t bad = 0;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) bits |= nonfinite_bits(vt[dt][0]) | nonfinite_bits(vt[dt][1]);
+      if (__any(any_nonfinite(bits))) {
+        if (any_nonfinite(bits)) dropped = 1;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          vt[dt][0] = drop_nonfinite(vt[dt][0]);
+          vt[dt][1] = drop_nonfinite(vt[dt][1]);
+        }
+      }
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          o[dt] = mfma_bf16(clean_values(ld16(tv + 16 * dt * kSlots + 8 * k), seen - (p0 + 16 * g + 8 * k), bad), pb[k],
-                            o[dt]);
-      if (bad) dropped = 1;
+        for (int k = 0; k < 2; ++k) o[dt] = mfma_bf16(vt[dt][k], pb[k], o[dt]);
     }
     // the waves' states through LDS
     l += __shfl_xor(l, 16, 64);
@@ -412,7 +449,7 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
     __syncthreads();
     if (tid == 0) dropped = 0;
     first_part = false;
-    left -= b1 - at.blk;
+    at.left -= b1 - at.blk;
     at.blk = 0;
     if (b1 == nb && ++at.h == c.Hkv) {
       at.h = 0;
@@ -442,19 +479,14 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
   if (tid == 0) dropped = 0;
   __syncthreads();
   Batch batch(p);
-  const int units = c.Hkv * batch.total;
-  const int per = run_length(p, units);
-  const int run0 = blockIdx.x * per;
-  int left = min(per, units - run0);
-  if (left <= 0) return;
-  Place at = place_of(p, batch, run0);
+  Share at = share_of(p, batch, blockIdx.x);
   const float sl0 = positive_scale(p.scale);
   const QuerySign sign(p.scale);
   const int nrows = p.T * p.rep;
   const int row = 32 * rt + r32;
   const int t = min(p.token_of(row), p.T - 1), rr = row - p.token_of(row) * p.rep;
   bool first_part = true;
-  while (left > 0) {
+  while (at.left > 0) {
     const int L = batch.length(at.b);
     const int seen = seen_positions(L, p.T, c.Smax);
     const int nb = (seen + kBlk - 1) >> 6;
@@ -462,7 +494,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
       ++at.b;
       continue;
     }
-    const int b1 = min(nb, at.blk + left);
+    const int b1 = min(nb, at.blk + at.left);
     const int base = min(L, c.Smax), done = base >> 6;
     const int64_t bh = (int64_t)at.b * c.Hkv + at.h;
     const int last = min(base + t, seen - 1);
@@ -471,7 +503,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
     // vrow + NT / 4 i, keys 16 (tid % 4) ..  (both steps multiples of 8: one swizzle).
     const int kkey = tid >> 3, vrow = tid >> 2;
     auto load_block = [&](int j) {
-      if (j >= done) return;
+      if (j >= min(done, b1)) return;
       const uint8_t* ksrc = c.keys(bh, j) + 16 * tid;
       const uint8_t* vsrc = c.values(bh, j) + 16 * tid;
 #pragma unroll
@@ -507,17 +539,23 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
         const int slot = (j & 1) * kBlk;
         const uint16_t* ksrc = c.tail_keys(bh) + (slot + kkey) * kHD + (tid & 7) * 16;
         const uint16_t* vsrc = c.tail_values(bh) + vrow * kSlots + slot + (tid & 3) * 16;
-        const int n = seen - (kBlk * j + 16 * (tid & 3));
-        uint32_t bad = 0;
+        u32x4 kt[PER][2], vt[PER][2];
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            kt[i][u] = ld16(ksrc + 16 * NT * i + 8 * u);
+            vt[i][u] = ld16(vsrc + 32 * NT * i + 8 * u);
+          }
+        uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          store_pair(kdst + 32 * NT * i, 2 * (tid & 7), kkey & 7, ld16(ksrc + 16 * NT * i), ld16(ksrc + 16 * NT * i + 8));
-          const u32x4 x = clean_values(ld16(vsrc + 32 * NT * i), n, bad);
-          const u32x4 y = clean_values(ld16(vsrc + 32 * NT * i + 8), n - 8, bad);
+          store_pair(kdst + 32 * NT * i, 2 * (tid & 7), kkey & 7, kt[i][0], kt[i][1]);
+          bits |= nonfinite_bits(vt[i][0]) | nonfinite_bits(vt[i][1]);
+          const u32x4 x = drop_nonfinite(vt[i][0]), y = drop_nonfinite(vt[i][1]);
           store_pair(vdst + 32 * NT * i, 2 * (tid & 3), vrow & 7, u32x4{x.x, x.y, y.x, y.y}, u32x4{x.z, x.w, y.z, y.w});
-          __builtin_amdgcn_sched_barrier(0);
         }
-        if (bad) dropped = 1;
+        if (any_nonfinite(bits)) dropped = 1;
       }
     };
     load_block(at.blk);
@@ -539,7 +577,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
         ks = c.ks[bh * c.nblk + j];
         vs = c.vs[bh * c.nblk + j];
       }
-      if (j + 1 < b1) load_block(j + 1);
+      load_block(j + 1);
       __syncthreads();
       const unsigned char* sk = buf + (32 * hf + r32) * 256;
       const unsigned char* sv = buf + BUF / 2 + r32 * 128;
@@ -624,7 +662,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
     __syncthreads();
     if (tid == 0) dropped = 0;
     first_part = false;
-    left -= b1 - at.blk;
+    at.left -= b1 - at.blk;
     at.blk = 0;
     if (b1 == nb && ++at.h == c.Hkv) {
       at.h = 0;
@@ -634,16 +672,22 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
 }
 
 // ------------------------------------------------------------------- merge
-// The parts of head bh: part of its first run, 2 w of the others up to run w1.
+// The parts of a head, in slots of the workspace (two a workgroup: one for the head that
+// its share starts in, one for a later one): `head` of workgroup w0, 2 w of the others up
+// to w1.
 struct Parts {
   int w0, w1, head;
   __device__ int at(int w) const { return w == w0 ? head : 2 * w; }
 };
 __device__ __forceinline__ Parts parts_of(const VerifyParams& p, Batch& batch, int b, int h, int nb) {
-  const int per = run_length(p, p.c.Hkv * batch.total);
-  const int u0 = p.c.Hkv * batch.before(b) + h * nb;
-  const int w0 = u0 / per;
-  return Parts{w0, (u0 + nb - 1) / per, 2 * w0 + (u0 > w0 * per ? 1 : 0)};
+  const int n = batch.units_of(nb);
+  const int u0 = p.c.Hkv * batch.before(b) + h * n;
+  if (batch.pieces) {
+    const int size = (nb + n - 1) / n;
+    return Parts{u0, u0 + (nb + size - 1) / size - 1, 2 * u0};
+  }
+  const int w0 = u0 / batch.per;
+  return Parts{w0, (u0 + nb - 1) / batch.per, 2 * w0 + (u0 > w0 * batch.per ? 1 : 0)};
 }
 
 // Running merge of the parts that one lane walks; V is the vector of outputs that it holds.
@@ -756,18 +800,17 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kerne
   if (live) store_gated(p, (int64_t)b * p.T + t, qh, d, a.o * (1.f / a.l));
 }
 
-// Rows of a part, blocks of a run at least (a short run's own work should cost more
-// than its part's way through the workspace), and the runs: what the device holds
-// at a time, or fewer for a small cache.
+// Rows of a part; blocks of a piece where there are few; workgroups: what the device holds at a time,
+// or fewer for a small cache.
 struct VerifyShape {
-  int part_rows, min_run, runs;
+  int part_rows, min_cut, runs;
 };
 VerifyShape verify_shape(int64_t B, int rows, int Hkv, int Smax) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
   VerifyShape v;
   v.part_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  v.min_run = rows <= 16 ? kWaves16 : 2;
-  v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(rows <= 16 ? cus : 2 * cus, ceil_div(B * Hkv * (Smax / kBlk), v.min_run)));
+  v.min_cut = 2;
+  v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(rows <= 16 ? cus : 2 * cus, B * Hkv * ceil_div(Smax / kBlk, v.min_cut)));
   return v;
 }
 
@@ -893,13 +936,12 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
           vw[u >> 1][2 * (u & 1) + 1] = y.y;
         }
       } else {
-        uint32_t bad = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           kw[u] = kv[i][u];
-          vw[u] = clean_values(vv[i][u], seen - (kBlk * j + 16 * (e & 3) + 8 * u), bad);
+          vw[u] = drop_nonfinite(vv[i][u]);
         }
-        if (bad) dropped = 1;
+        if (any_nonfinite(nonfinite_bits(vv[i][0]) | nonfinite_bits(vv[i][1]))) dropped = 1;
       }
       unsigned char* krow = buf + key * 256;
       const int c0 = 2 * (e & 7), sk = key & 7;
@@ -1136,7 +1178,7 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   p.rep_inv = 65536u / p.rep + 1;
   const VerifyShape v = verify_shape(B, T * p.rep, Hkv, p.c.Smax);
   p.part_rows = v.part_rows;
-  p.min_run = v.min_run;
+  p.min_cut = v.min_cut;
   p.runs = v.runs;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + (int64_t)2 * p.runs * p.part_rows * kHD;
