@@ -345,7 +345,7 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[4 * n + e] = acc[e];
         }
-        const float sl = sl0 * ks, lv = __log2f(vs), iv = 1.f / vs;
+        const float sl = sl0 * ks, lv = __log2f(vs), iv = __builtin_amdgcn_rcpf(vs);
         load_keys(next);
         ks = ksp[next];
         vs = vsp[next];
@@ -502,8 +502,16 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
     // Unit i of a thread: K's key kkey + NT / 8 i, features 16 (tid % 8) ..; V^T's feature
     // vrow + NT / 4 i, keys 16 (tid % 4) ..  (both steps multiples of 8: one swizzle).
     const int kkey = tid >> 3, vrow = tid >> 2;
+    float ks = 1.f, vs = 1.f;  // of the loaded block
+    const float* ksp = c.ks + bh * c.nblk;
+    const float* vsp = c.vs + bh * c.nblk;
     auto load_block = [&](int j) {
-      if (j >= min(done, b1)) return;
+      if (j >= min(done, b1)) {
+        ks = vs = 1.f;
+        return;
+      }
+      ks = ksp[j];
+      vs = vsp[j];
       const uint8_t* ksrc = c.keys(bh, j) + 16 * tid;
       const uint8_t* vsrc = c.values(bh, j) + 16 * tid;
 #pragma unroll
@@ -572,11 +580,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
       // one barrier a block: the buffer that block j + 1 goes to was read before this one
       unsigned char* buf = lds + (j & 1) * BUF;
       store_block(buf, j);
-      float ks = 1.f, vs = 1.f;
-      if (j < done) {
-        ks = c.ks[bh * c.nblk + j];
-        vs = c.vs[bh * c.nblk + j];
-      }
+      const float sl = sl0 * ks, lv = __log2f(vs), iv = __builtin_amdgcn_rcpf(vs);
       load_block(j + 1);
       __syncthreads();
       const unsigned char* sk = buf + (32 * hf + r32) * 256;
@@ -601,7 +605,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
         mx = fmaxf(mx, st[i]);
       }
       const f32x2 mb = both_halves(mx);
-      const float alpha = weights<16>(s, fmaxf(mb.x, mb.y), sl0 * ks, __log2f(vs), 1.f / vs, m, l, w);
+      const float alpha = weights<16>(s, fmaxf(mb.x, mb.y), sl, lv, iv, m, l, w);
       if (__any(alpha != 1.f)) {
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
@@ -985,7 +989,7 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     if (k0 < Lw) {
       const unsigned char* sk = buf + 64 * hf * 256;
       const unsigned char* sv = buf + kPBuf / 2 + hf * (kHD * 128);
-      const float sl = sl0 * ks, lv = __log2f(vs), iv = 1.f / vs;
+      const float sl = sl0 * ks, lv = __log2f(vs), iv = __builtin_amdgcn_rcpf(vs);
       f32x16 st[2];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
