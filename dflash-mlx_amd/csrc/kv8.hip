@@ -52,20 +52,94 @@ struct AppendParams {
   int T, Hq, rot;
   int nb;      // prompt: block tasks of a head
   int qtiles;  // prompt: 16-token query tiles of a sequence
-  double log2_base;
   float eps;
+  double freq[kHD / 2];  // base^(-2i/rot), i < rot / 2
 };
+
+// A head's row is held by 16 lanes, lane f of them features 8 f .. 8 f + 7 (16 bytes):
+// a wave normalizes and rotates four rows at a time, the sum of squares takes four DPP
+// adds, and the square root and division serve four rows.
+//
+// Cosine and sine of position pos at one frequency: the angle less its multiple of pi / 2
+// in fp64, then the Taylor series of both on [-pi / 4, pi / 4] in fp32 (the first terms left
+// out are below 2e-9), with what the reduced angle's rounding to fp32 loses put back to first
+// order.  Right to about an fp32 step at any position.
+__device__ __forceinline__ f32x2 cos_sin(int pos, double freq) {
+  const double half_pi = 1.5707963267948966192313216916398;
+  const double a = (double)pos * freq;
+  const double n = rint(a * (1.0 / half_pi));
+  const double r = fma(-n, half_pi, a);
+  const float x = (float)r, lo = (float)(r - (double)x), z = x * x;
+  float s = fmaf(z, 1.f / 362880.f, -1.f / 5040.f);
+  s = fmaf(z, s, 1.f / 120.f);
+  s = fmaf(z, s, -1.f / 6.f);
+  s = fmaf(z * x, s, x);
+  float c = fmaf(z, -1.f / 3628800.f, 1.f / 40320.f);
+  c = fmaf(z, c, -1.f / 720.f);
+  c = fmaf(z, c, 1.f / 24.f);
+  c = fmaf(z, c, -0.5f);
+  c = fmaf(z, c, 1.f);
+  const float sn = fmaf(c, lo, s), cs = fmaf(-s, lo, c);
+  const int q = (int)((int64_t)n & 3);  // quarter turns
+  const float u = q & 1 ? sn : cs, v = q & 1 ? cs : sn;
+  return f32x2{q == 1 || q == 2 ? -u : u, q >= 2 ? -v : v};
+}
+
+// The cosines and sines of N positions pos0 .. in LDS: [N][rot / 2] each, all
+// cosines first.  A thread keeps one frequency (256 is a multiple of rot / 2).
+template <int N>
+__device__ __forceinline__ void rotation_table(float* table, int pos0, const AppendParams& p) {
+  if (p.rot == 0) return;
+  const int half = p.rot >> 1, shift = __builtin_ctz(half);
+  const int i = threadIdx.x & (half - 1);
+  const double freq = p.freq[i];
+#pragma unroll 2
+  for (int t = threadIdx.x >> shift; t < N; t += 256 >> shift) {
+    const f32x2 cs = cos_sin(pos0 + t, freq);
+    table[t * half + i] = cs.x;
+    table[(N + t) * half + i] = cs.y;
+  }
+}
+
+// RMSNorm and rotary of a row's eight features at lane f: cosines cs[rot / 2], sines
+// sn[rot / 2].  fp32 throughout, rounded to bf16 once.
+__device__ __forceinline__ u32x4 norm_rotate8(u32x4 xw, u32x4 ww, const float* cs, const float* sn, int f, int rot,
+                                              float eps) {
+  float x[8], w[8];
+  unpack8(xw, x);
+  unpack8(ww, w);
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+  const float inv = 1.f / sqrtf(row16_sum(ss) / (float)kHD + eps);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
+  if (rot > 0) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __shfl_xor(x[i], rot >> 4, 64);
+    if (8 * f < rot) {
+      const int half = rot >> 1;
+      const bool low = 8 * f < half;
+      const int i0 = low ? 8 * f : 8 * f - half;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i0 + i], (low ? -y[i] : y[i]) * sn[i0 + i]);
+    }
+  }
+  return cvt8_bf16(x);
+}
 
 // ------------------------------------------------------------ draft append
 // Workgroups 0 .. 2 B Hkv - 1: the waiting block of one head, keys or values, if
-// any (4096 tokens of the tail's 16 KB in, 8 KB of codes out).  The others: a wave
-// a (token, head), as the bf16 cache's append; keys and values go to the tail.
+// any (16 KB of the tail in, 8 KB of codes out).  The others: 16 heads of a token, keys
+// and values to the tail.
 // The tail's slots that a waiting block is read from are not written by the same
 // call: it waits only where L % 64 <= 16, and the at most 16 new tokens then stay in
 // block L / 64, the other half of the slots.
 template <int TYPE>
 __global__ __launch_bounds__(256) void kv8_append_draft_kernel(const AppendParams p) {
   __shared__ uint32_t red[4];
+  __shared__ float table[kHD];
   const Kv8& c = p.c;
   const int nquant = 2 * c.B * c.Hkv;
   if ((int)blockIdx.x < nquant) {
@@ -74,77 +148,57 @@ __global__ __launch_bounds__(256) void kv8_append_draft_kernel(const AppendParam
     if (may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, (L >> 6) - 1, blockIdx.x & 1, red);
     return;
   }
-  const int slots = p.Hq + 2 * c.Hkv, groups = (slots + 3) >> 2;
+  const int slots = p.Hq + 2 * c.Hkv, groups = (slots + 15) >> 4;
   const int wg = blockIdx.x - nquant;
   const int bt = wg / groups;
-  const int slot = (wg - bt * groups) * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (slot >= slots) return;
+  const int tid = threadIdx.x, f = tid & 15;
+  const int slot = (wg - bt * groups) * 16 + (tid >> 4);
   const int b = bt / p.T;
   const int L = p.lens[b];
   const int pos = L + (bt - b * p.T);
   const bool in_cache = L >= 0 && L <= c.Smax && pos < c.Smax;
-  if (!in_cache && slot == 0 && lane == 0 && p.overflow != nullptr) p.overflow[b] = 1;
-  const int d0 = 2 * lane;
-  const uint16_t* row = p.proj + (int64_t)bt * p.row_stride + d0;
-  const int at = pos & (kSlots - 1);
-  if (slot >= p.Hq + c.Hkv) {
-    if (!in_cache) return;
-    const int h = slot - p.Hq - c.Hkv;
-    const uint32_t vv = *reinterpret_cast<const uint32_t*>(row + (2 * p.Hq + c.Hkv + h) * kHD);
-    uint16_t* col = c.tail_values((int64_t)b * c.Hkv + h) + d0 * kSlots + at;
-    col[0] = (uint16_t)vv;
-    col[kSlots] = (uint16_t)(vv >> 16);
-    return;
+  if (!in_cache && slot == 0 && f == 0 && p.overflow != nullptr) p.overflow[b] = 1;
+  const bool is_q = slot < p.Hq, is_k = !is_q && slot < p.Hq + c.Hkv;
+  const int head = is_q ? 2 * slot : p.Hq + slot;  // in units of 128 of the row: q | gate, k, v
+  u32x4 x = {0u, 0u, 0u, 0u}, w = x;
+  if (slot < slots) {
+    x = ld16(p.proj + (int64_t)bt * p.row_stride + head * kHD + 8 * f);
+    const uint16_t* wsrc = (is_q ? p.q_norm_w : p.k_norm_w) + 8 * f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(wsrc)[i];
   }
-  const bool is_q = slot < p.Hq;
-  const int h = is_q ? slot : slot - p.Hq;
-  const uint32_t xv = *reinterpret_cast<const uint32_t*>(row + (is_q ? 2 * h : 2 * p.Hq + h) * kHD);
-  const uint32_t wv = *reinterpret_cast<const uint32_t*>((is_q ? p.q_norm_w : p.k_norm_w) + d0);
-  const uint32_t packed = norm_rotate(
-      xv, wv, [&] { return rotation_of(pos, d0, p.rot, p.log2_base); }, d0, p.rot, p.eps);
+  if (tid < p.rot >> 1) {
+    const f32x2 cs = cos_sin(pos, p.freq[tid]);
+    table[tid] = cs.x;
+    table[(p.rot >> 1) + tid] = cs.y;
+  }
+  __syncthreads();
+  const u32x4 y = norm_rotate8(x, w, table, table + (p.rot >> 1), f, p.rot, p.eps);
+  const int at = pos & (kSlots - 1);
   if (is_q) {
-    *reinterpret_cast<uint32_t*>(p.q_out + ((int64_t)bt * p.Hq + h) * kHD + d0) = packed;
-  } else if (in_cache) {
-    *reinterpret_cast<uint32_t*>(c.tail_keys((int64_t)b * c.Hkv + h) + at * kHD + d0) = packed;
+    *reinterpret_cast<u32x4*>(p.q_out + ((int64_t)bt * p.Hq + slot) * kHD + 8 * f) = y;
+  } else if (is_k) {
+    if (in_cache)
+      *reinterpret_cast<u32x4*>(c.tail_keys((int64_t)b * c.Hkv + slot - p.Hq) + at * kHD + 8 * f) = y;
+  } else if (slot < slots && in_cache) {
+    uint16_t* col = c.tail_values((int64_t)b * c.Hkv + slot - p.Hq - c.Hkv) + 8 * f * kSlots + at;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) col[i * kSlots] = (uint16_t)(x[i >> 1] >> (16 * (i & 1)));
   }
 }
 
 // ----------------------------------------------------------- prompt append
-// Cosines and sines of N positions pos0 .. and the rot / 2 frequencies, to LDS
-// [N][rot / 2].  A thread keeps one frequency (256 is a multiple of rot / 2), so
-// its fp64 exponential is taken once; the angles are those of rotation_of.
-template <int N>
-__device__ __forceinline__ void rotation_table(f32x2* table, int pos0, int rot, double log2_base) {
-  if (rot == 0) return;
-  const int half = rot >> 1, shift = __builtin_ctz(half);
-  const int i = threadIdx.x & (half - 1);
-  for (int t = threadIdx.x >> shift; t < N; t += 256 >> shift) {
-    float sn, cs;
-    sincosf(rope_angle(pos0 + t, i, rot, log2_base), &sn, &cs);
-    table[t * half + i] = f32x2{cs, sn};
-  }
-}
-
-__device__ __forceinline__ Rotation table_rotation(const f32x2* table, int t, int d0, int rot) {
-  const int half = rot >> 1;
-  const int i0 = d0 < half ? d0 : d0 - half;
-  const f32x2 a = table[t * half + i0], b = table[t * half + i0 + 1];
-  return Rotation{a.y, a.x, b.y, b.x};
-}
-
 // Block j's 64 token rows of head h to LDS: positions of this call from proj (keys
 // normalized and rotated), earlier ones from the tail, others zero.  Ends with a
 // barrier.
 __device__ __forceinline__ void prompt_block_rows(const AppendParams& p, int b, int h, int L, int j, bool values,
-                                                  uint16_t (*rows)[kRow], f32x2* table) {
+                                                  uint16_t (*rows)[kRow], float* table) {
   const Kv8& c = p.c;
   const int64_t bh = (int64_t)b * c.Hkv + h;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, d0 = 2 * lane;
+  const int tid = threadIdx.x;
   const int end = min(L + p.T, c.Smax);
   const uint16_t* proj = p.proj + (int64_t)b * p.T * p.row_stride + (2 * p.Hq + h + (values ? c.Hkv : 0)) * kHD;
   __syncthreads();  // the rows and the table may still be read
-  if (!values) rotation_table<kBlk>(table, kBlk * j, p.rot, p.log2_base);
   if (values) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // 16-byte pieces: token e / 16, features 8 (e % 16)
@@ -168,24 +222,27 @@ __device__ __forceinline__ void prompt_block_rows(const AppendParams& p, int b, 
     __syncthreads();
     return;
   }
-  uint32_t xv[16];
+  const int f = tid & 15;  // four rows a thread: tid / 16 + 16 i
+  u32x4 x[4], w;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int pos = kBlk * j + 16 * wave + i;
-    xv[i] = 0u;
+  for (int i = 0; i < 4; ++i) {
+    const int pos = kBlk * j + (tid >> 4) + 16 * i;
+    x[i] = u32x4{0u, 0u, 0u, 0u};
     if (pos >= L && pos < end)
-      xv[i] = *reinterpret_cast<const uint32_t*>(proj + (int64_t)(pos - L) * p.row_stride + d0);
+      x[i] = ld16(proj + (int64_t)(pos - L) * p.row_stride + 8 * f);
     else if (pos < L)
-      xv[i] = *reinterpret_cast<const uint32_t*>(c.tail_keys(bh) + (pos & (kSlots - 1)) * kHD + d0);
+      x[i] = ld16(c.tail_keys(bh) + (pos & (kSlots - 1)) * kHD + 8 * f);
   }
-  const uint32_t wv = *reinterpret_cast<const uint32_t*>(p.k_norm_w + d0);
-  __syncthreads();  // the table is whole
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int tk = 16 * wave + i, pos = kBlk * j + tk;
-    if (pos >= L && pos < end)
-      xv[i] = norm_rotate(xv[i], wv, [&] { return table_rotation(table, tk, d0, p.rot); }, d0, p.rot, p.eps);
-    *reinterpret_cast<uint32_t*>(&rows[tk][d0]) = xv[i];
+  for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p.k_norm_w + 8 * f)[i];
+  rotation_table<kBlk>(table, kBlk * j, p);
+  __syncthreads();
+  const int half = p.rot >> 1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tk = (tid >> 4) + 16 * i, pos = kBlk * j + tk;
+    const u32x4 y = norm_rotate8(x[i], w, table + tk * half, table + (kBlk + tk) * half, f, p.rot, p.eps);
+    *reinterpret_cast<u32x4*>(&rows[tk][8 * f]) = pos >= L && pos < end ? y : x[i];
   }
   __syncthreads();
 }
@@ -240,15 +297,16 @@ __device__ __forceinline__ void rows_to_tail(const Kv8& c, int64_t bh, int j, bo
 }
 
 // Workgroups: nb block tasks for the keys and nb for the values of every head, then
-// 16 tokens x 4 query heads each.  Task i quantises block L / 64 + i if the prompt
-// completes it.  Task 0 alone touches the tail: it reads the waiting block and the
-// first block's earlier positions, and only then stores the last two blocks' rows
-// (they take the same slots).
+// 16 tokens x 4 query heads each.  Task i has block L / 64 + i: its codes if the prompt
+// completes it, its rows to the tail if it is one of the last two.  Where something is
+// read from the tail (a waiting block, the first block's earlier positions), task 0 alone
+// touches it: it reads first and stores the last two blocks' rows, which take the same
+// slots, afterwards.  Dynamic LDS: the rotation table, 64 rot floats.
 template <int TYPE>
 __global__ __launch_bounds__(256) void kv8_append_prompt_kernel(const AppendParams p) {
   __shared__ __attribute__((aligned(16))) uint16_t rows[kBlk][kRow];
-  __shared__ f32x2 table[kBlk * kHD / 2];
   __shared__ uint32_t red[4];
+  extern __shared__ __attribute__((aligned(16))) float table[];
   const Kv8& c = p.c;
   const int64_t ntask = (int64_t)c.B * c.Hkv * 2 * p.nb;
   int64_t id = blockIdx.x;
@@ -261,19 +319,21 @@ __global__ __launch_bounds__(256) void kv8_append_prompt_kernel(const AppendPara
     const int L = p.lens[b];
     if (L < 0 || L > c.Smax) return;
     const int first = L >> 6, end = min(L + p.T, c.Smax), done = end >> 6, j = first + i;
-    if (i == 0 && may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, first - 1, values, red);
-    if (j < done) {
-      prompt_block_rows(p, b, h, L, j, values, rows, table);
-      quantise_rows<TYPE>(c, bh, j, values, rows, red);
-    }
-    if (i != 0) return;
-    for (int jj = max(done - 1, first); jj <= done && kBlk * jj < end; ++jj) {
+    const bool reads_tail = (L & 63) != 0 || may_wait(L, c.Smax);
+    if (reads_tail && i == 0 && may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, first - 1, values, red);
+    const int tail0 = max(done - 1, first);  // the first block that the tail keeps
+#pragma unroll 1
+    for (int step = 0; step < (reads_tail && i == 0 ? 3 : 1); ++step) {
+      const int jj = step == 0 ? j : tail0 + step - 1;
+      const bool quantises = step == 0 && jj < done;
+      const bool keeps = step == 0 ? !reads_tail && jj >= tail0 : jj <= done;
+      if (kBlk * jj >= end || !(quantises || keeps)) continue;
       prompt_block_rows(p, b, h, L, jj, values, rows, table);
-      rows_to_tail(c, bh, jj, values, L, end, rows);
+      if (quantises) quantise_rows<TYPE>(c, bh, jj, values, rows, red);
+      if (keeps) rows_to_tail(c, bh, jj, values, L, end, rows);
     }
     return;
   }
-  // queries: a wave 4 tokens x 4 heads
   id -= ntask;
   const int hgroups = (p.Hq + 3) >> 2;
   const int h0 = 4 * (int)(id % hgroups);
@@ -282,22 +342,20 @@ __global__ __launch_bounds__(256) void kv8_append_prompt_kernel(const AppendPara
   const int L = p.lens[b], t0 = 16 * tile;
   if (h0 == 0 && tile == 0 && threadIdx.x == 0 && (L < 0 || L > c.Smax - p.T) && p.overflow != nullptr)
     p.overflow[b] = 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = 2 * lane;
-  uint32_t xv[16];
+  const int tk = threadIdx.x >> 4, f = threadIdx.x & 15, t = t0 + tk;  // a token a 16 lanes
+  const int64_t row = (int64_t)b * p.T + min(t, p.T - 1);
+  u32x4 x[4], w;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int t = min(t0 + 4 * wave + (i >> 2), p.T - 1), h = min(h0 + (i & 3), p.Hq - 1);
-    xv[i] = *reinterpret_cast<const uint32_t*>(p.proj + ((int64_t)b * p.T + t) * p.row_stride + 2 * h * kHD + d0);
-  }
-  const uint32_t wv = *reinterpret_cast<const uint32_t*>(p.q_norm_w + d0);
-  rotation_table<16>(table, L + t0, p.rot, p.log2_base);
+  for (int i = 0; i < 4; ++i) x[i] = ld16(p.proj + row * p.row_stride + 2 * min(h0 + i, p.Hq - 1) * kHD + 8 * f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p.q_norm_w + 8 * f)[i];
+  rotation_table<16>(table, L + t0, p);
   __syncthreads();
+  const int half = p.rot >> 1;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int tk = 4 * wave + (i >> 2), t = t0 + tk, h = h0 + (i & 3);
-    if (t >= p.T || h >= p.Hq) continue;
-    *reinterpret_cast<uint32_t*>(p.q_out + (((int64_t)b * p.T + t) * p.Hq + h) * kHD + d0) =
-        norm_rotate(xv[i], wv, [&] { return table_rotation(table, tk, d0, p.rot); }, d0, p.rot, p.eps);
+  for (int i = 0; i < 4; ++i) {
+    const u32x4 y = norm_rotate8(x[i], w, table + tk * half, table + (16 + tk) * half, f, p.rot, p.eps);
+    if (t < p.T && h0 + i < p.Hq) *reinterpret_cast<u32x4*>(p.q_out + (row * p.Hq + h0 + i) * kHD + 8 * f) = y;
   }
 }
 
@@ -430,13 +488,13 @@ bool fits_grid(int64_t wgs) { return wgs <= INT32_MAX; }
 
 using namespace dflash;
 
-#define DFLASH_KV8_LAUNCH(kernel, type, grid, stream, p)                                         \
+#define DFLASH_KV8_LAUNCH(kernel, type, grid, lds, stream, p)                                    \
   do {                                                                                           \
     if ((type) == DFLASH_KV_INT8)                                                                \
-      hipLaunchKernelGGL((kernel<DFLASH_KV_INT8>), dim3((unsigned)(grid)), dim3(256), 0,         \
+      hipLaunchKernelGGL((kernel<DFLASH_KV_INT8>), dim3((unsigned)(grid)), dim3(256), lds,       \
                          static_cast<hipStream_t>(stream), p);                                   \
     else                                                                                         \
-      hipLaunchKernelGGL((kernel<DFLASH_KV_E4M3>), dim3((unsigned)(grid)), dim3(256), 0,         \
+      hipLaunchKernelGGL((kernel<DFLASH_KV_E4M3>), dim3((unsigned)(grid)), dim3(256), lds,       \
                          static_cast<hipStream_t>(stream), p);                                   \
   } while (0)
 
@@ -456,7 +514,7 @@ extern "C" int dflash_kv8_append(const dflash_kv8_cache* cache, const void* proj
   if (proj == nullptr || q_norm_w == nullptr || k_norm_w == nullptr || lens == nullptr || q_out == nullptr)
     return DFLASH_ERR_NULL;
   if (((uintptr_t)proj & 15) || proj_row_stride % 8 || ((uintptr_t)q_norm_w & 3) || ((uintptr_t)k_norm_w & 3) ||
-      ((uintptr_t)q_out & 3))
+      ((uintptr_t)q_out & 15))
     return DFLASH_ERR_ALIGN;
   p.proj = static_cast<const uint16_t*>(proj);
   p.row_stride = proj_row_stride;
@@ -466,18 +524,18 @@ extern "C" int dflash_kv8_append(const dflash_kv8_cache* cache, const void* proj
   p.q_out = static_cast<uint16_t*>(q_out);
   p.overflow = overflow;
   p.T = T; p.Hq = Hq; p.rot = rot_dims;
-  p.log2_base = log2((double)rope_base);
+  for (int i = 0; i < rot_dims / 2; ++i) p.freq[i] = exp2(-2.0 * i / rot_dims * log2((double)rope_base));
   p.eps = eps;
   if (!prompt) {
-    const int64_t grid = (int64_t)2 * B * Hkv + (int64_t)B * T * ceil_div(Hq + 2 * Hkv, 4);
+    const int64_t grid = (int64_t)2 * B * Hkv + (int64_t)B * T * ceil_div(Hq + 2 * Hkv, 16);
     if (!fits_grid(grid)) return DFLASH_ERR_SHAPE;
-    DFLASH_KV8_LAUNCH(kv8_append_draft_kernel, cache->type, grid, stream, p);
+    DFLASH_KV8_LAUNCH(kv8_append_draft_kernel, cache->type, grid, 0, stream, p);
   } else {
     p.nb = (int)std::min<int64_t>(T / kBlk + 2, p.c.nblk);
     p.qtiles = (int)ceil_div(T, 16);
     const int64_t grid = (int64_t)2 * B * Hkv * p.nb + (int64_t)B * p.qtiles * ceil_div(Hq, 4);
     if (!fits_grid(grid)) return DFLASH_ERR_SHAPE;
-    DFLASH_KV8_LAUNCH(kv8_append_prompt_kernel, cache->type, grid, stream, p);
+    DFLASH_KV8_LAUNCH(kv8_append_prompt_kernel, cache->type, grid, (unsigned)(kBlk * rot_dims * sizeof(float)), stream, p);
   }
   return to_status(hipGetLastError());
 }
@@ -505,7 +563,7 @@ extern "C" int dflash_kv8_load(const dflash_kv8_cache* cache, const void* k, con
   p.nb = (int)ceil_div(std::min(S, p.c.Smax), kBlk);
   const int64_t grid = (int64_t)2 * p.c.B * p.c.Hkv * p.nb;
   if (!fits_grid(grid)) return DFLASH_ERR_SHAPE;
-  DFLASH_KV8_LAUNCH(kv8_load_kernel, cache->type, grid, stream, p);
+  DFLASH_KV8_LAUNCH(kv8_load_kernel, cache->type, grid, 0, stream, p);
   return to_status(hipGetLastError());
 }
 
@@ -526,6 +584,6 @@ extern "C" int dflash_kv8_read(const dflash_kv8_cache* cache, const int32_t* len
   p.v = static_cast<uint16_t*>(v_out);
   const int64_t grid = (int64_t)2 * p.c.B * p.c.Hkv * p.nb;
   if (!fits_grid(grid)) return DFLASH_ERR_SHAPE;
-  DFLASH_KV8_LAUNCH(kv8_read_kernel, cache->type, grid, stream, p);
+  DFLASH_KV8_LAUNCH(kv8_read_kernel, cache->type, grid, 0, stream, p);
   return to_status(hipGetLastError());
 }

@@ -75,8 +75,8 @@ typedef struct {
  *   prompt != 0: T committed tokens.  Every block that they complete is quantised,
  *     and the tail holds the last two blocks' positions.
  * overflow (or NULL): [B], set to 1 for a sequence with a position outside
- * [0, Smax).  rot_dims in {0, 16, 32, 64, 128}; Hq a multiple of Hkv; proj and
- * proj_row_stride 16-byte aligned.
+ * [0, Smax).  rot_dims in {0, 16, 32, 64, 128}; Hq a multiple of Hkv; proj, its rows
+ * and q_out 16-byte aligned.
  */
 int dflash_kv8_append(const dflash_kv8_cache* cache, const void* proj,
                       int64_t proj_row_stride, const void* q_norm_w,

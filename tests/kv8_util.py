@@ -64,18 +64,54 @@ def proj_rows(B, T, Hq, Hkv, seed, pad=0):
     return torch.randn(B, T, (2 * Hq + 2 * Hkv) * D + pad, generator=g).bfloat16()
 
 
-def bf16_append(device, proj, lens, Smax, Hq, Hkv, wq, wk, rot):
-    """dflash_attn_prep of the same rows: (q, keys, values [B, Hkv, Smax, D])."""
-    from dflash_mlx import _lib
+def norm_rotated(x, w, pos, rot):
+    """(values, slack) fp64 of RMSNorm(x) * w rotated at pos: x [B, T, H, D] bf16, pos
+    [B, T].  slack: what the kernels' fp32 may be off by before rounding, 2^-18 of the
+    pair that the rotation mixes (a sum of 128 squares, a square root, a division, two
+    products and the cosines' and sines' own 7e-8 each lose less than 2^-20)."""
+    x = x.double()
+    x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + EPS) * w.double()
+    mag = x.abs()
+    if rot:
+        inv = THETA ** (-2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)
+        ang = pos.double()[:, :, None, None] * inv
+        a, b = x[..., :rot // 2], x[..., rot // 2:rot]
+        both = a.abs() + b.abs()
+        x = torch.cat((a * ang.cos() - b * ang.sin(), b * ang.cos() + a * ang.sin(), x[..., rot:]), -1)
+        mag = torch.cat((both, both, mag[..., rot:]), -1)
+    return x, mag * 2.0 ** -18
+
+
+def rounded_right(got, want, slack):
+    """got (bf16) is want rounded to bf16, half a step (2^-8) of what was rounded."""
+    return bool(((got.double() - want).abs() <= 2.0 ** -8 * (want.abs() + slack) + slack).all())
+
+
+def appended_keys(device, proj, lens, Hq, Hkv, wk, rot, Smax, dtype):
+    """The keys [B, T, Hkv, D] that an append of these rows stores, taken from the same
+    kernel with the key rows in the queries' place (of a scratch cache)."""
+    import dflash_mlx as dm
 
     B, T = proj.shape[:2]
-    kc = torch.zeros(B, Hkv, Smax, D, dtype=torch.bfloat16, device=device)
-    vt = torch.zeros(B, Hkv, D, Smax, dtype=torch.bfloat16, device=device)
-    q = torch.empty(B, T, Hq, D, dtype=torch.bfloat16, device=device)
-    _lib.call("dflash_attn_prep", proj.data_ptr(), proj.stride(1), wq.data_ptr(), wk.data_ptr(), lens.data_ptr(),
-              kc.data_ptr(), vt.data_ptr(), q.data_ptr(), None, B, T, Hq, Hkv, D, Smax, rot, THETA, EPS,
-              _lib.stream_handle(device))
-    return q, kc, vt.transpose(2, 3)
+    rows = torch.zeros(B, T, 4 * Hkv * D, dtype=torch.bfloat16, device=device)
+    rows[..., :2 * Hkv * D].view(B, T, Hkv, 2, D)[:, :, :, 0] = \
+        proj[..., 2 * Hq * D:(2 * Hq + Hkv) * D].view(B, T, Hkv, D)
+    scratch = dm.QuantizedKVCache.zeros(B, Hkv, Smax, dtype, device)
+    return dm.attn_prep_q8(rows, wk, wk, lens, scratch, num_heads=Hkv, rot_dims=rot, rope_base=THETA, eps=EPS,
+                           prompt=True)
+
+
+def appended(device, k, v, proj, lens, Hq, Hkv, wk, rot, Smax, dtype):
+    """Histories k, v [B, Hkv, Smax, D] with the rows' keys and values at lens[b] + t."""
+    keys = appended_keys(device, proj, torch.tensor(lens, dtype=torch.int32, device=device), Hq, Hkv, wk, rot, Smax,
+                         dtype).cpu()
+    vals = proj[..., (2 * Hq + Hkv) * D:(2 * Hq + 2 * Hkv) * D].view(*proj.shape[:2], Hkv, D).cpu()
+    k, v = k.clone(), v.clone()
+    for b, L in enumerate(lens):
+        n = max(0, min(L + proj.shape[1], Smax) - L) if L >= 0 else 0
+        if n:
+            k[b, :, L:L + n], v[b, :, L:L + n] = keys[b, :n].transpose(0, 1), vals[b, :n].transpose(0, 1)
+    return k, v
 
 
 def attention_error(got, q, k, v, proj, lens, ends, dtype, scale):

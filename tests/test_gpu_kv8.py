@@ -1,16 +1,16 @@
 """The 8-bit key/value cache: quantising, loading, reading back and appending.
 
 Codes, scales and the values read back are compared bit for bit with the
-definition (oracle/kv8_oracle.py); appended queries and keys with the bf16
-cache's append (dflash_attn_prep), whose bits they must be."""
+definition (oracle/kv8_oracle.py); appended queries and keys with their
+formula in 64 bits, and the bf16 cache's append (dflash_attn_prep) with both."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 from oracle import kv8_oracle as orc
-from tests.kv8_util import (BLOCK, D, DTYPES, EPS, SLOTS, THETA, bf16_append, expected_read, loaded, proj_rows, random_kv,
-                            raw, tail_holds)
+from tests.kv8_util import (BLOCK, D, DTYPES, EPS, THETA, appended, appended_keys, expected_read, loaded, norm_rotated,
+                            proj_rows, random_kv, raw, rounded_right, tail_holds)
 
 pytestmark = pytest.mark.gpu
 
@@ -124,6 +124,47 @@ def _append(device, cache, proj, lens, Hq, Hkv, wq, wk, rot, prompt, overflow=No
                            prompt=prompt, overflow=overflow)
 
 
+def _queries_right(q, proj, lens, Hq, w, rot):
+    B, T = proj.shape[:2]
+    pos = torch.tensor(lens)[:, None] + torch.arange(T)
+    rows = proj[..., :2 * Hq * D].reshape(B, T, Hq, 2, D)[:, :, :, 0]
+    assert rounded_right(q.cpu(), *norm_rotated(rows.cpu(), w.cpu(), pos, rot))
+
+
+@pytest.mark.parametrize("rot", [0, 16, 32, 64, 128])
+def test_queries_and_keys_against_their_formula(device, rot):
+    """At positions from 0 to over 10^5, in both forms, with rows of every size: the
+    formula in 64 bits rounded once, and the bf16 cache's append within its own rounding."""
+    import dflash_mlx as dm
+    from dflash_mlx import _lib
+
+    B, T, Hq, Hkv, Smax = 5, 16, 6, 2, 131072
+    lens = [0, 1000, 40961, 99999, Smax - T]
+    proj = proj_rows(B, T, Hq, Hkv, seed=rot)
+    proj *= torch.tensor([1.0, 1e-4, 30.0, 0.0, 1e4]).bfloat16()[:, None, None]
+    g = torch.Generator().manual_seed(rot)
+    w = (1 + 0.2 * torch.randn(D, generator=g)).bfloat16().to(device)
+    proj, lens_d = proj.to(device), torch.tensor(lens, dtype=torch.int32, device=device)
+    cache = dm.QuantizedKVCache.zeros(B, Hkv, 64, torch.int8, device)  # positions past it are not written
+    q = _append(device, cache, proj, lens_d, Hq, Hkv, w, w, rot, False)
+    assert torch.equal(q, _append(device, cache, proj, lens_d, Hq, Hkv, w, w, rot, True))
+    _queries_right(q, proj, lens, Hq, w, rot)
+    keys = appended_keys(device, proj, lens_d, Hq, Hkv, w, rot, 64, torch.int8)
+    rows = proj[..., 2 * Hq * D:(2 * Hq + Hkv) * D].reshape(B, T, Hkv, D).cpu()
+    want, slack = norm_rotated(rows, w.cpu(), torch.tensor(lens)[:, None] + torch.arange(T), rot)
+    assert rounded_right(keys.cpu(), want, slack)
+    # the bf16 cache's append: an fp32 angle of up to 2 pi is off by 2.4e-7, so 2^-16 of the pair
+    kc = torch.zeros(1, Hkv, Smax, D, dtype=torch.bfloat16, device=device)
+    vt = torch.zeros(1, Hkv, D, Smax, dtype=torch.bfloat16, device=device)
+    for b, L in enumerate(lens):
+        qb = torch.empty(1, T, Hq, D, dtype=torch.bfloat16, device=device)
+        _lib.call("dflash_attn_prep", proj[b].data_ptr(), proj.stride(1), w.data_ptr(), w.data_ptr(),
+                  lens_d[b:].data_ptr(), kc.data_ptr(), vt.data_ptr(), qb.data_ptr(), None, 1, T, Hq, Hkv, D, Smax, rot,
+                  THETA, EPS, _lib.stream_handle(device))
+        got = kc[0, :, L:L + T].transpose(0, 1).cpu()
+        assert rounded_right(got, want[b], 4 * slack[b])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,Hq,Hkv,rot,lens", [
     (1, 4, 1, 32, [0, 63, 64, 80, 81]), (16, 16, 4, 32, [0, 48, 60, 64, 70]), (7, 8, 8, 128, [1, 121, 128, 144, 200]),
@@ -145,12 +186,10 @@ def test_draft_append(device, dtype, T, Hq, Hkv, rot, lens):
     g = torch.Generator().manual_seed(9)
     wq, wk = ((1 + 0.2 * torch.randn(D, generator=g)).bfloat16().to(device) for _ in range(2))
     q = _append(device, cache, proj, lens_d, Hq, Hkv, wq, wk, rot, False)
-    q_ref, k_new, v_new = bf16_append(device, proj, lens_d, Smax, Hq, Hkv, wq, wk, rot)
-    assert torch.equal(q, q_ref)
-    k_new, v_new = k_new.cpu(), v_new.cpu()
+    _queries_right(q, proj, lens, Hq, wq, rot)
+    ks, vs = appended(device, k, v, proj, lens, Hq, Hkv, wk, rot, Smax, dtype)
     for b, L in enumerate(lens):
-        kk, vv = k[b].clone(), v[b].clone()
-        kk[:, L:L + T], vv[:, L:L + T] = k_new[b, :, L:L + T], v_new[b, :, L:L + T]
+        kk, vv = ks[b], vs[b]
         _same_codes(cache, b, kk, vv, 0, L // BLOCK, dtype)
         lo = max(L // BLOCK - (L % BLOCK + T <= BLOCK), 0) * BLOCK
         assert tail_holds(cache, b, kk, vv, lo, L + T)
@@ -182,14 +221,11 @@ def test_prompt_append(device, dtype, T, Hq, Hkv, rot, lens):
     wq, wk = ((1 + 0.2 * torch.randn(D, generator=g)).bfloat16().to(device) for _ in range(2))
     flags = torch.zeros(B, dtype=torch.int32, device=device)
     q = _append(device, cache, proj, lens_d, Hq, Hkv, wq, wk, rot, True, flags)
-    q_ref, k_new, v_new = bf16_append(device, proj, lens_d, Smax, Hq, Hkv, wq, wk, rot)
-    assert torch.equal(q, q_ref)
+    _queries_right(q, proj, lens, Hq, wq, rot)
     assert flags.cpu().tolist() == [int(L + T > Smax) for L in lens]
-    k_new, v_new = k_new.cpu(), v_new.cpu()
+    ks, vs = appended(device, k, v, proj, lens, Hq, Hkv, wk, rot, Smax, dtype)
     for b, L in enumerate(lens):
-        kk, vv = k[b].clone(), v[b].clone()
-        end = min(L + T, Smax)
-        kk[:, L:end], vv[:, L:end] = k_new[b, :, L:end], v_new[b, :, L:end]
+        kk, vv, end = ks[b], vs[b], min(L + T, Smax)
         _same_codes(cache, b, kk, vv, 0, end // BLOCK, dtype)
         assert tail_holds(cache, b, kk, vv, max(end // BLOCK - 1, 0) * BLOCK, end)
 
@@ -214,10 +250,8 @@ def test_sequences_that_take_no_part_or_run_over(device, dtype, prompt):
     for i in range(6):
         for b in (0, 3):
             assert torch.equal(before[i][b], after[i][b]), (i, b)
-    _, k_new, v_new = bf16_append(device, proj, lens_d, Smax, Hq, Hkv, w, w, 32)
-    kk, vv = k[1].clone(), v[1].clone()
-    kk[:, 120:], vv[:, 120:] = k_new[1, :, 120:].cpu(), v_new[1, :, 120:].cpu()
-    assert tail_holds(cache, 1, kk, vv, 64, 128)
+    ks, vs = appended(device, k, v, proj, [-1, 120, -1, -1], Hq, Hkv, w, 32, Smax, dtype)
+    assert tail_holds(cache, 1, ks[1], vs[1], 64, 128)
     _same_codes(cache, 2, k[2], v[2], 0, 2, dtype)
     assert tail_holds(cache, 2, k[2], v[2], 64, 128)  # of a load: the last two blocks, 1 and (empty) 2
 
