@@ -40,6 +40,93 @@ __device__ __forceinline__ void quantise_tail_block(const Kv8& c, int64_t bh, in
 // Block L / 64 - 1 may have become complete since the last append.
 __device__ __forceinline__ bool may_wait(int L, int Smax) { return L >= kBlk && L <= Smax && (L & 63) <= kMaxDraft; }
 
+// A block's 64 rows in registers: piece i of a thread is token tid / 16 + 16 i, features
+// 8 (tid % 16) .. + 7.
+struct Rows {
+  u32x4 x[4];
+};
+
+// Four dwords as four rows of bytes, transposed.
+__device__ __forceinline__ void transpose4(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  const uint32_t ab0 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab2 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+  const uint32_t cd0 = __builtin_amdgcn_perm(d, c, 0x05010400u), cd2 = __builtin_amdgcn_perm(d, c, 0x07030602u);
+  a = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u);
+  b = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
+  c = __builtin_amdgcn_perm(cd2, ab2, 0x05040100u);
+  d = __builtin_amdgcn_perm(cd2, ab2, 0x07060302u);
+}
+
+// LDS of a block's values on their way from [position][feature] to [feature][position] or
+// back: codes, rows of 33 dwords (a wave's dwords of 8 rows 8 apart, 8 side by side each,
+// fall into 64 banks), or bf16.
+struct Turn {
+  union {
+    uint32_t codes[kBlk][kHD / 4 + 1];
+    uint16_t rows[kBlk][kRow];
+  };
+};
+
+// The codes of a block whose rows are in registers.  Values are stored transposed: a
+// thread turns 4 features x 8 positions, so that eight lanes store a feature's 64 bytes.
+template <int TYPE>
+__device__ __forceinline__ void store_codes(const Kv8& c, int64_t bh, int j, bool values, const Rows& r, Turn& lds,
+                                            uint32_t* red) {
+  const int t = threadIdx.x;
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a = max(a, abs_bits16(r.x[i]));
+  const f32x2 sm = block_scale<TYPE>(group_max_u32(a, red));
+  if (t == 0) (values ? c.vs : c.ks)[bh * c.nblk + j] = sm.x;
+  if (!values) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<u32x2*>(c.keys(bh, j) + 8 * (t + 256 * i)) = quantise8<TYPE>(r.x[i], sm.y);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const u32x2 q = quantise8<TYPE>(r.x[i], sm.y);
+    uint32_t* dst = &lds.codes[(t >> 4) + 16 * i][2 * (t & 15)];
+    dst[0] = q.x;
+    dst[1] = q.y;
+  }
+  __syncthreads();
+  const int p0 = 8 * (t & 7), quad = t >> 3;
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = lds.codes[p0 + i][quad];
+  transpose4(w[0], w[1], w[2], w[3]);
+  transpose4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<u32x2*>(c.values(bh, j) + (4 * quad + i) * kBlk + p0) = u32x2{w[i], w[4 + i]};
+  __syncthreads();
+}
+
+// The rows of block j at positions [from, to) into the tail.
+__device__ __forceinline__ void store_tail(const Kv8& c, int64_t bh, int j, bool values, const Rows& r, int from, int to,
+                                           Turn& lds) {
+  const int t = threadIdx.x;
+  if (!values) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = kBlk * j + (t >> 4) + 16 * i;
+      if (pos >= from && pos < to)
+        *reinterpret_cast<u32x4*>(c.tail_keys(bh) + (pos & (kSlots - 1)) * kHD + 8 * (t & 15)) = r.x[i];
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(&lds.rows[(t >> 4) + 16 * i][8 * (t & 15)]) = r.x[i];
+  __syncthreads();
+  uint16_t* dst = c.tail_values(bh) + (t >> 1) * kSlots + (j & 1) * kBlk;
+  for (int i = 0; i < 32; ++i) {
+    const int tk = (t & 1) * 32 + i, pos = kBlk * j + tk;
+    if (pos >= from && pos < to) dst[tk] = lds.rows[tk][t >> 1];
+  }
+  __syncthreads();
+}
+
 struct AppendParams {
   Kv8 c;
   const uint16_t* proj;  // [B*T, row_stride]: Hq x (q | gate), Hkv x k, Hkv x v
@@ -188,51 +275,46 @@ __global__ __launch_bounds__(256) void kv8_append_draft_kernel(const AppendParam
 }
 
 // ----------------------------------------------------------- prompt append
-// Block j's 64 token rows of head h to LDS: positions of this call from proj (keys
-// normalized and rotated), earlier ones from the tail, others zero.  Ends with a
-// barrier.
-__device__ __forceinline__ void prompt_block_rows(const AppendParams& p, int b, int h, int L, int j, bool values,
-                                                  uint16_t (*rows)[kRow], float* table) {
+// Block j's 64 rows of head h: positions of this call from proj (keys normalized and
+// rotated), earlier ones from the tail, others zero.
+__device__ __forceinline__ Rows prompt_rows(const AppendParams& p, int b, int h, int L, int j, bool values, Turn& lds,
+                                            float* table) {
   const Kv8& c = p.c;
   const int64_t bh = (int64_t)b * c.Hkv + h;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, f = tid & 15;
   const int end = min(L + p.T, c.Smax);
-  const uint16_t* proj = p.proj + (int64_t)b * p.T * p.row_stride + (2 * p.Hq + h + (values ? c.Hkv : 0)) * kHD;
-  __syncthreads();  // the rows and the table may still be read
-  if (values) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // 16-byte pieces: token e / 16, features 8 (e % 16)
-      const int e = tid + 256 * i, pos = kBlk * j + (e >> 4);
-      u32x4 w = {0u, 0u, 0u, 0u};
-      if (pos >= L && pos < end) w = ld16(proj + (int64_t)(pos - L) * p.row_stride + (e & 15) * 8);
-      if (pos >= L) *reinterpret_cast<u32x4*>(&rows[e >> 4][(e & 15) * 8]) = w;
-    }
-    if (kBlk * j < L) {  // the tail's values are transposed: thread (feature, 32 slots)
-      const uint16_t* src = c.tail_values(bh) + (tid >> 1) * kSlots + (j & 1) * kBlk + (tid & 1) * 32;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const u32x4 w = ld16(src + 8 * i);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int tk = (tid & 1) * 32 + 8 * i + u;
-          if (kBlk * j + tk < L) rows[tk][tid >> 1] = (uint16_t)(w[u >> 1] >> (16 * (u & 1)));
-        }
-      }
-    }
-    __syncthreads();
-    return;
-  }
-  const int f = tid & 15;  // four rows a thread: tid / 16 + 16 i
-  u32x4 x[4], w;
+  const uint16_t* proj = p.proj + (int64_t)b * p.T * p.row_stride + (2 * p.Hq + h + (values ? c.Hkv : 0)) * kHD + 8 * f;
+  Rows r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int pos = kBlk * j + (tid >> 4) + 16 * i;
-    x[i] = u32x4{0u, 0u, 0u, 0u};
+    r.x[i] = u32x4{0u, 0u, 0u, 0u};
     if (pos >= L && pos < end)
-      x[i] = ld16(proj + (int64_t)(pos - L) * p.row_stride + 8 * f);
-    else if (pos < L)
-      x[i] = ld16(c.tail_keys(bh) + (pos & (kSlots - 1)) * kHD + 8 * f);
+      r.x[i] = ld16(proj + (int64_t)(pos - L) * p.row_stride);
+    else if (pos < L && !values)
+      r.x[i] = ld16(c.tail_keys(bh) + (pos & (kSlots - 1)) * kHD + 8 * f);
   }
+  if (values) {
+    if (kBlk * j >= L) return r;
+    // the tail's values are transposed: thread (feature, 32 slots)
+    const uint16_t* src = c.tail_values(bh) + (tid >> 1) * kSlots + (j & 1) * kBlk + (tid & 1) * 32;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32x4 w = ld16(src + 8 * i);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        lds.rows[(tid & 1) * 32 + 8 * i + u][tid >> 1] = (uint16_t)(w[u >> 1] >> (16 * (u & 1)));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tk = (tid >> 4) + 16 * i;
+      if (kBlk * j + tk < L) r.x[i] = *reinterpret_cast<const u32x4*>(&lds.rows[tk][8 * f]);
+    }
+    __syncthreads();
+    return r;
+  }
+  u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p.k_norm_w + 8 * f)[i];
   rotation_table<kBlk>(table, kBlk * j, p);
@@ -241,59 +323,11 @@ __device__ __forceinline__ void prompt_block_rows(const AppendParams& p, int b, 
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int tk = (tid >> 4) + 16 * i, pos = kBlk * j + tk;
-    const u32x4 y = norm_rotate8(x[i], w, table + tk * half, table + (kBlk + tk) * half, f, p.rot, p.eps);
-    *reinterpret_cast<u32x4*>(&rows[tk][8 * f]) = pos >= L && pos < end ? y : x[i];
+    const u32x4 y = norm_rotate8(r.x[i], w, table + tk * half, table + (kBlk + tk) * half, f, p.rot, p.eps);
+    if (pos >= L && pos < end) r.x[i] = y;
   }
-  __syncthreads();
-}
-
-// The codes of the block in LDS rows.
-template <int TYPE>
-__device__ __forceinline__ void quantise_rows(const Kv8& c, int64_t bh, int j, bool values,
-                                              const uint16_t (*rows)[kRow], uint32_t* red) {
-  const int t = threadIdx.x;
-  u32x4 w[4];
-  if (values) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int tk = (t & 1) * 32 + 2 * i;
-      w[i >> 2][i & 3] = (uint32_t)rows[tk][t >> 1] | ((uint32_t)rows[tk + 1][t >> 1] << 16);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const u32x4*>(&rows[t >> 2][(t & 3) * 32 + 8 * i]);
-  }
-  uint32_t a = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) a = max(a, abs_bits16(w[i]));
-  const f32x2 sm = block_scale<TYPE>(group_max_u32(a, red));
-  uint8_t* dst = (values ? c.values(bh, j) : c.keys(bh, j)) + 32 * t;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const u32x2 lo = quantise8<TYPE>(w[2 * i], sm.y), hi = quantise8<TYPE>(w[2 * i + 1], sm.y);
-    *reinterpret_cast<u32x4*>(dst + 16 * i) = u32x4{lo.x, lo.y, hi.x, hi.y};
-  }
-  if (t == 0) (values ? c.vs : c.ks)[bh * c.nblk + j] = sm.x;
-}
-
-// The rows of block j at positions [from, to) into the tail.
-__device__ __forceinline__ void rows_to_tail(const Kv8& c, int64_t bh, int j, bool values, int from, int to,
-                                             const uint16_t (*rows)[kRow]) {
-  const int t = threadIdx.x;
-  if (values) {
-    uint16_t* dst = c.tail_values(bh) + (t >> 1) * kSlots + (j & 1) * kBlk;
-    for (int i = 0; i < 32; ++i) {
-      const int tk = (t & 1) * 32 + i, pos = kBlk * j + tk;
-      if (pos >= from && pos < to) dst[tk] = rows[tk][t >> 1];
-    }
-  } else {
-    const int pos = kBlk * j + (t >> 2);
-    if (pos < from || pos >= to) return;
-    uint16_t* dst = c.tail_keys(bh) + (pos & (kSlots - 1)) * kHD + (t & 3) * 32;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<u32x4*>(dst + 8 * i) = *reinterpret_cast<const u32x4*>(&rows[t >> 2][(t & 3) * 32 + 8 * i]);
-  }
+  __syncthreads();  // the table may be written again
+  return r;
 }
 
 // Workgroups: nb block tasks for the keys and nb for the values of every head, then
@@ -303,8 +337,8 @@ __device__ __forceinline__ void rows_to_tail(const Kv8& c, int64_t bh, int j, bo
 // touches it: it reads first and stores the last two blocks' rows, which take the same
 // slots, afterwards.  Dynamic LDS: the rotation table, 64 rot floats.
 template <int TYPE>
-__global__ __launch_bounds__(256) void kv8_append_prompt_kernel(const AppendParams p) {
-  __shared__ __attribute__((aligned(16))) uint16_t rows[kBlk][kRow];
+__global__ __launch_bounds__(256, 4) void kv8_append_prompt_kernel(const AppendParams p) {
+  __shared__ __attribute__((aligned(16))) Turn lds;
   __shared__ uint32_t red[4];
   extern __shared__ __attribute__((aligned(16))) float table[];
   const Kv8& c = p.c;
@@ -328,9 +362,9 @@ __global__ __launch_bounds__(256) void kv8_append_prompt_kernel(const AppendPara
       const bool quantises = step == 0 && jj < done;
       const bool keeps = step == 0 ? !reads_tail && jj >= tail0 : jj <= done;
       if (kBlk * jj >= end || !(quantises || keeps)) continue;
-      prompt_block_rows(p, b, h, L, jj, values, rows, table);
-      if (quantises) quantise_rows<TYPE>(c, bh, jj, values, rows, red);
-      if (keeps) rows_to_tail(c, bh, jj, values, L, end, rows);
+      const Rows r = prompt_rows(p, b, h, L, jj, values, lds, table);
+      if (quantises) store_codes<TYPE>(c, bh, jj, values, r, lds, red);
+      if (keeps) store_tail(c, bh, jj, values, r, L, end, lds);
     }
     return;
   }
@@ -369,11 +403,11 @@ struct LoadParams {
   int S, nb;
 };
 
-// Workgroup (block j, keys or values, head): 64 rows to LDS, codes if the block is
-// complete, the tail if it is one of the last two.
+// Workgroup (block j, keys or values, head): codes if the block is complete, the tail
+// if it is one of the last two.
 template <int TYPE>
 __global__ __launch_bounds__(256) void kv8_load_kernel(const LoadParams p) {
-  __shared__ __attribute__((aligned(16))) uint16_t rows[kBlk][kRow];
+  __shared__ __attribute__((aligned(16))) Turn lds;
   __shared__ uint32_t red[4];
   const Kv8& c = p.c;
   const int j = (int)(blockIdx.x % p.nb);
@@ -385,14 +419,12 @@ __global__ __launch_bounds__(256) void kv8_load_kernel(const LoadParams p) {
   if (kBlk * j >= n) return;
   const int64_t* st = values ? p.vs : p.ks;
   const uint16_t* src = (values ? p.v : p.k) + b * st[0] + h * st[1];
+  Rows r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = threadIdx.x + 256 * i, pos = min(kBlk * j + (e >> 4), n - 1);
-    *reinterpret_cast<u32x4*>(&rows[e >> 4][(e & 15) * 8]) = ld16(src + pos * st[2] + (e & 15) * 8);
-  }
-  __syncthreads();
-  if (j < n >> 6) quantise_rows<TYPE>(c, bh, j, values, rows, red);
-  if (j >= (n >> 6) - 1) rows_to_tail(c, bh, j, values, 0, n, rows);
+  for (int i = 0; i < 4; ++i)
+    r.x[i] = ld16(src + min(kBlk * j + (int)(threadIdx.x >> 4) + 16 * i, n - 1) * st[2] + 8 * (threadIdx.x & 15));
+  if (j < n >> 6) store_codes<TYPE>(c, bh, j, values, r, lds, red);
+  if (j >= (n >> 6) - 1) store_tail(c, bh, j, values, r, 0, n, lds);
 }
 
 // -------------------------------------------------------------------- read
@@ -405,12 +437,12 @@ struct ReadParams {
   uint16_t* v;
 };
 
-// Workgroup (block of positions, keys or values, head): a thread takes 32
-// neighbouring values in stored order, codes or tail, as bf16; the values' rows
-// turn through LDS.
+// Workgroup (block of positions, keys or values, head).  A block's rows come from its
+// codes (values turned by 4 features x 8 positions a thread) or from the tail, and go
+// out as whole rows, 16 bytes a lane.
 template <int TYPE>
 __global__ __launch_bounds__(256) void kv8_read_kernel(const ReadParams p) {
-  __shared__ __attribute__((aligned(16))) uint16_t rows[kBlk][kRow];
+  __shared__ __attribute__((aligned(16))) Turn lds;
   __shared__ uint32_t red[4];
   const Kv8& c = p.c;
   const int i = (int)(blockIdx.x % p.nb);
@@ -423,62 +455,79 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const ReadParams p) {
   const int L = p.lens[b];
   const int held = min(max(L, 0), c.Smax);
   const int64_t start = (int64_t)p.start + (p.starts ? p.starts[b] : 0);
-  // block j = floor(start / 64) + i covers the outputs 64 j - start ..
-  const int64_t j = (start >> 6) + i;
-  if (kBlk * j >= start + p.count) return;
-  u32x4 w[4];
+  // block floor(start / 64) + i covers the outputs 64 block - start ..
+  const int64_t block = (start >> 6) + i;
+  if (kBlk * block >= start + p.count) return;
+  Rows r;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) w[u] = u32x4{0u, 0u, 0u, 0u};
-  if (j >= 0 && kBlk * j < held) {
+  for (int u = 0; u < 4; ++u) r.x[u] = u32x4{0u, 0u, 0u, 0u};
+  if (block >= 0 && kBlk * block < held) {
+    const int j = (int)block;
     const bool waits = j == (held >> 6) - 1 && may_wait(L, c.Smax);
     if (j < held >> 6 && !waits) {
-      const uint8_t* src = (values ? c.values(bh, (int)j) : c.keys(bh, (int)j)) + 32 * t;
       const float s = (values ? c.vs : c.ks)[bh * c.nblk + j];
-      const u32x4 q[2] = {ld16(src), ld16(src + 16)};
+      u32x2 q[4];
+      if (!values) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const f32x4 f = codes_f32<TYPE>(q[u >> 2][u & 3]) * s;
-        w[u >> 1][2 * (u & 1)] = pack2(f.x, f.y);
-        w[u >> 1][2 * (u & 1) + 1] = pack2(f.z, f.w);
-      }
-    } else {
-      const int at = ((int)j & 1) * kBlk;
-      const uint16_t* src = values ? c.tail_values(bh) + (t >> 1) * kSlots + at + (t & 1) * 32
-                                   : c.tail_keys(bh) + (at + (t >> 2)) * kHD + (t & 3) * 32;
-      uint32_t a = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        w[u] = ld16(src + 8 * u);
-        a = max(a, abs_bits16(w[u]));
-      }
-      if (waits) {
-        const f32x2 sm = block_scale<TYPE>(group_max_u32(a, red));
+        for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const u32x2*>(c.keys(bh, j) + 8 * (t + 256 * u));
+      } else {
+        const int p0 = 8 * (t & 7), quad = t >> 3;
+        uint32_t w[8];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const u32x2 q = quantise8<TYPE>(w[u], sm.y);
-          const f32x4 lo = codes_f32<TYPE>(q.x) * sm.x, hi = codes_f32<TYPE>(q.y) * sm.x;
-          w[u] = u32x4{pack2(lo.x, lo.y), pack2(lo.z, lo.w), pack2(hi.x, hi.y), pack2(hi.z, hi.w)};
+          const u32x2 x = *reinterpret_cast<const u32x2*>(c.values(bh, j) + (4 * quad + u) * kBlk + p0);
+          w[u] = x.x;
+          w[4 + u] = x.y;
         }
+        transpose4(w[0], w[1], w[2], w[3]);
+        transpose4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) lds.codes[p0 + u][quad] = w[u];
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t* src = &lds.codes[(t >> 4) + 16 * u][2 * (t & 15)];
+          q[u] = u32x2{src[0], src[1]};
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) r.x[u] = values_bf16<TYPE>(q[u], s);
+    } else {
+      const int at = (j & 1) * kBlk;
+      if (!values) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          r.x[u] = ld16(c.tail_keys(bh) + (at + (t >> 4) + 16 * u) * kHD + 8 * (t & 15));
+      } else {
+        const uint16_t* src = c.tail_values(bh) + (t >> 1) * kSlots + at + (t & 1) * 32;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const u32x4 w = ld16(src + 8 * u);
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            lds.rows[(t & 1) * 32 + 8 * u + x][t >> 1] = (uint16_t)(w[x >> 1] >> (16 * (x & 1)));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) r.x[u] = *reinterpret_cast<const u32x4*>(&lds.rows[(t >> 4) + 16 * u][8 * (t & 15)]);
+      }
+      if (waits) {  // as it will read once it has its codes
+        uint32_t a = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) a = max(a, abs_bits16(r.x[u]));
+        const f32x2 sm = block_scale<TYPE>(group_max_u32(a, red));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) r.x[u] = values_bf16<TYPE>(quantise8<TYPE>(r.x[u], sm.y), sm.x);
       }
     }
   }
-  if (values) {
 #pragma unroll
-    for (int u = 0; u < 32; ++u)
-      rows[(t & 1) * 32 + u][t >> 1] = (uint16_t)(w[u >> 3][(u >> 1) & 3] >> (16 * (u & 1)));
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const u32x4*>(&rows[t >> 2][(t & 3) * 32 + 8 * u]);
+  for (int u = 0; u < 4; ++u) {
+    const int64_t pos = kBlk * block + (t >> 4) + 16 * u, o = pos - start;
+    if (o < 0 || o >= p.count) continue;
+    *reinterpret_cast<u32x4*>(out + (bh * p.count + o) * kHD + 8 * (t & 15)) =
+        pos < held ? r.x[u] : u32x4{0u, 0u, 0u, 0u};
   }
-  const int64_t pos = kBlk * j + (t >> 2), o = pos - start;
-  if (o < 0 || o >= p.count) return;
-  if (pos >= held) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = u32x4{0u, 0u, 0u, 0u};
-  }
-  uint16_t* dst = out + (bh * p.count + o) * kHD + (t & 3) * 32;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) *reinterpret_cast<u32x4*>(dst + 8 * u) = w[u];
 }
 
 bool fits_grid(int64_t wgs) { return wgs <= INT32_MAX; }

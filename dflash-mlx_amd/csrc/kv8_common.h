@@ -122,6 +122,14 @@ __device__ __forceinline__ u32x2 codes_bf16(uint32_t c) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true))};
 }
 
+// What eight codes stand for, rounded to bf16.
+template <int TYPE>
+__device__ __forceinline__ u32x4 values_bf16(u32x2 q, float scale) {
+  const f32x4 a = codes_f32<TYPE>(q.x) * scale, b = codes_f32<TYPE>(q.y) * scale;
+  const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  return cvt8_bf16(f);
+}
+
 // Largest magnitude's bits of two packed bf16, as fp32 bits.
 __device__ __forceinline__ uint32_t abs_bits2(uint32_t w) {
   return max(w & 0x7fff0000u, (w << 16) & 0x7fff0000u);
