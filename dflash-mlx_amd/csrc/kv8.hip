@@ -188,6 +188,8 @@ __device__ __forceinline__ void rotation_table(float* table, int pos0, const App
   }
 }
 
+constexpr int kDppQuadReverse = 0x1B;  // quad_perm [3,2,1,0]
+
 // RMSNorm and rotary of a row's eight features at lane f: cosines cs[rot / 2], sines
 // sn[rot / 2].  fp32 throughout, rounded to bf16 once.
 __device__ __forceinline__ u32x4 norm_rotate8(u32x4 xw, u32x4 ww, const float* cs, const float* sn, int f, int rot,
@@ -202,15 +204,33 @@ __device__ __forceinline__ u32x4 norm_rotate8(u32x4 xw, u32x4 ww, const float* c
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
   if (rot > 0) {
+    // the other half of the pair: lane f ^ (rot / 16) of the row
     float y[8];
+    if (rot == 32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __shfl_xor(x[i], rot >> 4, 64);
+      for (int i = 0; i < 8; ++i) y[i] = dpp_mov<kDppQuadSwap2>(x[i]);
+    } else if (rot == 16) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = dpp_mov<kDppQuadSwap1>(x[i]);
+    } else if (rot == 64) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = dpp_mov<kDppQuadReverse>(dpp_mov<kDppRowHalfMirror>(x[i]));  // f ^ 7 ^ 3
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = dpp_mov<kDppRowHalfMirror>(dpp_mov<kDppRowMirror>(x[i]));  // f ^ 15 ^ 7
+    }
     if (8 * f < rot) {
       const int half = rot >> 1;
       const bool low = 8 * f < half;
       const int i0 = low ? 8 * f : 8 * f - half;
+      f32x4 c[2], s[2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i0 + i], (low ? -y[i] : y[i]) * sn[i0 + i]);
+      for (int i = 0; i < 2; ++i) {
+        c[i] = *reinterpret_cast<const f32x4*>(cs + i0 + 4 * i);
+        s[i] = *reinterpret_cast<const f32x4*>(sn + i0 + 4 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], c[i >> 2][i & 3], (low ? -y[i] : y[i]) * s[i >> 2][i & 3]);
     }
   }
   return cvt8_bf16(x);
@@ -226,7 +246,7 @@ __device__ __forceinline__ u32x4 norm_rotate8(u32x4 xw, u32x4 ww, const float* c
 template <int TYPE>
 __global__ __launch_bounds__(256) void kv8_append_draft_kernel(const AppendParams p) {
   __shared__ uint32_t red[4];
-  __shared__ float table[kHD];
+  __shared__ __attribute__((aligned(16))) float table[kHD];
   const Kv8& c = p.c;
   const int nquant = 2 * c.B * c.Hkv;
   if ((int)blockIdx.x < nquant) {
