@@ -858,13 +858,13 @@ struct PrefillParams {
 
 constexpr int kPRows = 32;                     // query rows of a wave
 constexpr int kPKeys = 2 * kBlk;               // keys of a turn
-constexpr int kPBuf = 2 * kPKeys * kHD * 2;    // bytes of one turn's K and V^T in bf16
+constexpr int kPHalf = kPKeys * kHD * 2;       // bytes of one turn's K (or V^T) in bf16
 constexpr int kPMerge = 66 * 64;               // floats of a wave's O, m and l
 constexpr int kPPitch = kHD + 4;               // floats of a normalized row in LDS
 
 constexpr int prefill_lds(int pairs) {
   const int merge = 4 * pairs * (kPMerge + kPRows * kPPitch);
-  return merge > 2 * kPBuf ? merge : 2 * kPBuf;
+  return merge > 4 * kPHalf ? merge : 4 * kPHalf;
 }
 
 template <int TYPE, int REP, int RB>
@@ -898,165 +898,202 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
   const int turns = len < 0 ? 0 : (min(base + min(t0 + RB * kPRows, p.P), c.Smax) + kPKeys - 1) / kPKeys;
   const int Lw = len >= 0 && (RB == 1 || tw < p.P) ? min(base + min(tw + kPRows, p.P), c.Smax) : 0;
   if (tid == 0) dropped = 0;
-  u32x4 kv[PER][2], vv[PER][2];
+  u32x4 kv[PER], vv[PER];
   // K unit e: key e / 8, features 16 (e % 8) ..; V^T unit e: block e / 512, feature
   // (e / 4) % 128, keys 16 (e % 4) ..  Blocks past the cache's last are clamped.
-  auto load_turn = [&](int turn) {
+  auto unit_of = [&](int i) { return min(tid + NT * i, UNITS - 1); };
+  auto block_of = [&](int turn, int e) { return min(2 * turn + (e >> 9), c.nblk - 1); };
+  auto load_keys = [&](int turn, u32x4 (&kv)[PER]) {
+    if (turn >= turns) return;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int e = min(tid + NT * i, UNITS - 1);
-      const int j = min(2 * turn + (e >> 9), c.nblk - 1);
-      const int key = (e >> 3) & 63, d = (e >> 2) & 127;
-      if (j < done) {
-        kv[i][0] = ld16(c.keys(bh, j) + key * kHD + (e & 7) * 16);
-        vv[i][0] = ld16(c.values(bh, j) + d * kBlk + (e & 3) * 16);
-      } else {
-        const int at = (j & 1) * kBlk;
-        const uint16_t* ks = c.tail_keys(bh) + (at + key) * kHD + (e & 7) * 16;
-        const uint16_t* vs = c.tail_values(bh) + d * kSlots + at + (e & 3) * 16;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          kv[i][u] = ld16(ks + 8 * u);
-          vv[i][u] = ld16(vs + 8 * u);
-        }
-      }
+      const int e = unit_of(i), j = block_of(turn, e);
+      if (j < done) kv[i] = ld16(c.keys(bh, j) + 16 * (e & 511));
     }
   };
-  auto store_turn = [&](unsigned char* buf, int turn) {
+  auto load_values = [&](int turn) {
+    if (turn >= turns) return;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = unit_of(i), j = block_of(turn, e);
+      if (j < done) vv[i] = ld16(c.values(bh, j) + 16 * (e & 511));
+    }
+  };
+  auto store_pair = [&](unsigned char* row, int piece, int swizzle, u32x4 x, u32x4 y) {
+    *reinterpret_cast<u32x4*>(row + ((piece ^ swizzle) << 4)) = x;
+    *reinterpret_cast<u32x4*>(row + (((piece + 1) ^ swizzle) << 4)) = y;
+  };
+  auto store_keys = [&](int turn, const u32x4 (&kv)[PER]) {
+    if (turn >= turns) return;
+    unsigned char* buf = lds + (turn & 1) * kPHalf;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = tid + NT * i;
       if (UNITS % NT != 0 && e >= UNITS) continue;
-      const int j = min(2 * turn + (e >> 9), c.nblk - 1);
-      const int key = e >> 3, d = (e >> 2) & 127;
-      u32x4 kw[2], vw[2];
+      const int j = block_of(turn, e), key = e >> 3;
+      unsigned char* row = buf + key * 256;
       if (j < done) {
+        u32x2 x[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const u32x2 x = codes_bf16<TYPE>(kv[i][0][u]), y = codes_bf16<TYPE>(vv[i][0][u]);
-          kw[u >> 1][2 * (u & 1)] = x.x;
-          kw[u >> 1][2 * (u & 1) + 1] = x.y;
-          vw[u >> 1][2 * (u & 1)] = y.x;
-          vw[u >> 1][2 * (u & 1) + 1] = y.y;
-        }
+        for (int u = 0; u < 4; ++u) x[u] = codes_bf16<TYPE>(kv[i][u]);
+        store_pair(row, 2 * (e & 7), key & 7, u32x4{x[0].x, x[0].y, x[1].x, x[1].y}, u32x4{x[2].x, x[2].y, x[3].x, x[3].y});
       } else {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          kw[u] = kv[i][u];
-          vw[u] = drop_nonfinite(vv[i][u]);
-        }
-        if (any_nonfinite(nonfinite_bits(vv[i][0]) | nonfinite_bits(vv[i][1]))) dropped = 1;
+        const uint16_t* src = c.tail_keys(bh) + ((j & 1) * kBlk + (key & 63)) * kHD + (e & 7) * 16;
+        store_pair(row, 2 * (e & 7), key & 7, ld16(src), ld16(src + 8));
       }
-      unsigned char* krow = buf + key * 256;
-      const int c0 = 2 * (e & 7), sk = key & 7;
-      *reinterpret_cast<u32x4*>(krow + ((c0 ^ sk) << 4)) = kw[0];
-      *reinterpret_cast<u32x4*>(krow + (((c0 + 1) ^ sk) << 4)) = kw[1];
-      // 16 keys: the first piece keeps 0-3 and 8-11 (hl = 0), the second 4-7 and 12-15
-      unsigned char* vrow = buf + kPBuf / 2 + (e >> 9) * (kHD * 128) + d * 128;
-      const int c1 = 2 * (e & 3), sv = d & 7;
-      *reinterpret_cast<u32x4*>(vrow + ((c1 ^ sv) << 4)) = u32x4{vw[0].x, vw[0].y, vw[1].x, vw[1].y};
-      *reinterpret_cast<u32x4*>(vrow + (((c1 + 1) ^ sv) << 4)) = u32x4{vw[0].z, vw[0].w, vw[1].z, vw[1].w};
     }
   };
-  load_turn(0);
+  auto store_values = [&](int turn) {
+    if (turn >= turns) return;
+    unsigned char* buf = lds + 2 * kPHalf + (turn & 1) * kPHalf;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = tid + NT * i;
+      if (UNITS % NT != 0 && e >= UNITS) continue;
+      const int j = block_of(turn, e), d = (e >> 2) & 127;
+      unsigned char* row = buf + (e >> 9) * (kHD * 128) + d * 128;
+      // 16 keys: the first piece keeps 0-3 and 8-11 (hl = 0), the second 4-7 and 12-15
+      if (j < done) {
+        u32x2 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = codes_bf16<TYPE>(vv[i][u]);
+        store_pair(row, 2 * (e & 3), d & 7, u32x4{x[0].x, x[0].y, x[2].x, x[2].y}, u32x4{x[1].x, x[1].y, x[3].x, x[3].y});
+      } else {
+        const uint16_t* src = c.tail_values(bh) + d * kSlots + (j & 1) * kBlk + (e & 3) * 16;
+        const u32x4 v0 = ld16(src), v1 = ld16(src + 8);
+        if (any_nonfinite(nonfinite_bits(v0) | nonfinite_bits(v1))) dropped = 1;
+        const u32x4 x = drop_nonfinite(v0), y = drop_nonfinite(v1);
+        store_pair(row, 2 * (e & 3), d & 7, u32x4{x.x, x.y, y.x, y.y}, u32x4{x.z, x.w, y.z, y.w});
+      }
+    }
+  };
+  u32x4 kv1[PER];
+  load_keys(0, kv);
+  load_values(0);
+  load_keys(1, kv1);
   const QuerySign sign(p.scale);
   const uint16_t* qr = p.q + (((int64_t)b * p.P + min(tw + r32, p.P - 1)) * p.Hq + qh) * kHD + hl * 8;
   u32x4 qb[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) qb[k] = sign(ld16(qr + 16 * k));
   __syncthreads();  // dropped is 0
-  store_turn(lds, 0);
-  if (turns > 1) load_turn(1);
+  store_keys(0, kv);
+  store_values(0);
+  store_keys(1, kv1);
+  load_keys(2, kv);
+  load_values(1);
   float m = -INFINITY, l = 0.f;
   f32x16 o[4];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) o[dt] = f32x16{};
   const float sl0 = positive_scale(p.scale);
   const int last = min(base + tw + r32, Lw - 1);  // the last key this lane's row sees
-  __syncthreads();
-  for (int j = 0; j < turns; ++j) {
-    const unsigned char* buf = lds + (j & 1) * kPBuf;
-    const int kb = 2 * j + hf, k0 = kBlk * kb;
-    float ks = 1.f, vs = 1.f;
+  f32x16 st[2];
+  u32x4 pb[4];
+  float ks = 1.f, vs = 1.f;  // of the block whose scores are in st
+  auto sees = [&](int turn) { return kBlk * (2 * turn + hf) < Lw; };
+  auto scores = [&](int turn) {
+    const int kb = 2 * turn + hf;
+    ks = vs = 1.f;
     if (kb < done) {
       ks = c.ks[bh * c.nblk + kb];
       vs = c.vs[bh * c.nblk + kb];
     }
-    if (j + 1 < turns) {
-      store_turn(lds + ((j + 1) & 1) * kPBuf, j + 1);
-      if (j + 2 < turns) load_turn(j + 2);
+    const unsigned char* sk = lds + (turn & 1) * kPHalf + 64 * hf * 256;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      st[kt] = f32x16{};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
+                                           sk + (32 * kt + r32) * 256 + (((2 * k + hl) ^ (r32 & 7)) << 4))),
+            __builtin_bit_cast(bf16x8, qb[k]), st[kt], 0, 0, 0);
     }
-    if (k0 < Lw) {
-      const unsigned char* sk = buf + 64 * hf * 256;
-      const unsigned char* sv = buf + kPBuf / 2 + hf * (kHD * 128);
-      const float sl = sl0 * ks, lv = __log2f(vs), iv = __builtin_amdgcn_rcpf(vs);
-      f32x16 st[2];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        st[kt] = f32x16{};
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
-                                             sk + (32 * kt + r32) * 256 + (((2 * k + hl) ^ (r32 & 7)) << 4))),
-              __builtin_bit_cast(bf16x8, qb[k]), st[kt], 0, 0, 0);
-      }
-      const bool masked = k0 + 63 > base + tw;  // some row does not see the whole block
-      if (masked) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = k0 + 32 * kt + 8 * (i >> 2) + 4 * hl + (i & 3);
-            if (key > last) st[kt][i] = -INFINITY;
-          }
-      }
-      float mx = st[0][0];
+  };
+  auto softmax = [&](int turn) {
+    const int k0 = kBlk * (2 * turn + hf);
+    const float sl = sl0 * ks, lv = __log2f(vs), iv = __builtin_amdgcn_rcpf(vs);
+    const bool masked = k0 + 63 > base + tw;  // some row does not see the whole block
+    if (masked) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[kt][i]);
-      const f32x2 mb = both_halves(mx);
-      mx = fmaf(fmaxf(mb.x, mb.y), sl, lv);
-      if (__any(mx > m)) {
-        const float mn = fmaxf(m, mx);
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        l *= alpha;
+        for (int i = 0; i < 16; ++i)
+          if (k0 + 32 * kt + 8 * (i >> 2) + 4 * hl + (i & 3) > last) st[kt][i] = -INFINITY;
+    }
+    float mx = st[0][0];
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
-        m = mn;
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[kt][i]);
+    const f32x2 mb = both_halves(mx);
+    mx = fmaf(fmaxf(mb.x, mb.y), sl, lv);
+    if (__any(mx > m)) {
+      const float mn = fmaxf(m, mx);
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
+      m = mn;
+    }
+    const float off = lv - (m == -INFINITY ? 0.f : m);
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float pe[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        pe[i] = __builtin_amdgcn_exp2f(fmaf(st[s >> 1][8 * (s & 1) + i], sl, off));
+        sum += pe[i];
       }
-      const float off = lv - (m == -INFINITY ? 0.f : m);
-      float sum = 0.f;
-      u32x4 pb[4];
+      pb[s] = cvt8_bf16(pe);
+    }
+    if (masked && !(sl + off == sl + off) && k0 > last) {
+      // a block that reads as NaN, past the row's last key: its weights are NaN here, not 0
+      sum = 0.f;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        float pe[8];
+      for (int s = 0; s < 4; ++s) pb[s] = u32x4{0u, 0u, 0u, 0u};
+    }
+    l = fmaf(sum, iv, l);
+  };
+  auto outputs = [&](int turn) {
+    const unsigned char* sv = lds + 2 * kPHalf + (turn & 1) * kPHalf + hf * (kHD * 128);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          pe[i] = __builtin_amdgcn_exp2f(fmaf(st[s >> 1][8 * (s & 1) + i], sl, off));
-          sum += pe[i];
-        }
-        pb[s] = cvt8_bf16(pe);
-      }
-      if (masked && !(sl + off == sl + off)) {
-        // a block that reads as NaN, past some rows' last key: nothing of it for a row
-        // that does not see it (its whole weight is NaN here, not 0)
-        if (k0 > last) {
-          sum = 0.f;
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-          for (int s = 0; s < 4; ++s) pb[s] = u32x4{0u, 0u, 0u, 0u};
-        }
-      }
-      l = fmaf(sum, iv, l);
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
-                                             sv + (32 * dt + r32) * 128 + (((2 * s + hl) ^ (r32 & 7)) << 4))),
-              __builtin_bit_cast(bf16x8, pb[s]), o[dt], 0, 0, 0);
+      for (int dt = 0; dt < 4; ++dt)
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
+                                           sv + (32 * dt + r32) * 128 + (((2 * s + hl) ^ (r32 & 7)) << 4))),
+            __builtin_bit_cast(bf16x8, pb[s]), o[dt], 0, 0, 0);
+  };
+  // K j + 2 and V j + 1 to LDS: the buffers of K j and V j - 1, both read in turn j - 1
+  auto stage = [&](int j) {
+    store_keys(j + 2, kv);
+    store_values(j + 1);
+    load_keys(j + 3, kv);
+    load_values(j + 2);
+  };
+  __syncthreads();
+  if (sees(0)) {
+    scores(0);
+    if (hf == 1) softmax(0);
+  }
+  __syncthreads();  // K 0 is read: its buffer takes K 2
+  // Turn j: the products of K j + 1 and V j.  The first half's waves do their softmax and
+  // staging before them, the second half's after: a SIMD holds one wave of each, and the
+  // matrix unit has one's products beside the other's arithmetic.
+  for (int j = 0; j < turns; ++j) {
+    if (hf == 0) {
+      if (sees(j)) softmax(j);
+      stage(j);
+    }
+    if (sees(j)) outputs(j);
+    if (j + 1 < turns && sees(j + 1)) scores(j + 1);
+    if (hf == 1) {
+      if (j + 1 < turns && sees(j + 1)) softmax(j + 1);
+      stage(j);
     }
     __syncthreads();
   }
