@@ -35,6 +35,7 @@ from .kv8 import (
     attn_verify_q8_workspace_bytes,
     kv_load_q8,
     kv_read_q8,
+    kv_rewind_q8,
 )
 from .runtime import (
     DFlashRuntimeEvent,
@@ -85,6 +86,7 @@ __all__ = [
     "greedy_accept",
     "kv_load_q8",
     "kv_read_q8",
+    "kv_rewind_q8",
     "lm_head_argmax",
     "lm_head_greedy_accept",
     "longest_prefix_match",

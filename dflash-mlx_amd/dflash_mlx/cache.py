@@ -55,6 +55,9 @@ class KVCache:
         self.offset = need
         return self.keys[:, :, :need], self.values[:, :, :need]
 
+    def prepare(self) -> None:
+        """Called before a forward that appends at ``offset``."""
+
     def is_trimmable(self) -> bool:
         return True
 

@@ -44,6 +44,7 @@ import torch
 
 from . import _lib
 from .gdn_layer import QK_NORM_EPS, GatedDeltaConfig, GatedDeltaWeights
+from .kv8 import QuantizedKVCache, attn_verify_q8_workspace_bytes, kv_load_q8
 
 
 @dataclass(frozen=True)
@@ -206,7 +207,7 @@ class HybridVerifyRunner:
 
     def __init__(self, cfg: HybridConfig, weights: HybridWeights, B: int, T: int, Smax: int,
                  device: torch.device, weight_layout: str = "tiled", fused_prologue: bool = True,
-                 fused_norms: bool = True):
+                 fused_norms: bool = True, kv_dtype: torch.dtype = torch.bfloat16):
         """weight_layout: "tiled" streams weights re-laid out once as MFMA
         fragments (dflash_weight_tile_bf16, cached in the layer dicts as
         "<name>_tiled"; same sums bit for bit) wherever the row count is a
@@ -271,12 +272,23 @@ class HybridVerifyRunner:
         # attention layers: KV caches (zero-filled: positions past the live
         # length are read with zero weight and must stay finite)
         self.aproj = e(M, cfg.attn_proj_rows)
-        self.k_cache = [z(B, Hkv, Smax, D) for _ in range(na)]
-        self.vt_cache = [z(B, Hkv, D, Smax) for _ in range(na)]
+        self.kv_dtype = kv_dtype
+        self.k_cache, self.vt_cache, self.kv = [], [], []
+        if kv_dtype is bf:
+            self.k_cache = [z(B, Hkv, Smax, D) for _ in range(na)]
+            self.vt_cache = [z(B, Hkv, D, Smax) for _ in range(na)]
+        else:
+            if D != 128:
+                raise ValueError(f"a cache in 8 bits needs attention heads of 128, got {D}")
+            self.kv = [QuantizedKVCache.zeros(B, Hkv, Smax, kv_dtype, device) for _ in range(na)]
         self.q = e(B, T, Hq, D)
         self.attn_out = e(M, Hq * D)
         lib = _lib.load()
-        self.attn_ws = e(int(lib.dflash_attn_verify_workspace_bytes(B, Hq, Hkv, Smax)), dt=torch.uint8)
+        if kv_dtype is bf:
+            ws = int(lib.dflash_attn_verify_workspace_bytes(B, Hq, Hkv, Smax))
+        else:
+            ws = max(attn_verify_q8_workspace_bytes(B, t, Hq, Hkv, Smax) for t in range(1, T + 1))
+        self.attn_ws = e(ws, dt=torch.uint8)
         # accept / commit
         self.lens = z(B, dt=i32)
         self.keep = z(B, dt=i32)  # 0: the first step starts from `state`
@@ -534,18 +546,30 @@ class HybridVerifyRunner:
                 if self.splits["w_qkv"]:
                     fwd.append(("dflash_splitk_reduce", (pp, self.splits["w_qkv"], M, arows,
                                                          self.aproj.data_ptr(), arows)))
-                fwd.append(("dflash_attn_prep",
-                            (self.aproj.data_ptr(), arows, lw["q_norm"].data_ptr(),
-                             lw["k_norm"].data_ptr(), self.lens.data_ptr(),
-                             self.k_cache[ai].data_ptr(), self.vt_cache[ai].data_ptr(),
-                             self.q.data_ptr(), self.overflow.data_ptr(), B, T, Hq, Hkv, D,
-                             self.Smax, cfg.rot_dims, float(cfg.rope_theta), eps)))
-                fwd.append(("dflash_attn_verify",
-                            (self.q.data_ptr(), self.k_cache[ai].data_ptr(),
-                             self.vt_cache[ai].data_ptr(), self.lens.data_ptr(),
-                             self.aproj.data_ptr(), arows, self.attn_out.data_ptr(), B, T, Hq, Hkv,
-                             D, self.Smax, self.Smax, float(D ** -0.5), self.attn_ws.data_ptr(),
-                             self.attn_ws.numel())))
+                if self.kv:
+                    kv = self.kv[ai]
+                    fwd.append(("dflash_kv8_append",
+                                (kv._ptr, self.aproj.data_ptr(), arows, lw["q_norm"].data_ptr(),
+                                 lw["k_norm"].data_ptr(), self.lens.data_ptr(), self.q.data_ptr(),
+                                 self.overflow.data_ptr(), T, Hq, cfg.rot_dims, float(cfg.rope_theta),
+                                 eps, 0)))
+                    fwd.append(("dflash_attn_verify_q8",
+                                (kv._ptr, self.q.data_ptr(), self.lens.data_ptr(),
+                                 self.aproj.data_ptr(), arows, self.attn_out.data_ptr(), T, Hq,
+                                 float(D ** -0.5), self.attn_ws.data_ptr(), self.attn_ws.numel())))
+                else:
+                    fwd.append(("dflash_attn_prep",
+                                (self.aproj.data_ptr(), arows, lw["q_norm"].data_ptr(),
+                                 lw["k_norm"].data_ptr(), self.lens.data_ptr(),
+                                 self.k_cache[ai].data_ptr(), self.vt_cache[ai].data_ptr(),
+                                 self.q.data_ptr(), self.overflow.data_ptr(), B, T, Hq, Hkv, D,
+                                 self.Smax, cfg.rot_dims, float(cfg.rope_theta), eps)))
+                    fwd.append(("dflash_attn_verify",
+                                (self.q.data_ptr(), self.k_cache[ai].data_ptr(),
+                                 self.vt_cache[ai].data_ptr(), self.lens.data_ptr(),
+                                 self.aproj.data_ptr(), arows, self.attn_out.data_ptr(), B, T, Hq, Hkv,
+                                 D, self.Smax, self.Smax, float(D ** -0.5), self.attn_ws.data_ptr(),
+                                 self.attn_ws.numel())))
                 if post:
                     fwd.append(self._residual_norm_op(lw, "w_o", self.attn_out, M, None))
                 else:
@@ -608,15 +632,28 @@ class HybridVerifyRunner:
         keys / values [B,Hkv,S<=Smax,D] (positions >= S are zeroed).  Clears the
         pending accept (the next step starts from `rec`) and the overflow
         flags.  Raises unless 0 <= lens[b] and lens[b] + T <= Smax, the room
-        the next block's keys need."""
-        self.lens.copy_(check_cache_lengths(lens, self.B, self.T, self.Smax))
+        the next block's keys need.  Caches in 8 bits take lengths above 0 only
+        with their keys and values (their tails follow the length)."""
+        checked = check_cache_lengths(lens, self.B, self.T, self.Smax)
+        if self.kv and k is None and self.B and int(checked.max()) > 0:
+            raise ValueError("the lengths of caches in 8 bits are set with their keys and values")
+        self.lens.copy_(checked)
         self.keep.zero_()
         self.overflow.zero_()
         for dst, src in ((self.conv, conv), (self.state, rec)):
             if src is not None:
                 for d_, s_ in zip(dst, src):
                     d_.copy_(s_)
-        if k is not None:
+        if k is not None and self.kv:
+            for kv, kk, vv in zip(self.kv, k, v):
+                S = kk.shape[2]
+                if S > self.Smax:
+                    raise ValueError(f"{S} cached positions exceed Smax = {self.Smax}")
+                pad = max(0, int(checked.max()) - S)
+                kk, vv = (torch.nn.functional.pad(t, (0, 0, 0, pad)).to(self.device, torch.bfloat16)
+                          for t in (kk, vv))
+                kv_load_q8(kk, vv, self.lens, kv)
+        elif k is not None:
             for kc, vc, kk, vv in zip(self.k_cache, self.vt_cache, k, v):
                 S = kk.shape[2]
                 if S > self.Smax:

@@ -5,9 +5,11 @@ contexts; a cache in 8 bits halves them (and the memory).  ``QuantizedKVCache``
 holds complete blocks of 64 positions as int8 or e4m3 codes with one fp32
 scale per block and head, keys and values apart, and the latest two blocks of
 positions in bf16 (the tail).  A block gets its codes only once all its
-positions are committed, from the tail: its scale never depends on draft
-tokens that are rejected later, so speculative decoding over this cache still
-gives the tokens that the target alone would give over it.
+positions are committed, from the tail: what the cache holds of the kept
+tokens never depends on draft tokens that were rejected.  A step at committed
+length L reads the blocks below L // 64 from their codes, so a token that ends a
+block is read in bf16 by the steps that start before its end and from its code
+by those after.
 
 The ops take the place of the bf16 cache's append (q/k RMSNorm, rotary, KV
 append; custom_qwen35_model.py:496-522) and attention (causal SDPA over the
@@ -90,7 +92,7 @@ class QuantizedKVCache:
 
     @classmethod
     def zeros(cls, B: int, Hkv: int, Smax: int, dtype: torch.dtype, device) -> "QuantizedKVCache":
-        """An empty cache (1.016 bytes a value and 64 KB of tail a sequence and head)."""
+        """An empty cache: every position reads as zero."""
         if dtype not in _TYPES:
             raise TypeError(f"codes must be int8 or float8_e4m3fn, got {dtype}")
         if B < 0 or Hkv <= 0 or Smax <= 0 or Smax % BLOCK:
@@ -98,8 +100,9 @@ class QuantizedKVCache:
         nb, D, bf = Smax // BLOCK, HEAD_DIM, torch.bfloat16
         z = lambda dt, *s: torch.zeros(*s, dtype=dt, device=device)  # noqa: E731
         codes = lambda *s: z(torch.uint8, *s).view(dtype)  # noqa: E731
-        return cls(codes(B, Hkv, Smax, D), codes(B, Hkv, nb, D, BLOCK), z(torch.float32, B, Hkv, nb),
-                   z(torch.float32, B, Hkv, nb), z(bf, B, Hkv, SLOTS, D), z(bf, B, Hkv, D, SLOTS))
+        ones = lambda: torch.ones(B, Hkv, nb, dtype=torch.float32, device=device)  # noqa: E731
+        return cls(codes(B, Hkv, Smax, D), codes(B, Hkv, nb, D, BLOCK), ones(), ones(), z(bf, B, Hkv, SLOTS, D),
+                   z(bf, B, Hkv, D, SLOTS))
 
     def __repr__(self):
         return f"QuantizedKVCache({self.dtype}, B={self.B}, Hkv={self.Hkv}, Smax={self.Smax}, {self.device})"
@@ -292,3 +295,37 @@ def kv_read_q8(cache: QuantizedKVCache, lens, count: int, *, start=0):
     _call("dflash_kv8_read", cache.device, cache._ptr, lens.data_ptr(), _lib.ptr(starts), int(start), count,
           k.data_ptr(), v.data_ptr())
     return k, v
+
+
+def kv_rewind_q8(cache: QuantizedKVCache, length: int, written: int) -> int:
+    """Make the tail ready for a call at committed length `length` of every sequence
+    after positions up to `written` - 1 have been appended (rejected drafts
+    included): what the call reads from the tail and later positions have
+    overwritten comes back from the codes, rounded to bf16.  Returns what to pass as
+    `written` next time, with the positions appended from here on.  Nothing is
+    launched for the rewinds of a decode loop."""
+    _check_cache(cache)
+    length, written = int(length), int(written)
+    if not 0 <= length <= cache.Smax or written < length:
+        raise ValueError(f"need 0 <= length <= {cache.Smax} and written >= length, got {length} and {written}")
+    blk, rest = divmod(length, BLOCK)
+
+    def intact(x):  # no later position has taken block x's slots
+        return x < 0 or written <= x * BLOCK + SLOTS
+
+    def refill(x):
+        # as read at a length past it: from its codes, which it got before its slots were taken
+        lens = torch.full((cache.B,), (x + 2) * BLOCK + BLOCK // 2, dtype=torch.int32, device=cache.device)
+        k, v = kv_read_q8(cache, lens, BLOCK, start=x * BLOCK)
+        s = x * BLOCK % SLOTS
+        cache.tail_k[:, :, s:s + BLOCK] = k
+        cache.tail_vt[:, :, :, s:s + BLOCK] = v.transpose(2, 3)
+
+    if rest and not intact(blk):
+        refill(blk)
+    if intact(blk - 1):
+        return length
+    if rest <= MAX_DRAFT:  # the next append may quantise block blk - 1 again
+        refill(blk - 1)
+        return length
+    return min(written, blk * BLOCK + SLOTS)  # (block blk is there, block blk - 1 is not)

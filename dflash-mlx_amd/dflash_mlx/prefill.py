@@ -404,13 +404,22 @@ class HybridPrefill:
             else:
                 ap = self.aproj.data_ptr()
                 self._bf16_proj(tw["w_qkv"], xn, H, P, ap, arows, False, stream)
-                call("dflash_attn_prep", ap, arows, lw["q_norm"].data_ptr(), lw["k_norm"].data_ptr(),
-                     run.lens.data_ptr(), run.k_cache[ai].data_ptr(), run.vt_cache[ai].data_ptr(),
-                     self.q.data_ptr(), run.overflow.data_ptr(), 1, P, Hq, Hkv, D, run.Smax,
-                     cfg.rot_dims, float(cfg.rope_theta), eps, stream)
-                call("dflash_attn_prefill", self.q.data_ptr(), run.k_cache[ai].data_ptr(),
-                     run.vt_cache[ai].data_ptr(), run.lens.data_ptr(), ap, arows,
-                     self.attn_out.data_ptr(), P, Hq, Hkv, D, run.Smax, float(D ** -0.5), stream)
+                if run.kv:
+                    kv = run.kv[ai]._ptr
+                    call("dflash_kv8_append", kv, ap, arows, lw["q_norm"].data_ptr(),
+                         lw["k_norm"].data_ptr(), run.lens.data_ptr(), self.q.data_ptr(),
+                         run.overflow.data_ptr(), P, Hq, cfg.rot_dims, float(cfg.rope_theta), eps, 1,
+                         stream)
+                    call("dflash_attn_prefill_q8", kv, self.q.data_ptr(), run.lens.data_ptr(), ap,
+                         arows, self.attn_out.data_ptr(), P, Hq, float(D ** -0.5), stream)
+                else:
+                    call("dflash_attn_prep", ap, arows, lw["q_norm"].data_ptr(), lw["k_norm"].data_ptr(),
+                         run.lens.data_ptr(), run.k_cache[ai].data_ptr(), run.vt_cache[ai].data_ptr(),
+                         self.q.data_ptr(), run.overflow.data_ptr(), 1, P, Hq, Hkv, D, run.Smax,
+                         cfg.rot_dims, float(cfg.rope_theta), eps, stream)
+                    call("dflash_attn_prefill", self.q.data_ptr(), run.k_cache[ai].data_ptr(),
+                         run.vt_cache[ai].data_ptr(), run.lens.data_ptr(), ap, arows,
+                         self.attn_out.data_ptr(), P, Hq, Hkv, D, run.Smax, float(D ** -0.5), stream)
                 branch = self._to_residual(tw["w_o"], self.attn_out.data_ptr(), Hq * D, P, stream)
                 ai += 1
             self._add_norm(branch, lw["ln_post"], None, P, stream)

@@ -12,7 +12,8 @@ LoadedTargetModel facade (adapters.py:341-570, :729-826).
   to ``block_size``, ``max_seq_len`` cache positions) and returns its caches
   as the reference's per-layer list: an ``ArraysCache`` [conv window, state]
   per gated-delta layer and a ``DeviceKVCache`` per attention layer, all views
-  of the runner's device buffers.
+  of the runner's device buffers (``DeviceQuantizedKVCache`` with
+  ``kv_dtype`` int8 or float8_e4m3fn).
 * ``forward_dflash(inputs, cache, layer_ids, return_rollback_records)`` runs
   a verify block (at most ``block_size`` tokens) through the runner, and a
   longer input (a prompt) in one pass with launches sized to it
@@ -47,6 +48,7 @@ from . import _lib
 from .adapters import make_rollback_record
 from .cache import ArraysCache, KVCache
 from .hybrid_model import HybridConfig, HybridVerifyRunner, HybridWeights
+from .kv8 import QuantizedKVCache, kv_read_q8, kv_rewind_q8
 from .prefill import HybridPrefill
 
 
@@ -78,6 +80,52 @@ class DeviceKVCache(KVCache):
         raise NotImplementedError("the runner's attention kernels append to this cache")
 
 
+class DeviceQuantizedKVCache(KVCache):
+    """A full-attention layer's KV cache in 8 bits (kv8.QuantizedKVCache): ``offset``
+    as DeviceKVCache's, ``keys`` and ``values`` read back in bf16.  ``written``
+    counts the positions ever written since the tail was made ready, rejected
+    drafts included: prepare() looks whether the tail still holds what a call
+    at ``offset`` reads."""
+
+    def __init__(self, cache: QuantizedKVCache):
+        self.cache = cache
+        self.written = 0
+        self._offset = 0
+
+    @property
+    def offset(self) -> int:
+        return self._offset
+
+    @offset.setter
+    def offset(self, n: int) -> None:
+        self._offset = n
+        self.written = max(self.written, n)
+
+    def prepare(self) -> None:
+        """Before a forward at ``offset``."""
+        if self._offset < self.written:
+            self.written = kv_rewind_q8(self.cache, self._offset, self.written)
+
+    @property
+    def capacity(self) -> int:
+        return self.cache.Smax
+
+    def _read(self):
+        lens = torch.full((self.cache.B,), self._offset, dtype=torch.int32, device=self.cache.device)
+        return kv_read_q8(self.cache, lens, self._offset)
+
+    @property
+    def keys(self) -> torch.Tensor:
+        return self._read()[0]
+
+    @property
+    def values(self) -> torch.Tensor:
+        return self._read()[1]
+
+    def update_and_fetch(self, keys, values):
+        raise NotImplementedError("the runner's attention kernels append to this cache")
+
+
 class HybridCache(list):
     """The per-layer cache list of one sequence, bound to its runner."""
 
@@ -93,11 +141,12 @@ class HybridTargetModel:
     def __init__(self, cfg: HybridConfig, weights: HybridWeights, device: torch.device,
                  max_seq_len: int = 4096, block_size: int = 16, weight_layout: str = "tiled",
                  eos_token_ids: set[int] | None = None, prompt_pass: str = "prefill",
-                 prefill_rows: int = 8192):
+                 prefill_rows: int = 8192, kv_dtype: torch.dtype = torch.bfloat16):
         """prompt_pass: "prefill" runs inputs longer than block_size in one
         pass (prefill.HybridPrefill, up to prefill_rows rows per pass);
         "blocks" runs them through the verify runner block_size tokens at a
-        time."""
+        time.  kv_dtype: torch.int8 or torch.float8_e4m3fn hold the attention
+        layers' caches in 8 bits (kv8.QuantizedKVCache)."""
         if prompt_pass not in ("prefill", "blocks"):
             raise ValueError(f"prompt_pass must be 'prefill' or 'blocks', got {prompt_pass!r}")
         self.cfg, self.weights, self.device = cfg, weights, torch.device(device)
@@ -106,6 +155,7 @@ class HybridTargetModel:
         self.weight_layout = weight_layout
         self.prompt_pass = prompt_pass
         self.prefill_rows = int(prefill_rows)
+        self.kv_dtype = kv_dtype
         self.eos_token_ids = set(eos_token_ids or ())
         self._smax = -(-(self.max_seq_len + self.block_size) // 64) * 64
 
@@ -116,7 +166,7 @@ class HybridTargetModel:
         runner."""
         cfg = self.cfg
         run = HybridVerifyRunner(cfg, self.weights, 1, self.block_size, self._smax, self.device,
-                                 weight_layout=self.weight_layout)
+                                 weight_layout=self.weight_layout, kv_dtype=self.kv_dtype)
         run.snapshot_conv()
         cache = HybridCache()
         cache.runner = run
@@ -129,7 +179,8 @@ class HybridTargetModel:
                 cache.linear_idx.append(i)
                 gi += 1
             else:
-                c = DeviceKVCache(run.k_cache[ai], run.vt_cache[ai])
+                c = (DeviceQuantizedKVCache(run.kv[ai]) if run.kv
+                     else DeviceKVCache(run.k_cache[ai], run.vt_cache[ai]))
                 cache.attn_idx.append(i)
                 ai += 1
             cache.append(c)
@@ -168,6 +219,8 @@ class HybridTargetModel:
             raise ValueError(f"{n_new} new tokens at cache length {off} exceed the "
                              f"{run.Smax}-position cache (max_seq_len {self.max_seq_len} "
                              f"+ one block, rounded up to 64)")
+        for i in cache.attn_idx:
+            cache[i].prepare()
         return off
 
     @staticmethod
