@@ -18,8 +18,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // query head r of the group at token t, against the positions that they see.  Work is
 // counted in blocks of 64 positions over all heads and sequences and shared by the
 // launch's workgroups whatever the sequences' lengths (Batch).  That cuts heads into
-// parts, which go to the workspace for a second launch to merge; a head that one
-// workgroup has to itself is finished there.
+// parts, which go to the workspace and are merged by the workgroup that brings a head's
+// last one (up to 16 rows: 8 KB a part at most) or by a second launch (a part of 64 rows is
+// 32 KB: one workgroup would take longer over a head's than the launch does); a head that
+// one workgroup has to itself is finished there.
 //   - Products on MFMA in transposed form, S^T = K Q^T and O^T = V^T P^T: a lane
 //     holds one row's scores and outputs, and P stays in its registers.
 //   - A block's key scale is one factor of its scores; its value scale goes into
@@ -35,6 +37,7 @@ struct VerifyParams {
   uint16_t* out;    // [B, T, Hq * D]
   float* part_o;    // [2 * runs][part_rows][D], in the order that the kernel's lanes hold them
   float* part_ml;   // [2 * runs][part_rows][2]
+  int32_t* count;   // [B, Hkv] parts that have arrived (up to 16 rows); zero between calls
   int T, Hq, rep, runs, min_cut;
   int part_rows;  // rows of a part in the workspace
   uint32_t rep_inv;
@@ -245,6 +248,39 @@ __device__ __forceinline__ float weights(const float (&s)[N], float mx, float sl
   return alpha;
 }
 
+// The parts of a head, in slots of the workspace (two a workgroup: one for the head that
+// its share starts in, one for a later one): `head` of workgroup w0, 2 w of the others up
+// to w1.
+struct Parts {
+  int w0, w1, head;
+  __device__ int at(int w) const { return w == w0 ? head : 2 * w; }
+};
+__device__ __forceinline__ Parts parts_of(const VerifyParams& p, Batch& batch, int b, int h, int nb) {
+  const int n = batch.units_of(nb);
+  const int u0 = p.c.Hkv * batch.before(b) + h * n;
+  if (batch.pieces) {
+    const int size = (nb + n - 1) / n;
+    return Parts{u0, u0 + (nb + size - 1) / size - 1, 2 * u0};
+  }
+  const int w0 = u0 / batch.per;
+  return Parts{w0, (u0 + nb - 1) / batch.per, 2 * w0 + (u0 > w0 * batch.per ? 1 : 0)};
+}
+
+// Running merge of the parts that one lane walks; V is the vector of outputs that it holds.
+template <class V>
+struct Merged {
+  float m = -INFINITY, l = 0.f;
+  V o = V{};
+  __device__ void add(float pm, float pl, V po) {
+    const float mn = fmaxf(m, pm);
+    const float ca = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    const float cb = pm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm - mn);
+    l = l * ca + pl * cb;
+    o = o * ca + po * cb;
+    m = mn;
+  }
+};
+
 // ------------------------------------------------- up to 16 rows (single tokens)
 // Eight waves, block by block in turn, straight from memory to registers: nothing is
 // shared.  v_mfma_f32_16x16x32_bf16; lane (r, g) = (lane % 16, lane / 16) has row r.
@@ -253,12 +289,30 @@ __device__ __forceinline__ float weights(const float (&s)[N], float mx, float sl
 // the ones whose values lie side by side in a row of V^T.  The next block's keys
 // are loaded once these are consumed, its values likewise.
 constexpr int kWaves16 = 8;
+constexpr int kPartsAhead = 8;
+
+// Parts of up to 16 rows are merged by the workgroup that brings the last one: stored and
+// loaded at agent scope, counted after the stores are acknowledged (the protocol and the
+// hardware ordering that it rests on are in device_common.h).  In order of their runs,
+// whichever comes last.
+__device__ __forceinline__ void store_part(float* base, int64_t i, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(base) + i,
+                     (uint64_t)__float_as_uint(x) | ((uint64_t)__float_as_uint(y) << 32), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 load_part(const float* base, int64_t i) {
+  const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(base) + i, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  return f32x2{__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32))};
+}
+
 
 template <int TYPE>
 __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel(const VerifyParams p) {
   __shared__ __attribute__((aligned(16))) float so[kWaves16][16][kHD + 4];
   __shared__ float sml[kWaves16][16][2];
   __shared__ int dropped;  // the tail's values hold a NaN or an infinity
+  __shared__ int arrived;
   const Kv8& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -266,6 +320,13 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
   if (tid == 0) dropped = 0;
   __syncthreads();
   Batch batch(p);
+  // sequences that take no part: their rows are zero
+  for (int b = blockIdx.x; b < c.B; b += gridDim.x) {
+    if (batch.length(b) >= 0) continue;
+    const int n = p.T * p.Hq * kHD / 2;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out) + (int64_t)b * n;
+    for (int i = tid; i < n; i += 64 * kWaves16) dst[i] = 0u;
+  }
   Share at = share_of(p, batch, blockIdx.x);
   const float sl0 = positive_scale(p.scale);
   const QuerySign sign(p.scale);
@@ -442,8 +503,52 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
         const int qh = at.h * p.rep + row - tt * p.rep;
         store_gated(p, (int64_t)at.b * p.T + tt, qh, d, oo * (1.f / ll));
       } else {
-        *reinterpret_cast<f32x4*>(p.part_o + (part * p.part_rows + row) * kHD + d) = oo;
-        if (d == 0) *reinterpret_cast<f32x2*>(p.part_ml + (part * p.part_rows + row) * 2) = f32x2{mm, ll};
+        const int64_t at2 = ((part * p.part_rows + row) * kHD + d) / 2;
+        store_part(p.part_o, at2, oo.x, oo.y);
+        store_part(p.part_o, at2 + 1, oo.z, oo.w);
+        if (d == 0) store_part(p.part_ml, part * p.part_rows + row, mm, ll);
+      }
+    }
+    if (!whole) {
+      const Parts parts = parts_of(p, batch, at.b, at.h, nb);
+      __builtin_amdgcn_s_waitcnt(0);  // this thread's part is where every XCD sees it
+      __syncthreads();
+      if (tid == 0)
+        arrived = __hip_atomic_fetch_add(p.count + bh, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (arrived == parts.w1 - parts.w0) {  // the last: merge them, in their order
+        if (tid == 0) __hip_atomic_store(p.count + bh, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int items = nrows * 32, groups = min(64 * kWaves16 / items, kWaves16);
+        const int group = tid / items, i = tid - group * items, row = i >> 5, d = (i & 31) * 4;
+        Merged<f32x4> a;
+        if (group < groups) {
+          for (int w = parts.w0 + group; w <= parts.w1; w += groups * kPartsAhead) {
+            f32x2 ml[kPartsAhead], o0[kPartsAhead], o1[kPartsAhead];
+#pragma unroll
+            for (int u = 0; u < kPartsAhead; ++u) {
+              const int64_t x = (int64_t)parts.at(min(w + groups * u, parts.w1)) * p.part_rows + row;
+              ml[u] = load_part(p.part_ml, x);
+              o0[u] = load_part(p.part_o, (x * kHD + d) / 2);
+              o1[u] = load_part(p.part_o, (x * kHD + d) / 2 + 1);
+            }
+#pragma unroll
+            for (int u = 0; u < kPartsAhead; ++u)
+              if (w + groups * u <= parts.w1) a.add(ml[u].x, ml[u].y, f32x4{o0[u].x, o0[u].y, o1[u].x, o1[u].y});
+          }
+          if (d == 0) {
+            sml[group][row][0] = a.m;
+            sml[group][row][1] = a.l;
+          }
+          *reinterpret_cast<f32x4*>(&so[group][row][d]) = a.o;
+        }
+        __syncthreads();
+        if (group == 0) {
+          const int n = min(groups, parts.w1 - parts.w0 + 1);
+          for (int x = 1; x < n; ++x)
+            a.add(sml[x][row][0], sml[x][row][1], *reinterpret_cast<const f32x4*>(&so[x][row][d]));
+          const int tt = p.token_of(row);
+          store_gated(p, (int64_t)at.b * p.T + tt, at.h * p.rep + row - tt * p.rep, d, a.o * (1.f / a.l));
+        }
       }
     }
     __syncthreads();
@@ -676,87 +781,9 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
 }
 
 // ------------------------------------------------------------------- merge
-// The parts of a head, in slots of the workspace (two a workgroup: one for the head that
-// its share starts in, one for a later one): `head` of workgroup w0, 2 w of the others up
-// to w1.
-struct Parts {
-  int w0, w1, head;
-  __device__ int at(int w) const { return w == w0 ? head : 2 * w; }
-};
-__device__ __forceinline__ Parts parts_of(const VerifyParams& p, Batch& batch, int b, int h, int nb) {
-  const int n = batch.units_of(nb);
-  const int u0 = p.c.Hkv * batch.before(b) + h * n;
-  if (batch.pieces) {
-    const int size = (nb + n - 1) / n;
-    return Parts{u0, u0 + (nb + size - 1) / size - 1, 2 * u0};
-  }
-  const int w0 = u0 / batch.per;
-  return Parts{w0, (u0 + nb - 1) / batch.per, 2 * w0 + (u0 > w0 * batch.per ? 1 : 0)};
-}
-
-// Running merge of the parts that one lane walks; V is the vector of outputs that it holds.
-template <class V>
-struct Merged {
-  float m = -INFINITY, l = 0.f;
-  V o = V{};
-  __device__ void add(float pm, float pl, V po) {
-    const float mn = fmaxf(m, pm);
-    const float ca = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-    const float cb = pm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm - mn);
-    l = l * ca + pl * cb;
-    o = o * ca + po * cb;
-    m = mn;
-  }
-};
-
-// Up to 16 rows: a workgroup per (token, query head); lane l has features 2 l, 2 l + 1.
-// The waves take the parts in turn, kMergeAhead loads in flight: up to 128 parts (one
-// sequence, two key/value heads on 256 runs) cost one trip to memory.
+// The waves take the parts in turn, kMergeAhead loads in flight: up to 128 parts cost one
+// trip to memory.
 constexpr int kMergeWaves = 16, kMergeAhead = 8;
-
-__global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge16_kernel(const VerifyParams p) {
-  __shared__ float sm[kMergeWaves], sl[kMergeWaves];
-  __shared__ f32x2 so[kMergeWaves][64];
-  const int bt = blockIdx.x, qh = blockIdx.y;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int b = bt / p.T, t = bt - b * p.T, h = qh / p.rep, row = t * p.rep + qh - h * p.rep;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + ((int64_t)bt * p.Hq + qh) * kHD + 2 * lane);
-  Batch batch(p);
-  const int nb = seen_blocks(__builtin_amdgcn_readfirstlane(p.lens[b]), p.T, p.c.Smax);
-  if (nb == 0) {  // takes no part
-    if (wave == 0) *dst = 0u;
-    return;
-  }
-  const Parts parts = parts_of(p, batch, b, h, nb);
-  if (parts.w0 == parts.w1) return;  // finished by its one run
-  const uint32_t gv =
-      *reinterpret_cast<const uint32_t*>(p.gate + (int64_t)bt * p.gate_stride + qh * 2 * kHD + kHD + 2 * lane);
-  Merged<f32x2> a;
-  for (int w = parts.w0 + wave; w <= parts.w1; w += kMergeWaves * kMergeAhead) {
-    f32x2 ml[kMergeAhead], os[kMergeAhead];
-#pragma unroll
-    for (int u = 0; u < kMergeAhead; ++u) {
-      const int64_t i = (int64_t)parts.at(min(w + kMergeWaves * u, parts.w1)) * p.part_rows + row;
-      ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * i);
-      os[u] = *reinterpret_cast<const f32x2*>(p.part_o + i * kHD + 2 * lane);
-    }
-#pragma unroll
-    for (int u = 0; u < kMergeAhead; ++u)
-      if (w + kMergeWaves * u <= parts.w1) a.add(ml[u].x, ml[u].y, os[u]);
-  }
-  if (lane == 0) {
-    sm[wave] = a.m;
-    sl[wave] = a.l;
-  }
-  so[wave][lane] = a.o;
-  __syncthreads();
-  if (wave != 0) return;
-  const int n = min(kMergeWaves, parts.w1 - parts.w0 + 1);
-  for (int k = 1; k < n; ++k) a.add(sm[k], sl[k], so[k][lane]);
-  const float inv = 1.f / a.l;
-  const float g0 = 1.f / (1.f + __expf(-bf16_lo(gv))), g1 = 1.f / (1.f + __expf(-bf16_hi(gv)));
-  *dst = pack2(a.o.x * inv * g0, a.o.y * inv * g1);
-}
 
 // Up to 64 rows: a workgroup per (sequence, key/value head, tile, sixteenth q of its
 // outputs), a part's outputs as the lanes stored them; the waves take the parts in turn.
@@ -817,6 +844,8 @@ VerifyShape verify_shape(int64_t B, int rows, int Hkv, int Smax) {
   v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(rows <= 16 ? cus : 2 * cus, B * Hkv * ceil_div(Smax / kBlk, v.min_cut)));
   return v;
 }
+
+size_t count_bytes(int64_t B, int Hkv) { return (size_t)ceil_div(B * Hkv * 4, 256) * 256; }
 
 template <int TYPE>
 void launch_verify(const VerifyParams& p, hipStream_t s) {
@@ -1190,7 +1219,7 @@ extern "C" size_t dflash_attn_verify_q8_workspace_bytes(int B, int T, int Hq, in
       Smax <= 0 || Smax % kBlk != 0)
     return 0;
   const VerifyShape v = verify_shape(B, T * (Hq / Hkv), Hkv, Smax);
-  return (size_t)2 * v.runs * v.part_rows * (kHD + 2) * sizeof(float);
+  return count_bytes(B, Hkv) + (size_t)2 * v.runs * v.part_rows * (kHD + 2) * sizeof(float);
 }
 
 extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* q, const int32_t* lens,
@@ -1221,19 +1250,16 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   p.part_rows = v.part_rows;
   p.min_cut = v.min_cut;
   p.runs = v.runs;
-  p.part_o = static_cast<float*>(workspace);
+  p.count = static_cast<int32_t*>(workspace);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + count_bytes(B, Hkv));
   p.part_ml = p.part_o + (int64_t)2 * p.runs * p.part_rows * kHD;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache->type == DFLASH_KV_INT8) launch_verify<DFLASH_KV_INT8>(p, s);
   else launch_verify<DFLASH_KV_E4M3>(p, s);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return (int)e;
-  if (p.part_rows == 16)
-    hipLaunchKernelGGL(attn_verify_q8_merge16_kernel, dim3((unsigned)(B * T), (unsigned)Hq),
-                       dim3(64 * kMergeWaves), 0, s, p);
-  else
-    hipLaunchKernelGGL(attn_verify_q8_merge64_kernel, dim3((unsigned)(Hkv * p.part_rows / 2), (unsigned)B),
-                       dim3(64 * kMergeWaves), 0, s, p);
+  if (e != hipSuccess || p.part_rows == 16) return to_status(e);
+  hipLaunchKernelGGL(attn_verify_q8_merge64_kernel, dim3((unsigned)(Hkv * p.part_rows / 2), (unsigned)B),
+                     dim3(64 * kMergeWaves), 0, s, p);
   return to_status(hipGetLastError());
 }
 

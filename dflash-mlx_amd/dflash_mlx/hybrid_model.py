@@ -288,7 +288,7 @@ class HybridVerifyRunner:
             ws = int(lib.dflash_attn_verify_workspace_bytes(B, Hq, Hkv, Smax))
         else:
             ws = max(attn_verify_q8_workspace_bytes(B, t, Hq, Hkv, Smax) for t in range(1, T + 1))
-        self.attn_ws = e(ws, dt=torch.uint8)
+        self.attn_ws = z(ws, dt=torch.uint8)  # (the 8-bit cache's attention counts in it)
         # accept / commit
         self.lens = z(B, dt=i32)
         self.keep = z(B, dt=i32)  # 0: the first step starts from `state`

@@ -61,7 +61,7 @@ class QuantizedKVCache:
     one device."""
 
     __slots__ = ("k_codes", "v_codes", "k_scale", "v_scale", "tail_k", "tail_vt", "B", "Hkv", "Smax", "dtype",
-                 "device", "_struct", "_ptr")
+                 "device", "_struct", "_ptr", "_lens_shape", "_ws_bytes", "_workspaces")
 
     def __init__(self, k_codes, v_codes, k_scale, v_scale, tail_k, tail_vt):
         _require_device("k_codes", k_codes)
@@ -89,6 +89,9 @@ class QuantizedKVCache:
         self._struct = _CCache(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                tail_k.data_ptr(), tail_vt.data_ptr(), _TYPES[k_codes.dtype], B, Hkv, Smax)
         self._ptr = ctypes.addressof(self._struct)
+        self._lens_shape = (B,)
+        self._ws_bytes = {}    # attn_verify_q8's, by (T, heads)
+        self._workspaces = {}  # by stream: calls on one stream do not overlap
 
     @classmethod
     def zeros(cls, B: int, Hkv: int, Smax: int, dtype: torch.dtype, device) -> "QuantizedKVCache":
@@ -117,14 +120,17 @@ def _call(fn: str, dev: torch.device, *args) -> None:
             _lib.call(fn, *args, _lib.stream_handle(dev))
 
 
+# The checks below test for what is right in one expression and say what is wrong
+# only afterwards: a small call's time is all host work.
+
 def _check_cache(cache) -> None:
     if not isinstance(cache, QuantizedKVCache):
         raise TypeError(f"cache must be a QuantizedKVCache, got {type(cache).__name__}")
 
 
 def _check_lens(name: str, lens, cache) -> None:
-    if isinstance(lens, torch.Tensor) and (lens.dtype is torch.int32 and lens.device == cache.device
-                                           and lens.shape == (cache.B,) and lens.is_contiguous()):
+    if isinstance(lens, torch.Tensor) and (lens.dtype is torch.int32 and lens.shape == cache._lens_shape
+                                           and lens.device == cache.device and lens.is_contiguous()):
         return
     _require_device(name, lens, cache.device)
     if lens.dtype is not torch.int32:
@@ -135,29 +141,46 @@ def _check_lens(name: str, lens, cache) -> None:
 def _row_stride(name: str, proj, cache, T: int | None, width: int) -> int:
     """Row stride of the projection rows [B, T, >= width], which are evenly
     spaced and 16-byte aligned."""
+    if isinstance(proj, torch.Tensor) and proj.dim() == 3:
+        (b, t, w), (sb, st, se) = proj.shape, proj.stride()
+        row = st if t > 1 else sb if b > 1 else max(st, w)
+        if (proj.dtype is torch.bfloat16 and proj.device == cache.device and b == cache.B and (T is None or t == T)
+                and w >= width and se == 1 and row >= w and (b == 1 or t == 1 or sb == t * row) and row % 8 == 0
+                and proj.data_ptr() % 16 == 0):
+            return row
     _require_device(name, proj, cache.device)
     if proj.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {proj.dtype}")
     if proj.dim() != 3 or proj.shape[0] != cache.B or (T is not None and proj.shape[1] != T) or proj.shape[2] < width:
         raise ValueError(f"{name} must be [{cache.B}, {'T' if T is None else T}, at least {width}], "
                          f"got {tuple(proj.shape)}")
-    B, T, w = proj.shape
-    sb, st, se = proj.stride()
-    row = st if T > 1 else sb if B > 1 else max(st, w)
-    if se != 1 or row < w or (B > 1 and T > 1 and sb != T * row) or row % 8 or proj.data_ptr() % 16:
-        raise ValueError(f"{name} rows must be contiguous, evenly spaced over [B, T] and 16-byte aligned, "
-                         f"got strides {(sb, st, se)}")
-    return row
+    if proj.numel() == 0:
+        return -(-width // 8) * 8
+    raise ValueError(f"{name} rows must be contiguous, evenly spaced over [B, T] and 16-byte aligned, "
+                     f"got strides {tuple(proj.stride())}")
 
 
 def _check_queries(q, cache):
+    if isinstance(q, torch.Tensor) and q.dim() == 4:
+        b, t, h, d = q.shape
+        if (q.dtype is torch.bfloat16 and b == cache.B and d == HEAD_DIM and h and h % cache.Hkv == 0
+                and q.device == cache.device):
+            return t, h
     _require_device("q", q, cache.device)
     if q.dtype is not torch.bfloat16:
         raise TypeError(f"q must be bfloat16, got {q.dtype}")
-    if q.dim() != 4 or q.shape[0] != cache.B or q.shape[3] != HEAD_DIM or q.shape[2] == 0 \
-            or q.shape[2] % cache.Hkv:
-        raise ValueError(f"q must be [{cache.B}, T, a multiple of {cache.Hkv} heads, {HEAD_DIM}], got {tuple(q.shape)}")
-    return q.shape[1], q.shape[2]
+    raise ValueError(f"q must be [{cache.B}, T, a multiple of {cache.Hkv} heads, {HEAD_DIM}], got {tuple(q.shape)}")
+
+
+_NORM_SHAPE = (HEAD_DIM,)
+
+
+def _check_norm(name: str, w, cache) -> None:
+    if isinstance(w, torch.Tensor) and (w.dtype is torch.bfloat16 and w.shape == _NORM_SHAPE
+                                        and w.device == cache.device and w.is_contiguous()):
+        return
+    _require_device(name, w, cache.device)
+    raise ValueError(f"{name} must be contiguous bfloat16 [{HEAD_DIM}], got {w.dtype} {tuple(w.shape)}")
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -187,10 +210,8 @@ def attn_prep_q8(proj, q_norm, k_norm, lens, cache: QuantizedKVCache, *, num_hea
     T = proj.shape[1]
     if not prompt and T > MAX_DRAFT:
         raise ValueError(f"a draft append takes at most {MAX_DRAFT} tokens, got {T} (prompt=True for committed ones)")
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        _require_device(name, w, cache.device)
-        if w.dtype is not torch.bfloat16 or w.shape != (HEAD_DIM,) or not w.is_contiguous():
-            raise ValueError(f"{name} must be contiguous bfloat16 [{HEAD_DIM}]")
+    _check_norm("q_norm", q_norm, cache)
+    _check_norm("k_norm", k_norm, cache)
     if overflow is not None:
         _check_lens("overflow", overflow, cache)
     q = torch.empty((cache.B, T, num_heads, HEAD_DIM), dtype=torch.bfloat16, device=cache.device)
@@ -205,14 +226,32 @@ def attn_verify_q8_workspace_bytes(B: int, T: int, num_heads: int, Hkv: int, Sma
     return int(_lib.load().dflash_attn_verify_q8_workspace_bytes(B, T, num_heads, Hkv, Smax))
 
 
+def _verify_workspace(cache: QuantizedKVCache, T: int, Hq: int) -> torch.Tensor:
+    """The cache's workspace of the current stream; of a captured graph its own."""
+    n = cache._ws_bytes.get((T, Hq))
+    if n is None:
+        with torch.cuda.device(cache.device):
+            n = cache._ws_bytes[(T, Hq)] = attn_verify_q8_workspace_bytes(cache.B, T, Hq, cache.Hkv, cache.Smax)
+    capturing = torch.cuda.is_current_stream_capturing()
+    stream = _lib.stream_handle(cache.device)
+    ws = None if capturing else cache._workspaces.get(stream)
+    if ws is None or ws.numel() < n:
+        ws = torch.empty(n, dtype=torch.uint8, device=cache.device)
+        ws[:4 * cache.B * cache.Hkv].zero_()
+        if not capturing:
+            cache._workspaces[stream] = ws
+    return ws
+
+
 def attn_verify_q8(q, cache: QuantizedKVCache, lens, proj, *, scale: float | None = None, workspace=None):
     """Attention of the T <= 16 tokens a sequence that attn_prep_q8 (prompt=False)
     appended at lens[b]: token t sees positions 0 .. lens[b] + t.
 
     q: bf16 [B, T, Hq, 128]; proj: the projection rows (the gate of head h at
     256 h + 128); T * Hq / Hkv <= 64; scale: 128 ** -0.5 by default.  workspace
-    (optional): uint8, attn_verify_q8_workspace_bytes bytes, kept by a caller
-    that replays graphs; calls that overlap in time must not share it.  Returns
+    (optional): uint8, attn_verify_q8_workspace_bytes bytes, the first 4 B Hkv zero
+    before its first use; calls that overlap in time must not share it.  By default
+    the cache keeps one a stream, and a captured graph gets its own.  Returns
     softmax(scale q k^T) v * sigmoid(gate), bf16 [B, T, Hq * 128]."""
     _check_cache(cache)
     _check_lens("lens", lens, cache)
@@ -220,20 +259,17 @@ def attn_verify_q8(q, cache: QuantizedKVCache, lens, proj, *, scale: float | Non
     if T > MAX_DRAFT or T * (Hq // cache.Hkv) > 64:
         raise ValueError(f"at most {MAX_DRAFT} tokens and 64 query rows a key/value head, got T = {T}, {Hq} heads")
     row = _row_stride("proj", proj, cache, T, 2 * Hq * HEAD_DIM)
-    dev = cache.device
-    out = torch.empty((cache.B, T, Hq * HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    out = torch.empty((cache.B, T, Hq * HEAD_DIM), dtype=torch.bfloat16, device=cache.device)
     if out.numel() == 0:
         return out
     if workspace is None:
-        with torch.cuda.device(dev):
-            n = attn_verify_q8_workspace_bytes(cache.B, T, Hq, cache.Hkv, cache.Smax)
-        workspace = torch.empty(n, dtype=torch.uint8, device=dev)
+        workspace = _verify_workspace(cache, T, Hq)
     else:
-        _require_device("workspace", workspace, dev)
+        _require_device("workspace", workspace, cache.device)
         if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous uint8")
     q = _aligned(q)
-    _call("dflash_attn_verify_q8", dev, cache._ptr, q.data_ptr(), lens.data_ptr(), proj.data_ptr(), row,
+    _call("dflash_attn_verify_q8", cache.device, cache._ptr, q.data_ptr(), lens.data_ptr(), proj.data_ptr(), row,
           out.data_ptr(), T, Hq, HEAD_DIM ** -0.5 if scale is None else float(scale), workspace.data_ptr(),
           workspace.numel())
     return out
@@ -290,8 +326,8 @@ def kv_read_q8(cache: QuantizedKVCache, lens, count: int, *, start=0):
         starts, start = start, 0
     elif not -2 ** 31 <= start < 2 ** 31:
         raise ValueError(f"start {start} is not a 32-bit position")
-    k, v = (torch.empty((cache.B, cache.Hkv, count, HEAD_DIM), dtype=torch.bfloat16, device=cache.device)
-            for _ in range(2))
+    k = torch.empty((cache.B, cache.Hkv, count, HEAD_DIM), dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty_like(k)
     _call("dflash_kv8_read", cache.device, cache._ptr, lens.data_ptr(), _lib.ptr(starts), int(start), count,
           k.data_ptr(), v.data_ptr())
     return k, v

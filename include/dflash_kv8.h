@@ -113,8 +113,9 @@ int dflash_kv8_read(const dflash_kv8_cache* cache, const int32_t* lens,
  * lens[b] + t:
  *   out[b, t, h*128 ..] = bf16(softmax(scale * q k^T) v * sigmoid(gate))
  * with the gate of head h at h*256 + 128 of row b*T + t of gate_src.  T * Hq / Hkv
- * <= 64.  workspace: dflash_attn_verify_q8_workspace_bytes bytes, no initial
- * contents, not shared by calls that overlap in time.
+ * <= 64.  workspace: dflash_attn_verify_q8_workspace_bytes bytes (enough for any
+ * smaller T and Hq too), its first 4 * B * Hkv bytes zero before the first call (every call leaves them
+ * zero), not shared by calls that overlap in time.
  */
 size_t dflash_attn_verify_q8_workspace_bytes(int B, int T, int Hq, int Hkv,
                                              int Smax);

@@ -189,3 +189,117 @@ def test_verify_blocks_that_read_as_nan(device, dtype):
         scales[1, 0, 2] = good
         assert got[1, :, :2].isnan().all()
         assert torch.isfinite(got[0].float()).all() and torch.isfinite(got[1, :, 2:].float()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,lens", [(1, [3000, 17, 900]), (16, [3000, 17, 900])])
+def test_calls_on_two_streams_and_captured(device, dtype, T, lens):
+    """Two streams at once over one cache, and two graphs captured on one stream and
+    replayed beside each other and eager calls: all as the call alone."""
+    import dflash_mlx as dm
+
+    Hq, Hkv, Smax = 8, 2, 3136
+    cache, lens_d, k, v, q, proj, _ = _case(device, dtype, T, Hq, Hkv, lens, Smax, 5, False)
+    qs = [q.to(device), (q.float() * -0.5).bfloat16().to(device)]
+    proj = proj.to(device)
+    want = [dm.attn_verify_q8(x, cache, lens_d, proj) for x in qs]
+    again = [dm.attn_verify_q8(x, cache, lens_d, proj) for x in qs]
+    assert all(torch.equal(a, b) for a, b in zip(want, again))  # whichever part comes last
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(dm.attn_verify_q8(qs[i], cache, lens_d, proj))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for x in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(dm.attn_verify_q8(x, cache, lens_d, proj))
+        graphs.append(g)
+    for turn in range(6):
+        for o in outs:
+            o.fill_(0)
+        torch.cuda.synchronize()
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].replay()
+        eager = dm.attn_verify_q8(qs[turn % 2], cache, lens_d, proj)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[turn % 2])
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_workspace_serves_every_shape(device, dtype):
+    """One workspace for calls of growing and falling sizes: every call leaves its
+    counts zero, and one that is too small is refused."""
+    import dflash_mlx as dm
+    from dflash_mlx import _lib
+
+    Hq, Hkv, Smax = 8, 2, 4096
+    n = dm.attn_verify_q8_workspace_bytes(3, 16, Hq, Hkv, Smax)
+    ws = torch.zeros(n, dtype=torch.uint8, device=device)
+    for T in (1, 16, 4, 8, 1, 3):
+        cache, lens_d, k, v, q, proj, _ = _case(device, dtype, T, Hq, Hkv, [4000, 100, 2000], Smax, T, False)
+        assert dm.attn_verify_q8_workspace_bytes(3, T, Hq, Hkv, Smax) <= n
+        a = dm.attn_verify_q8(q.to(device), cache, lens_d, proj.to(device), workspace=ws)
+        b = dm.attn_verify_q8(q.to(device), cache, lens_d, proj.to(device))
+        assert torch.equal(a, b) and (ws[:4 * 3 * Hkv] == 0).all()
+    with pytest.raises(_lib.DFlashError, match="workspace"):
+        dm.attn_verify_q8(q.to(device), cache, lens_d, proj.to(device), workspace=ws[:1024])
+
+
+def test_refusals(device):
+    import dflash_mlx as dm
+
+    cache, lens, k, v, q, proj, _ = _case(device, torch.int8, 4, 4, 2, [100, 30], 128, 1, False)
+    q, proj = q.to(device), proj.to(device)
+    w = torch.ones(D, dtype=torch.bfloat16, device=device)
+    prep = dict(num_heads=4, rot_dims=32, rope_base=1e5)
+    for fn, exc, text in (
+            (lambda: dm.attn_verify_q8(q.float(), cache, lens, proj), TypeError, "q must be bfloat16"),
+            (lambda: dm.attn_verify_q8(q[:1], cache, lens, proj), ValueError, "q must be"),
+            (lambda: dm.attn_verify_q8(q[:, :, :3], cache, lens, proj), ValueError, "q must be"),
+            (lambda: dm.attn_verify_q8(q.cpu(), cache, lens, proj), ValueError, "no CPU path"),
+            (lambda: dm.attn_verify_q8(q, cache, lens.long(), proj), TypeError, "lens must be int32"),
+            (lambda: dm.attn_verify_q8(q, cache, lens[:1], proj), ValueError, "lens must be contiguous"),
+            (lambda: dm.attn_verify_q8(q, cache, lens.cpu(), proj), ValueError, "no CPU path"),
+            (lambda: dm.attn_verify_q8(q, cache, lens, proj[:, :3]), ValueError, "proj must be"),
+            (lambda: dm.attn_verify_q8(q, cache, lens, proj[..., :900]), ValueError, "proj must be"),
+            (lambda: dm.attn_verify_q8(q, cache, lens, proj[..., 1:]), ValueError, "16-byte aligned"),
+            (lambda: dm.attn_verify_q8(q.repeat(1, 5, 1, 1)[:, :17], cache, lens, proj.repeat(1, 5, 1)[:, :17]), ValueError,
+             "at most 16 tokens"),
+            (lambda: dm.attn_verify_q8(q.repeat(1, 4, 5, 1), cache, lens, proj.repeat(1, 4, 1)), ValueError, "64 query rows"),
+            (lambda: dm.attn_verify_q8(q, cache, lens, proj, workspace=torch.zeros(9)), ValueError, "no CPU path"),
+            (lambda: dm.attn_verify_q8(q, None, lens, proj), TypeError, "QuantizedKVCache"),
+            (lambda: dm.attn_prefill_q8(q, cache, lens, proj[:, :2]), ValueError, "proj must be"),
+            (lambda: dm.attn_prep_q8(proj.repeat(1, 5, 1), w, w, lens, cache, **prep), ValueError, "at most 16 tokens"),
+            (lambda: dm.attn_prep_q8(proj, w[:64], w, lens, cache, **prep), ValueError, "q_norm must be"),
+            (lambda: dm.attn_prep_q8(proj, w, w.float(), lens, cache, **prep), ValueError, "k_norm must be"),
+            (lambda: dm.attn_prep_q8(proj, w, w, lens, cache, num_heads=3, rot_dims=32, rope_base=1e5), ValueError,
+             "num_heads"),
+            (lambda: dm.attn_prep_q8(proj, w, w, lens, cache, num_heads=4, rot_dims=48, rope_base=1e5), RuntimeError,
+             "not supported"),
+            (lambda: dm.attn_prep_q8(proj[..., :1400], w, w, lens, cache, **prep), ValueError, "proj must be"),
+            (lambda: dm.kv_read_q8(cache, lens, -1), ValueError, "count"),
+            (lambda: dm.kv_read_q8(cache, lens, 4, start=lens.long()), TypeError, "start must be int32"),
+            (lambda: dm.kv_read_q8(cache, lens, 4, start=2 ** 31), ValueError, "32-bit"),
+            (lambda: dm.kv_load_q8(k.to(device), v.to(device).float(), lens, cache), TypeError, "v must be bfloat16"),
+            (lambda: dm.kv_load_q8(k.to(device), v.to(device)[:, :, :5], lens, cache), ValueError, "v must be"),
+            (lambda: dm.kv_rewind_q8(cache, 129, 200), ValueError, "length"),
+            (lambda: dm.kv_rewind_q8(cache, 50, 49), ValueError, "written")):
+        with pytest.raises(exc, match=text):
+            fn()
+    # empty calls
+    assert dm.attn_verify_q8(q[:, :0], cache, lens, proj[:, :0]).shape == (2, 0, 512)
+    assert dm.attn_prefill_q8(q[:, :0], cache, lens, proj[:, :0]).shape == (2, 0, 512)
+    assert dm.attn_prep_q8(proj[:, :0], w, w, lens, cache, **prep).shape == (2, 0, 4, D)
+    assert dm.kv_read_q8(cache, lens, 0)[0].shape == (2, 2, 0, D)
+    none = dm.QuantizedKVCache.zeros(0, 2, 64, torch.int8, device)
+    assert dm.attn_verify_q8(q[:0], none, lens[:0], proj[:0]).shape == (0, 4, 512)
