@@ -929,23 +929,27 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
   if (tid == 0) dropped = 0;
   u32x4 kv[PER], vv[PER];
   // K unit e: key e / 8, features 16 (e % 8) ..; V^T unit e: block e / 512, feature
-  // (e / 4) % 128, keys 16 (e % 4) ..  Blocks past the cache's last are clamped.
-  auto unit_of = [&](int i) { return min(tid + NT * i, UNITS - 1); };
-  auto block_of = [&](int turn, int e) { return min(2 * turn + (e >> 9), c.nblk - 1); };
+  // (e / 4) % 128, keys 16 (e % 4) ..  A wave's 64 units lie in one block of the turn,
+  // half_of: the block's address and the choice between codes and tail are the wave's.
+  // Blocks past the cache's last are clamped.
+  auto half_of = [&](int i) { return NT == 512 ? i : min(64 * wave + NT * i, UNITS - 1) >> 9; };
+  auto block_of = [&](int turn, int i) { return min(2 * turn + half_of(i), c.nblk - 1); };
+  auto unit_of = [&](int i) { return NT == 512 ? tid : (tid + NT * i) & 511; };
+  auto beyond = [&](int i) { return UNITS % NT != 0 && 64 * wave + NT * i >= UNITS; };
   auto load_keys = [&](int turn, u32x4 (&kv)[PER]) {
     if (turn >= turns) return;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int e = unit_of(i), j = block_of(turn, e);
-      if (j < done) kv[i] = ld16(c.keys(bh, j) + 16 * (e & 511));
+      const int j = block_of(turn, i);
+      if (j < done) kv[i] = ld16(c.keys(bh, j) + 16 * unit_of(i));
     }
   };
   auto load_values = [&](int turn) {
     if (turn >= turns) return;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int e = unit_of(i), j = block_of(turn, e);
-      if (j < done) vv[i] = ld16(c.values(bh, j) + 16 * (e & 511));
+      const int j = block_of(turn, i);
+      if (j < done) vv[i] = ld16(c.values(bh, j) + 16 * unit_of(i));
     }
   };
   auto store_pair = [&](unsigned char* row, int piece, int swizzle, u32x4 x, u32x4 y) {
@@ -957,17 +961,16 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     unsigned char* buf = lds + (turn & 1) * kPHalf;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int e = tid + NT * i;
-      if (UNITS % NT != 0 && e >= UNITS) continue;
-      const int j = block_of(turn, e), key = e >> 3;
-      unsigned char* row = buf + key * 256;
+      if (beyond(i)) continue;
+      const int e = unit_of(i), j = block_of(turn, i), key = e >> 3;
+      unsigned char* row = buf + half_of(i) * (kBlk * 256) + key * 256;
       if (j < done) {
         u32x2 x[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) x[u] = codes_bf16<TYPE>(kv[i][u]);
         store_pair(row, 2 * (e & 7), key & 7, u32x4{x[0].x, x[0].y, x[1].x, x[1].y}, u32x4{x[2].x, x[2].y, x[3].x, x[3].y});
       } else {
-        const uint16_t* src = c.tail_keys(bh) + ((j & 1) * kBlk + (key & 63)) * kHD + (e & 7) * 16;
+        const uint16_t* src = c.tail_keys(bh) + ((j & 1) * kBlk + key) * kHD + (e & 7) * 16;
         store_pair(row, 2 * (e & 7), key & 7, ld16(src), ld16(src + 8));
       }
     }
@@ -977,10 +980,9 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     unsigned char* buf = lds + 2 * kPHalf + (turn & 1) * kPHalf;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int e = tid + NT * i;
-      if (UNITS % NT != 0 && e >= UNITS) continue;
-      const int j = block_of(turn, e), d = (e >> 2) & 127;
-      unsigned char* row = buf + (e >> 9) * (kHD * 128) + d * 128;
+      if (beyond(i)) continue;
+      const int e = unit_of(i), j = block_of(turn, i), d = e >> 2;
+      unsigned char* row = buf + half_of(i) * (kHD * 128) + d * 128;
       // 16 keys: the first piece keeps 0-3 and 8-11 (hl = 0), the second 4-7 and 12-15
       if (j < done) {
         u32x2 x[4];
@@ -1029,16 +1031,15 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
       vs = c.vs[bh * c.nblk + kb];
     }
     const unsigned char* sk = lds + (turn & 1) * kPHalf + 64 * hf * 256;
+    st[0] = st[1] = f32x16{};
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      st[kt] = f32x16{};
+    for (int k = 0; k < 8; ++k)
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int kt = 0; kt < 2; ++kt)
         st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
             __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
                                            sk + (32 * kt + r32) * 256 + (((2 * k + hl) ^ (r32 & 7)) << 4))),
             __builtin_bit_cast(bf16x8, qb[k]), st[kt], 0, 0, 0);
-    }
   };
   auto softmax = [&](int turn) {
     const int k0 = kBlk * (2 * turn + hf);
