@@ -896,6 +896,18 @@ constexpr int prefill_lds(int pairs) {
   return merge > 4 * kPHalf ? merge : 4 * kPHalf;
 }
 
+// Orders a run of N products with one LDS read each so that READS reads stay ahead of them.
+template <int N, int READS>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+  for (int i = 0; i < N - READS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, READS, 0);
+}
+
 template <int TYPE, int REP, int RB>
 __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(const PrefillParams p) {
   constexpr int PAIRS = REP * RB;
@@ -1040,6 +1052,7 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
             __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
                                            sk + (32 * kt + r32) * 256 + (((2 * k + hl) ^ (r32 & 7)) << 4))),
             __builtin_bit_cast(bf16x8, qb[k]), st[kt], 0, 0, 0);
+    reads_ahead<16, 4>();
   };
   auto softmax = [&](int turn) {
     const int k0 = kBlk * (2 * turn + hf);
@@ -1097,6 +1110,7 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
             __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(
                                            sv + (32 * dt + r32) * 128 + (((2 * s + hl) ^ (r32 & 7)) << 4))),
             __builtin_bit_cast(bf16x8, pb[s]), o[dt], 0, 0, 0);
+    reads_ahead<16, 4>();
   };
   // K j + 2 and V j + 1 to LDS: the buffers of K j and V j - 1, both read in turn j - 1
   auto stage = [&](int j) {
