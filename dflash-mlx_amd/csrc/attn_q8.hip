@@ -882,6 +882,9 @@ struct PrefillParams {
   int heads, groups;  // launched head groups (Hkv * groups) and groups of a key/value head
   int nblk;           // row blocks
   int xcds;           // XCDs that a launched head group owns (0: groups in order)
+  int splits;         // most workgroups that share a row block's turns
+  float* part_o;      // [splits, B, P, Hq, D] of a split: softmax . v over its keys alone
+  float* part_w;      // [splits, B, P, Hq]: log2 of the sum of its exponentials
   float scale;
 };
 
@@ -890,6 +893,16 @@ constexpr int kPKeys = 2 * kBlk;               // keys of a turn
 constexpr int kPHalf = kPKeys * kHD * 2;       // bytes of one turn's K (or V^T) in bf16
 constexpr int kPMerge = 66 * 64;               // floats of a wave's O, m and l
 constexpr int kPPitch = kHD + 4;               // floats of a normalized row in LDS
+
+constexpr int kSplitTurns = 2;                 // least turns of a split
+
+// Turns of the row block that ends before row `end`, and the splits that share them.
+__device__ __forceinline__ int prefill_turns(const PrefillParams& p, int len, int end) {
+  return len < 0 ? 0 : (min(min(len, p.c.Smax) + min(end, p.P), p.c.Smax) + kPKeys - 1) / kPKeys;
+}
+__device__ __forceinline__ int prefill_splits(const PrefillParams& p, int turns) {
+  return max(1, min(p.splits, turns / kSplitTurns));
+}
 
 constexpr int prefill_lds(int pairs) {
   const int merge = 4 * pairs * (kPMerge + kPRows * kPPitch);
@@ -936,7 +949,10 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
   const int qh = hg * REP + (RB == 1 ? pair : pair % REP);
   const int seen = len < 0 ? 0 : min(base + p.P, c.Smax);  // positions of the cache
   const int done = seen >> 6;
-  const int turns = len < 0 ? 0 : (min(base + min(t0 + RB * kPRows, p.P), c.Smax) + kPKeys - 1) / kPKeys;
+  const int all = prefill_turns(p, len, t0 + RB * kPRows);
+  const int splits = prefill_splits(p, all), split = blockIdx.z;
+  if (split >= splits) return;
+  const int first = all * split / splits, turns = all * (split + 1) / splits;  // this split's: first .. turns - 1
   const int Lw = len >= 0 && (RB == 1 || tw < p.P) ? min(base + min(tw + kPRows, p.P), c.Smax) : 0;
   if (tid == 0) dropped = 0;
   u32x4 kv[PER], vv[PER];
@@ -1011,20 +1027,20 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     }
   };
   u32x4 kv1[PER];
-  load_keys(0, kv);
-  load_values(0);
-  load_keys(1, kv1);
+  load_keys(first, kv);
+  load_values(first);
+  load_keys(first + 1, kv1);
   const QuerySign sign(p.scale);
   const uint16_t* qr = p.q + (((int64_t)b * p.P + min(tw + r32, p.P - 1)) * p.Hq + qh) * kHD + hl * 8;
   u32x4 qb[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) qb[k] = sign(ld16(qr + 16 * k));
   __syncthreads();  // dropped is 0
-  store_keys(0, kv);
-  store_values(0);
-  store_keys(1, kv1);
-  load_keys(2, kv);
-  load_values(1);
+  store_keys(first, kv);
+  store_values(first);
+  store_keys(first + 1, kv1);
+  load_keys(first + 2, kv);
+  load_values(first + 1);
   float m = -INFINITY, l = 0.f;
   f32x16 o[4];
 #pragma unroll
@@ -1120,15 +1136,15 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     load_values(j + 2);
   };
   __syncthreads();
-  if (sees(0)) {
-    scores(0);
-    if (hf == 1) softmax(0);
+  if (sees(first)) {
+    scores(first);
+    if (hf == 1) softmax(first);
   }
-  __syncthreads();  // K 0 is read: its buffer takes K 2
+  __syncthreads();  // the first K is read: its buffer takes the third
   // Turn j: the products of K j + 1 and V j.  The first half's waves do their softmax and
   // staging before them, the second half's after: a SIMD holds one wave of each, and the
   // matrix unit has one's products beside the other's arithmetic.
-  for (int j = 0; j < turns; ++j) {
+  for (int j = first; j < turns; ++j) {
     if (hf == 0) {
       if (sees(j)) softmax(j);
       stage(j);
@@ -1157,11 +1173,13 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
   auto row_of = [&](int e) { return t0 + (RB == 1 ? 0 : (e >> 9) / REP * kPRows) + ((e >> 4) & 31); };
   auto head_of = [&](int e) { return hg * REP + (RB == 1 ? e >> 9 : (e >> 9) % REP); };
   u32x4 gt[OUT];
+  if (splits == 1) {
 #pragma unroll
-  for (int i = 0; i < OUT; ++i) {
-    const int e = tid + NT * i;
-    gt[i] = ld16(p.gate + ((int64_t)b * p.P + min(row_of(e), p.P - 1)) * p.gate_stride + head_of(e) * 2 * kHD + kHD +
-                 (e & 15) * 8);
+    for (int i = 0; i < OUT; ++i) {
+      const int e = tid + NT * i;
+      gt[i] = ld16(p.gate + ((int64_t)b * p.P + min(row_of(e), p.P - 1)) * p.gate_stride + head_of(e) * 2 * kHD + kHD +
+                   (e & 15) * 8);
+    }
   }
   __syncthreads();
   if (hf == 0) {
@@ -1174,6 +1192,8 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     const float inv = ls == 0.f ? 0.f : 1.f / ls;  // 0: the sequence takes no part
     c0 *= inv;
     c1 *= inv;
+    const int64_t part = ((int64_t)split * c.B + b) * p.P;
+    if (splits > 1 && hl == 0 && tw + r32 < p.P) p.part_w[(part + tw + r32) * p.Hq + qh] = mn + __log2f(ls);
     float* row = rows + (pair * kPRows + r32) * kPPitch;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
@@ -1197,11 +1217,54 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
       for (int u = 0; u < 8; ++u)
         row[u] += dropped_values(c, bh, (e & 15) * 8 + u, kBlk * done, min(base + t, seen - 1));
     }
+    if (splits > 1) {
+      float* dst = p.part_o + ((((int64_t)split * c.B + b) * p.P + t) * p.Hq + head_of(e)) * kHD + (e & 15) * 8;
+      *reinterpret_cast<f32x4*>(dst) = *reinterpret_cast<const f32x4*>(row);
+      *reinterpret_cast<f32x4*>(dst + 4) = *reinterpret_cast<const f32x4*>(row + 4);
+      continue;
+    }
     unpack8(gt[i], g);
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = row[u] * (1.f / (1.f + __expf(-g[u])));
     *reinterpret_cast<u32x4*>(p.out + (((int64_t)b * p.P + t) * p.Hq + head_of(e)) * kHD + (e & 15) * 8) = pack8(v);
   }
+}
+
+// The splits of a row joined, gated and stored: 16 lanes a row of a head, 8 features each.
+// A feature that is not finite in a split is so in the row, whatever the split's weight.
+__global__ __launch_bounds__(256) void attn_prefill_q8_merge_kernel(const PrefillParams p, int block_rows) {
+  const int b = blockIdx.y;
+  const int64_t e = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (e >= (int64_t)p.P * p.Hq) return;
+  const int t = (int)(e / p.Hq), h = (int)(e % p.Hq), f = (threadIdx.x & 15) * 8;
+  const int splits = prefill_splits(p, prefill_turns(p, p.lens[b], (t / block_rows + 1) * block_rows));
+  if (splits == 1) return;  // the row is stored
+  const int64_t row = (int64_t)b * p.P * p.Hq + e, step = (int64_t)p.c.B * p.P * p.Hq;
+  const u32x4 gt = ld16(p.gate + ((int64_t)b * p.P + t) * p.gate_stride + h * 2 * kHD + kHD + f);
+  float mx = -INFINITY;
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) mx = fmaxf(mx, p.part_w[k * step + row]);
+  float sum = 0.f;
+  float v[8] = {};
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) {
+    const float w = p.part_w[k * step + row];
+    const float x = w == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w - mx);
+    const float* o = p.part_o + (k * step + row) * kHD + f;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(o), c = *reinterpret_cast<const f32x4*>(o + 4);
+    sum += x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = i < 4 ? a[i & 3] : c[i & 3];
+      v[i] += fabsf(y) < INFINITY ? x * y : y;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  float g[8];
+  unpack8(gt, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (1.f / (1.f + __expf(-g[i])));
+  *reinterpret_cast<u32x4*>(p.out + row * kHD + f) = pack8(v);
 }
 
 // Row blocks of a workgroup: as many as make eight waves, two a SIMD (six with three
@@ -1212,6 +1275,25 @@ template <int TYPE, int REP>
 void launch_prefill(const PrefillParams& p, dim3 grid, hipStream_t s) {
   constexpr int RB = prefill_row_blocks(REP);
   hipLaunchKernelGGL((attn_prefill_q8_kernel<TYPE, REP, RB>), grid, dim3(128 * REP * RB), 0, s, p);
+}
+
+// The launched heads: up to four query heads of a key/value head together.
+int prefill_rep(int per_kv) {
+  int rep = 4;
+  while (per_kv % rep != 0) --rep;
+  return rep;
+}
+
+// Splits of a row block's keys: a workgroup fills a CU and takes its time for a turn
+// whatever the others do, so as many as the rows' workgroups leave CUs for.
+int most_prefill_splits(int64_t wgs, int Smax) {
+  const int64_t cus = device_cus() > 0 ? device_cus() : 256;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({cus / wgs, Smax / kPKeys / kSplitTurns, 64}));
+}
+
+int prefill_splits_of(int64_t B, int64_t P, int Hq, int Hkv, int Smax) {
+  const int rep = prefill_rep(Hq / Hkv);
+  return most_prefill_splits(B * ceil_div(P, kPRows * prefill_row_blocks(rep)) * (Hq / rep), Smax);
 }
 
 template <int TYPE>
@@ -1278,9 +1360,15 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   return to_status(hipGetLastError());
 }
 
+extern "C" size_t dflash_attn_prefill_q8_workspace_bytes(int B, int P, int Hq, int Hkv, int Smax) {
+  if (B <= 0 || P <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || Hq / Hkv > 16 || Smax <= 0 || Smax % kBlk != 0) return 0;
+  const int splits = prefill_splits_of(B, P, Hq, Hkv, Smax);
+  return splits == 1 ? 0 : (size_t)splits * B * P * Hq * (kHD + 1) * sizeof(float);
+}
+
 extern "C" int dflash_attn_prefill_q8(const dflash_kv8_cache* cache, const void* q, const int32_t* lens,
                                       const void* gate_src, int64_t gate_row_stride, void* out, int P, int Hq,
-                                      float scale, void* stream) {
+                                      float scale, void* workspace, size_t workspace_bytes, void* stream) {
   PrefillParams p{};
   if (const int rc = check_cache(cache, &p.c)) return rc;
   const int B = p.c.B, Hkv = p.c.Hkv;
@@ -1290,9 +1378,11 @@ extern "C" int dflash_attn_prefill_q8(const dflash_kv8_cache* cache, const void*
   if (q == nullptr || lens == nullptr || gate_src == nullptr || out == nullptr) return DFLASH_ERR_NULL;
   if (((uintptr_t)q & 15) || ((uintptr_t)gate_src & 15) || gate_row_stride % 8 || ((uintptr_t)out & 15))
     return DFLASH_ERR_ALIGN;
-  // the launched heads: up to four query heads of a key/value head together
-  int rep = 4;
-  while (Hq / Hkv % rep != 0) --rep;
+  if (workspace != nullptr) {
+    if ((uintptr_t)workspace & 15) return DFLASH_ERR_ALIGN;
+    if (workspace_bytes < dflash_attn_prefill_q8_workspace_bytes(B, P, Hq, Hkv, p.c.Smax)) return DFLASH_ERR_WORKSPACE;
+  }
+  const int rep = prefill_rep(Hq / Hkv);
   p.q = static_cast<const uint16_t*>(q);
   p.lens = lens;
   p.gate = static_cast<const uint16_t*>(gate_src);
@@ -1306,9 +1396,16 @@ extern "C" int dflash_attn_prefill_q8(const dflash_kv8_cache* cache, const void*
   p.scale = scale;
   const int64_t wgs = p.xcds ? 8 * ceil_div(p.nblk, p.xcds) : (int64_t)p.nblk * p.heads;
   if (wgs > INT32_MAX) return DFLASH_ERR_SHAPE;
-  const dim3 grid((unsigned)wgs, (unsigned)B);
+  p.splits = workspace == nullptr ? 1 : prefill_splits_of(B, P, Hq, Hkv, p.c.Smax);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_w = p.part_o + (int64_t)p.splits * B * P * Hq * kHD;
+  const dim3 grid((unsigned)wgs, (unsigned)B, (unsigned)p.splits);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache->type == DFLASH_KV_INT8) launch_prefill<DFLASH_KV_INT8>(p, rep, grid, s);
   else launch_prefill<DFLASH_KV_E4M3>(p, rep, grid, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return to_status(e);
+  hipLaunchKernelGGL(attn_prefill_q8_merge_kernel, dim3((unsigned)ceil_div((int64_t)P * Hq, 16), (unsigned)B), dim3(256),
+                     0, s, p, kPRows * prefill_row_blocks(rep));
   return to_status(hipGetLastError());
 }

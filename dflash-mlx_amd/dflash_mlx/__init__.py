@@ -30,6 +30,7 @@ from .gated_delta import (
 from .kv8 import (
     QuantizedKVCache,
     attn_prefill_q8,
+    attn_prefill_q8_workspace_bytes,
     attn_prep_q8,
     attn_verify_q8,
     attn_verify_q8_workspace_bytes,
@@ -74,6 +75,7 @@ __all__ = [
     "adapter_for_model_type",
     "advance_gated_delta_states",
     "attn_prefill_q8",
+    "attn_prefill_q8_workspace_bytes",
     "attn_prep_q8",
     "attn_verify_q8",
     "attn_verify_q8_workspace_bytes",

@@ -120,8 +120,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dflash_attn_verify_q8_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
     "dflash_attn_verify_q8": (
         _I, [_VP, _VP, _VP, _VP, _I64, _VP, _I, _I, ctypes.c_float, _VP, _SZ, _VP]),
+    "dflash_attn_prefill_q8_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
     "dflash_attn_prefill_q8": (
-        _I, [_VP, _VP, _VP, _VP, _I64, _VP, _I, _I, ctypes.c_float, _VP]),
+        _I, [_VP, _VP, _VP, _VP, _I64, _VP, _I, _I, ctypes.c_float, _VP, _SZ, _VP]),
     "dflash_commit_accept": (_I, [_VP, _VP, _VP, _I, _I, _VP]),
     "dflash_greedy_accept_workspace_bytes": (_SZ, [_I, _I, _I]),
     "dflash_greedy_accept_noalloc_max_bytes": (_SZ, []),

@@ -275,6 +275,11 @@ def attn_verify_q8(q, cache: QuantizedKVCache, lens, proj, *, scale: float | Non
     return out
 
 
+def attn_prefill_q8_workspace_bytes(B: int, P: int, num_heads: int, Hkv: int, Smax: int) -> int:
+    """Bytes of attn_prefill_q8's workspace: 0 where the rows alone fill the device."""
+    return int(_lib.load().dflash_attn_prefill_q8_workspace_bytes(B, P, num_heads, Hkv, Smax))
+
+
 def attn_prefill_q8(q, cache: QuantizedKVCache, lens, proj, *, scale: float | None = None):
     """attn_verify_q8 over the P rows a sequence that attn_prep_q8 (prompt=True)
     appended at lens[b]: row i sees positions 0 .. lens[b] + i."""
@@ -283,9 +288,12 @@ def attn_prefill_q8(q, cache: QuantizedKVCache, lens, proj, *, scale: float | No
     P, Hq = _check_queries(q, cache)
     row = _row_stride("proj", proj, cache, P, 2 * Hq * HEAD_DIM)
     out = torch.empty((cache.B, P, Hq * HEAD_DIM), dtype=torch.bfloat16, device=cache.device)
+    n = attn_prefill_q8_workspace_bytes(cache.B, P, Hq, cache.Hkv, cache.Smax)
+    workspace = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
     q = _aligned(q)
     _call("dflash_attn_prefill_q8", cache.device, cache._ptr, q.data_ptr(), lens.data_ptr(), proj.data_ptr(), row,
-          out.data_ptr(), P, Hq, HEAD_DIM ** -0.5 if scale is None else float(scale))
+          out.data_ptr(), P, Hq, HEAD_DIM ** -0.5 if scale is None else float(scale),
+          workspace.data_ptr() if n else None, n)
     return out
 
 

@@ -240,6 +240,7 @@ class HybridPrefill:
         self.run, self.cfg = runner, cfg
         self.max_rows = int(max_rows)
         self.rows_cap = 0
+        self.kv_ws = torch.empty(0, dtype=torch.uint8, device=runner.device)  # attention over the 8-bit cache
         self._lib = _lib.load()
         self.cus = torch.cuda.get_device_properties(runner.device).multi_processor_count
         self._weights()
@@ -382,6 +383,11 @@ class HybridPrefill:
         scan_strides = (ctypes.c_int64 * 13)(P * C, C, Dk, P * C, C, Dk, P * C, C, Dv,
                                              P * Hv, Hv, P * Hv, Hv)
         arows = cfg.attn_proj_rows
+        if run.kv:
+            n = self._lib.dflash_attn_prefill_q8_workspace_bytes(1, P, Hq, Hkv, run.Smax)
+            if self.kv_ws.numel() < n:
+                self.kv_ws = torch.empty(n, dtype=torch.uint8, device=run.device)
+            kv_ws = (self.kv_ws.data_ptr(), self.kv_ws.numel())
         gi = ai = 0
         for i in range(L):
             lw, tw = layers[i], self.w[i]
@@ -411,7 +417,7 @@ class HybridPrefill:
                          run.overflow.data_ptr(), P, Hq, cfg.rot_dims, float(cfg.rope_theta), eps, 1,
                          stream)
                     call("dflash_attn_prefill_q8", kv, self.q.data_ptr(), run.lens.data_ptr(), ap,
-                         arows, self.attn_out.data_ptr(), P, Hq, float(D ** -0.5), stream)
+                         arows, self.attn_out.data_ptr(), P, Hq, float(D ** -0.5), *kv_ws, stream)
                 else:
                     call("dflash_attn_prep", ap, arows, lw["q_norm"].data_ptr(), lw["k_norm"].data_ptr(),
                          run.lens.data_ptr(), run.k_cache[ai].data_ptr(), run.vt_cache[ai].data_ptr(),

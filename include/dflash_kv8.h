@@ -114,8 +114,8 @@ int dflash_kv8_read(const dflash_kv8_cache* cache, const int32_t* lens,
  *   out[b, t, h*128 ..] = bf16(softmax(scale * q k^T) v * sigmoid(gate))
  * with the gate of head h at h*256 + 128 of row b*T + t of gate_src.  T * Hq / Hkv
  * <= 64.  workspace: dflash_attn_verify_q8_workspace_bytes bytes (enough for any
- * smaller T and Hq too), its first 4 * B * Hkv bytes zero before the first call (every call leaves them
- * zero), not shared by calls that overlap in time.
+ * smaller T and Hq too), its first 4 * B * Hkv bytes zero before the first call
+ * (every call leaves them zero), not shared by calls that overlap in time.
  */
 size_t dflash_attn_verify_q8_workspace_bytes(int B, int T, int Hq, int Hkv,
                                              int Smax);
@@ -128,12 +128,17 @@ int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* q,
 /*
  * The same over P prompt rows a sequence that dflash_kv8_append (prompt != 0) has put
  * at lens[b]: row i attends to positions 0 .. lens[b] + i.  q [B, P, Hq, 128],
- * out [B, P, Hq*128].  No workspace.
+ * out [B, P, Hq*128].  workspace: dflash_attn_prefill_q8_workspace_bytes bytes for
+ * these sizes, of any content, not shared by calls that overlap in time: few rows have
+ * their keys split over workgroups, which meet there.  NULL (or 0 bytes needed): no split.
  */
+size_t dflash_attn_prefill_q8_workspace_bytes(int B, int P, int Hq, int Hkv,
+                                              int Smax);
 int dflash_attn_prefill_q8(const dflash_kv8_cache* cache, const void* q,
                            const int32_t* lens, const void* gate_src,
                            int64_t gate_row_stride, void* out, int P, int Hq,
-                           float scale, void* stream);
+                           float scale, void* workspace, size_t workspace_bytes,
+                           void* stream);
 
 #ifdef __cplusplus
 }

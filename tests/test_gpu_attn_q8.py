@@ -99,6 +99,70 @@ def test_prompt(device, dtype, T, Hq, Hkv, lens, Smax):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Hq,Hkv,lens,Smax", [
+    (1, 4, 1, [3900], 4032),              # one row block: as many splits as turns allow
+    (33, 16, 4, [2000, 130, -1, 0], 2112),  # sequences of many splits, of two, of one and none
+    (600, 8, 4, [700], 1344),
+    (70, 3, 1, [1900, 1980], 1984),
+    (129, 4, 4, [1500], 1664),
+])
+def test_prompt_with_split_keys(device, dtype, T, Hq, Hkv, lens, Smax):
+    import dflash_mlx as dm
+
+    assert dm.attn_prefill_q8_workspace_bytes(len(lens), T, Hq, Hkv, Smax) > 0
+    _check(device, dtype, T, Hq, Hkv, lens, Smax, seed=T + Hq + len(lens), prompt=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_split_keys_that_are_not_finite(device, dtype):
+    """An infinite value is in its rows whatever its split weighs, a NaN block in the
+    rows of every split that joins it, and neither in other rows."""
+    import dflash_mlx as dm
+
+    T, Hq, Hkv, L = 40, 4, 2, 1100
+    cache, lens_d, k, v, q, proj, ends = _case(device, dtype, T, Hq, Hkv, [L], 1216, 5, True)
+    attend = lambda: dm.attn_prefill_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(T, Hq, D)  # noqa: E731
+    clean = attend()
+    cache.tail_vt[0, 1, 17, 1120 % SLOTS] = float("inf")
+    cache.tail_k[0, 1, 1120 % SLOTS] = -8 * q[0, 25, 2].to(device)  # its weight in row 25 of head 2 underflows
+    got = attend()
+    assert got[20:, 2:, 17].isinf().sum() >= 1 and not torch.isfinite(got[20:, 2:, 17].float()).any()
+    assert torch.equal(got[:20], clean[:20]) and torch.equal(got[:, :2], clean[:, :2])
+    assert torch.isfinite(got[20:, 2:, :17].float()).all() and torch.isfinite(got[20:, 2:, 18:].float()).all()
+    for t in (cache.tail_vt, cache.tail_k):
+        t.nan_to_num_(posinf=0.5)
+    cache.v_scale[0, 0, 2] = float("nan")
+    assert attend()[:, :2].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_split_prompt_captured_and_on_two_streams(device, dtype):
+    import dflash_mlx as dm
+
+    T, Hq, Hkv, lens = 50, 8, 2, [1500, 200]
+    cache, lens_d, k, v, q, proj, ends = _case(device, dtype, T, Hq, Hkv, lens, 1600, 9, True)
+    qd, pd = q.to(device), proj.to(device)
+    attend = lambda: dm.attn_prefill_q8(qd, cache, lens_d, pd)  # noqa: E731
+    want = attend()
+    torch.cuda.synchronize()
+    outs, streams = [], [torch.cuda.Stream(device) for _ in range(2)]
+    for i in range(8):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(attend())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = attend()
+    for _ in range(3):
+        captured.zero_()
+        graph.replay()
+        assert torch.equal(attend(), want)
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("prompt", [False, True])
 @pytest.mark.parametrize("scale", [0.5, -0.1, 0.0])
 def test_scales(device, dtype, prompt, scale):

@@ -38,8 +38,8 @@ def _verify(lib, c, q=P, lens=P, gate=P, stride=32 * 128, out=P, T=4, Hq=16, ws=
     return lib.dflash_attn_verify_q8(ctypes.addressof(c), q, lens, gate, stride, out, T, Hq, 0.1, ws, nbytes, None)
 
 
-def _prefill(lib, c, q=P, lens=P, gate=P, stride=32 * 128, out=P, T=40, Hq=16):
-    return lib.dflash_attn_prefill_q8(ctypes.addressof(c), q, lens, gate, stride, out, T, Hq, 0.1, None)
+def _prefill(lib, c, q=P, lens=P, gate=P, stride=32 * 128, out=P, T=40, Hq=16, ws=None, nbytes=0):
+    return lib.dflash_attn_prefill_q8(ctypes.addressof(c), q, lens, gate, stride, out, T, Hq, 0.1, ws, nbytes, None)
 
 
 def _read(lib, c, lens=P, count=5, k=P, v=P):
@@ -57,7 +57,8 @@ def test_every_declared_entry_point_is_exported_and_bound(lib):
     text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "dflash_kv8.h").read_text(), flags=re.S)
     names = set(re.findall(r"\b(dflash_[a-z0-9_]+)\s*\(", text))
     assert names == {"dflash_kv8_append", "dflash_kv8_load", "dflash_kv8_read", "dflash_attn_verify_q8",
-                     "dflash_attn_verify_q8_workspace_bytes", "dflash_attn_prefill_q8"}
+                     "dflash_attn_verify_q8_workspace_bytes", "dflash_attn_prefill_q8",
+                     "dflash_attn_prefill_q8_workspace_bytes"}
     for name in names:
         assert hasattr(lib, name) and name in _lib.SIGNATURES
 
@@ -121,6 +122,21 @@ def test_prefill_refusals(lib):
     assert _prefill(lib, c, gate=P + 8) == ALIGN
     assert _prefill(lib, _cache(B=65536)) == SHAPE
     assert _prefill(lib, c, T=0) == 0
+
+
+def test_prefill_workspace(lib):
+    need = lib.dflash_attn_prefill_q8_workspace_bytes
+    # one row block of four head groups over 32 turns of keys: split; a device's worth of row blocks: not
+    n = need(1, 40, 16, 4, 4096)
+    assert n > 0 and n % (40 * 16 * 129 * 4) == 0
+    assert need(1, 100000, 16, 4, 4096) == 0 and need(64, 200, 16, 4, 4096) == 0
+    assert need(1, 40, 16, 4, 256) == 0  # too few turns
+    for bad in ((0, 40, 16, 4, 4096), (1, 0, 16, 4, 4096), (1, 40, 16, 0, 4096), (1, 40, 15, 4, 4096), (1, 40, 68, 4, 4096),
+                (1, 40, 16, 4, 100), (1, 40, 16, 4, 0), (1, 40, 0, 4, 4096)):
+        assert need(*bad) == 0, bad
+    c = _cache(B=1, Smax=4096)
+    assert _prefill(lib, c, ws=P, nbytes=n - 1) == WORKSPACE
+    assert _prefill(lib, c, ws=P + 8, nbytes=n) == ALIGN
 
 
 def test_read_and_load_refusals(lib):
