@@ -891,7 +891,7 @@ struct PrefillParams {
 constexpr int kPRows = 32;                     // query rows of a wave
 constexpr int kPKeys = 2 * kBlk;               // keys of a turn
 constexpr int kPHalf = kPKeys * kHD * 2;       // bytes of one turn's K (or V^T) in bf16
-constexpr int kPMerge = 66 * 64;               // floats of a wave's O, m and l
+constexpr int kPMerge = 68 * 64;               // floats that the two waves of a row tile exchange
 constexpr int kPPitch = kHD + 4;               // floats of a normalized row in LDS
 
 constexpr int kSplitTurns = 2;                 // least turns of a split
@@ -903,6 +903,10 @@ __device__ __forceinline__ int prefill_turns(const PrefillParams& p, int len, in
 __device__ __forceinline__ int prefill_splits(const PrefillParams& p, int turns) {
   return max(1, min(p.splits, turns / kSplitTurns));
 }
+
+// The reciprocal is off by one unit in the last place of 32 bits, under a 2^16th of the
+// rounding of the bf16 result.
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
 
 constexpr int prefill_lds(int pairs) {
   const int merge = 4 * pairs * (kPMerge + kPRows * kPPitch);
@@ -955,6 +959,9 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
   const int first = all * split / splits, turns = all * (split + 1) / splits;  // this split's: first .. turns - 1
   const int Lw = len >= 0 && (RB == 1 || tw < p.P) ? min(base + min(tw + kPRows, p.P), c.Smax) : 0;
   if (tid == 0) dropped = 0;
+  constexpr int OUT = PAIRS * kPRows * 16 / NT;  // pieces of 8 features of the rows a thread loads and stores
+  auto row_of = [&](int e) { return t0 + (RB == 1 ? 0 : (e >> 9) / REP * kPRows) + ((e >> 4) & 31); };
+  auto head_of = [&](int e) { return hg * REP + (RB == 1 ? e >> 9 : (e >> 9) % REP); };
   u32x4 kv[PER], vv[PER];
   // K unit e: key e / 8, features 16 (e % 8) ..; V^T unit e: block e / 512, feature
   // (e / 4) % 128, keys 16 (e % 4) ..  A wave's 64 units lie in one block of the turn,
@@ -1026,16 +1033,29 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
       }
     }
   };
-  u32x4 kv1[PER];
+  // The queries' rows come whole, 16 lanes a row, and are read back from LDS as the
+  // products take them; they stand in the buffer of V first + 1.
+  unsigned char* sq = lds + 2 * kPHalf + ((first + 1) & 1) * kPHalf;
+  const QuerySign sign(p.scale);
+  u32x4 qv[OUT], kv1[PER];
+#pragma unroll
+  for (int i = 0; i < OUT; ++i) {
+    const int e = tid + NT * i;
+    qv[i] = ld16(p.q + (((int64_t)b * p.P + min(row_of(e), p.P - 1)) * p.Hq + head_of(e)) * kHD + (e & 15) * 8);
+  }
   load_keys(first, kv);
   load_values(first);
   load_keys(first + 1, kv1);
-  const QuerySign sign(p.scale);
-  const uint16_t* qr = p.q + (((int64_t)b * p.P + min(tw + r32, p.P - 1)) * p.Hq + qh) * kHD + hl * 8;
+#pragma unroll
+  for (int i = 0; i < OUT; ++i) {
+    const int e = tid + NT * i;
+    *reinterpret_cast<u32x4*>(sq + (e >> 4) * 256 + (((e & 15) ^ ((e >> 4) & 7)) << 4)) = sign(qv[i]);
+  }
+  __syncthreads();  // the queries are there, and dropped is 0
   u32x4 qb[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) qb[k] = sign(ld16(qr + 16 * k));
-  __syncthreads();  // dropped is 0
+  for (int k = 0; k < 8; ++k)
+    qb[k] = *reinterpret_cast<const u32x4*>(sq + (pair * kPRows + r32) * 256 + (((2 * k + hl) ^ (r32 & 7)) << 4));
   store_keys(first, kv);
   store_values(first);
   store_keys(first + 1, kv1);
@@ -1157,33 +1177,37 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     }
     __syncthreads();
   }
-  // The second key half's sums go to the first through LDS, which leaves the
-  // normalized rows there; every wave then gates and stores whole rows.
+  int te = tid;  // its rows' addresses are computed again rather than kept through the turns
+  asm volatile("" : "+v"(te));
+  // The two waves of a row tile exchange halves of their sums through LDS, which each
+  // merges and leaves there as normalized rows; every wave then gates and stores whole rows.
   float* red = reinterpret_cast<float*>(lds) + pair * kPMerge + lane;
   float* rows = reinterpret_cast<float*>(lds) + PAIRS * kPMerge;  // [PAIRS][32][kPPitch]
-  if (hf == 1) {
+  auto give = [&](const f32x16& x, const f32x16& y) {
+    float* to = red + hf * (34 * 64);
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) red[(16 * dt + i) * 64] = o[dt][i];
-    red[64 * 64] = m;
-    red[65 * 64] = l;
-  }
-  constexpr int OUT = PAIRS * kPRows * 16 / NT;  // pieces of 8 features a thread stores
-  auto row_of = [&](int e) { return t0 + (RB == 1 ? 0 : (e >> 9) / REP * kPRows) + ((e >> 4) & 31); };
-  auto head_of = [&](int e) { return hg * REP + (RB == 1 ? e >> 9 : (e >> 9) % REP); };
+    for (int i = 0; i < 16; ++i) {
+      to[i * 64] = x[i];
+      to[(16 + i) * 64] = y[i];
+    }
+    to[32 * 64] = m;
+    to[33 * 64] = l;
+  };
+  if (hf == 0) give(o[2], o[3]);
+  else give(o[0], o[1]);
   u32x4 gt[OUT];
   if (splits == 1) {
 #pragma unroll
     for (int i = 0; i < OUT; ++i) {
-      const int e = tid + NT * i;
+      const int e = te + NT * i;
       gt[i] = ld16(p.gate + ((int64_t)b * p.P + min(row_of(e), p.P - 1)) * p.gate_stride + head_of(e) * 2 * kHD + kHD +
                    (e & 15) * 8);
     }
   }
   __syncthreads();
-  if (hf == 0) {
-    const float m1 = red[64 * 64], l1 = red[65 * 64];
+  {
+    const float* from = red + (1 - hf) * (34 * 64);
+    const float m1 = from[32 * 64], l1 = from[33 * 64];
     const float mn = fmaxf(m, m1);
     float c0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
     float c1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - mn);
@@ -1193,22 +1217,29 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     c0 *= inv;
     c1 *= inv;
     const int64_t part = ((int64_t)split * c.B + b) * p.P;
-    if (splits > 1 && hl == 0 && tw + r32 < p.P) p.part_w[(part + tw + r32) * p.Hq + qh] = mn + __log2f(ls);
-    float* row = rows + (pair * kPRows + r32) * kPPitch;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+    if (splits > 1 && hf == 0 && hl == 0 && tw + r32 < p.P) p.part_w[(part + tw + r32) * p.Hq + qh] = mn + __log2f(ls);
+    float* row = rows + (pair * kPRows + r32) * kPPitch + 64 * hf + 4 * hl;
+    auto merge = [&](const f32x16& x, int dt) {
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = o[dt][4 * i4 + e] * c0 + red[(16 * dt + 4 * i4 + e) * 64] * c1;
-        *reinterpret_cast<f32x4*>(row + 32 * dt + 8 * i4 + 4 * hl) = v;
+        for (int e = 0; e < 4; ++e) v[e] = x[4 * i4 + e] * c0 + from[(16 * dt + 4 * i4 + e) * 64] * c1;
+        *reinterpret_cast<f32x4*>(row + 32 * dt + 8 * i4) = v;
       }
+    };
+    if (hf == 0) {
+      merge(o[0], 0);
+      merge(o[1], 1);
+    } else {
+      merge(o[2], 0);
+      merge(o[3], 1);
+    }
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < OUT; ++i) {
-    const int e = tid + NT * i, t = row_of(e);
+    const int e = te + NT * i, t = row_of(e);
     if (t >= p.P) continue;
     float* row = rows + (e >> 4) * kPPitch + (e & 15) * 8;
     float g[8], v[8];
@@ -1225,7 +1256,7 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     }
     unpack8(gt[i], g);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = row[u] * (1.f / (1.f + __expf(-g[u])));
+    for (int u = 0; u < 8; ++u) v[u] = row[u] * sigmoid(g[u]);
     *reinterpret_cast<u32x4*>(p.out + (((int64_t)b * p.P + t) * p.Hq + head_of(e)) * kHD + (e & 15) * 8) = pack8(v);
   }
 }
@@ -1263,7 +1294,7 @@ __global__ __launch_bounds__(256) void attn_prefill_q8_merge_kernel(const Prefil
   float g[8];
   unpack8(gt, g);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (1.f / (1.f + __expf(-g[i])));
+  for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * sigmoid(g[i]);
   *reinterpret_cast<u32x4*>(p.out + row * kHD + f) = pack8(v);
 }
 
