@@ -27,7 +27,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 //   - A block's key scale is one factor of its scores; its value scale goes into
 //     the exponent (weights 2^(x + log2 scale - m), m the running maximum of that),
 //     and the sum takes the weights times 1 / scale.
-//   - Weights are rounded to bf16 for P V; the maximum's is 1 exactly.
+//   - Weights are rounded to bf16 for P V (the codes are exact in it): off by at most
+//     2^-8 of themselves, where the codes are by 2^-8 of the block's largest value (int8)
+//     or 2^-4 of their own (e4m3).  Sums, maxima and outputs stay in fp32.
+// Every position's 256 bytes of codes are read once, which bounds the kernel where rows
+// are few: 32 sequences of up to 8191 positions (16 heads on 4, one token, int8), 204 MB
+// in 46 us, 4.4 TB/s of the 5.2 that a large copy reaches.
 struct VerifyParams {
   Kv8 c;
   const uint16_t* q;  // [B, T, Hq, D]
@@ -69,8 +74,11 @@ __device__ __forceinline__ int wave_scan(int x) {
 // workgroup's even share, at least min_cut.  Where every head cut into pieces of at most
 // that gives no more pieces than workgroups, a workgroup takes one piece of one head
 // (`pieces`); otherwise all blocks, in order of sequence and head, are cut into runs of
-// the even share, which cross from head to head.  Units: pieces, or blocks.  Lane i of chunk c has sequence 64 c + i; up to
-// 64 sequences are loaded once and stay in the lanes.
+// the even share, which cross from head to head.  Pieces have a part each and are merged
+// in even numbers (16 tokens after 4096: 15.7 us, as runs 17.7); runs fill the device
+// where heads do not divide it (12 sequences of 8 heads: 21.4 us).  Units: pieces, or
+// blocks.  Lane i of chunk c has sequence 64 c + i; up to 64 sequences are loaded once and
+// stay in the lanes.
 struct Batch {
   const VerifyParams& p;
   int len, incl;  // of the first chunk: lengths, and units of one head up to and with the lane's
@@ -287,14 +295,16 @@ struct Merged {
 // Operand row i of K's tile n is position 16 (i / 4) + 8 (n / 2) + 4 (n % 2) + i % 4,
 // so that result rows 4 g + e of tiles 2 s and 2 s + 1 are positions 16 g + 8 s .. + 7,
 // the ones whose values lie side by side in a row of V^T.  The next block's keys
-// are loaded once these are consumed, its values likewise.
+// are loaded once these are consumed, its values likewise: 16 KB a wave in flight, and no
+// barrier before the merge.  Few rows leave the matrix unit idle anyway; what counts is
+// bytes in flight.
 constexpr int kWaves16 = 8;
 constexpr int kPartsAhead = 8;
 
 // Parts of up to 16 rows are merged by the workgroup that brings the last one: stored and
 // loaded at agent scope, counted after the stores are acknowledged (the protocol and the
 // hardware ordering that it rests on are in device_common.h).  In order of their runs,
-// whichever comes last.
+// whichever comes last.  A second launch instead: 17.9 us against 11.2 (1 token after 500).
 __device__ __forceinline__ void store_part(float* base, int64_t i, float x, float y) {
   __hip_atomic_store(reinterpret_cast<uint64_t*>(base) + i,
                      (uint64_t)__float_as_uint(x) | ((uint64_t)__float_as_uint(y) << 32), __ATOMIC_RELAXED,
@@ -305,7 +315,6 @@ __device__ __forceinline__ f32x2 load_part(const float* base, int64_t i) {
                                        __HIP_MEMORY_SCOPE_AGENT);
   return f32x2{__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32))};
 }
-
 
 template <int TYPE>
 __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel(const VerifyParams p) {
@@ -569,6 +578,11 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
 // (lane / 32) + i % 4 of its half in result element i).  All waves read the same
 // block: its codes are loaded once, a block ahead, and become bf16 on their way
 // to the other of two LDS buffers, as the prompt kernel's.
+// 16 tokens after 131000 (16 heads on 4, int8): 40 us and 8 us of merge for 134 MB and
+// 17.2 GFLOP.  Two waves a SIMD go through conversion, barrier, scores, softmax and
+// products block by block, 1.9 us each, and that chain bounds it: two blocks ahead (46.6
+// us a call against 45.9), four LDS reads ahead of the products and the scales in lanes
+// (no change) left it alone; codes straight to every wave's registers took 50.2.
 template <int TYPE, int RT>
 __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(const VerifyParams p) {
   constexpr int NT = 128 * RT, PER = kBlk * kHD / 16 / NT;
@@ -831,8 +845,11 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kerne
   if (live) store_gated(p, (int64_t)b * p.T + t, qh, d, a.o * (1.f / a.l));
 }
 
-// Rows of a part; blocks of a piece where there are few; workgroups: what the device holds at a time,
-// or fewer for a small cache.
+// Rows of a part: the least tile that holds them.  One tile larger, us a call: up to 16
+// rows 13.8 for 11.1 (1 token after 500), 72.5 for 46.3 (32 sequences after 8191); up to
+// 32 rows 47.4 for 41.5 (8 sequences of 8 tokens after 16000, 16 heads on 4).
+// Blocks of a piece where there are few: 2 (16 tokens after 4096: 16.5 us; 1: 17.1, 4:
+// 17.0, 6: 17.6).  Workgroups: what the device holds at a time, or fewer for a small cache.
 struct VerifyShape {
   int part_rows, min_cut, runs;
 };
@@ -871,6 +888,13 @@ void launch_verify(const VerifyParams& p, hipStream_t s) {
 //   - A turn's codes are loaded once per workgroup, a turn ahead, and become bf16 on
 //     their way to the other of two LDS buffers: 16-byte piece c of row r at slot
 //     c ^ (r % 8).
+//   - Weights are rounded to bf16 for P V, as in the verify kernel.
+// 4 D operations a pair of positions bound it.  16 heads on 4, e4m3: 4096 rows 86 us, 803
+// TFLOP/s; 2048 rows after 14336 273 us, 942 TFLOP/s; a large library product of bf16
+// reaches 1300.  int8 takes 92 us for 4096 rows (its bytes take more instructions to
+// become bf16).  A turn takes 5000 cycles, of which the matrix unit works 2048; one wave's
+// softmax (1400) and staging (1100) run beside the other's products, and what is left over
+// is the wait for LDS and for the slower wave at the barrier.
 struct PrefillParams {
   Kv8 c;
   const uint16_t* q;  // [B, P, Hq, D]
@@ -894,7 +918,9 @@ constexpr int kPHalf = kPKeys * kHD * 2;       // bytes of one turn's K (or V^T)
 constexpr int kPMerge = 68 * 64;               // floats that the two waves of a row tile exchange
 constexpr int kPPitch = kHD + 4;               // floats of a normalized row in LDS
 
-constexpr int kSplitTurns = 2;                 // least turns of a split
+// Least turns of a split: 2 (600 rows after 1000 29.2 us, 64 after 500 17.5, 300 alone
+// 14.4; 1: 29.3, 17.0, 15.4; 4: 30.0, 18.7, 14.4).
+constexpr int kSplitTurns = 2;
 
 // Turns of the row block that ends before row `end`, and the splits that share them.
 __device__ __forceinline__ int prefill_turns(const PrefillParams& p, int len, int end) {
@@ -913,7 +939,9 @@ constexpr int prefill_lds(int pairs) {
   return merge > 4 * kPHalf ? merge : 4 * kPHalf;
 }
 
-// Orders a run of N products with one LDS read each so that READS reads stay ahead of them.
+// Orders a run of N products with one LDS read each so that READS reads stay ahead of them
+// (2048 rows after 14336: 289 us as the compiler orders them, 277 with two, 276 with
+// four, 278 with six).
 template <int N, int READS>
 __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
@@ -1263,6 +1291,7 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
 
 // The splits of a row joined, gated and stored: 16 lanes a row of a head, 8 features each.
 // A feature that is not finite in a split is so in the row, whatever the split's weight.
+// Bound by the fp32 rows, read once: 600 rows of 16 heads in three splits, 14.7 MB, 5.6 us.
 __global__ __launch_bounds__(256) void attn_prefill_q8_merge_kernel(const PrefillParams p, int block_rows) {
   const int b = blockIdx.y;
   const int64_t e = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -1299,7 +1328,8 @@ __global__ __launch_bounds__(256) void attn_prefill_q8_merge_kernel(const Prefil
 }
 
 // Row blocks of a workgroup: as many as make eight waves, two a SIMD (six with three
-// heads), as in the bf16 cache's kernel.
+// heads), as in the bf16 cache's kernel.  600 rows after 1000 on two heads a workgroup, four
+// waves: 46.5 us for 39.5 (before keys were split).
 constexpr int prefill_row_blocks(int rep) { return rep == 1 ? 4 : rep == 2 ? 2 : 1; }
 
 template <int TYPE, int REP>
@@ -1316,7 +1346,9 @@ int prefill_rep(int per_kv) {
 }
 
 // Splits of a row block's keys: a workgroup fills a CU and takes its time for a turn
-// whatever the others do, so as many as the rows' workgroups leave CUs for.
+// whatever the others do, so as many as the rows' workgroups leave CUs for.  Unsplit, 512
+// rows after 32256 took 488 us for 153, 100 after 8000 132 for 35; more splits than one
+// round of the device holds are slower where rows see few keys (1500 rows: 51 us for 33).
 int most_prefill_splits(int64_t wgs, int Smax) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   return (int)std::max<int64_t>(1, std::min<int64_t>({cus / wgs, Smax / kPKeys / kSplitTurns, 64}));
@@ -1423,6 +1455,7 @@ extern "C" int dflash_attn_prefill_q8(const dflash_kv8_cache* cache, const void*
   p.heads = Hq / rep;
   p.groups = p.heads / Hkv;
   p.nblk = (int)ceil_div(P, kPRows * prefill_row_blocks(rep));
+  // an XCD keeps to one head group, whose codes stay in its L2: 4096 rows 89 us, groups in order 124
   p.xcds = 8 % p.heads == 0 ? 8 / p.heads : 0;
   p.scale = scale;
   const int64_t wgs = p.xcds ? 8 * ceil_div(p.nblk, p.xcds) : (int64_t)p.nblk * p.heads;
