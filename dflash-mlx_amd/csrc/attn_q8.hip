@@ -232,12 +232,34 @@ struct QuerySign {
 };
 __device__ __forceinline__ float positive_scale(float scale) { return (scale == 0.f ? 1.f : fabsf(scale)) * kLog2e; }
 
+// A block's value scale as the weights take it: lv, its logarithm, goes into the weights'
+// exponent; lc, the same no further out than 2^-40 and 2^40, into the running maximum's; iv =
+// 2^-lc is what the sum takes its weights times.  Past 2^-40 or 2^40 (`apart`) the sum's are
+// of their own, 2^(lc - lv) of those for P V: or weights that count in it would be lost
+// beside a block of 2^100 times their scale (values that are all zero have 2^-107).  NaN
+// stays NaN.
+constexpr int kMostScale = 40;
+struct ValueScale {
+  float lv, lc, iv;
+  bool apart;
+  __device__ __forceinline__ explicit ValueScale(float vs) {
+    lc = lv = __log2f(vs);
+    iv = __builtin_amdgcn_rcpf(vs);
+    const uint32_t least = (127u - kMostScale) << 23, bits = __builtin_amdgcn_readfirstlane(__float_as_uint(vs));
+    apart = bits - least > (2u * kMostScale) << 23;
+    if (apart) {
+      lc = lv > kMostScale ? kMostScale : lv < 0.f ? -(float)kMostScale : lv;
+      iv = __builtin_amdgcn_exp2f(-lc);
+    }
+  }
+};
+
 // N scores of one row and block to weights w[], the running maximum m, sum l and the
 // outputs' factor (1 if the maximum stays).
 template <int N>
-__device__ __forceinline__ float weights(const float (&s)[N], float mx, float sl, float lv, float iv, float& m, float& l,
-                                         float (&w)[N]) {
-  mx = fmaf(mx, sl, lv);
+__device__ __forceinline__ float weights(const float (&s)[N], float mx, float sl, const ValueScale& vs, float& m,
+                                         float& l, float (&w)[N]) {
+  mx = fmaf(mx, sl, vs.lc);
   float alpha = 1.f;
   if (__any(mx > m)) {
     const float mn = fmaxf(m, mx);
@@ -245,14 +267,19 @@ __device__ __forceinline__ float weights(const float (&s)[N], float mx, float sl
     l *= alpha;
     m = mn;
   }
-  const float off = lv - (m == -INFINITY ? 0.f : m);
-  float sum = 0.f;
+  const float top = m == -INFINITY ? 0.f : m;
+  const float off = vs.lv - top;
+  float sum = 0.f, own = 0.f;
+  if (vs.apart) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) own += __builtin_amdgcn_exp2f(fmaf(s[i], sl, vs.lc - top));
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sl, off));
     sum += w[i];
   }
-  l = fmaf(sum, iv, l);
+  l = fmaf(vs.apart ? own : sum, vs.iv, l);
   return alpha;
 }
 
@@ -367,11 +394,11 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
     for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float s[16], w[16];
     u32x4 pb[2];
-    auto softmax = [&](float sl, float lv, float iv) {
+    auto softmax = [&](float sl, const ValueScale& scale) {
       float mx = s[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-      const float alpha = weights<16>(s, max_over_groups(mx), sl, lv, iv, m, l, w);
+      const float alpha = weights<16>(s, max_over_groups(mx), sl, scale, m, l, w);
       if (__any(alpha != 1.f)) {
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) o[dt] *= alpha;
@@ -415,11 +442,12 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[4 * n + e] = acc[e];
         }
-        const float sl = sl0 * ks, lv = __log2f(vs), iv = __builtin_amdgcn_rcpf(vs);
+        const float sl = sl0 * ks;
+        const ValueScale scale(vs);
         load_keys(next);
         ks = ksp[next];
         vs = vsp[next];
-        softmax(sl, lv, iv);
+        softmax(sl, scale);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
@@ -456,7 +484,7 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) vt[dt][1] = ld16(tv + 16 * dt * kSlots + 8);
-      softmax(sl0, 0.f, 1.f);
+      softmax(sl0, ValueScale(1.f));
       uint32_t bits = 0;
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) bits |= nonfinite_bits(vt[dt][0]) | nonfinite_bits(vt[dt][1]);
@@ -699,7 +727,8 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
       // one barrier a block: the buffer that block j + 1 goes to was read before this one
       unsigned char* buf = lds + (j & 1) * BUF;
       store_block(buf, j);
-      const float sl = sl0 * ks, lv = __log2f(vs), iv = __builtin_amdgcn_rcpf(vs);
+      const float sl = sl0 * ks;
+      const ValueScale scale(vs);
       load_block(j + 1);
       __syncthreads();
       const unsigned char* sk = buf + (32 * hf + r32) * 256;
@@ -724,7 +753,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
         mx = fmaxf(mx, st[i]);
       }
       const f32x2 mb = both_halves(mx);
-      const float alpha = weights<16>(s, fmaxf(mb.x, mb.y), sl, lv, iv, m, l, w);
+      const float alpha = weights<16>(s, fmaxf(mb.x, mb.y), sl, scale, m, l, w);
       if (__any(alpha != 1.f)) {
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
@@ -1120,7 +1149,8 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
   };
   auto softmax = [&](int turn) {
     const int k0 = kBlk * (2 * turn + hf);
-    const float sl = sl0 * ks, lv = __log2f(vs), iv = __builtin_amdgcn_rcpf(vs);
+    const float sl = sl0 * ks;
+    const ValueScale scale(vs);
     const bool masked = k0 + 63 > base + tw;  // some row does not see the whole block
     if (masked) {
 #pragma unroll
@@ -1135,7 +1165,7 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[kt][i]);
     const f32x2 mb = both_halves(mx);
-    mx = fmaf(fmaxf(mb.x, mb.y), sl, lv);
+    mx = fmaf(fmaxf(mb.x, mb.y), sl, scale.lc);
     if (__any(mx > m)) {
       const float mn = fmaxf(m, mx);
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
@@ -1144,8 +1174,13 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
       for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
       m = mn;
     }
-    const float off = lv - (m == -INFINITY ? 0.f : m);
-    float sum = 0.f;
+    const float top = m == -INFINITY ? 0.f : m;
+    const float off = scale.lv - top;
+    float sum = 0.f, own = 0.f, iv = scale.iv;
+    if (scale.apart) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) own += __builtin_amdgcn_exp2f(fmaf(st[i >> 4][i & 15], sl, scale.lc - top));
+    }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       float pe[8];
@@ -1158,11 +1193,11 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     }
     if (masked && !(sl + off == sl + off) && k0 > last) {
       // a block that reads as NaN, past the row's last key: its weights are NaN here, not 0
-      sum = 0.f;
+      sum = own = iv = 0.f;
 #pragma unroll
       for (int s = 0; s < 4; ++s) pb[s] = u32x4{0u, 0u, 0u, 0u};
     }
-    l = fmaf(sum, iv, l);
+    l = fmaf(scale.apart ? own : sum, iv, l);
   };
   auto outputs = [&](int turn) {
     const unsigned char* sv = lds + 2 * kPHalf + (turn & 1) * kPHalf + hf * (kHD * 128);

@@ -194,6 +194,30 @@ def test_value_scales_of_every_size(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,rep,prompt", [(2, 1, False), (16, 2, False), (16, 4, False), (40, 2, True)])
+@pytest.mark.parametrize("large", [2.0 ** 20, 2.0 ** 110])
+def test_zero_values_beside_large_ones(device, dtype, T, rep, prompt, large):
+    """One block's values are large, all others zero (their scale is the least there is)
+    or, beside the largest, ordinary: the sum of weights counts every block."""
+    import dflash_mlx as dm
+
+    L, Smax = 1000 if prompt else 1040, 1088
+    cache, lens_d, k, v, q, proj, ends = _case(device, dtype, T, 2 * rep, 2, [L], Smax, 8, prompt, qstd=0.5)
+    held = ends[0][0]
+    v[:, :, 64:128] = (v[:, :, 64:128].float() * large).bfloat16()
+    if large < 2.0 ** 100:
+        v[:, :, :64] = 0
+        v[:, :, 128:] = 0
+    dm.kv_load_q8(k.to(device), v.to(device), torch.tensor([held if prompt else L], dtype=torch.int32, device=device), cache)
+    p = torch.arange(L // BLOCK * BLOCK if not prompt else held // BLOCK * BLOCK, held)
+    cache.tail_k[0, :, p % SLOTS] = k[0, :, p].to(device)
+    cache.tail_vt[0, :, :, p % SLOTS] = v[0, :, p].transpose(1, 2).to(device)
+    attend = dm.attn_prefill_q8 if prompt else dm.attn_verify_q8
+    got = attend(q.to(device), cache, lens_d, proj.to(device)).cpu()
+    assert attention_error(got, q, k, v, proj, [L], ends, dtype, D ** -0.5) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_values_that_are_not_finite(device, dtype, bad):
     """A draft token's value that is not finite is seen by its own row and the
@@ -239,6 +263,25 @@ def test_prompt_values_that_are_not_finite(device, dtype):
         assert got[64:, :2].isnan().all()
         assert torch.equal(got[:64], clean[:64])
         assert torch.isfinite(got[64:, 2:].float()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L", [10, 40, 1])
+def test_prompt_rows_before_a_block_that_reads_as_nan(device, dtype, L):
+    """Rows of one tile on both sides of the block's first position."""
+    import dflash_mlx as dm
+
+    T, Hq, Hkv = 150, 4, 2
+    cache, lens_d, k, v, q, proj, ends = _case(device, dtype, T, Hq, Hkv, [L], 192, 3, True)
+    attend = lambda: dm.attn_prefill_q8(q.to(device), cache, lens_d, proj.to(device)).cpu().view(T, Hq, D)  # noqa: E731
+    clean = attend()
+    for scales in (cache.k_scale, cache.v_scale):
+        good = scales[0, 0, 1].clone()
+        scales[0, 0, 1] = float("nan")  # positions 64 .. 127 of key/value head 0
+        got = attend()
+        scales[0, 0, 1] = good
+        assert got[64 - L:, :2].isnan().all()
+        assert torch.equal(got[:64 - L], clean[:64 - L]) and torch.equal(got[:, 2:], clean[:, 2:])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
