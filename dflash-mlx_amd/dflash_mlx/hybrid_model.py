@@ -280,6 +280,9 @@ class HybridVerifyRunner:
         else:
             if D != 128:
                 raise ValueError(f"a cache in 8 bits needs attention heads of 128, got {D}")
+            if T * (Hq // Hkv) > 64:
+                raise ValueError(f"over a cache in 8 bits a block has at most 64 query rows a key/value head, "
+                                 f"got {T} tokens of {Hq} heads on {Hkv}")
             self.kv = [QuantizedKVCache.zeros(B, Hkv, Smax, kv_dtype, device) for _ in range(na)]
         self.q = e(B, T, Hq, D)
         self.attn_out = e(M, Hq * D)

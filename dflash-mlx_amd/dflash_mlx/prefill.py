@@ -383,11 +383,6 @@ class HybridPrefill:
         scan_strides = (ctypes.c_int64 * 13)(P * C, C, Dk, P * C, C, Dk, P * C, C, Dv,
                                              P * Hv, Hv, P * Hv, Hv)
         arows = cfg.attn_proj_rows
-        if run.kv:
-            n = self._lib.dflash_attn_prefill_q8_workspace_bytes(1, P, Hq, Hkv, run.Smax)
-            if self.kv_ws.numel() < n:
-                self.kv_ws = torch.empty(n, dtype=torch.uint8, device=run.device)
-            kv_ws = (self.kv_ws.data_ptr(), self.kv_ws.numel())
         gi = ai = 0
         for i in range(L):
             lw, tw = layers[i], self.w[i]
@@ -411,13 +406,14 @@ class HybridPrefill:
                 ap = self.aproj.data_ptr()
                 self._bf16_proj(tw["w_qkv"], xn, H, P, ap, arows, False, stream)
                 if run.kv:
-                    kv = run.kv[ai]._ptr
+                    kv, ws = run.kv[ai]._ptr, self._kv_workspace(P)
                     call("dflash_kv8_append", kv, ap, arows, lw["q_norm"].data_ptr(),
                          lw["k_norm"].data_ptr(), run.lens.data_ptr(), self.q.data_ptr(),
                          run.overflow.data_ptr(), P, Hq, cfg.rot_dims, float(cfg.rope_theta), eps, 1,
                          stream)
                     call("dflash_attn_prefill_q8", kv, self.q.data_ptr(), run.lens.data_ptr(), ap,
-                         arows, self.attn_out.data_ptr(), P, Hq, float(D ** -0.5), *kv_ws, stream)
+                         arows, self.attn_out.data_ptr(), P, Hq, float(D ** -0.5), ws.data_ptr(), ws.numel(),
+                         stream)
                 else:
                     call("dflash_attn_prep", ap, arows, lw["q_norm"].data_ptr(), lw["k_norm"].data_ptr(),
                          run.lens.data_ptr(), run.k_cache[ai].data_ptr(), run.vt_cache[ai].data_ptr(),
@@ -501,6 +497,15 @@ class HybridPrefill:
             _lib.call("dflash_gemm_bf16_tiled_prefill", x_ptr, K, wt.data_ptr(), self.r.data_ptr(),
                       self.cfg.hidden_size, P, n, K, stream)
         return used
+
+    def _kv_workspace(self, P: int) -> torch.Tensor:
+        """The workspace of the attention over a cache in 8 bits (empty: no split)."""
+        cfg = self.cfg
+        n = self._lib.dflash_attn_prefill_q8_workspace_bytes(
+            1, P, cfg.num_attention_heads, cfg.num_key_value_heads, self.run.Smax)
+        if self.kv_ws.numel() < n:
+            self.kv_ws = torch.empty(n, dtype=torch.uint8, device=self.run.device)
+        return self.kv_ws
 
     def _partials(self, floats: int) -> int:
         """The partials' buffer, which _ensure made large enough for any plan."""

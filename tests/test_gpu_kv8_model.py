@@ -7,6 +7,8 @@ codes, and the decode loop with itself: what a cache holds after blocks with
 rejected drafts, trims and prompts is what the kept tokens alone leave."""
 from __future__ import annotations
 
+import dataclasses
+
 import pytest
 import torch
 
@@ -158,3 +160,12 @@ def test_lengths_come_with_their_keys(weights, device, dtype):
     run.set_state([0])
     with pytest.raises(TypeError, match="int8 or float8_e4m3fn"):
         HybridVerifyRunner(CFG, weights, 1, 16, 128, device, kv_dtype=torch.float16)
+
+
+def test_refusals(weights, device):
+    with pytest.raises(ValueError, match="64 query rows"):
+        HybridVerifyRunner(dataclasses.replace(CFG, num_attention_heads=5), weights, 1, 16, 512, device, kv_dtype=torch.int8)
+    with pytest.raises(ValueError, match="heads of 128"):
+        HybridVerifyRunner(dataclasses.replace(CFG, head_dim=64), weights, 1, 16, 512, device, kv_dtype=torch.int8)
+    with pytest.raises(TypeError, match="codes must be"):
+        HybridVerifyRunner(CFG, weights, 1, 16, 512, device, kv_dtype=torch.float16)
