@@ -201,12 +201,18 @@ __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
                                                  0, 0);
 }
 
+// The reciprocal is off by one unit in the last place of 32 bits, under a 2^16th of the
+// rounding of the bf16 result.
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+
 // Four normalized features of a row, times the sigmoid of their gates.
-__device__ __forceinline__ void store_gated(const VerifyParams& p, int64_t bt, int qh, int d, f32x4 v) {
-  const u32x2 g = *reinterpret_cast<const u32x2*>(p.gate + bt * p.gate_stride + qh * 2 * kHD + kHD + d);
+__device__ __forceinline__ u32x2 load_gate(const VerifyParams& p, int64_t bt, int qh, int d) {
+  return *reinterpret_cast<const u32x2*>(p.gate + bt * p.gate_stride + qh * 2 * kHD + kHD + d);
+}
+__device__ __forceinline__ void store_gated(const VerifyParams& p, int64_t bt, int qh, int d, f32x4 v, u32x2 g) {
   const float ga[4] = {bf16_lo(g.x), bf16_hi(g.x), bf16_lo(g.y), bf16_hi(g.y)};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] *= 1.f / (1.f + __expf(-ga[e]));
+  for (int e = 0; e < 4; ++e) v[e] *= sigmoid(ga[e]);
   *reinterpret_cast<u32x2*>(p.out + (bt * p.Hq + qh) * kHD + d) = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
 }
 
@@ -301,17 +307,26 @@ __device__ __forceinline__ Parts parts_of(const VerifyParams& p, Batch& batch, i
   return Parts{w0, (u0 + nb - 1) / batch.per, 2 * w0 + (u0 > w0 * batch.per ? 1 : 0)};
 }
 
-// Running merge of the parts that one lane walks; V is the vector of outputs that it holds.
+// Running merge of the parts that one lane walks, N at a time (a maximum of -infinity: no
+// part); V is the vector of outputs that it holds.
 template <class V>
 struct Merged {
   float m = -INFINITY, l = 0.f;
   V o = V{};
-  __device__ void add(float pm, float pl, V po) {
-    const float mn = fmaxf(m, pm);
+  template <int N>
+  __device__ __forceinline__ void add(const f32x2 (&ml)[N], const V (&po)[N]) {
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < N; ++u) mn = fmaxf(mn, ml[u].x);
     const float ca = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-    const float cb = pm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm - mn);
-    l = l * ca + pl * cb;
-    o = o * ca + po * cb;
+    l *= ca;
+    o *= ca;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const float f = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mn);
+      l = fmaf(ml[u].y, f, l);
+      o += po[u] * f;
+    }
     m = mn;
   }
 };
@@ -515,6 +530,9 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
     const int64_t part = 2 * (int64_t)blockIdx.x + (first_part ? 0 : 1);
     for (int i = tid; i < nrows * 32; i += 64 * kWaves16) {
       const int row = i >> 5, d = (i & 31) * 4;
+      const int tt = p.token_of(row), qh = at.h * p.rep + row - tt * p.rep;
+      u32x2 gate = {0u, 0u};
+      if (whole) gate = load_gate(p, (int64_t)at.b * p.T + tt, qh, d);
       float mm = -INFINITY, ll = 0.f;
 #pragma unroll
       for (int x = 0; x < kWaves16; ++x) mm = fmaxf(mm, sml[x][row][0]);
@@ -526,7 +544,6 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
         ll = fmaf(sml[x][row][1], f, ll);
         oo += *reinterpret_cast<const f32x4*>(&so[x][row][d]) * f;
       }
-      const int tt = p.token_of(row);
       if (dropped)
 #pragma unroll 1
         for (int e = 0; e < 4; ++e) {
@@ -537,8 +554,7 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
           oo.w += e == 3 ? x : 0.f;
         }
       if (whole) {
-        const int qh = at.h * p.rep + row - tt * p.rep;
-        store_gated(p, (int64_t)at.b * p.T + tt, qh, d, oo * (1.f / ll));
+        store_gated(p, (int64_t)at.b * p.T + tt, qh, d, oo * (1.f / ll), gate);
       } else {
         const int64_t at2 = ((part * p.part_rows + row) * kHD + d) / 2;
         store_part(p.part_o, at2, oo.x, oo.y);
@@ -557,20 +573,25 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
         if (tid == 0) __hip_atomic_store(p.count + bh, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const int items = nrows * 32, groups = min(64 * kWaves16 / items, kWaves16);
         const int group = tid / items, i = tid - group * items, row = i >> 5, d = (i & 31) * 4;
+        const int tt = p.token_of(row), qh = at.h * p.rep + row - tt * p.rep;
         Merged<f32x4> a;
+        u32x2 gate = {0u, 0u};
+        if (group == 0) gate = load_gate(p, (int64_t)at.b * p.T + tt, qh, d);
         if (group < groups) {
           for (int w = parts.w0 + group; w <= parts.w1; w += groups * kPartsAhead) {
-            f32x2 ml[kPartsAhead], o0[kPartsAhead], o1[kPartsAhead];
+            f32x2 ml[kPartsAhead];
+            f32x4 os[kPartsAhead];
 #pragma unroll
             for (int u = 0; u < kPartsAhead; ++u) {
               const int64_t x = (int64_t)parts.at(min(w + groups * u, parts.w1)) * p.part_rows + row;
               ml[u] = load_part(p.part_ml, x);
-              o0[u] = load_part(p.part_o, (x * kHD + d) / 2);
-              o1[u] = load_part(p.part_o, (x * kHD + d) / 2 + 1);
+              const f32x2 o0 = load_part(p.part_o, (x * kHD + d) / 2), o1 = load_part(p.part_o, (x * kHD + d) / 2 + 1);
+              os[u] = f32x4{o0.x, o0.y, o1.x, o1.y};
             }
 #pragma unroll
             for (int u = 0; u < kPartsAhead; ++u)
-              if (w + groups * u <= parts.w1) a.add(ml[u].x, ml[u].y, f32x4{o0[u].x, o0[u].y, o1[u].x, o1[u].y});
+              if (w + groups * u > parts.w1) ml[u].x = -INFINITY;
+            a.add(ml, os);
           }
           if (d == 0) {
             sml[group][row][0] = a.m;
@@ -581,10 +602,18 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
         __syncthreads();
         if (group == 0) {
           const int n = min(groups, parts.w1 - parts.w0 + 1);
-          for (int x = 1; x < n; ++x)
-            a.add(sml[x][row][0], sml[x][row][1], *reinterpret_cast<const f32x4*>(&so[x][row][d]));
-          const int tt = p.token_of(row);
-          store_gated(p, (int64_t)at.b * p.T + tt, at.h * p.rep + row - tt * p.rep, d, a.o * (1.f / a.l));
+          for (int x = 1; x < n; x += 4) {
+            f32x2 ml[4];
+            f32x4 os[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int y = min(x + u, n - 1);
+              ml[u] = f32x2{x + u < n ? sml[y][row][0] : -INFINITY, sml[y][row][1]};
+              os[u] = *reinterpret_cast<const f32x4*>(&so[y][row][d]);
+            }
+            a.add(ml, os);
+          }
+          store_gated(p, (int64_t)at.b * p.T + tt, qh, d, a.o * (1.f / a.l), gate);
         }
       }
     }
@@ -807,7 +836,9 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
       if (!whole) {
         *reinterpret_cast<f32x4*>(p.part_o + part * (32 * kHD) + 256 * q + 4 * lane) = v;
       } else if (row < nrows) {
-        store_gated(p, (int64_t)at.b * p.T + t, at.h * p.rep + rr, d, v);
+        const int64_t bt = (int64_t)at.b * p.T + t;
+        const int qh = at.h * p.rep + rr;
+        store_gated(p, bt, qh, d, v, load_gate(p, bt, qh, d));
       }
     }
     if (!whole && hf == 0 && hl == 0) *reinterpret_cast<f32x2*>(p.part_ml + (part * 32 + r32) * 2) = f32x2{mn, ls};
@@ -848,6 +879,8 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kerne
   }
   const Parts parts = parts_of(p, batch, b, h, nb);
   if (parts.w0 == parts.w1) return;  // finished by its one run
+  u32x2 gate = {0u, 0u};
+  if (wave == 0 && live) gate = load_gate(p, (int64_t)b * p.T + t, qh, d);
   Merged<f32x4> a;
   for (int w = parts.w0 + wave; w <= parts.w1; w += kMergeWaves * kMergeAhead) {
     f32x2 ml[kMergeAhead];
@@ -860,7 +893,8 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kerne
     }
 #pragma unroll
     for (int u = 0; u < kMergeAhead; ++u)
-      if (w + kMergeWaves * u <= parts.w1) a.add(ml[u].x, ml[u].y, os[u]);
+      if (w + kMergeWaves * u > parts.w1) ml[u].x = -INFINITY;
+    a.add(ml, os);
   }
   if (hl == 0) {
     sm[wave][r32] = a.m;
@@ -869,9 +903,15 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kerne
   so[wave][lane] = a.o;
   __syncthreads();
   if (wave != 0) return;
-  const int n = min(kMergeWaves, parts.w1 - parts.w0 + 1);
-  for (int k = 1; k < n; ++k) a.add(sm[k][r32], sl[k][r32], so[k][lane]);
-  if (live) store_gated(p, (int64_t)b * p.T + t, qh, d, a.o * (1.f / a.l));
+  f32x2 ml[kMergeWaves - 1];
+  f32x4 os[kMergeWaves - 1];
+#pragma unroll
+  for (int k = 1; k < kMergeWaves; ++k) {  // (a wave without a part left -infinity)
+    ml[k - 1] = f32x2{sm[k][r32], sl[k][r32]};
+    os[k - 1] = so[k][lane];
+  }
+  a.add(ml, os);
+  if (live) store_gated(p, (int64_t)b * p.T + t, qh, d, a.o * (1.f / a.l), gate);
 }
 
 // Rows of a part: the least tile that holds them.  One tile larger, us a call: up to 16
@@ -958,10 +998,6 @@ __device__ __forceinline__ int prefill_turns(const PrefillParams& p, int len, in
 __device__ __forceinline__ int prefill_splits(const PrefillParams& p, int turns) {
   return max(1, min(p.splits, turns / kSplitTurns));
 }
-
-// The reciprocal is off by one unit in the last place of 32 bits, under a 2^16th of the
-// rounding of the bf16 result.
-__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
 
 constexpr int prefill_lds(int pairs) {
   const int merge = 4 * pairs * (kPMerge + kPRows * kPPitch);
