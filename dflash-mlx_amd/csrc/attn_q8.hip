@@ -578,19 +578,23 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
         u32x2 gate = {0u, 0u};
         if (group == 0) gate = load_gate(p, (int64_t)at.b * p.T + tt, qh, d);
         if (group < groups) {
-          for (int w = parts.w0 + group; w <= parts.w1; w += groups * kPartsAhead) {
+          for (int w0 = parts.w0; w0 <= parts.w1; w0 += groups * kPartsAhead) {
             f32x2 ml[kPartsAhead];
             f32x4 os[kPartsAhead];
 #pragma unroll
             for (int u = 0; u < kPartsAhead; ++u) {
-              const int64_t x = (int64_t)parts.at(min(w + groups * u, parts.w1)) * p.part_rows + row;
-              ml[u] = load_part(p.part_ml, x);
+              ml[u] = f32x2{-INFINITY, 0.f};
+              os[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+              if (w0 + groups * u > parts.w1) continue;  // (no group has a part left)
+              const int w = w0 + groups * u + group;
+              const int64_t x = (int64_t)parts.at(min(w, parts.w1)) * p.part_rows + row;
               const f32x2 o0 = load_part(p.part_o, (x * kHD + d) / 2), o1 = load_part(p.part_o, (x * kHD + d) / 2 + 1);
+              ml[u] = load_part(p.part_ml, x);
               os[u] = f32x4{o0.x, o0.y, o1.x, o1.y};
             }
 #pragma unroll
             for (int u = 0; u < kPartsAhead; ++u)
-              if (w + groups * u > parts.w1) ml[u].x = -INFINITY;
+              if (w0 + groups * u + group > parts.w1) ml[u].x = -INFINITY;
             a.add(ml, os);
           }
           if (d == 0) {
@@ -887,13 +891,13 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kerne
     f32x4 os[kMergeAhead];
 #pragma unroll
     for (int u = 0; u < kMergeAhead; ++u) {
-      const int64_t i = (int64_t)parts.at(min(w + kMergeWaves * u, parts.w1)) * tiles + rt;
+      ml[u] = f32x2{-INFINITY, 0.f};
+      os[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (w + kMergeWaves * u > parts.w1) continue;
+      const int64_t i = (int64_t)parts.at(w + kMergeWaves * u) * tiles + rt;
       ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + (i * 32 + r32) * 2);
       os[u] = *reinterpret_cast<const f32x4*>(p.part_o + i * (32 * kHD) + 256 * q + 4 * lane);
     }
-#pragma unroll
-    for (int u = 0; u < kMergeAhead; ++u)
-      if (w + kMergeWaves * u > parts.w1) ml[u].x = -INFINITY;
     a.add(ml, os);
   }
   if (hl == 0) {
