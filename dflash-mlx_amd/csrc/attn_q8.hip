@@ -1376,29 +1376,40 @@ __global__ __launch_bounds__(256) void attn_prefill_q8_merge_kernel(const Prefil
   if (splits == 1) return;  // the row is stored
   const int64_t row = (int64_t)b * p.P * p.Hq + e, step = (int64_t)p.c.B * p.P * p.Hq;
   const u32x4 gt = ld16(p.gate + ((int64_t)b * p.P + t) * p.gate_stride + h * 2 * kHD + kHD + f);
-  float mx = -INFINITY;
-#pragma unroll 4
-  for (int k = 0; k < splits; ++k) mx = fmaxf(mx, p.part_w[k * step + row]);
-  float sum = 0.f;
-  float v[8] = {};
-#pragma unroll 4
-  for (int k = 0; k < splits; ++k) {
-    const float w = p.part_w[k * step + row];
-    const float x = w == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w - mx);
-    const float* o = p.part_o + (k * step + row) * kHD + f;
-    const f32x4 a = *reinterpret_cast<const f32x4*>(o), c = *reinterpret_cast<const f32x4*>(o + 4);
-    sum += x;
+  typedef float f32x8 __attribute__((ext_vector_type(8)));
+  constexpr int AHEAD = 4;
+  Merged<f32x8> a;
+  f32x8 bad = {};
+  for (int k0 = 0; k0 < splits; k0 += AHEAD) {
+    f32x2 ml[AHEAD];
+    f32x8 os[AHEAD];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = i < 4 ? a[i & 3] : c[i & 3];
-      v[i] += fabsf(y) < INFINITY ? x * y : y;
+    for (int u = 0; u < AHEAD; ++u) {
+      ml[u] = f32x2{-INFINITY, 1.f};
+      os[u] = f32x8{};
+      if (k0 + u >= splits) continue;
+      const int64_t at = (k0 + u) * step + row;
+      ml[u].x = p.part_w[at];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + at * kHD + f);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p.part_o + at * kHD + f + 4);
+      os[u] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = os[u][i];
+        const bool finite = fabsf(y) < INFINITY;
+        os[u][i] = finite ? y : 0.f;
+        bad[i] += finite ? 0.f : y;
+      }
+    a.add(ml, os);
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  float g[8];
+  const float inv = a.l == 0.f ? 0.f : 1.f / a.l;
+  float g[8], v[8];
   unpack8(gt, g);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * sigmoid(g[i]);
+  for (int i = 0; i < 8; ++i) v[i] = (a.o[i] * inv + bad[i]) * sigmoid(g[i]);
   *reinterpret_cast<u32x4*>(p.out + row * kHD + f) = pack8(v);
 }
 
