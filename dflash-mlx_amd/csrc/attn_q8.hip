@@ -32,7 +32,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 //     or 2^-4 of their own (e4m3).  Sums, maxima and outputs stay in fp32.
 // Every position's 256 bytes of codes are read once, which bounds the kernel where rows
 // are few: 32 sequences of up to 8191 positions (16 heads on 4, one token, int8), 204 MB
-// in 46 us, 4.4 TB/s of the 5.2 that a large copy reaches.
+// in 45 us, 4.5 TB/s of the 5.2 that a large copy reaches.
 struct VerifyParams {
   Kv8 c;
   const uint16_t* q;  // [B, T, Hq, D]
@@ -75,8 +75,8 @@ __device__ __forceinline__ int wave_scan(int x) {
 // that gives no more pieces than workgroups, a workgroup takes one piece of one head
 // (`pieces`); otherwise all blocks, in order of sequence and head, are cut into runs of
 // the even share, which cross from head to head.  Pieces have a part each and are merged
-// in even numbers (16 tokens after 4096: 15.7 us, as runs 17.7); runs fill the device
-// where heads do not divide it (12 sequences of 8 heads: 21.4 us).  Units: pieces, or
+// in even numbers (16 tokens after 4096: 14.7 us, as runs 16.5); runs fill the device
+// where there are more heads than pieces can be had of (12 sequences of 8 heads).  Units: pieces, or
 // blocks.  Lane i of chunk c has sequence 64 c + i; up to 64 sequences are loaded once and
 // stay in the lanes.
 struct Batch {
@@ -639,11 +639,12 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
 // (lane / 32) + i % 4 of its half in result element i).  All waves read the same
 // block: its codes are loaded once, a block ahead, and become bf16 on their way
 // to the other of two LDS buffers, as the prompt kernel's.
-// 16 tokens after 131000 (16 heads on 4, int8): 40 us and 8 us of merge for 134 MB and
+// 16 tokens after 131000 (16 heads on 4, int8): 40 us and 6.5 us of merge for 134 MB and
 // 17.2 GFLOP.  Two waves a SIMD go through conversion, barrier, scores, softmax and
-// products block by block, 1.9 us each, and that chain bounds it: two blocks ahead (46.6
-// us a call against 45.9), four LDS reads ahead of the products and the scales in lanes
-// (no change) left it alone; codes straight to every wave's registers took 50.2.
+// products block by block, 1.9 us each (4.4 TB/s), and that chain bounds it beside 10 us of
+// start and end: two blocks ahead (46.6 us a call against 45.9), four LDS reads ahead of
+// the products and the scales in lanes (no change) left it alone; codes straight to every
+// wave's registers took 50.2.
 template <int TYPE, int RT>
 __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(const VerifyParams p) {
   constexpr int NT = 128 * RT, PER = kBlk * kHD / 16 / NT;
@@ -919,10 +920,9 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kerne
 }
 
 // Rows of a part: the least tile that holds them.  One tile larger, us a call: up to 16
-// rows 13.8 for 11.1 (1 token after 500), 72.5 for 46.3 (32 sequences after 8191); up to
-// 32 rows 47.4 for 41.5 (8 sequences of 8 tokens after 16000, 16 heads on 4).
-// Blocks of a piece where there are few: 2 (16 tokens after 4096: 16.5 us; 1: 17.1, 4:
-// 17.0, 6: 17.6).  Workgroups: what the device holds at a time, or fewer for a small cache.
+// rows 13.3 for 10.8 (1 token after 500), 77.8 for 45.3 (32 sequences after 8191); up to
+// 32 rows 46.5 for 42.6 (8 sequences of 8 tokens after 16000, 16 heads on 4).
+// Blocks of a piece where there are few: 2 (16 tokens after 4096: 14.7 us; 1: 15.7, 4: 15.4).  Workgroups: what the device holds at a time, or fewer for a small cache.
 struct VerifyShape {
   int part_rows, min_cut, runs;
 };
@@ -962,8 +962,8 @@ void launch_verify(const VerifyParams& p, hipStream_t s) {
 //     their way to the other of two LDS buffers: 16-byte piece c of row r at slot
 //     c ^ (r % 8).
 //   - Weights are rounded to bf16 for P V, as in the verify kernel.
-// 4 D operations a pair of positions bound it.  16 heads on 4, e4m3: 4096 rows 86 us, 803
-// TFLOP/s; 2048 rows after 14336 273 us, 942 TFLOP/s; a large library product of bf16
+// 4 D operations a pair of positions bound it.  16 heads on 4, e4m3: 4096 rows 87 us, 790
+// TFLOP/s; 2048 rows after 14336 276 us, 930 TFLOP/s; a large library product of bf16
 // reaches 1300.  int8 takes 92 us for 4096 rows (its bytes take more instructions to
 // become bf16).  A turn takes 5000 cycles, of which the matrix unit works 2048; one wave's
 // softmax (1400) and staging (1100) run beside the other's products, and what is left over
@@ -991,8 +991,8 @@ constexpr int kPHalf = kPKeys * kHD * 2;       // bytes of one turn's K (or V^T)
 constexpr int kPMerge = 68 * 64;               // floats that the two waves of a row tile exchange
 constexpr int kPPitch = kHD + 4;               // floats of a normalized row in LDS
 
-// Least turns of a split: 2 (600 rows after 1000 29.2 us, 64 after 500 17.5, 300 alone
-// 14.4; 1: 29.3, 17.0, 15.4; 4: 30.0, 18.7, 14.4).
+// Least turns of a split: 2 (600 rows after 1000 29.2 us, 64 after 500 17.0, 300 alone
+// 14.6; 1: 29.2, 15.4, 15.4; 4: 29.9, 18.6, 14.6).
 constexpr int kSplitTurns = 2;
 
 // Turns of the row block that ends before row `end`, and the splits that share them.
@@ -1009,8 +1009,8 @@ constexpr int prefill_lds(int pairs) {
 }
 
 // Orders a run of N products with one LDS read each so that READS reads stay ahead of them
-// (2048 rows after 14336: 289 us as the compiler orders them, 277 with two, 276 with
-// four, 278 with six).
+// (2048 rows after 14336: 289 us as the compiler orders them, 276 with four; two are the
+// same, six 1 % slower).
 template <int N, int READS>
 __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
@@ -1366,7 +1366,7 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
 
 // The splits of a row joined, gated and stored: 16 lanes a row of a head, 8 features each.
 // A feature that is not finite in a split is so in the row, whatever the split's weight.
-// Bound by the fp32 rows, read once: 600 rows of 16 heads in three splits, 14.7 MB, 5.6 us.
+// The fp32 rows are read once: 600 rows of 16 heads in three splits, 14.7 MB, 5.2 us.
 __global__ __launch_bounds__(256) void attn_prefill_q8_merge_kernel(const PrefillParams p, int block_rows) {
   const int b = blockIdx.y;
   const int64_t e = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -1433,7 +1433,7 @@ int prefill_rep(int per_kv) {
 
 // Splits of a row block's keys: a workgroup fills a CU and takes its time for a turn
 // whatever the others do, so as many as the rows' workgroups leave CUs for.  Unsplit, 512
-// rows after 32256 took 488 us for 153, 100 after 8000 132 for 35; more splits than one
+// rows after 32256 took 488 us for 154, 100 after 8000 132 for 28; more splits than one
 // round of the device holds are slower where rows see few keys (1500 rows: 51 us for 33).
 int most_prefill_splits(int64_t wgs, int Smax) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
