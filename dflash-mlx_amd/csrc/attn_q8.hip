@@ -1360,7 +1360,8 @@ __global__ __launch_bounds__(128 * REP * RB, 2) void attn_prefill_q8_kernel(cons
     unpack8(gt[i], g);
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = row[u] * sigmoid(g[u]);
-    *reinterpret_cast<u32x4*>(p.out + (((int64_t)b * p.P + t) * p.Hq + head_of(e)) * kHD + (e & 15) * 8) = pack8(v);
+    *reinterpret_cast<u32x4*>(p.out + (((int64_t)b * p.P + t) * p.Hq + head_of(e)) * kHD + (e & 15) * 8) =
+        len < 0 ? u32x4{0u, 0u, 0u, 0u} : pack8(v);  // (whatever the gate holds)
   }
 }
 

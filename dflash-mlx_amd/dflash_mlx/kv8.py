@@ -199,9 +199,11 @@ def attn_prep_q8(proj, q_norm, k_norm, lens, cache: QuantizedKVCache, *, num_hea
     rotary over the first rot_dims (0, 16, 32, 64 or 128) features.
 
     prompt=False: T <= 16 draft tokens, of which any number may be rejected (the
-    next call's lens says how many were kept).  prompt=True: T committed tokens.
+    next call's lens says how many were kept).  prompt=True: T committed tokens, all
+    of them: lens grows by T.  (Prompts of several lengths, which padding would
+    commit too: a call for each length, with lens -1 for the other sequences.)
     overflow (int32 [B], optional) is set to 1 for a sequence with positions
-    outside the cache, which are not written."""
+    outside the cache, lens -1 among them, which are not written."""
     _check_cache(cache)
     _check_lens("lens", lens, cache)
     if num_heads <= 0 or num_heads % cache.Hkv:

@@ -72,8 +72,8 @@ typedef struct {
  *   prompt == 0: T <= 16 draft tokens.  They go to the tail; block lens[b] / 64 - 1
  *     is quantised from the tail if lens[b] % 64 <= 16 (it may have become complete
  *     since the last append; the same codes again otherwise).
- *   prompt != 0: T committed tokens.  Every block that they complete is quantised,
- *     and the tail holds the last two blocks' positions.
+ *   prompt != 0: T committed tokens (lens grows by T).  Every block that they complete
+ *     is quantised, and the tail holds the last two blocks' positions.
  * overflow (or NULL): [B], set to 1 for a sequence with a position outside
  * [0, Smax).  rot_dims in {0, 16, 32, 64, 128}; Hq a multiple of Hkv; proj, its rows
  * and q_out 16-byte aligned.

@@ -138,3 +138,30 @@ def test_offsets_past_32_bits(device, dtype):
         got = dm.kv_read_q8(cache, torch.where(lens < 0, lens, at), 150, start=at - 150)
         for x, want in zip(got, (kk, vv)):
             assert torch.equal(x[-1].cpu(), want[:, at - 150:at].float().bfloat16()) and (x[:-1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_of_several_lengths(device, dtype):
+    """A call for each length, the other sequences at -1: every sequence's cache and rows
+    are those of a cache of its own."""
+    import dflash_mlx as dm
+
+    sizes = (130, 64, 7)
+    w = torch.ones(D, dtype=torch.bfloat16, device=device)
+    rows = [proj_rows(1, n, HQ, HKV, 30 + n).to(device) for n in sizes]
+    kw = dict(num_heads=HQ, rot_dims=32, rope_base=THETA, eps=EPS, prompt=True)
+
+    def lens(*x):
+        return torch.tensor(x, dtype=torch.int32, device=device)
+
+    cache = dm.QuantizedKVCache.zeros(len(sizes), HKV, 192, dtype, device)
+    for b, (n, r) in enumerate(zip(sizes, rows)):
+        own = dm.QuantizedKVCache.zeros(1, HKV, 192, dtype, device)
+        want = dm.attn_prefill_q8(dm.attn_prep_q8(r, w, w, lens(0), own, **kw), own, lens(0), r)
+        batch = torch.full((len(sizes), *r.shape[1:]), float("nan"), dtype=r.dtype, device=device)
+        batch[b] = r[0]
+        at = lens(*(0 if i == b else -1 for i in range(len(sizes))))
+        got = dm.attn_prefill_q8(dm.attn_prep_q8(batch, w, w, at, cache, **kw), cache, at, batch)
+        assert torch.equal(got[b], want[0]) and (got[[i for i in range(len(sizes)) if i != b]] == 0).all()
+        for x, y in zip(dm.kv_read_q8(cache, lens(*sizes), n), dm.kv_read_q8(own, lens(n), n)):
+            assert torch.equal(x[b], y[0])
