@@ -45,6 +45,7 @@ struct VerifyParams {
   int32_t* count;   // [B, Hkv] parts that have arrived (up to 16 rows); zero between calls
   int T, Hq, rep, runs, min_cut;
   int part_rows;  // rows of a part in the workspace
+  int sliced;     // the merge of more than 16 rows: a workgroup per sixteenth of a head's outputs
   uint32_t rep_inv;
   float scale;
 
@@ -864,73 +865,85 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
 // trip to memory.
 constexpr int kMergeWaves = 16, kMergeAhead = 8;
 
-// Up to 64 rows: a workgroup per (sequence, key/value head, tile, sixteenth q of its
-// outputs), a part's outputs as the lanes stored them; the waves take the parts in turn.
+// Up to 64 rows, a part's outputs as the lanes stored them.  With few heads (p.sliced), a
+// workgroup per (sequence, key/value head, tile, sixteenth q of its outputs), whose waves
+// take the parts in turn; with many, which have few parts each if any, a workgroup per
+// (sequence, head, tile) and a wave per sixteenth.  Slices for all: 128 sequences of 16
+// tokens after 200 150 us for 31, 16 after 4096 42 for 29, nearly all workgroups without a
+// part; for none: 16 tokens after 131000 75.9 for 46.4, after 4096 22.4 for 15.2.
 __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kernel(const VerifyParams p) {
   __shared__ float sm[kMergeWaves][32], sl[kMergeWaves][32];
   __shared__ f32x4 so[kMergeWaves][64];
   const int tiles = p.part_rows >> 5;
-  const int q = blockIdx.x & 15, rt = (blockIdx.x >> 4) % tiles, h = (blockIdx.x >> 4) / tiles, b = blockIdx.y;
+  const int hx = p.sliced ? blockIdx.x >> 4 : blockIdx.x;
+  const int rt = hx % tiles, h = hx / tiles, b = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int q = p.sliced ? blockIdx.x & 15 : wave;
+  const int first = p.sliced ? wave : 0, stride = p.sliced ? kMergeWaves : 1;  // of the wave's parts
   const int r32 = lane & 31, hl = lane >> 5, row = 32 * rt + r32;
   const int t = p.token_of(row), qh = h * p.rep + row - t * p.rep, d = 32 * (q >> 2) + 8 * (q & 3) + 4 * hl;
   const bool live = row < p.T * p.rep;
   Batch batch(p);
   const int nb = seen_blocks(__builtin_amdgcn_readfirstlane(p.lens[b]), p.T, p.c.Smax);
   if (nb == 0) {  // takes no part
-    if (wave == 0 && live)
+    if (first == 0 && live)
       *reinterpret_cast<u32x2*>(p.out + (((int64_t)b * p.T + t) * p.Hq + qh) * kHD + d) = u32x2{0u, 0u};
     return;
   }
   const Parts parts = parts_of(p, batch, b, h, nb);
   if (parts.w0 == parts.w1) return;  // finished by its one run
   u32x2 gate = {0u, 0u};
-  if (wave == 0 && live) gate = load_gate(p, (int64_t)b * p.T + t, qh, d);
+  if (first == 0 && live) gate = load_gate(p, (int64_t)b * p.T + t, qh, d);
   Merged<f32x4> a;
-  for (int w = parts.w0 + wave; w <= parts.w1; w += kMergeWaves * kMergeAhead) {
+  for (int w = parts.w0 + first; w <= parts.w1; w += stride * kMergeAhead) {
     f32x2 ml[kMergeAhead];
     f32x4 os[kMergeAhead];
 #pragma unroll
     for (int u = 0; u < kMergeAhead; ++u) {
       ml[u] = f32x2{-INFINITY, 0.f};
       os[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (w + kMergeWaves * u > parts.w1) continue;
-      const int64_t i = (int64_t)parts.at(w + kMergeWaves * u) * tiles + rt;
+      if (w + stride * u > parts.w1) continue;
+      const int64_t i = (int64_t)parts.at(w + stride * u) * tiles + rt;
       ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + (i * 32 + r32) * 2);
       os[u] = *reinterpret_cast<const f32x4*>(p.part_o + i * (32 * kHD) + 256 * q + 4 * lane);
     }
     a.add(ml, os);
   }
-  if (hl == 0) {
-    sm[wave][r32] = a.m;
-    sl[wave][r32] = a.l;
-  }
-  so[wave][lane] = a.o;
-  __syncthreads();
-  if (wave != 0) return;
-  f32x2 ml[kMergeWaves - 1];
-  f32x4 os[kMergeWaves - 1];
+  if (p.sliced) {
+    if (hl == 0) {
+      sm[wave][r32] = a.m;
+      sl[wave][r32] = a.l;
+    }
+    so[wave][lane] = a.o;
+    __syncthreads();
+    if (wave != 0) return;
+    f32x2 ml[kMergeWaves - 1];
+    f32x4 os[kMergeWaves - 1];
 #pragma unroll
-  for (int k = 1; k < kMergeWaves; ++k) {  // (a wave without a part left -infinity)
-    ml[k - 1] = f32x2{sm[k][r32], sl[k][r32]};
-    os[k - 1] = so[k][lane];
+    for (int k = 1; k < kMergeWaves; ++k) {  // (a wave without a part left -infinity)
+      ml[k - 1] = f32x2{sm[k][r32], sl[k][r32]};
+      os[k - 1] = so[k][lane];
+    }
+    a.add(ml, os);
   }
-  a.add(ml, os);
   if (live) store_gated(p, (int64_t)b * p.T + t, qh, d, a.o * (1.f / a.l), gate);
 }
 
 // Rows of a part: the least tile that holds them.  One tile larger, us a call: up to 16
 // rows 13.3 for 10.8 (1 token after 500), 77.8 for 45.3 (32 sequences after 8191); up to
 // 32 rows 46.5 for 42.6 (8 sequences of 8 tokens after 16000, 16 heads on 4).
-// Blocks of a piece where there are few: 2 (16 tokens after 4096: 14.7 us; 1: 15.7, 4: 15.4).  Workgroups: what the device holds at a time, or fewer for a small cache.
+// Blocks of a piece where there are few: 2 (16 tokens after 4096: 14.7 us; 1: 15.7, 4: 15.4).
+// Workgroups: what the device holds at a time, or fewer for a small cache.  sliced: where
+// that makes the merge two rounds of the device at most.
 struct VerifyShape {
-  int part_rows, min_cut, runs;
+  int part_rows, min_cut, runs, sliced;
 };
 VerifyShape verify_shape(int64_t B, int rows, int Hkv, int Smax) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
   VerifyShape v;
   v.part_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   v.min_cut = 2;
+  v.sliced = B * Hkv * v.part_rows / 2 <= 2 * cus;
   v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(rows <= 16 ? cus : 2 * cus, B * Hkv * ceil_div(Smax / kBlk, v.min_cut)));
   return v;
 }
@@ -1497,6 +1510,7 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   p.part_rows = v.part_rows;
   p.min_cut = v.min_cut;
   p.runs = v.runs;
+  p.sliced = v.sliced;
   p.count = static_cast<int32_t*>(workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + count_bytes(B, Hkv));
   p.part_ml = p.part_o + (int64_t)2 * p.runs * p.part_rows * kHD;
@@ -1505,7 +1519,7 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   else launch_verify<DFLASH_KV_E4M3>(p, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.part_rows == 16) return to_status(e);
-  hipLaunchKernelGGL(attn_verify_q8_merge64_kernel, dim3((unsigned)(Hkv * p.part_rows / 2), (unsigned)B),
+  hipLaunchKernelGGL(attn_verify_q8_merge64_kernel, dim3((unsigned)(Hkv * p.part_rows / 32 * (p.sliced ? 16 : 1)), (unsigned)B),
                      dim3(64 * kMergeWaves), 0, s, p);
   return to_status(hipGetLastError());
 }

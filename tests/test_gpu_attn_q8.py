@@ -76,6 +76,17 @@ def test_verify(device, dtype, T, Hq, Hkv, lens, Smax):
     _check(device, dtype, T, Hq, Hkv, lens, Smax, seed=T + Hq + len(lens), prompt=False)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Hq,Hkv,lens,Smax", [
+    (16, 16, 4, [2000, 70, -1, 900, 0, 1300], 2048),  # many heads of 64 rows, in parts and whole
+    (8, 8, 2, [1500] + [40] * 20 + [-1, 700], 1536),  # of 32 rows
+    (16, 1, 1, [4000], 4032),                         # one head of 16 rows in few parts
+    (16, 2, 2, [2500, 100], 2560),
+])
+def test_verify_merges(device, dtype, T, Hq, Hkv, lens, Smax):
+    _check(device, dtype, T, Hq, Hkv, lens, Smax, seed=T + Hq + len(lens), prompt=False)
+
+
 PROMPT = [
     (1, 4, 1, [0], 64),
     (17, 16, 4, [0], 64),
