@@ -71,6 +71,17 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
+// Largest of the wave's values, 0 or more.
+__device__ __forceinline__ int wave_most(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // How the launch's workgroups share the blocks, from the lengths: `cut` blocks are a
 // workgroup's even share, at least min_cut.  Where every head cut into pieces of at most
 // that gives no more pieces than workgroups, a workgroup takes one piece of one head
@@ -80,6 +91,10 @@ __device__ __forceinline__ int wave_scan(int x) {
 // where there are more heads than pieces can be had of (12 sequences of 8 heads).  Units: pieces, or
 // blocks.  Lane i of chunk c has sequence 64 c + i; up to 64 sequences are loaded once and
 // stay in the lanes.
+// A head of up to 16 rows is merged by one workgroup, which takes about a 32nd of a row for
+// each part of what a block takes: its parts are at most so many that the merge is no longer
+// than the part before it, sqrt(blocks rows / 32) blocks each (1 key/value head, 16 rows
+// after 32768: 20 us, else 40; 4 heads 21.4, else 24.6).
 struct Batch {
   const VerifyParams& p;
   int len, incl;  // of the first chunk: lengths, and units of one head up to and with the lane's
@@ -89,13 +104,16 @@ struct Batch {
   int units;      // of the launch
 
   __device__ __forceinline__ explicit Batch(const VerifyParams& params) : p(params) {
-    int nblk = 0, n = 0;
+    int nblk = 0, n = 0, longest = 0;
     for (int c = chunks() - 1; c >= 0; --c) {
       load(c);
-      nblk += __builtin_amdgcn_readlane(wave_scan(seen_blocks(len, p.T, p.c.Smax)), 63);
+      const int nb = seen_blocks(len, p.T, p.c.Smax);
+      nblk += __builtin_amdgcn_readlane(wave_scan(nb), 63);
+      if (p.part_rows == 16) longest = max(longest, wave_most(nb));
     }
     nblk *= p.c.Hkv;
     cut = max(p.min_cut, (nblk + p.runs - 1) / p.runs);
+    if (p.part_rows == 16) cut = max(cut, (int)sqrtf((float)longest * (float)(p.T * p.rep) * (1.f / 32.f)));
     pieces = true;
     for (int c = chunks() - 1; c >= 0; --c) {
       if (p.c.B > 64) load(c);
