@@ -44,6 +44,7 @@ struct VerifyParams {
   float* part_ml;   // [2 * runs][part_rows][2]
   int32_t* count;   // [B, Hkv] parts that have arrived (up to 16 rows); zero between calls
   int T, Hq, rep, runs, min_cut;
+  int waves;      // of a workgroup (up to 16 rows)
   int part_rows;  // rows of a part in the workspace
   int sliced;     // the merge of more than 16 rows: a workgroup per sixteenth of a head's outputs
   uint32_t rep_inv;
@@ -351,7 +352,7 @@ struct Merged {
 };
 
 // ------------------------------------------------- up to 16 rows (single tokens)
-// Eight waves, block by block in turn, straight from memory to registers: nothing is
+// W waves, block by block in turn, straight from memory to registers: nothing is
 // shared.  v_mfma_f32_16x16x32_bf16; lane (r, g) = (lane % 16, lane / 16) has row r.
 // Operand row i of K's tile n is position 16 (i / 4) + 8 (n / 2) + 4 (n % 2) + i % 4,
 // so that result rows 4 g + e of tiles 2 s and 2 s + 1 are positions 16 g + 8 s .. + 7,
@@ -359,7 +360,6 @@ struct Merged {
 // are loaded once these are consumed, its values likewise: 16 KB a wave in flight, and no
 // barrier before the merge.  Few rows leave the matrix unit idle anyway; what counts is
 // bytes in flight.
-constexpr int kWaves16 = 8;
 constexpr int kPartsAhead = 8;
 
 // Parts of up to 16 rows are merged by the workgroup that brings the last one: stored and
@@ -377,10 +377,10 @@ __device__ __forceinline__ f32x2 load_part(const float* base, int64_t i) {
   return f32x2{__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32))};
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel(const VerifyParams p) {
-  __shared__ __attribute__((aligned(16))) float so[kWaves16][16][kHD + 4];
-  __shared__ float sml[kWaves16][16][2];
+template <int TYPE, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const VerifyParams p) {
+  __shared__ __attribute__((aligned(16))) float so[W][16][kHD + 4];
+  __shared__ float sml[W][16][2];
   __shared__ int dropped;  // the tail's values hold a NaN or an infinity
   __shared__ int arrived;
   const Kv8& c = p.c;
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
     if (batch.length(b) >= 0) continue;
     const int n = p.T * p.Hq * kHD / 2;
     uint32_t* dst = reinterpret_cast<uint32_t*>(p.out) + (int64_t)b * n;
-    for (int i = tid; i < n; i += 64 * kWaves16) dst[i] = 0u;
+    for (int i = tid; i < n; i += 64 * W) dst[i] = 0u;
   }
   Share at = share_of(p, batch, blockIdx.x);
   const float sl0 = positive_scale(p.scale);
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
       ks = ksp[j];
       vs = vsp[j];
       do {
-        const int next = min(j + kWaves16, coded - 1);  // (past the last: loaded again, not used)
+        const int next = min(j + W, coded - 1);  // (past the last: loaded again, not used)
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -490,10 +490,10 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
             o[dt] = mfma_bf16(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[k], o[dt]);
           }
         load_values(next);
-        j += kWaves16;
+        j += W;
       } while (j < coded);
     }
-    for (; j < b1; j += kWaves16) {  // the tail, in bf16
+    for (; j < b1; j += W) {  // the tail, in bf16
       const int slot = (j & 1) * kBlk, p0 = kBlk * j;
       const uint16_t* tk = c.tail_keys(bh) + (slot + key0) * kHD + 16 * g;
       const uint16_t* tv = c.tail_values(bh) + r * kSlots + slot + 16 * g;
@@ -547,17 +547,17 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
     __syncthreads();
     const bool whole = at.blk == 0 && b1 == nb;
     const int64_t part = 2 * (int64_t)blockIdx.x + (first_part ? 0 : 1);
-    for (int i = tid; i < nrows * 32; i += 64 * kWaves16) {
+    for (int i = tid; i < nrows * 32; i += 64 * W) {
       const int row = i >> 5, d = (i & 31) * 4;
       const int tt = p.token_of(row), qh = at.h * p.rep + row - tt * p.rep;
       u32x2 gate = {0u, 0u};
       if (whole) gate = load_gate(p, (int64_t)at.b * p.T + tt, qh, d);
       float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int x = 0; x < kWaves16; ++x) mm = fmaxf(mm, sml[x][row][0]);
+      for (int x = 0; x < W; ++x) mm = fmaxf(mm, sml[x][row][0]);
       f32x4 oo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < kWaves16; ++x) {
+      for (int x = 0; x < W; ++x) {
         const float mw = sml[x][row][0];
         const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
         ll = fmaf(sml[x][row][1], f, ll);
@@ -590,53 +590,56 @@ __global__ __launch_bounds__(64 * kWaves16, 2) void attn_verify_q8_rows16_kernel
       __syncthreads();
       if (arrived == parts.w1 - parts.w0) {  // the last: merge them, in their order
         if (tid == 0) __hip_atomic_store(p.count + bh, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const int items = nrows * 32, groups = min(64 * kWaves16 / items, kWaves16);
-        const int group = tid / items, i = tid - group * items, row = i >> 5, d = (i & 31) * 4;
-        const int tt = p.token_of(row), qh = at.h * p.rep + row - tt * p.rep;
-        Merged<f32x4> a;
-        u32x2 gate = {0u, 0u};
-        if (group == 0) gate = load_gate(p, (int64_t)at.b * p.T + tt, qh, d);
-        if (group < groups) {
-          for (int w0 = parts.w0; w0 <= parts.w1; w0 += groups * kPartsAhead) {
-            f32x2 ml[kPartsAhead];
-            f32x4 os[kPartsAhead];
+        const int items = min(nrows * 32, 64 * W), groups = min(64 * W / items, W), group = tid / items;
+        for (int i0 = 0; i0 < nrows * 32; i0 += items) {
+          const int i = i0 + tid - group * items, row = min(i >> 5, nrows - 1), d = (i & 31) * 4;
+          const int tt = p.token_of(row), qh = at.h * p.rep + row - tt * p.rep;
+          Merged<f32x4> a;
+          u32x2 gate = {0u, 0u};
+          if (group == 0) gate = load_gate(p, (int64_t)at.b * p.T + tt, qh, d);
+          if (group < groups) {
+            for (int w0 = parts.w0; w0 <= parts.w1; w0 += groups * kPartsAhead) {
+              f32x2 ml[kPartsAhead];
+              f32x4 os[kPartsAhead];
 #pragma unroll
-            for (int u = 0; u < kPartsAhead; ++u) {
-              ml[u] = f32x2{-INFINITY, 0.f};
-              os[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-              if (w0 + groups * u > parts.w1) continue;  // (no group has a part left)
-              const int w = w0 + groups * u + group;
-              const int64_t x = (int64_t)parts.at(min(w, parts.w1)) * p.part_rows + row;
-              const f32x2 o0 = load_part(p.part_o, (x * kHD + d) / 2), o1 = load_part(p.part_o, (x * kHD + d) / 2 + 1);
-              ml[u] = load_part(p.part_ml, x);
-              os[u] = f32x4{o0.x, o0.y, o1.x, o1.y};
+              for (int u = 0; u < kPartsAhead; ++u) {
+                ml[u] = f32x2{-INFINITY, 0.f};
+                os[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (w0 + groups * u > parts.w1) continue;  // (no group has a part left)
+                const int w = w0 + groups * u + group;
+                const int64_t x = (int64_t)parts.at(min(w, parts.w1)) * p.part_rows + row;
+                const f32x2 o0 = load_part(p.part_o, (x * kHD + d) / 2), o1 = load_part(p.part_o, (x * kHD + d) / 2 + 1);
+                ml[u] = load_part(p.part_ml, x);
+                os[u] = f32x4{o0.x, o0.y, o1.x, o1.y};
+              }
+#pragma unroll
+              for (int u = 0; u < kPartsAhead; ++u)
+                if (w0 + groups * u + group > parts.w1) ml[u].x = -INFINITY;
+              a.add(ml, os);
             }
-#pragma unroll
-            for (int u = 0; u < kPartsAhead; ++u)
-              if (w0 + groups * u + group > parts.w1) ml[u].x = -INFINITY;
-            a.add(ml, os);
-          }
-          if (d == 0) {
-            sml[group][row][0] = a.m;
-            sml[group][row][1] = a.l;
-          }
-          *reinterpret_cast<f32x4*>(&so[group][row][d]) = a.o;
-        }
-        __syncthreads();
-        if (group == 0) {
-          const int n = min(groups, parts.w1 - parts.w0 + 1);
-          for (int x = 1; x < n; x += 4) {
-            f32x2 ml[4];
-            f32x4 os[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int y = min(x + u, n - 1);
-              ml[u] = f32x2{x + u < n ? sml[y][row][0] : -INFINITY, sml[y][row][1]};
-              os[u] = *reinterpret_cast<const f32x4*>(&so[y][row][d]);
+            if (d == 0) {
+              sml[group][row][0] = a.m;
+              sml[group][row][1] = a.l;
             }
-            a.add(ml, os);
+            *reinterpret_cast<f32x4*>(&so[group][row][d]) = a.o;
           }
-          store_gated(p, (int64_t)at.b * p.T + tt, qh, d, a.o * (1.f / a.l), gate);
+          __syncthreads();
+          if (group == 0) {
+            const int n = min(groups, parts.w1 - parts.w0 + 1);
+            for (int x = 1; x < n; x += 4) {
+              f32x2 ml[4];
+              f32x4 os[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const int y = min(x + u, n - 1);
+                ml[u] = f32x2{x + u < n ? sml[y][row][0] : -INFINITY, sml[y][row][1]};
+                os[u] = *reinterpret_cast<const f32x4*>(&so[y][row][d]);
+              }
+              a.add(ml, os);
+            }
+            if (i < nrows * 32) store_gated(p, (int64_t)at.b * p.T + tt, qh, d, a.o * (1.f / a.l), gate);
+          }
+          if (64 * W >= 16 * 32) break;  // (one round)
         }
       }
     }
@@ -952,17 +955,22 @@ __global__ __launch_bounds__(64 * kMergeWaves) void attn_verify_q8_merge64_kerne
 // 32 rows 46.5 for 42.6 (8 sequences of 8 tokens after 16000, 16 heads on 4).
 // Blocks of a piece where there are few: 2 (16 tokens after 4096: 14.7 us; 1: 15.7, 4: 15.4).
 // Workgroups: what the device holds at a time, or fewer for a small cache.  sliced: where
-// that makes the merge two rounds of the device at most.
+// that makes the merge two rounds of the device at most.  waves (up to 16 rows): eight; two,
+// in four times the workgroups, where there are at least as many heads as those, which then
+// go side by side instead of one after another: one token of 256 sequences of 4 heads after
+// 60 13.9 us for 21.9, after 500 40 for 48, after 4000 159 for 154, 512 of 2 after 100 18.8
+// for 36.9; more than 8 rows lose more at length than they gain (4 tokens after 500 55 for 52).
 struct VerifyShape {
-  int part_rows, min_cut, runs, sliced;
+  int part_rows, min_cut, runs, sliced, waves;
 };
 VerifyShape verify_shape(int64_t B, int rows, int Hkv, int Smax) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
   VerifyShape v;
   v.part_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   v.min_cut = 2;
+  v.waves = rows <= 8 && B * Hkv >= 4 * cus ? 2 : 8;
   v.sliced = B * Hkv * v.part_rows / 2 <= 2 * cus;
-  v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(rows <= 16 ? cus : 2 * cus, B * Hkv * ceil_div(Smax / kBlk, v.min_cut)));
+  v.runs = (int)std::max<int64_t>(1, std::min<int64_t>(rows > 16 ? 2 * cus : cus * 8 / v.waves, B * Hkv * ceil_div(Smax / kBlk, v.min_cut)));
   return v;
 }
 
@@ -971,8 +979,10 @@ size_t count_bytes(int64_t B, int Hkv) { return (size_t)ceil_div(B * Hkv * 4, 25
 template <int TYPE>
 void launch_verify(const VerifyParams& p, hipStream_t s) {
   const dim3 grid((unsigned)p.runs);
-  if (p.part_rows == 16)
-    hipLaunchKernelGGL((attn_verify_q8_rows16_kernel<TYPE>), grid, dim3(64 * kWaves16), 0, s, p);
+  if (p.part_rows == 16 && p.waves == 2)
+    hipLaunchKernelGGL((attn_verify_q8_rows16_kernel<TYPE, 2>), grid, dim3(64 * 2), 0, s, p);
+  else if (p.part_rows == 16)
+    hipLaunchKernelGGL((attn_verify_q8_rows16_kernel<TYPE, 8>), grid, dim3(64 * 8), 0, s, p);
   else if (p.part_rows == 32)
     hipLaunchKernelGGL((attn_verify_q8_rows64_kernel<TYPE, 1>), grid, dim3(128), 0, s, p);
   else
@@ -1496,8 +1506,11 @@ extern "C" size_t dflash_attn_verify_q8_workspace_bytes(int B, int T, int Hq, in
   if (B <= 0 || T <= 0 || T > kMaxDraft || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || (int64_t)T * (Hq / Hkv) > 64 ||
       Smax <= 0 || Smax % kBlk != 0)
     return 0;
-  const VerifyShape v = verify_shape(B, T * (Hq / Hkv), Hkv, Smax);
-  return count_bytes(B, Hkv) + (size_t)2 * v.runs * v.part_rows * (kHD + 2) * sizeof(float);
+  const int rows = T * (Hq / Hkv);
+  const VerifyShape v = verify_shape(B, rows, Hkv, Smax);
+  int runs = v.runs;
+  if (v.part_rows == 16) runs = std::max(runs, verify_shape(B, 1, Hkv, Smax).runs);  // (fewer rows may have more)
+  return count_bytes(B, Hkv) + (size_t)2 * runs * v.part_rows * (kHD + 2) * sizeof(float);
 }
 
 extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* q, const int32_t* lens,
@@ -1529,6 +1542,7 @@ extern "C" int dflash_attn_verify_q8(const dflash_kv8_cache* cache, const void* 
   p.min_cut = v.min_cut;
   p.runs = v.runs;
   p.sliced = v.sliced;
+  p.waves = v.waves;
   p.count = static_cast<int32_t*>(workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + count_bytes(B, Hkv));
   p.part_ml = p.part_o + (int64_t)2 * p.runs * p.part_rows * kHD;

@@ -82,6 +82,9 @@ def test_verify(device, dtype, T, Hq, Hkv, lens, Smax):
     (8, 8, 2, [1500] + [40] * 20 + [-1, 700], 1536),  # of 32 rows
     (16, 1, 1, [4000], 4032),                         # one head of 16 rows in few parts
     (16, 2, 2, [2500, 100], 2560),
+    (1, 8, 4, [(37 * i) % 190 - (i % 50 == 7) * 500 for i in range(270)] + [1400], 1472),  # more heads than workgroups
+    (2, 16, 4, [(53 * i) % 130 for i in range(256)] + [700, 1000], 1024),
+    (5, 17, 17, [(29 * i) % 140 for i in range(64)], 192),
 ])
 def test_verify_merges(device, dtype, T, Hq, Hkv, lens, Smax):
     _check(device, dtype, T, Hq, Hkv, lens, Smax, seed=T + Hq + len(lens), prompt=False)

@@ -111,6 +111,14 @@ def test_verify_refusals(lib):
         assert lib.dflash_attn_verify_q8_workspace_bytes(*bad) == 0, bad
 
 
+@pytest.mark.parametrize("B,Hkv,Smax", [(1, 4, 4096), (12, 1, 64), (300, 4, 1024), (256, 8, 64), (2000, 1, 8192)])
+def test_verify_workspace_serves_smaller_calls(lib, B, Hkv, Smax):
+    need = lib.dflash_attn_verify_q8_workspace_bytes
+    sizes = {(T, rep): need(B, T, Hkv * rep, Hkv, Smax) for T in range(1, 17) for rep in (1, 2, 3, 4, 8, 16) if T * rep <= 64}
+    for (T, rep), n in sizes.items():
+        assert all(n >= m > 0 for (t, r), m in sizes.items() if t <= T and r <= rep), (T, rep)
+
+
 def test_prefill_refusals(lib):
     c = _cache()
     for name in ("q", "lens", "gate", "out"):
