@@ -103,7 +103,9 @@ __device__ __forceinline__ void store_codes(const Kv8& c, int64_t bh, int j, boo
   __syncthreads();
 }
 
-// The rows of block j at positions [from, to) into the tail.
+// The rows of block j at positions [from, to) into the tail: values turned, 8 positions a
+// store (one by one, a load of 4 sequences of 8192 took 42 us for 18: the last block's
+// workgroup outlasted the rest).
 __device__ __forceinline__ void store_tail(const Kv8& c, int64_t bh, int j, bool values, const Rows& r, int from, int to,
                                            Turn& lds) {
   const int t = threadIdx.x;
@@ -120,9 +122,19 @@ __device__ __forceinline__ void store_tail(const Kv8& c, int64_t bh, int j, bool
   for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(&lds.rows[(t >> 4) + 16 * i][8 * (t & 15)]) = r.x[i];
   __syncthreads();
   uint16_t* dst = c.tail_values(bh) + (t >> 1) * kSlots + (j & 1) * kBlk;
-  for (int i = 0; i < 32; ++i) {
-    const int tk = (t & 1) * 32 + i, pos = kBlk * j + tk;
-    if (pos >= from && pos < to) dst[tk] = lds.rows[tk][t >> 1];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int tk = (t & 1) * 32 + 8 * g, pos = kBlk * j + tk;
+    if (pos >= from && pos + 8 <= to) {
+      u32x4 w;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        w[u] = lds.rows[tk + 2 * u][t >> 1] | ((uint32_t)lds.rows[tk + 2 * u + 1][t >> 1] << 16);
+      *reinterpret_cast<u32x4*>(dst + tk) = w;
+    } else {
+      for (int i = 0; i < 8; ++i)
+        if (pos + i >= from && pos + i < to) dst[tk + i] = lds.rows[tk + i][t >> 1];
+    }
   }
   __syncthreads();
 }
@@ -357,7 +369,7 @@ __device__ __forceinline__ Rows prompt_rows(const AppendParams& p, int b, int h,
 // read from the tail (a waiting block, the first block's earlier positions), task 0 alone
 // touches it: it reads first and stores the last two blocks' rows, which take the same
 // slots, afterwards.  Dynamic LDS: the rotation table, 64 rot floats.
-// Bound by memory: 4096 tokens of 16 heads on 4, 59 MB in 15.2 us, 3.9 TB/s of the 5.2
+// Bound by memory: 4096 tokens of 16 heads on 4, 59 MB in 13.1 us, 4.5 TB/s of the 5.2
 // that a large copy reaches; the rest is a workgroup's way from its loads through the
 // block's maximum to its codes.  (More waves a CU spill.)
 template <int TYPE>
@@ -428,7 +440,8 @@ struct LoadParams {
 };
 
 // Workgroup (block j, keys or values, head): codes if the block is complete, the tail
-// if it is one of the last two.
+// if it is one of the last two.  Bound by memory: 4 sequences of 8192 positions, 101 MB
+// in 18 us, 5.5 TB/s.
 template <int TYPE>
 __global__ __launch_bounds__(256) void kv8_load_kernel(const LoadParams p) {
   __shared__ __attribute__((aligned(16))) Turn lds;
