@@ -20,7 +20,6 @@ rotary are the package's own configuration (16 query and 4 key/value heads of
 128) and generic ones around it.
 """
 import sys
-from functools import lru_cache
 from pathlib import Path
 
 import torch
@@ -181,7 +180,6 @@ def prepare(case, seed):
     return state
 
 
-@lru_cache(maxsize=1)
 def _package():
     root = str(Path(__file__).resolve().parent.parent / "dflash-mlx_amd")
     if root not in sys.path:
