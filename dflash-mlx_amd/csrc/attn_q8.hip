@@ -381,13 +381,13 @@ template <int TYPE, int W>
 __global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const VerifyParams p) {
   __shared__ __attribute__((aligned(16))) float so[W][16][kHD + 4];
   __shared__ float sml[W][16][2];
-  __shared__ int dropped;  // the tail's values hold a NaN or an infinity
+  __shared__ int dropped[2];  // a head's tail values hold a NaN or an infinity
   __shared__ int arrived;
   const Kv8& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  if (tid == 0) dropped = 0;
+  if (tid == 0) dropped[0] = 0;
   __syncthreads();
   Batch batch(p);
   // sequences that take no part: their rows are zero
@@ -404,6 +404,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const 
   const int t = min(p.token_of(r), p.T - 1), rr = r - p.token_of(r) * p.rep;
   const int key0 = 16 * (r >> 2) + (r & 3);  // operand row r of tile n: + 8 (n / 2) + 4 (n % 2)
   bool first_part = true;
+  int flag = 0;  // the head's of dropped[]
   while (at.left > 0) {
     const int L = batch.length(at.b);
     const int seen = seen_positions(L, p.T, c.Smax);
@@ -412,6 +413,9 @@ __global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const 
       ++at.b;
       continue;
     }
+    // The next head's flag, last read before the barrier that ended the head before this
+    // one, is cleared ahead of this head's barriers: behind them a wave may set it.
+    if (tid == 0) dropped[flag ^ 1] = 0;
     const int b1 = min(nb, at.blk + at.left);
     const int base = min(L, c.Smax), done = base >> 6;
     const int64_t bh = (int64_t)at.b * c.Hkv + at.h;
@@ -523,7 +527,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const 
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) bits |= nonfinite_bits(vt[dt][0]) | nonfinite_bits(vt[dt][1]);
       if (__any(any_nonfinite(bits))) {
-        if (any_nonfinite(bits)) dropped = 1;
+        if (any_nonfinite(bits)) dropped[flag] = 1;
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
           vt[dt][0] = drop_nonfinite(vt[dt][0]);
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const 
         ll = fmaf(sml[x][row][1], f, ll);
         oo += *reinterpret_cast<const f32x4*>(&so[x][row][d]) * f;
       }
-      if (dropped)
+      if (dropped[flag])
 #pragma unroll 1
         for (int e = 0; e < 4; ++e) {
           const float x = dropped_values(c, bh, d + e, kBlk * max(done, at.blk), min(min(base + tt, seen - 1), kBlk * b1 - 1));
@@ -644,7 +648,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const 
       }
     }
     __syncthreads();
-    if (tid == 0) dropped = 0;
+    flag ^= 1;
     first_part = false;
     at.left -= b1 - at.blk;
     at.blk = 0;
@@ -673,13 +677,13 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
   constexpr int BUF = 2 * kBlk * kHD * 2;  // bytes of a block's K and V^T in bf16
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
   __shared__ f32x2 sml[RT][2][32];
-  __shared__ int dropped;  // the tail's values hold a NaN or an infinity
+  __shared__ int dropped[2];  // a head's tail values hold a NaN or an infinity
   const Kv8& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, hl = lane >> 5;
   const int hf = wave / RT, rt = wave % RT;
-  if (tid == 0) dropped = 0;
+  if (tid == 0) dropped[0] = 0;
   __syncthreads();
   Batch batch(p);
   Share at = share_of(p, batch, blockIdx.x);
@@ -689,6 +693,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
   const int row = 32 * rt + r32;
   const int t = min(p.token_of(row), p.T - 1), rr = row - p.token_of(row) * p.rep;
   bool first_part = true;
+  int flag = 0;  // the head's of dropped[]
   while (at.left > 0) {
     const int L = batch.length(at.b);
     const int seen = seen_positions(L, p.T, c.Smax);
@@ -697,6 +702,9 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
       ++at.b;
       continue;
     }
+    // The next head's flag, last read before the barrier that ended the head before this
+    // one, is cleared ahead of this head's barriers: behind them a wave may set it.
+    if (tid == 0) dropped[flag ^ 1] = 0;
     const int b1 = min(nb, at.blk + at.left);
     const int base = min(L, c.Smax), done = base >> 6;
     const int64_t bh = (int64_t)at.b * c.Hkv + at.h;
@@ -766,7 +774,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
           const u32x4 x = drop_nonfinite(vt[i][0]), y = drop_nonfinite(vt[i][1]);
           store_pair(vdst + 32 * NT * i, 2 * (tid & 3), vrow & 7, u32x4{x.x, x.y, y.x, y.y}, u32x4{x.z, x.w, y.z, y.w});
         }
-        if (any_nonfinite(bits)) dropped = 1;
+        if (any_nonfinite(bits)) dropped[flag] = 1;
       }
     };
     load_block(at.blk);
@@ -851,7 +859,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
     for (int q = 8 * hf; q < 8 * hf + 8; ++q) {
       f32x4 v = so[q * 64] * c0 + so[(16 + q) * 64] * c1;
       const int d = 32 * (q >> 2) + 8 * (q & 3) + 4 * hl;
-      if (dropped)
+      if (dropped[flag])
 #pragma unroll 1
         for (int e = 0; e < 4; ++e) {
           const float x = dropped_values(c, bh, d + e, kBlk * max(done, at.blk), min(last, kBlk * b1 - 1));
@@ -870,7 +878,7 @@ __global__ __launch_bounds__(128 * RT, 2) void attn_verify_q8_rows64_kernel(cons
     }
     if (!whole && hf == 0 && hl == 0) *reinterpret_cast<f32x2*>(p.part_ml + (part * 32 + r32) * 2) = f32x2{mn, ls};
     __syncthreads();
-    if (tid == 0) dropped = 0;
+    flag ^= 1;
     first_part = false;
     at.left -= b1 - at.blk;
     at.blk = 0;
