@@ -369,9 +369,12 @@ def kv_rewind_q8(cache: QuantizedKVCache, length: int, written: int) -> int:
 
     if rest and not intact(blk):
         refill(blk)
+    # what a later rewind finds: block blk's slots are its own, or, at a block's end with later
+    # positions written, no longer block blk - 2's
+    kept = length if rest else min(written, length + 1)
     if intact(blk - 1):
-        return length
+        return kept
     if rest <= MAX_DRAFT:  # the next append may quantise block blk - 1 again
         refill(blk - 1)
-        return length
+        return kept
     return min(written, blk * BLOCK + SLOTS)  # (block blk is there, block blk - 1 is not)
