@@ -324,7 +324,8 @@ def kv_load_q8(k, v, lens, cache: QuantizedKVCache) -> None:
 def kv_read_q8(cache: QuantizedKVCache, lens, count: int, *, start=0):
     """(keys, values) bf16 [B, Hkv, count, 128] at positions start + i, as an
     attention at committed length lens[b] reads them; positions outside [0,
-    lens[b]) are zero.  start: an int, or int32 [B] on the device."""
+    lens[b]) are zero.  A length below one already written to is read after
+    kv_rewind_q8, like any call at it.  start: an int, or int32 [B] on the device."""
     _check_cache(cache)
     _check_lens("lens", lens, cache)
     count = int(count)

@@ -85,7 +85,7 @@ class DeviceQuantizedKVCache(KVCache):
     as DeviceKVCache's, ``keys`` and ``values`` read back in bf16.  ``written``
     counts the positions ever written since the tail was made ready, rejected
     drafts included: prepare() looks whether the tail still holds what a call
-    at ``offset`` reads."""
+    at ``offset`` reads, and refills it if not."""
 
     def __init__(self, cache: QuantizedKVCache):
         self.cache = cache
@@ -102,7 +102,7 @@ class DeviceQuantizedKVCache(KVCache):
         self.written = max(self.written, n)
 
     def prepare(self) -> None:
-        """Before a forward at ``offset``."""
+        """Before a forward or a read at ``offset``."""
         if self._offset < self.written:
             self.written = kv_rewind_q8(self.cache, self._offset, self.written)
 
@@ -111,6 +111,7 @@ class DeviceQuantizedKVCache(KVCache):
         return self.cache.Smax
 
     def _read(self):
+        self.prepare()  # after a trim the tail may hold later positions
         lens = torch.full((self.cache.B,), self._offset, dtype=torch.int32, device=self.cache.device)
         return kv_read_q8(self.cache, lens, self._offset)
 

@@ -100,8 +100,8 @@ int dflash_kv8_load(const dflash_kv8_cache* cache, const void* k,
  * [B, Hkv, count, 128] (either may be NULL), as an attention at committed length
  * lens[b] would see them: blocks below lens[b] / 64 as their codes stand for
  * (block lens[b] / 64 - 1, if it may still wait for its codes, as they will stand
- * for), the rest from the tail.  Positions outside [0, min(lens[b], Smax)) read as
- * zero.  starts may be NULL.
+ * for), the rest from the tail, which has to hold them at that length (Lengths
+ * above).  Positions outside [0, min(lens[b], Smax)) read as zero.  starts may be NULL.
  */
 int dflash_kv8_read(const dflash_kv8_cache* cache, const int32_t* lens,
                     const int32_t* starts, int start, int count, void* k_out,
