@@ -37,8 +37,12 @@ __device__ __forceinline__ void quantise_tail_block(const Kv8& c, int64_t bh, in
   if (t == 0) (values ? c.vs : c.ks)[bh * c.nblk + j] = sm.x;
 }
 
-// Block L / 64 - 1 may have become complete since the last append.
-__device__ __forceinline__ bool may_wait(int L, int Smax) { return L >= kBlk && L <= Smax && (L & 63) <= kMaxDraft; }
+// Block L / 64 - 1 may have become complete since the last append: with L past the cache's
+// end by a draft block's tokens, its last block.
+__device__ __forceinline__ bool may_wait(int L, int Smax) {
+  return L >= kBlk && L - kMaxDraft <= Smax && (L & 63) <= kMaxDraft;
+}
+__device__ __forceinline__ int waiting_block(int L, int Smax) { return (min(L, Smax) >> 6) - 1; }
 
 // A block's 64 rows in registers: piece i of a thread is token tid / 16 + 16 i, features
 // 8 (tid % 16) .. + 7.
@@ -265,7 +269,7 @@ __global__ __launch_bounds__(256) void kv8_append_draft_kernel(const AppendParam
   if ((int)blockIdx.x < nquant) {
     const int64_t bh = blockIdx.x >> 1;
     const int L = p.lens[bh / c.Hkv];
-    if (may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, (L >> 6) - 1, blockIdx.x & 1, red);
+    if (may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, waiting_block(L, c.Smax), blockIdx.x & 1, red);
     return;
   }
   const int slots = p.Hq + 2 * c.Hkv, groups = (slots + 15) >> 4;
@@ -387,10 +391,10 @@ __global__ __launch_bounds__(256, 4) void kv8_append_prompt_kernel(const AppendP
     const int64_t bh = id >> 1;
     const int b = (int)(bh / c.Hkv), h = (int)(bh % c.Hkv);
     const int L = p.lens[b];
+    if (i == 0 && may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, waiting_block(L, c.Smax), values, red);
     if (L < 0 || L > c.Smax) return;
     const int first = L >> 6, end = min(L + p.T, c.Smax), done = end >> 6, j = first + i;
     const bool reads_tail = (L & 63) != 0 || may_wait(L, c.Smax);
-    if (reads_tail && i == 0 && may_wait(L, c.Smax)) quantise_tail_block<TYPE>(c, bh, first - 1, values, red);
     const int tail0 = max(done - 1, first);  // the first block that the tail keeps
 #pragma unroll 1
     for (int step = 0; step < (reads_tail && i == 0 ? 3 : 1); ++step) {
@@ -501,7 +505,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const ReadParams p) {
   for (int u = 0; u < 4; ++u) r.x[u] = u32x4{0u, 0u, 0u, 0u};
   if (block >= 0 && kBlk * block < held) {
     const int j = (int)block;
-    const bool waits = j == (held >> 6) - 1 && may_wait(L, c.Smax);
+    const bool waits = j == waiting_block(L, c.Smax) && may_wait(L, c.Smax);
     if (j < held >> 6 && !waits) {
       const float s = (values ? c.vs : c.ks)[bh * c.nblk + j];
       u32x2 q[4];

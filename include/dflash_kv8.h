@@ -32,8 +32,10 @@
  *
  * Lengths: lens[b] (device int32) is sequence b's committed length before the
  * call's tokens.  lens[b] < 0 marks a sequence that takes no part: nothing of it
- * is written to the cache and its output rows are zero.  Positions at or past
- * Smax are never written nor read.  Between two draft appends (at most 16 tokens) lens[b]
+ * is written to the cache, and an attention's or a read's rows of it are zero (the
+ * append's queries are computed all the same).  Positions at or past Smax are never
+ * written nor read; a length that draft tokens carry past Smax stands for the
+ * positions below it.  Between two draft appends (at most 16 tokens) lens[b]
  * grows by at most the tokens of the first; it may fall (a rewind) to L as long as
  * the tail still holds what the next call reads: with W the largest position
  * written since the tail was last loaded, plus one, W <= 64 (L / 64) + 64 where
@@ -71,7 +73,8 @@ typedef struct {
  * and values appended at positions lens[b] + t.
  *   prompt == 0: T <= 16 draft tokens.  They go to the tail; block lens[b] / 64 - 1
  *     is quantised from the tail if lens[b] % 64 <= 16 (it may have become complete
- *     since the last append; the same codes again otherwise).
+ *     since the last append; the same codes again otherwise), the cache's last block if
+ *     Smax <= lens[b] <= Smax + 16.
  *   prompt != 0: T committed tokens (lens grows by T).  Every block that they complete
  *     is quantised, and the tail holds the last two blocks' positions.
  * overflow (or NULL): [B], set to 1 for a sequence with a position outside
