@@ -618,7 +618,10 @@ __global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const 
               }
 #pragma unroll
               for (int u = 0; u < kPartsAhead; ++u)
-                if (w0 + groups * u + group > parts.w1) ml[u].x = -INFINITY;
+                if (w0 + groups * u + group > parts.w1) {  // (the last again, not to be added: it may be infinite)
+                  ml[u].x = -INFINITY;
+                  os[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
               a.add(ml, os);
             }
             if (d == 0) {
@@ -638,6 +641,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_verify_q8_rows16_kernel(const 
                 const int y = min(x + u, n - 1);
                 ml[u] = f32x2{x + u < n ? sml[y][row][0] : -INFINITY, sml[y][row][1]};
                 os[u] = *reinterpret_cast<const f32x4*>(&so[y][row][d]);
+                if (x + u >= n) os[u] = f32x4{0.f, 0.f, 0.f, 0.f};
               }
               a.add(ml, os);
             }
