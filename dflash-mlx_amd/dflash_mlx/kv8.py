@@ -229,11 +229,13 @@ def attn_verify_q8_workspace_bytes(B: int, T: int, num_heads: int, Hkv: int, Sma
 
 
 def _verify_workspace(cache: QuantizedKVCache, T: int, Hq: int) -> torch.Tensor:
-    """The cache's workspace of the current stream; of a captured graph its own."""
+    """The cache's workspace of its device's current stream; of a captured graph its own."""
+    if torch.cuda.current_device() != cache.device.index:  # (the capture's state is the current device's)
+        with torch.cuda.device(cache.device):
+            return _verify_workspace(cache, T, Hq)
     n = cache._ws_bytes.get((T, Hq))
     if n is None:
-        with torch.cuda.device(cache.device):
-            n = cache._ws_bytes[(T, Hq)] = attn_verify_q8_workspace_bytes(cache.B, T, Hq, cache.Hkv, cache.Smax)
+        n = cache._ws_bytes[(T, Hq)] = attn_verify_q8_workspace_bytes(cache.B, T, Hq, cache.Hkv, cache.Smax)
     capturing = torch.cuda.is_current_stream_capturing()
     stream = _lib.stream_handle(cache.device)
     ws = None if capturing else cache._workspaces.get(stream)
