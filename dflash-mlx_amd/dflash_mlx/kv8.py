@@ -359,8 +359,10 @@ def kv_rewind_q8(cache: QuantizedKVCache, length: int, written: int) -> int:
         raise ValueError(f"need 0 <= length <= {cache.Smax} and written >= length, got {length} and {written}")
     blk, rest = divmod(length, BLOCK)
 
-    def intact(x):  # no later position has taken block x's slots
-        return x < 0 or written <= x * BLOCK + SLOTS
+    def intact(x):
+        # no later position has taken block x's slots, nor did a prompt or a load end where the
+        # block after it does, which keeps that one alone
+        return x < 0 or written < x * BLOCK + SLOTS
 
     def refill(x):
         # as read at a length past it: from its codes, which it got before its slots were taken
@@ -372,12 +374,9 @@ def kv_rewind_q8(cache: QuantizedKVCache, length: int, written: int) -> int:
 
     if rest and not intact(blk):
         refill(blk)
-    # what a later rewind finds: block blk's slots are its own, or, at a block's end with later
-    # positions written, no longer block blk - 2's
-    kept = length if rest else min(written, length + 1)
     if intact(blk - 1):
-        return kept
+        return length
     if rest <= MAX_DRAFT:  # the next append may quantise block blk - 1 again
         refill(blk - 1)
-        return kept
-    return min(written, blk * BLOCK + SLOTS)  # (block blk is there, block blk - 1 is not)
+        return length
+    return min(written, blk * BLOCK + SLOTS - 1)  # (block blk is there, block blk - 1 is not)

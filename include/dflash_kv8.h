@@ -38,8 +38,9 @@
  * positions below it.  Between two draft appends (at most 16 tokens) lens[b]
  * grows by at most the tokens of the first; it may fall (a rewind) to L as long as
  * the tail still holds what the next call reads: with W the largest position
- * written since the tail was last loaded, plus one, W <= 64 (L / 64) + 64 where
- * L % 64 <= 16, else W <= 64 (L / 64) + 128.  dflash_kv8_load sets any state anew.
+ * written since the tail was last loaded, plus one, W < 64 (L / 64) + 64 where
+ * L % 64 <= 16, else W < 64 (L / 64) + 128 (L = 0 takes nothing from it).
+ * dflash_kv8_load sets any state anew.
  */
 #ifndef DFLASH_KV8_H
 #define DFLASH_KV8_H
@@ -76,7 +77,7 @@ typedef struct {
  *     since the last append; the same codes again otherwise), the cache's last block if
  *     Smax <= lens[b] <= Smax + 16.
  *   prompt != 0: T committed tokens (lens grows by T).  Every block that they complete
- *     is quantised, and the tail holds the last two blocks' positions.
+ *     is quantised, and the tail holds the last of those and the open block.
  * overflow (or NULL): [B], set to 1 for a sequence with a position outside
  * [0, Smax).  rot_dims in {0, 16, 32, 64, 128}; Hq a multiple of Hkv; proj, its rows
  * and q_out 16-byte aligned.
@@ -91,7 +92,7 @@ int dflash_kv8_append(const dflash_kv8_cache* cache, const void* proj,
  * Load: positions [0, lens[b]) of every sequence (lens clamped to [0, min(S, Smax)])
  * from bf16 keys and values k, v [B, Hkv, S, 128], the last axis contiguous and
  * the others strided (k_strides, v_strides: b, h, position, in elements, multiples
- * of 8), complete blocks quantised and the last two blocks' positions to the tail.
+ * of 8), complete blocks quantised, the last of them and the open block to the tail.
  */
 int dflash_kv8_load(const dflash_kv8_cache* cache, const void* k,
                     const int64_t* k_strides, const void* v,

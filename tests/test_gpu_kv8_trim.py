@@ -36,10 +36,24 @@ def test_read_after_trims(weights, device, dtype, cuts):  # noqa: F811
     cache = m.make_cache()
     m.forward_dflash(_tokens(330), cache, [3])
     m.forward_dflash(_tokens(16, seed=3), cache, [3])
+    cache[cache.attn_idx[0]].trim(16)  # a rejected block
+    _trim_and_read(m, cache, 330, cuts, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [128, 320])
+@pytest.mark.parametrize("cuts", [(1,), (47,), (50,), (60,), (64,), (80,), (110,), (64, 50)])
+def test_read_after_trims_of_a_prompt_of_whole_blocks(weights, device, dtype, n, cuts):  # noqa: F811
+    """The prompt leaves its last block in the tail, and none before it."""
+    m = _model(weights, device, dtype)
+    cache = m.make_cache()
+    m.forward_dflash(_tokens(n), cache, [3])
+    _trim_and_read(m, cache, n, cuts, dtype)
+
+
+def _trim_and_read(m, cache, n, cuts, dtype):
     c = cache[cache.attn_idx[0]]
-    c.trim(16)  # a rejected block
     before = [x.clone() for x in _keys_values(cache)]
-    n = 330
     for cut in cuts:
         c.trim(cut)
         n -= cut

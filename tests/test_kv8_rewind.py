@@ -41,7 +41,7 @@ class Sequence:
         assert torch.equal(self.cache.tail_k[0, 0, p, 0], self.cache.tail_vt[0, 0, 0, p])
         return self.cache.tail_k[0, 0, p, 0]
 
-    def append(self, T, keep):
+    def append(self, T, keep, prompt=False):
         L = self.length
         blk = L // BLOCK
         assert torch.equal(self._slots(blk * BLOCK, L), self.kept[blk * BLOCK:]), f"the open block at {L}"
@@ -52,10 +52,15 @@ class Sequence:
         T = min(T, SMAX - L)
         new = self.tokens + 1.0 + torch.arange(T)
         self.tokens += T
-        p = torch.arange(L, L + T) % SLOTS
-        self.cache.tail_k[0, 0, p, 0] = self.cache.tail_vt[0, 0, 0, p] = new
-        self.written = max(self.written, L + T)
         self.kept = torch.cat((self.kept, new[:keep]))
+        lo = L
+        if prompt:  # codes of what it completes; the tail takes the last block with codes and the open one
+            done = self.length // BLOCK
+            self.codes[blk:done] = self.kept[blk * BLOCK:done * BLOCK].view(-1, BLOCK)
+            lo = max(L, (done - 1) * BLOCK)
+        p = torch.arange(lo, L + T) % SLOTS
+        self.cache.tail_k[0, 0, p, 0] = self.cache.tail_vt[0, 0, 0, p] = new[lo - L:]
+        self.written = max(self.written, L + T)
 
     def rewind(self, length):
         self.written = kv8.kv_rewind_q8(self.cache, length, self.written)
@@ -72,6 +77,15 @@ def test_two_rewinds_in_a_row(monkeypatch):
     s.append(5, 5)
 
 
+@pytest.mark.parametrize("n,length", [(448, 384), (448, 398), (448, 330), (128, 64), (450, 384), (447, 384)])
+def test_a_rewind_after_a_prompt(monkeypatch, n, length):
+    """One that ends a block leaves no earlier one in the tail."""
+    s = Sequence(monkeypatch)
+    s.append(n, n, prompt=True)
+    s.rewind(length)
+    s.append(5, 5)
+
+
 @pytest.mark.parametrize("seed", range(20))
 def test_any_chain_of_appends_and_rewinds(monkeypatch, seed):
     rng = random.Random(seed)
@@ -79,8 +93,14 @@ def test_any_chain_of_appends_and_rewinds(monkeypatch, seed):
     again = False
     for _ in range(1500):
         if rng.random() < (0.4 if again else 0.97) and s.length + 16 <= SMAX:
-            T = rng.randint(1, 16)
-            s.append(T, rng.choice([T, T, rng.randint(0, T)]))
+            if rng.random() < 0.1:
+                n = min(rng.randint(1, 200), SMAX - s.length)
+                if rng.random() < 0.5:  # up to a block's end
+                    n = max(1, (s.length + n) // BLOCK * BLOCK - s.length)
+                s.append(n, n, prompt=True)
+            else:
+                T = rng.randint(1, 16)
+                s.append(T, rng.choice([T, T, rng.randint(0, T)]))
             again = False
         else:
             length = rng.randint(max(0, s.length - 150), s.length)
