@@ -1,5 +1,6 @@
-// Device helpers shared by the attention kernels of the bf16 cache
-// (model_ops.hip) and of the 8-bit cache (kv8.hip, attn_q8.hip).
+// Device helpers of the attention kernels: of the bf16 cache's (model_ops.hip) and of
+// the 8-bit cache's (kv8.hip, attn_q8.hip).  Rotation, norm_rotate and the sums and
+// roundings that they use are the bf16 cache's alone.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -1016,7 +1016,7 @@ void launch_verify(const VerifyParams& p, hipStream_t s) {
 //     c ^ (r % 8).
 //   - Weights are rounded to bf16 for P V, as in the verify kernel.
 // 4 D operations a pair of positions bound it.  16 heads on 4, e4m3: 4096 rows 87 us, 790
-// TFLOP/s; 2048 rows after 14336 276 us, 930 TFLOP/s; a large library product of bf16
+// TFLOP/s; 2048 rows after 14336 280 us, 920 TFLOP/s; a large library product of bf16
 // reaches 1300.  int8 takes 92 us for 4096 rows (its bytes take more instructions to
 // become bf16).  A turn takes 5000 cycles, of which the matrix unit works 2048; one wave's
 // softmax (1400) and staging (1100) run beside the other's products, and what is left over

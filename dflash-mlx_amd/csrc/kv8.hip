@@ -373,9 +373,10 @@ __device__ __forceinline__ Rows prompt_rows(const AppendParams& p, int b, int h,
 // read from the tail (a waiting block, the first block's earlier positions), task 0 alone
 // touches it: it reads first and stores the last two blocks' rows, which take the same
 // slots, afterwards.  Dynamic LDS: the rotation table, 64 rot floats.
-// Bound by memory: 4096 tokens of 16 heads on 4, 59 MB in 13.1 us, 4.5 TB/s of the 5.2
-// that a large copy reaches; the rest is a workgroup's way from its loads through the
-// block's maximum to its codes.  (More waves a CU spill.)
+// 4096 tokens of 16 heads on 4 move 46 MB in 13 us, 3.5 TB/s of the 5.2 that a large copy
+// reaches: a workgroup's way from its loads through the block's maximum to its codes, and
+// the query tiles' rotation tables, computed again for every four heads, are not hidden.
+// (More waves a CU spill.)
 template <int TYPE>
 __global__ __launch_bounds__(256, 4) void kv8_append_prompt_kernel(const AppendParams p) {
   __shared__ __attribute__((aligned(16))) Turn lds;

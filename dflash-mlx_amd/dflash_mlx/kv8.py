@@ -194,8 +194,8 @@ def attn_prep_q8(proj, q_norm, k_norm, lens, cache: QuantizedKVCache, *, num_hea
     """Queries [B, T, num_heads, 128] bf16 from the projection rows, the new keys
     and values appended to the cache at lens[b] + t.
 
-    proj: bf16 [B, T, >= (2 num_heads + 2 Hkv) 128] laid out [heads x (query |
-    gate), Hkv x key, Hkv x value]; q_norm, k_norm: bf16 [128] RMSNorm weights;
+    proj: bf16 [B, T, >= (2 num_heads + 2 Hkv) 128], rows evenly spaced and 16-byte
+    aligned, laid out [heads x (query | gate), Hkv x key, Hkv x value]; q_norm, k_norm: bf16 [128] RMSNorm weights;
     rotary over the first rot_dims (0, 16, 32, 64 or 128) features.
 
     prompt=False: T <= 16 draft tokens, of which any number may be rejected (the
