@@ -38,6 +38,7 @@ from .kv8 import (
     kv_read_q8,
     kv_rewind_q8,
 )
+from .logits import LogitsState, process_logits
 from .runtime import (
     DFlashRuntimeEvent,
     dflash_generate,
@@ -70,6 +71,7 @@ __all__ = [
     "verify_block_parallel_lazy_logits",
     "verify_block_stream",
     "KVCache",
+    "LogitsState",
     "QuantizedKVCache",
     "Qwen35TargetAdapter",
     "adapter_for_model_type",
@@ -93,6 +95,7 @@ __all__ = [
     "lm_head_greedy_accept",
     "longest_prefix_match",
     "make_rollback_record",
+    "process_logits",
     "rewind_kv_caches",
     "rollback_linear_caches",
     "sample_tokens",

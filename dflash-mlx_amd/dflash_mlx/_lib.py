@@ -1,5 +1,5 @@
-"""ctypes binding of libdflash_gfx950.so (declared in include/dflash_gdn.h and
-include/dflash_kv8.h).
+"""ctypes binding of libdflash_gfx950.so (declared in include/dflash_gdn.h,
+include/dflash_kv8.h and include/dflash_logits.h).
 
 The library is loaded after ``import torch`` so that it binds to the HIP
 runtime torch already loaded (both use the soname libamdhip64.so.7); loading
@@ -22,7 +22,7 @@ DFLASH_DTYPE_F32 = 0
 DFLASH_DTYPE_BF16 = 1
 DFLASH_DTYPE_F16 = 2
 
-# Every entry point of both headers, with its ctypes signature.
+# Every entry point of the headers, with its ctypes signature.
 _VP = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -131,6 +131,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dflash_greedy_accept": (
         _I,
         [_VP, _I, _I64, _I64, _VP, _I64, _I, _VP, _VP, _VP, _I, _I, _I, _VP, _SZ, _VP],
+    ),
+    "dflash_logits_state_reset": (_I, [_VP, _VP]),
+    "dflash_logits_state_add": (_I, [_VP, _VP, _I64, _I, _VP, _I, _VP]),
+    "dflash_logits_state_set_bias": (_I, [_VP, _VP, _I64, _VP, _I64, _I, _VP]),
+    "dflash_logits_process": (
+        _I, [_VP, _I, _I64, _I64, _VP, _VP, _I64, _I, _VP, _I64, _I64, _VP, _I64, _I64, _I, _I, _I, _VP]),
+    "dflash_greedy_accept_processed": (
+        _I,
+        [_VP, _I, _I64, _I64, _VP, _I64, _I, _VP, _VP, _I64, _I64, _VP, _VP, _VP, _I, _I, _I, _VP, _SZ, _VP],
     ),
     "dflash_gdn_prologue": (
         _I,

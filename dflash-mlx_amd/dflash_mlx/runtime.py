@@ -38,6 +38,8 @@ import torch
 
 from . import _lib
 from .gated_delta import _require_device
+from .kv8 import _call
+from .logits import LogitsState, check_draft, check_mask, check_state
 
 
 def _as_3d(logits: torch.Tensor) -> torch.Tensor:
@@ -55,6 +57,8 @@ def greedy_accept(
     draft: torch.Tensor | Sequence[int] | Sequence[Sequence[int]] | None = None,
     *,
     want_posterior: bool = True,
+    state: LogitsState | None = None,
+    mask: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor, torch.Tensor]:
     """Fused greedy verify on the device.
 
@@ -63,11 +67,17 @@ def greedy_accept(
     (posterior [B,N] or None, matched [B], bonus [B]) with
     posterior = argmax(logits, -1) (lowest index on ties),
     matched = leading positions where draft == posterior (<= min(n, N)),
-    bonus = posterior[matched] or -1 when matched == N."""
+    bonus = posterior[matched] or -1 when matched == N.
+
+    state, mask: the argmax is of the processed logits (logits.process_logits, in
+    fp32 whatever the logits' type), which are not stored; draft i is then known
+    to the rows from i + 1 on.  A row that its mask leaves nothing gives token 0."""
     _require_device("logits", logits, None)
     lg = _as_3d(logits)
     if lg.stride(-1) != 1:
         lg = lg.contiguous()
+    if state is not None or mask is not None:
+        return _greedy_accept_processed(lg, draft, want_posterior, state, mask)
     B, N, V = lg.shape
     dev = lg.device
     if draft is None:
@@ -103,6 +113,28 @@ def greedy_accept(
         _lib.ptr(post), matched.data_ptr(), bonus.data_ptr(), B, N, V,
         ws.data_ptr(), ws.numel(), _lib.stream_handle(dev),
     )
+    return post, matched, bonus
+
+
+def _greedy_accept_processed(lg, draft, want_posterior, state, mask):
+    """greedy_accept of [B, N, V] logits under a state and a mask."""
+    B, N, V = lg.shape
+    dev = lg.device
+    sp = check_state(state, B, V, dev)
+    d = check_draft(draft, B, N, dev, state is not None)
+    mp, mb, mr = check_mask(mask, B, N, V, dev) if mask is not None else (None, 0, 0)
+    post = torch.empty((B, N), dtype=torch.int32, device=dev) if want_posterior else None
+    ends = torch.empty((2, B), dtype=torch.int32, device=dev)
+    matched, bonus = ends[0], ends[1]
+    if B == 0:
+        return post, matched, bonus
+    if N == 0 or V == 0:
+        raise ValueError(f"logits need at least one row and one vocabulary entry, got {tuple(lg.shape)}")
+    ws_bytes = int(_lib.load().dflash_greedy_accept_workspace_bytes(B, N, V))
+    ws = torch.empty((max(ws_bytes, 8),), dtype=torch.uint8, device=dev)
+    _call("dflash_greedy_accept_processed", dev, lg.data_ptr(), _lib.dtype_tag(lg.dtype), lg.stride(0), lg.stride(1),
+          _lib.ptr(d), d.stride(0) if d is not None else 0, d.shape[1] if d is not None else 0, sp, mp, mb, mr,
+          _lib.ptr(post), matched.data_ptr(), bonus.data_ptr(), B, N, V, ws.data_ptr(), ws.numel())
     return post, matched, bonus
 
 
