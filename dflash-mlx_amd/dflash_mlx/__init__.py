@@ -27,6 +27,7 @@ from .gated_delta import (
     gated_delta_verify_rollback,
     tape_select,
 )
+from .int8 import Int8Weight, linear_i8, matmul_i8, pack_weight_i8, quantize_rows_i8, quantize_weight_i8
 from .kv8 import (
     QuantizedKVCache,
     attn_prefill_q8,
@@ -70,6 +71,7 @@ __all__ = [
     "verify_block_parallel_greedy_argmax",
     "verify_block_parallel_lazy_logits",
     "verify_block_stream",
+    "Int8Weight",
     "KVCache",
     "LogitsState",
     "QuantizedKVCache",
@@ -91,11 +93,16 @@ __all__ = [
     "kv_load_q8",
     "kv_read_q8",
     "kv_rewind_q8",
+    "linear_i8",
     "lm_head_argmax",
     "lm_head_greedy_accept",
     "longest_prefix_match",
     "make_rollback_record",
+    "matmul_i8",
+    "pack_weight_i8",
     "process_logits",
+    "quantize_rows_i8",
+    "quantize_weight_i8",
     "rewind_kv_caches",
     "rollback_linear_caches",
     "sample_tokens",

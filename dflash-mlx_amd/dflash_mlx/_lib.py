@@ -1,5 +1,5 @@
 """ctypes binding of libdflash_gfx950.so (declared in include/dflash_gdn.h,
-include/dflash_kv8.h and include/dflash_logits.h).
+include/dflash_kv8.h, include/dflash_int8.h and include/dflash_logits.h).
 
 The library is loaded after ``import torch`` so that it binds to the HIP
 runtime torch already loaded (both use the soname libamdhip64.so.7); loading
@@ -132,6 +132,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I,
         [_VP, _I, _I64, _I64, _VP, _I64, _I, _VP, _VP, _VP, _I, _I, _I, _VP, _SZ, _VP],
     ),
+    "dflash_weight_i8_bytes": (_SZ, [_I, _I, _I]),
+    "dflash_weight_i8_scales": (_SZ, [_I, _I]),
+    "dflash_weight_pack_i8": (_I, [_VP, _I64, _VP, _VP, _VP, _I, _I, _I, _VP]),
+    "dflash_quantize_rows_i8": (_I, [_VP, _I, _I64, _VP, _I64, _VP, _I, _I, _VP]),
+    "dflash_gemm_i8": (_I, [_VP, _I64, _VP, _VP, _VP, _VP, _I, _I64, _I, _I, _I, _I, _VP]),
     "dflash_logits_state_reset": (_I, [_VP, _VP]),
     "dflash_logits_state_add": (_I, [_VP, _VP, _I64, _I, _VP, _I, _VP]),
     "dflash_logits_state_set_bias": (_I, [_VP, _VP, _I64, _VP, _I64, _I, _VP]),
