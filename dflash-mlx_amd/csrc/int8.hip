@@ -8,20 +8,12 @@
 #include "device_common.h"
 #include "dflash_int8.h"
 #include "host_common.h"
+#include "int8_common.h"
 
 namespace dflash {
 namespace {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x4 u32x4_e2 __attribute__((aligned(2)));  // a vector at any element of 16 bits
-typedef u32x2 u32x2_e2 __attribute__((aligned(2)));
-typedef f32x4 f32x4_e4 __attribute__((aligned(4)));
-
-inline int k_steps(int K) { return 2 * (int)ceil_div(K, 128); }
-inline int channel_tiles(int N, int gated) {
-  return gated ? 2 * (int)ceil_div(N / 2, 16) : (int)ceil_div(N, 16);
-}
 
 // ------------------------------------------------------------------ quantise
 
@@ -133,86 +125,9 @@ __global__ __launch_bounds__(256) void pack_kernel(const int8_t* codes, int64_t 
 
 // ------------------------------------------------------------------- product
 
-struct GemmParams {
-  const uint8_t* x;
-  int64_t xs;
-  const float* sx;
-  const u32x4* w;
-  const float* sw;
-  void* out;
-  int64_t os;
-  int M, cols;  // output rows and columns
-  int K, k_steps, tiles;
-};
-
-template <typename T>
-struct Out;
-template <>
-struct Out<float> {
-  static __device__ void store4(float* p, const float (&v)[4]) {
-    *reinterpret_cast<f32x4_e4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-  }
-  static __device__ float one(float v) { return v; }
-};
-template <>
-struct Out<uint16_t> {  // bf16
-  static __device__ void store4(uint16_t* p, const float (&v)[4]) {
-    *reinterpret_cast<u32x2_e2*>(p) = u32x2{f32_to_bf16_rne(v[0]) | (uint32_t)f32_to_bf16_rne(v[1]) << 16,
-                                            f32_to_bf16_rne(v[2]) | (uint32_t)f32_to_bf16_rne(v[3]) << 16};
-  }
-  static __device__ uint16_t one(float v) { return f32_to_bf16_rne(v); }
-};
-template <>
-struct Out<_Float16> {
-  static __device__ void store4(_Float16* p, const float (&v)[4]) {
-    typedef _Float16 h4 __attribute__((ext_vector_type(4), aligned(2)));
-    *reinterpret_cast<h4*>(p) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-  }
-  static __device__ _Float16 one(float v) { return (_Float16)v; }
-};
-
-// 4 neighbouring output columns from col on of row m (those below cols).
-template <typename T>
-__device__ __forceinline__ void store_cols(const GemmParams& p, int m, int col, const float (&v)[4]) {
-  T* o = static_cast<T*>(p.out) + (int64_t)m * p.os + col;
-  if (col + 4 <= p.cols) {
-    Out<T>::store4(o, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (col + e < p.cols) o[e] = Out<T>::one(v[e]);
-  }
-}
-
-__device__ __forceinline__ float silu(float g) { return g / (1.f + expf(-g)); }
-
-// Lane (r16, g) of a 16 x 16 tile of sums holds channels 4g .. 4g + 3 of the tile for
-// row r16: the outputs of the channel tiles t and t + 1 (a gate and its up where
-// GATED) for row m.
-template <typename T, bool GATED>
-__device__ __forceinline__ void store_pair(const GemmParams& p, int t, int g, int m, const i32x4& a, const i32x4& b,
-                                           float sx) {
-  const f32x4 sa = *reinterpret_cast<const f32x4*>(p.sw + 16 * t + 4 * g);
-  float v[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = (float)a[e] * sa[e] * sx;
-  if (!GATED) store_cols<T>(p, m, 16 * t + 4 * g, v);
-  if (t + 1 >= p.tiles) return;
-  const f32x4 sb = *reinterpret_cast<const f32x4*>(p.sw + 16 * (t + 1) + 4 * g);
-  if (GATED) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = silu(v[e]) * ((float)b[e] * sb[e] * sx);
-    store_cols<T>(p, m, 8 * t + 4 * g, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)b[e] * sb[e] * sx;
-    store_cols<T>(p, m, 16 * (t + 1) + 4 * g, v);
-  }
-}
-
 // A wave takes two channel tiles and MT row tiles over all of K.
 template <typename T, bool GATED, int MT>
-__global__ __launch_bounds__(256) void gemm_i8_kernel(const GemmParams p) {
+__global__ __launch_bounds__(256) void gemm_i8_kernel(const GemmI8 p) {
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const int t = 2 * (blockIdx.x * 4 + (threadIdx.x >> 6));
   if (t >= p.tiles) return;
@@ -241,7 +156,8 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(const GemmParams p) {
 }
 
 template <typename T, bool GATED>
-hipError_t launch_gemm(const GemmParams& p, hipStream_t s) {
+hipError_t launch_gemm(const GemmI8& p, hipStream_t s) {
+  if (p.M > 256) return launch_prompt_i8<T, GATED>(p, s);
   const unsigned gx = (unsigned)ceil_div(p.tiles, 8);
   if (p.M <= 16)
     hipLaunchKernelGGL((gemm_i8_kernel<T, GATED, 1>), dim3(gx, 1), dim3(256), 0, s, p);
@@ -251,7 +167,7 @@ hipError_t launch_gemm(const GemmParams& p, hipStream_t s) {
 }
 
 template <typename T>
-hipError_t launch_gemm(const GemmParams& p, int gated, hipStream_t s) {
+hipError_t launch_gemm(const GemmI8& p, int gated, hipStream_t s) {
   return gated ? launch_gemm<T, true>(p, s) : launch_gemm<T, false>(p, s);
 }
 
@@ -304,9 +220,11 @@ extern "C" int dflash_gemm_i8(const void* x, int64_t x_row_stride, const float* 
                               const float* packed_scale, void* out, int out_dtype, int64_t out_row_stride, int M,
                               int N, int K, int gated, void* stream) {
   if (M < 0 || bad_weight(N, K, gated)) return DFLASH_ERR_SHAPE;
-  GemmParams p{};
+  GemmI8 p{};
   p.cols = gated ? N / 2 : N;
   if (M > 1 && (x_row_stride < 16 * ceil_div(K, 16) || out_row_stride < p.cols)) return DFLASH_ERR_SHAPE;
+  // the prompt kernel's row offsets are 32-bit, its tiles counted in an int
+  if (x_row_stride > (1 << 23) || ceil_div(M, 256) * ceil_div(N, 128) > INT32_MAX / 2) return DFLASH_ERR_SHAPE;
   if (M == 0) return DFLASH_OK;
   if (x == nullptr || x_scale == nullptr || packed_codes == nullptr || packed_scale == nullptr || out == nullptr)
     return DFLASH_ERR_NULL;

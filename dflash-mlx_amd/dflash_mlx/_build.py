@@ -20,7 +20,7 @@ LIB_PATH = PKG_DIR / LIB_NAME
 
 SOURCES = ["gdn_scan.hip", "gdn_layer_ops.hip", "gdn_chunked.hip", "greedy_accept.hip", "lm_head_argmax.hip",
            "rollback.hip", "model_ops.hip", "skinny_gemm.hip", "prefill_gemm.hip", "block_gemm.hip", "kv8.hip",
-           "attn_q8.hip", "int8.hip", "logits.hip", "abi.cpp"]
+           "attn_q8.hip", "int8.hip", "int8_prompt.hip", "logits.hip", "abi.cpp"]
 
 # -packed-fp32-ops off: v_pk_{add,mul,fma}_f32 have given silent wrong results
 # on these machines, so the compiler must not form them from scalar code.
