@@ -151,7 +151,8 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(const GemmI8 p) {
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     const int m = m0 + 16 * j + r16;
-    if (m < p.M) store_pair<T, GATED>(p, t, g, m, acc[0][j], acc[1][j], p.sx[m]);
+    if (m < p.M)
+      store_pair<T, GATED>(p, t, g, static_cast<T*>(p.out) + (int64_t)m * p.os, 4 * g, acc[0][j], acc[1][j], tile_scales(p, t, g), tile_scales(p, t + 1, g), p.sx[m]);
   }
 }
 
@@ -223,8 +224,8 @@ extern "C" int dflash_gemm_i8(const void* x, int64_t x_row_stride, const float* 
   GemmI8 p{};
   p.cols = gated ? N / 2 : N;
   if (M > 1 && (x_row_stride < 16 * ceil_div(K, 16) || out_row_stride < p.cols)) return DFLASH_ERR_SHAPE;
-  // the prompt kernel's row offsets are 32-bit, its tiles counted in an int
-  if (x_row_stride > (1 << 23) || ceil_div(M, 256) * ceil_div(N, 128) > INT32_MAX / 2) return DFLASH_ERR_SHAPE;
+  // the prompt kernel's offsets in a block of rows are 32-bit, its tiles counted in an int
+  if (x_row_stride > (1 << 23) || out_row_stride > (1 << 26) || ceil_div(M, 256) * ceil_div(N, 128) > INT32_MAX / 2) return DFLASH_ERR_SHAPE;
   if (M == 0) return DFLASH_OK;
   if (x == nullptr || x_scale == nullptr || packed_codes == nullptr || packed_scale == nullptr || out == nullptr)
     return DFLASH_ERR_NULL;

@@ -26,6 +26,12 @@ __device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, uint32_t
                :: "v"(voff), "s"(sbase), "s"(lds) : "memory");
 }
 
+// The same with 4 bytes a lane, at lds + 4 l.
+__device__ __forceinline__ void dma4(const void* sbase, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1"
+               :: "v"(voff), "s"(sbase), "s"(lds) : "memory");
+}
+
 // Wait until at most N loads of this wave are outstanding (loads complete
 // in issue order).
 template <int N>

@@ -3,8 +3,10 @@
 Codes have to be equal: they are defined by real arithmetic.  An output is the exact sum,
 rounded to fp32 (2^-24), times two scales (2^-24 each), and half a step of its type.  A
 gated one is silu(g) u: g is off by 3 * 2^-24 of itself, which silu amplifies by at most
-1 + |g|; its exponential, sum, quotient and the product with u (off by 3 * 2^-24) come to
-less than 9 * 2^-24 together (the exponential within 2 ulp)."""
+1 + |g|; the exponential's argument g log2(e) rounds once and its constant once, 2 |g| *
+2^-24 of the exponential; the exponential itself, the sum, the quotient and the product
+with u (off by 3 * 2^-24) come to less than 9 * 2^-24 (exponential and reciprocal within
+2 ulp)."""
 from __future__ import annotations
 
 import pytest
@@ -35,7 +37,7 @@ def product(codes, scale, w_codes, w_scale, gated=False):
 
 def check(got, want, gate=None):
     gate = torch.zeros_like(want) if gate is None else gate
-    tol = (12 + 3 * gate.abs()) * 2.0 ** -24 * want.abs() + torch.finfo(got.dtype).eps / 2 * want.abs()
+    tol = (12 + 5 * gate.abs()) * 2.0 ** -24 * want.abs() + torch.finfo(got.dtype).eps / 2 * want.abs()
     tol += torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps  # a step of the least values
     bad = (got.cpu().double() - want).abs() > tol
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} beyond the tolerance"
