@@ -125,51 +125,153 @@ __global__ __launch_bounds__(256) void pack_kernel(const int8_t* codes, int64_t 
 
 // ------------------------------------------------------------------- product
 
-// A wave takes two channel tiles and MT row tiles over all of K.
-template <typename T, bool GATED, int MT>
-__global__ __launch_bounds__(256) void gemm_i8_kernel(const GemmI8 p) {
+// Few rows: the weight is streamed once.  A workgroup takes VT channel tiles and all
+// rows; its KW waves share K, each with a stretch of its own: no barrier while they
+// stream, weights D k-steps ahead in registers, rows (which every workgroup reads) from
+// the L2.  Their sums meet in LDS, integers, so their order does not matter.
+template <typename T, bool GATED, int MT, int VT, int KW, int D>
+__global__ __launch_bounds__(64 * KW) void stream_i8_kernel(const GemmI8 p) {
+  __shared__ i32x4 sums[KW][VT * MT][64];
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-  const int t = 2 * (blockIdx.x * 4 + (threadIdx.x >> 6));
-  if (t >= p.tiles) return;
-  const int m0 = blockIdx.y * 16 * MT;
-  const int t1 = min(t + 1, p.tiles - 1);
-  const int last = (p.K - 1) >> 4;  // the row's last 16-byte piece; the weight is 0 behind K
-  i32x4 acc[2][MT] = {};
-  for (int ks = 0; ks < p.k_steps; ++ks) {
-    const u32x4* w = p.w + (int64_t)ks * p.tiles * 64 + lane;
-    const i32x4 a0 = __builtin_bit_cast(i32x4, w[(int64_t)t * 64]);
-    const i32x4 a1 = __builtin_bit_cast(i32x4, w[(int64_t)t1 * 64]);
-    const int piece = min(4 * ks + g, last);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int t0 = VT * blockIdx.x;
+  const int all = (p.K + 63) >> 6, per = (all + KW - 1) / KW;
+  const int k0 = min(wave * per, all), n = min(per, all - k0);
+  const int last = (p.K - 1) >> 4;  // a row's last 16-byte piece; the weight is 0 behind K
+  const u32x4* w[VT];
+  const uint8_t* x[MT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const int m = min(m0 + 16 * j + r16, p.M - 1);
-      const i32x4 b = *reinterpret_cast<const i32x4*>(p.x + (int64_t)m * p.xs + 16 * piece);
-      acc[0][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, b, acc[0][j], 0, 0, 0);
-      acc[1][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, b, acc[1][j], 0, 0, 0);
+  for (int v = 0; v < VT; ++v)
+    w[v] = p.w + ((int64_t)k0 * p.tiles + min(t0 + v, p.tiles - 1)) * 64 + lane;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) x[j] = p.x + (int64_t)min(16 * j + r16, p.M - 1) * p.xs;
+  struct Stage {
+    i32x4 a[VT], b[MT];
+  } ring[D];
+  auto load = [&](Stage& s, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int v = 0; v < VT; ++v)
+      s.a[v] = __builtin_bit_cast(i32x4, __builtin_nontemporal_load(w[v] + (int64_t)i * p.tiles * 64));
+    const int piece = min(4 * (k0 + i) + g, last);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) s.b[j] = *reinterpret_cast<const i32x4*>(x[j] + 16 * piece);
+  };
+  i32x4 acc[VT][MT] = {};
+  auto multiply = [&](const Stage& s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int v = 0; v < VT; ++v)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+        acc[v][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.a[v], s.b[j], acc[v][j], 0, 0, 0);
+  };
+  // Loads past the stretch read its last step again, so that every turn has as many in flight.
+  if (n > 0) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(ring[d], min(d, n - 1));
+    int i = 0;
+    for (; i + D <= n; i += D) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        multiply(ring[d]);
+        load(ring[d], min(i + D + d, n - 1));
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (i + d < n) multiply(ring[d]);
+  }
+  // Wave k adds up and stores the pairs (of channel tiles, by row tile) k, k + KW, ...
+#pragma unroll
+  for (int v = 0; v < VT; ++v)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sums[wave][v * MT + j][lane] = acc[v][j];
+  constexpr int kPair = VT > 1 ? 2 : 1;
+  __syncthreads();
+  for (int q = wave; q < VT / kPair * MT; q += KW) {
+    const int v = q / MT * kPair, j = q % MT, t = t0 + v, m = 16 * j + r16;
+    i32x4 a = sums[0][v * MT + j][lane], b = sums[0][(v + kPair - 1) * MT + j][lane];
+#pragma unroll
+    for (int k = 1; k < KW; ++k) {
+      a += sums[k][v * MT + j][lane];
+      if (VT > 1) b += sums[k][(v + kPair - 1) * MT + j][lane];
+    }
+    if (t < p.tiles && m < p.M) {
+      T* row = static_cast<T*>(p.out) + (int64_t)m * p.os;
+      const f32x4 sa = tile_scales(p, t, g);
+      const float sx = p.sx[m];
+      if (VT > 1) {
+        store_pair<T, GATED>(p, t, g, row, 4 * g, a, b, sa, tile_scales(p, t + 1, g), sx);
+      } else {
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (float)a[e] * sa[e] * sx;
+        store_cols<T, false>(p, row, 4 * g, 16 * t, g, o);
+      }
     }
   }
-#pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int m = m0 + 16 * j + r16;
-    if (m < p.M)
-      store_pair<T, GATED>(p, t, g, static_cast<T*>(p.out) + (int64_t)m * p.os, 4 * g, acc[0][j], acc[1][j], tile_scales(p, t, g), tile_scales(p, t + 1, g), p.sx[m]);
-  }
+}
+
+template <typename T, bool GATED, int MT, int VT, int KW, int D>
+hipError_t launch_stream(const GemmI8& p, hipStream_t s) {
+  hipLaunchKernelGGL((stream_i8_kernel<T, GATED, MT, VT, KW, D>), dim3((unsigned)ceil_div(p.tiles, VT)), dim3(64 * KW),
+                     0, s, p);
+  return hipGetLastError();
+}
+
+// Measured in replayed graphs over weights that are not in the cache (MI355X, us, the
+// launch's gap with it), 16 rows, one channel tile and 8 waves / two and 4 / four and 4:
+// 2560 x 9216 9.3 / 12.3 / 17.0, 2560 x 4096 6.1 / 7.0 / 9.3, 5120 x 2560 7.7 / 5.7 / 7.2,
+// 18432 x 2560 gated - / 13.2 / 13.4, 151936 x 2560 117 / 80 / 71.
+template <typename T, bool GATED, int MT>
+hipError_t launch_rows(const GemmI8& p, hipStream_t s) {
+  if (p.tiles <= 256) return launch_stream<T, GATED, MT, GATED ? 2 : 1, 8, 4>(p, s);
+  if (p.tiles <= 2048) return launch_stream<T, GATED, MT, 2, 4, 4>(p, s);
+  return launch_stream<T, GATED, MT, 4, 4, 4>(p, s);
 }
 
 template <typename T, bool GATED>
 hipError_t launch_gemm(const GemmI8& p, hipStream_t s) {
-  if (p.M > 256) return launch_prompt_i8<T, GATED>(p, s);
-  const unsigned gx = (unsigned)ceil_div(p.tiles, 8);
-  if (p.M <= 16)
-    hipLaunchKernelGGL((gemm_i8_kernel<T, GATED, 1>), dim3(gx, 1), dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL((gemm_i8_kernel<T, GATED, 4>), dim3(gx, (unsigned)ceil_div(p.M, 64)), dim3(256), 0, s, p);
-  return hipGetLastError();
+  if (p.plan.kind != PlanI8::kStream) return launch_prompt_i8<T, GATED>(p, s);
+  if (p.M <= 16) return launch_rows<T, GATED, 1>(p, s);
+  if (p.M <= 32) return launch_rows<T, GATED, 2>(p, s);
+  return launch_rows<T, GATED, 4>(p, s);
 }
 
 template <typename T>
 hipError_t launch_gemm(const GemmI8& p, int gated, hipStream_t s) {
   return gated ? launch_gemm<T, true>(p, s) : launch_gemm<T, false>(p, s);
+}
+
+// The plan of the least estimated time, in us, fitted to times of replayed graphs (MI355X).
+//   stream: its bytes, the weight's and the rows' for every group of channel tiles, at 5.8
+//     TB/s, for up to 64 rows;
+//   wide: 0.62 a k-step of 64 and 8 a tile's outputs, a round of the compute units;
+//   narrow: 0.45 a k-step where two workgroups share a unit, 0.27 alone, and 4 a tile; the
+//     splits' sums are written and read at 4 TB/s by a launch of 2.5.
+// Within 15 % of the measured times of 64 to 4096 rows, 2560 to 151936 channels and 1001 to
+// 9216 features; it picked the fastest or one within 7 % of it.
+PlanI8 plan_i8(int M, int tiles, int k_steps) {
+  PlanI8 best{PlanI8::kStream, 1};
+  if (M <= 16) return best;
+  const double cus = std::max(device_cus(), 1);
+  double least = 1e30;
+  if (M <= 64) {
+    const int vt = tiles <= 256 ? 1 : tiles <= 2048 ? 2 : 4;
+    const double rows = (double)ceil_div(tiles, vt) * 16 * ceil_div(M, 16);
+    least = 3 + (rows + 16. * tiles) * 64 * k_steps / 5.8e6;
+  }
+  const double wide = 4 + ceil_div(ceil_div(tiles, 16) * ceil_div(M, 256), (int64_t)cus) * (0.62 * k_steps + 8);
+  if (wide < least) least = wide, best = {PlanI8::kWide, 1};
+  const int64_t narrow_tiles = ceil_div(tiles, 8) * ceil_div(M, 128);
+  for (int n = 1; n <= 16 && 4 * n <= k_steps; ++n) {
+    const int steps = 2 * (int)ceil_div(k_steps / 2, n);
+    if (n > 1 && narrow_tiles * n > 2 * cus) break;
+    const int64_t units = narrow_tiles * n, whole = units / (int64_t)(2 * cus), rest = units % (int64_t)(2 * cus);
+    double t = 4 + whole * (0.45 * steps + 4) + (rest == 0 ? 0 : rest <= cus ? 0.27 * steps + 4 : 0.45 * steps + 4);
+    if (n > 1) t += 2.5 + 8. * n * M * 16 * tiles / 4e6;
+    if (t < least) least = t, best = {PlanI8::kNarrow, (int)ceil_div(k_steps, steps)};
+  }
+  return best;
 }
 
 bool bad_weight(int N, int K, int gated) {
@@ -217,9 +319,15 @@ extern "C" int dflash_quantize_rows_i8(const void* x, int x_dtype, int64_t x_row
   return to_status(hipGetLastError());
 }
 
+extern "C" size_t dflash_gemm_i8_workspace_bytes(int M, int N, int K, int gated) {
+  if (M <= 0 || bad_weight(N, K, gated)) return 0;
+  const int tiles = channel_tiles(N, gated), splits = plan_i8(M, tiles, k_steps(K)).splits;
+  return splits > 1 ? (size_t)splits * M * tiles * 64 : 0;
+}
+
 extern "C" int dflash_gemm_i8(const void* x, int64_t x_row_stride, const float* x_scale, const void* packed_codes,
                               const float* packed_scale, void* out, int out_dtype, int64_t out_row_stride, int M,
-                              int N, int K, int gated, void* stream) {
+                              int N, int K, int gated, void* workspace, size_t workspace_bytes, void* stream) {
   if (M < 0 || bad_weight(N, K, gated)) return DFLASH_ERR_SHAPE;
   GemmI8 p{};
   p.cols = gated ? N / 2 : N;
@@ -238,6 +346,11 @@ extern "C" int dflash_gemm_i8(const void* x, int64_t x_row_stride, const float* 
   p.w = static_cast<const u32x4*>(packed_codes), p.sw = packed_scale;
   p.out = out, p.os = out_row_stride;
   p.M = M, p.K = K, p.k_steps = k_steps(K), p.tiles = channel_tiles(N, gated);
+  p.plan = plan_i8(M, p.tiles, p.k_steps);
+  if (p.plan.splits > 1 && workspace_bytes < (size_t)p.plan.splits * M * p.tiles * 64) return DFLASH_ERR_WORKSPACE;
+  if (p.plan.splits > 1 && workspace == nullptr) return DFLASH_ERR_NULL;
+  if ((uintptr_t)workspace % 16) return DFLASH_ERR_ALIGN;
+  p.workspace = workspace;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return to_status(f32                                ? launch_gemm<float>(p, gated, s)
                    : out_dtype == DFLASH_DTYPE_BF16 ? launch_gemm<uint16_t>(p, gated, s)

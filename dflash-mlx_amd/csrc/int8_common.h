@@ -21,6 +21,13 @@ inline int channel_tiles(int N, int gated) {
   return gated ? 2 * (int)ceil_div(N / 2, 16) : (int)ceil_div(N, 16);
 }
 
+// How a product runs: as a stream of the weight (int8.hip), or by tiles of 256 x 256 or
+// 128 x 128 with K in so many splits (int8_prompt.hip).
+struct PlanI8 {
+  enum Kind { kStream, kNarrow, kWide } kind;
+  int splits;
+};
+
 struct GemmI8 {
   const uint8_t* x;
   int64_t xs;
@@ -31,6 +38,8 @@ struct GemmI8 {
   int64_t os;
   int M, cols;  // output rows and columns
   int K, k_steps, tiles;
+  PlanI8 plan;
+  void* workspace;  // where the splits' sums go
 };
 
 template <typename T>
@@ -113,7 +122,7 @@ __device__ __forceinline__ void store_pair(const GemmI8& p, int t, int g, T* row
   }
 }
 
-// Products of many rows (int8_prompt.hip).
+// Products by tiles (int8_prompt.hip).
 template <typename T, bool GATED>
 hipError_t launch_prompt_i8(const GemmI8& p, hipStream_t s);
 

@@ -181,9 +181,11 @@ def matmul_i8(codes: torch.Tensor, scale: torch.Tensor, weight: Int8Weight, *, o
     if not fits or rows.data_ptr() % 16 or M > 1 and (rows.stride(0) % 16 or rows.stride(0) < Kp):
         rows = torch.nn.functional.pad(rows, (0, Kp - K)) if Kp > K else rows.clone(memory_format=torch.contiguous_format)
     scale = scale.contiguous()
+    n = int(_lib.load().dflash_gemm_i8_workspace_bytes(M, weight.N, K, int(weight.gated)))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call("dflash_gemm_i8", dev, rows.data_ptr(), rows.stride(0) if M > 1 else Kp, scale.data_ptr(),
           weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), _OUT[out.dtype], os, M, weight.N, K,
-          int(weight.gated))
+          int(weight.gated), _lib.ptr(ws), n)
     return out
 
 

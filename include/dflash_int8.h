@@ -52,10 +52,13 @@ int dflash_quantize_rows_i8(const void* x, int x_dtype, int64_t x_row_stride, vo
 
 /* The product of codes x [M, K] (16-byte aligned, rows x_row_stride bytes apart, a multiple
  * of 16; rows are read up to K rounded up to 16, whatever is there) with a packed
- * weight.  out: bf16, fp16 or fp32, out_row_stride elements apart, at least N (gated: N / 2). */
+ * weight.  out: bf16, fp16 or fp32, out_row_stride elements apart, at least N (gated: N / 2).
+ * workspace: dflash_gemm_i8_workspace_bytes(M, N, K, gated) bytes (for the current device; may be
+ * 0), 16-byte aligned. */
+size_t dflash_gemm_i8_workspace_bytes(int M, int N, int K, int gated);
 int dflash_gemm_i8(const void* x, int64_t x_row_stride, const float* x_scale, const void* packed_codes,
                    const float* packed_scale, void* out, int out_dtype, int64_t out_row_stride, int M, int N,
-                   int K, int gated, void* stream);
+                   int K, int gated, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

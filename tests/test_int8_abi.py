@@ -28,8 +28,8 @@ def _quantize(lib, x=P, dtype=1, xs=200, codes=P, cs=208, scale=P, M=4, K=200):
     return lib.dflash_quantize_rows_i8(x, dtype, xs, codes, cs, scale, M, K, None)
 
 
-def _gemm(lib, x=P, xs=208, sx=P, w=P, sw=P, out=P, dtype=1, os=64, M=4, N=64, K=200, gated=0):
-    return lib.dflash_gemm_i8(x, xs, sx, w, sw, out, dtype, os, M, N, K, gated, None)
+def _gemm(lib, x=P, xs=208, sx=P, w=P, sw=P, out=P, dtype=1, os=64, M=4, N=64, K=200, gated=0, ws=P, nbytes=1 << 40):
+    return lib.dflash_gemm_i8(x, xs, sx, w, sw, out, dtype, os, M, N, K, gated, ws, nbytes, None)
 
 
 def test_every_declared_entry_point_is_exported_and_bound(lib):
@@ -38,7 +38,7 @@ def test_every_declared_entry_point_is_exported_and_bound(lib):
     text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "dflash_int8.h").read_text(), flags=re.S)
     names = set(re.findall(r"\b(dflash_[a-z0-9_]+)\s*\(", text))
     assert names == {"dflash_weight_i8_bytes", "dflash_weight_i8_scales", "dflash_weight_pack_i8",
-                     "dflash_quantize_rows_i8", "dflash_gemm_i8"}
+                     "dflash_quantize_rows_i8", "dflash_gemm_i8", "dflash_gemm_i8_workspace_bytes"}
     for name in names:
         assert hasattr(lib, name) and name in _lib.SIGNATURES
 
