@@ -356,3 +356,39 @@ extern "C" int dflash_gemm_i8(const void* x, int64_t x_row_stride, const float* 
                    : out_dtype == DFLASH_DTYPE_BF16 ? launch_gemm<uint16_t>(p, gated, s)
                                                       : launch_gemm<_Float16>(p, gated, s));
 }
+
+namespace {
+// Where a linear's codes, scales and splits' sums lie in its workspace.
+size_t codes_bytes(int M, int K) { return (size_t)M * 16 * ceil_div(K, 16); }
+size_t scales_bytes(int M) { return 16 * (size_t)ceil_div(M, 4); }
+}  // namespace
+
+extern "C" size_t dflash_linear_i8_workspace_bytes(int M, int N, int K, int gated) {
+  if (M <= 0 || bad_weight(N, K, gated)) return 0;
+  return codes_bytes(M, K) + scales_bytes(M) + dflash_gemm_i8_workspace_bytes(M, N, K, gated);
+}
+
+extern "C" int dflash_linear_i8(const void* x, int x_dtype, int64_t x_row_stride, const void* packed_codes,
+                                const float* packed_scale, void* out, int out_dtype, int64_t out_row_stride, int M,
+                                int N, int K, int gated, void* workspace, size_t workspace_bytes, void* stream) {
+  if (M < 0 || bad_weight(N, K, gated)) return DFLASH_ERR_SHAPE;
+  const int cols = gated ? N / 2 : N;
+  if (x_row_stride < 0 || (M > 1 && out_row_stride < cols) || out_row_stride > (1 << 26)) return DFLASH_ERR_SHAPE;
+  if (M == 0) return DFLASH_OK;
+  // what the product would refuse is refused before anything is launched
+  if (packed_codes == nullptr || packed_scale == nullptr || out == nullptr || workspace == nullptr) return DFLASH_ERR_NULL;
+  const bool f32 = out_dtype == DFLASH_DTYPE_F32;
+  if (!f32 && out_dtype != DFLASH_DTYPE_BF16 && out_dtype != DFLASH_DTYPE_F16) return DFLASH_ERR_UNSUPPORTED;
+  if ((uintptr_t)packed_codes % 16 || (uintptr_t)packed_scale % 16 || (uintptr_t)out % (f32 ? 4 : 2) ||
+      (uintptr_t)workspace % 16)
+    return DFLASH_ERR_ALIGN;
+  if (workspace_bytes < dflash_linear_i8_workspace_bytes(M, N, K, gated)) return DFLASH_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  const size_t cb = codes_bytes(M, K), sb = scales_bytes(M);
+  float* scale = reinterpret_cast<float*>(ws + cb);
+  const int64_t cs = 16 * ceil_div(K, 16);
+  const int e = dflash_quantize_rows_i8(x, x_dtype, x_row_stride, ws, cs, scale, M, K, stream);
+  if (e) return e;
+  return dflash_gemm_i8(ws, cs, scale, packed_codes, packed_scale, out, out_dtype, out_row_stride, M, N, K, gated,
+                        ws + cb + sb, workspace_bytes - cb - sb, stream);
+}

@@ -138,6 +138,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dflash_quantize_rows_i8": (_I, [_VP, _I, _I64, _VP, _I64, _VP, _I, _I, _VP]),
     "dflash_gemm_i8_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "dflash_gemm_i8": (_I, [_VP, _I64, _VP, _VP, _VP, _VP, _I, _I64, _I, _I, _I, _I, _VP, _SZ, _VP]),
+    "dflash_linear_i8_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "dflash_linear_i8": (
+        _I, [_VP, _I, _I64, _VP, _VP, _VP, _I, _I64, _I, _I, _I, _I, _VP, _SZ, _VP]),
     "dflash_logits_state_reset": (_I, [_VP, _VP]),
     "dflash_logits_state_add": (_I, [_VP, _VP, _I64, _I, _VP, _I, _VP]),
     "dflash_logits_state_set_bias": (_I, [_VP, _VP, _I64, _VP, _I64, _I, _VP]),

@@ -32,7 +32,7 @@ class Int8Weight:
     pack_weight_i8 make it): codes as the matrix unit's fragments, one fp32 scale a
     channel.  gated: the weight is [gate; up] and the products are silu(gate) * up."""
 
-    __slots__ = ("codes", "scales", "N", "K", "gated", "cols", "device")
+    __slots__ = ("codes", "scales", "N", "K", "gated", "cols", "device", "_codes_ptr", "_scales_ptr", "_gated", "_ws_bytes")
 
     def __init__(self, codes, scales, N: int, K: int, gated: bool):
         lib = _lib.load()
@@ -49,6 +49,8 @@ class Int8Weight:
         self.codes, self.scales, self.N, self.K, self.gated = codes, scales, int(N), int(K), bool(gated)
         self.cols = self.N // 2 if self.gated else self.N
         self.device = codes.device
+        self._codes_ptr, self._scales_ptr, self._gated = codes.data_ptr(), scales.data_ptr(), int(self.gated)
+        self._ws_bytes = {}  # by entry point and rows
 
     def __repr__(self):
         return f"Int8Weight(N={self.N}, K={self.K}, gated={self.gated}, {self.device})"
@@ -122,6 +124,17 @@ def quantize_rows_i8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return (codes if Kp == K else codes[..., :K]), scale
 
 
+def _workspace_bytes(fn: str, M: int, weight: Int8Weight) -> int:
+    """The entry point's workspace for M rows (on the weight's device)."""
+    n = weight._ws_bytes.get((fn, M))
+    if n is None:
+        with torch.cuda.device(weight.device):
+            n = int(getattr(_lib.load(), fn)(M, weight.N, weight.K, weight._gated))
+        if len(weight._ws_bytes) < 4096:
+            weight._ws_bytes[(fn, M)] = n
+    return n
+
+
 def _output(out, out_dtype, lead, weight):
     """(the output tensor, its rows' stride)."""
     if out is None:
@@ -181,11 +194,11 @@ def matmul_i8(codes: torch.Tensor, scale: torch.Tensor, weight: Int8Weight, *, o
     if not fits or rows.data_ptr() % 16 or M > 1 and (rows.stride(0) % 16 or rows.stride(0) < Kp):
         rows = torch.nn.functional.pad(rows, (0, Kp - K)) if Kp > K else rows.clone(memory_format=torch.contiguous_format)
     scale = scale.contiguous()
-    n = int(_lib.load().dflash_gemm_i8_workspace_bytes(M, weight.N, K, int(weight.gated)))
+    n = _workspace_bytes("dflash_gemm_i8_workspace_bytes", M, weight)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call("dflash_gemm_i8", dev, rows.data_ptr(), rows.stride(0) if M > 1 else Kp, scale.data_ptr(),
-          weight.codes.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), _OUT[out.dtype], os, M, weight.N, K,
-          int(weight.gated), _lib.ptr(ws), n)
+          weight._codes_ptr, weight._scales_ptr, out.data_ptr(), _OUT[out.dtype], os, M, weight.N, K, weight._gated,
+          _lib.ptr(ws), n)
     return out
 
 
@@ -199,6 +212,15 @@ def linear_i8(x: torch.Tensor, weight: Int8Weight, *, out_dtype: torch.dtype | N
         raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
     if x.dim() == 0:
         raise ValueError("x must be [..., K]")
-    _check_weight(weight, x.shape[-1], x.device)
-    codes, scale = quantize_rows_i8(x)
-    return matmul_i8(codes, scale, weight, out_dtype=x.dtype if out_dtype is None else out_dtype, out=out)
+    lead, K, dev = x.shape[:-1], x.shape[-1], x.device
+    _check_weight(weight, K, dev)
+    out, os = _output(out, x.dtype if out_dtype is None else out_dtype, lead, weight)
+    if out.numel() == 0:
+        return out
+    rows = _rows_of(x)
+    M = rows.shape[0]
+    n = _workspace_bytes("dflash_linear_i8_workspace_bytes", M, weight)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _call("dflash_linear_i8", dev, rows.data_ptr(), _IN[x.dtype], rows.stride(0), weight._codes_ptr, weight._scales_ptr,
+          out.data_ptr(), _OUT[out.dtype], os, M, weight.N, K, weight._gated, ws.data_ptr(), n)
+    return out

@@ -60,6 +60,14 @@ int dflash_gemm_i8(const void* x, int64_t x_row_stride, const float* x_scale, co
                    const float* packed_scale, void* out, int out_dtype, int64_t out_row_stride, int M, int N,
                    int K, int gated, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Both in one call: rows x (bf16 or fp16) quantised and multiplied, the same bits.  workspace:
+ * dflash_linear_i8_workspace_bytes(M, N, K, gated) bytes (for the current device), 16-byte
+ * aligned. */
+size_t dflash_linear_i8_workspace_bytes(int M, int N, int K, int gated);
+int dflash_linear_i8(const void* x, int x_dtype, int64_t x_row_stride, const void* packed_codes,
+                     const float* packed_scale, void* out, int out_dtype, int64_t out_row_stride, int M, int N,
+                     int K, int gated, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 ROOT = Path(__file__).resolve().parent.parent
-NULL, SHAPE, UNSUPPORTED, ALIGN = -1, -2, -3, -4
+NULL, SHAPE, UNSUPPORTED, ALIGN, WORKSPACE = -1, -2, -3, -4, -5
 P = 0x1000  # stands for a device pointer: no call below gets as far as a launch
 
 
@@ -38,7 +38,8 @@ def test_every_declared_entry_point_is_exported_and_bound(lib):
     text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "dflash_int8.h").read_text(), flags=re.S)
     names = set(re.findall(r"\b(dflash_[a-z0-9_]+)\s*\(", text))
     assert names == {"dflash_weight_i8_bytes", "dflash_weight_i8_scales", "dflash_weight_pack_i8",
-                     "dflash_quantize_rows_i8", "dflash_gemm_i8", "dflash_gemm_i8_workspace_bytes"}
+                     "dflash_quantize_rows_i8", "dflash_gemm_i8", "dflash_gemm_i8_workspace_bytes",
+                     "dflash_linear_i8", "dflash_linear_i8_workspace_bytes"}
     for name in names:
         assert hasattr(lib, name) and name in _lib.SIGNATURES
 
@@ -88,6 +89,24 @@ def test_products_that_are_refused(lib):
                dict(out=P + 2, dtype=0)):
         assert _gemm(lib, **kw) == ALIGN
     assert _gemm(lib, M=0, x=None) == 0
+
+
+def _linear(lib, x=P, xd=1, xs=200, w=P, sw=P, out=P, dtype=1, os=64, M=4, N=64, K=200, gated=0, ws=P, nbytes=1 << 40):
+    return lib.dflash_linear_i8(x, xd, xs, w, sw, out, dtype, os, M, N, K, gated, ws, nbytes, None)
+
+
+def test_linears_that_are_refused(lib):
+    for kw in (dict(M=-1), dict(xs=-1), dict(os=63), dict(N=0), dict(K=131073), dict(N=63, gated=1), dict(os=1 << 27)):
+        assert _linear(lib, **kw) == SHAPE
+    for name in ("x", "w", "sw", "out", "ws"):
+        assert _linear(lib, **{name: None}) == NULL
+    assert _linear(lib, dtype=3) == UNSUPPORTED and _linear(lib, xd=0) == UNSUPPORTED
+    for kw in (dict(x=P + 1), dict(w=P + 8), dict(sw=P + 8), dict(out=P + 1), dict(out=P + 2, dtype=0), dict(ws=P + 8)):
+        assert _linear(lib, **kw) == ALIGN
+    assert _linear(lib, nbytes=4 * 208 + 15) == WORKSPACE
+    assert _linear(lib, M=0, x=None) == 0
+    assert lib.dflash_linear_i8_workspace_bytes(4, 64, 200, 0) == 4 * 208 + 16
+    assert lib.dflash_linear_i8_workspace_bytes(0, 64, 200, 0) == 0
 
 
 def test_python_refuses_host_tensors():
