@@ -77,26 +77,35 @@ __device__ __forceinline__ u32x4 load_row8(const uint16_t* x, int c, int K) {
   return v;
 }
 
-constexpr int kQThreads = 256;
-
-// A workgroup a row.
-template <bool BF16>
-__global__ __launch_bounds__(kQThreads) void quantize_rows_kernel(const uint16_t* x, int64_t xs, uint8_t* codes,
-                                                                  int64_t cs, float* scale, int K) {
-  __shared__ uint32_t best[kQThreads / 64];
+// A workgroup of NT threads a row, which they keep in registers: one trip to memory for
+// rows of up to 32 NT values, and another to the L2 for longer ones.
+template <bool BF16, int NT>
+__global__ __launch_bounds__(NT) void quantize_rows_kernel(const uint16_t* x, int64_t xs, uint8_t* codes, int64_t cs,
+                                                           float* scale, int K) {
+  constexpr int R = 4;
+  __shared__ uint32_t best[NT / 64];
   const uint16_t* xr = x + (int64_t)blockIdx.x * xs;
+  uint8_t* cr = codes + (int64_t)blockIdx.x * cs;
   const int chunks = 2 * ((K + 15) >> 4);  // pieces of 8, up to K rounded up to 16
+  u32x4 held[R] = {};
   uint32_t m = 0;
-  for (int c = threadIdx.x; c < chunks; c += kQThreads) m = largest8(load_row8(xr, c, K), m);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (const int c = threadIdx.x + i * NT; c < chunks) held[i] = load_row8(xr, c, K);
+#pragma unroll
+  for (int i = 0; i < R; ++i) m = largest8(held[i], m);
+  for (int c = threadIdx.x + R * NT; c < chunks; c += NT) m = largest8(load_row8(xr, c, K), m);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
   if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kQThreads / 64; ++w) m = max(m, best[w]);
+  for (int w = 0; w < NT / 64; ++w) m = max(m, best[w]);
   const RowScale r = row_scale<BF16>(m);
-  uint8_t* cr = codes + (int64_t)blockIdx.x * cs;
-  for (int c = threadIdx.x; c < chunks; c += kQThreads)
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (const int c = threadIdx.x + i * NT; c < chunks) *reinterpret_cast<u32x2*>(cr + 8 * c) = codes8<BF16>(held[i], r);
+  for (int c = threadIdx.x + R * NT; c < chunks; c += NT)
     *reinterpret_cast<u32x2*>(cr + 8 * c) = codes8<BF16>(load_row8(xr, c, K), r);
   if (threadIdx.x == 0) scale[blockIdx.x] = r.scale;
 }
@@ -312,8 +321,12 @@ extern "C" int dflash_quantize_rows_i8(const void* x, int x_dtype, int64_t x_row
   if (x_dtype != DFLASH_DTYPE_BF16 && x_dtype != DFLASH_DTYPE_F16) return DFLASH_ERR_UNSUPPORTED;
   if ((uintptr_t)x % 2 || (uintptr_t)codes % 16 || codes_row_stride % 16 || (uintptr_t)scale % 4)
     return DFLASH_ERR_ALIGN;
-  const auto kernel = x_dtype == DFLASH_DTYPE_BF16 ? quantize_rows_kernel<true> : quantize_rows_kernel<false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)M), dim3(kQThreads), 0, static_cast<hipStream_t>(stream),
+  const bool bf = x_dtype == DFLASH_DTYPE_BF16;
+  // Few rows leave most of the device idle, whose threads then share a row.
+  const bool wide = M <= 512 && K > 2048;
+  const auto kernel = wide ? (bf ? quantize_rows_kernel<true, 1024> : quantize_rows_kernel<false, 1024>)
+                           : (bf ? quantize_rows_kernel<true, 256> : quantize_rows_kernel<false, 256>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)M), dim3(wide ? 1024 : 256), 0, static_cast<hipStream_t>(stream),
                      static_cast<const uint16_t*>(x), x_row_stride, static_cast<uint8_t*>(codes), codes_row_stride,
                      scale, K);
   return to_status(hipGetLastError());

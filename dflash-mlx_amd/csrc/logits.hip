@@ -2,14 +2,14 @@
 // grammar masks, applied on the way to the greedy accept or written out for a
 // sampler (include/dflash_logits.h has the formulas).
 //
-// All of it is bound by the logits' bytes (600 KB a row of 151 936 in fp32), so
-// the state is kept such that a pass reads little else: a bit a token says
-// whether the token has a count or a bias at all, and only where one of eight
-// neighbouring bits is set are those eight counts and biases read.  Draft tokens
-// before a row are counted from a list in LDS of those that fall into the
-// workgroup's slice, mostly none.
+// All of it is bound by the logits' bytes (600 KB a row of 151 936 in fp32), so the state is
+// kept such that a pass reads little else: a bit a token says whether the token has a count
+// or a bias at all, and only those few are looked up.  Draft tokens before a row are counted
+// from a list in LDS of those that fall into the workgroup's slice, mostly none.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "accept_common.h"
 #include "argmax_common.h"
@@ -46,6 +46,7 @@ struct ProcessParams {
   int64_t obs, ors;
   uint64_t* keys;
   int N, V, chunk, splits;
+  unsigned rows;
 };
 
 template <typename T>
@@ -115,9 +116,7 @@ __device__ __forceinline__ float penalised(float l, uint32_t count, float bias, 
 // the workgroup's slice (in LDS; nd of them).
 struct RowState {
   const int32_t* counts;
-  const uint8_t* known;
   const float* bias;
-  const uint8_t* mask;
   float rep, pres, freq;
   const int32_t* drafts;
   int nd;
@@ -129,104 +128,205 @@ __device__ __forceinline__ int times_drafted(const RowState& s, int v) {
   return n;
 }
 
-// Which of entries 8c .. 8c + 7 have a count or a bias.
-__device__ __forceinline__ uint32_t known_bits(const RowState& s, int c) {
-  uint32_t bits = s.counts != nullptr ? s.known[c] : 0;
-  for (int k = 0; k < s.nd; ++k)
-    if ((s.drafts[k] >> 3) == c) bits |= 1u << (s.drafts[k] & 7);
-  return bits;
+// The entries whose bit of `keep` is 0 as -inf.
+__device__ __forceinline__ void keep_bits(float (&x)[8], uint32_t keep) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = keep >> e & 1 ? x[e] : -__builtin_inff();
 }
 
-// Eight whole entries 8c .. 8c + 7.
-__device__ __forceinline__ void process8(const RowState& s, int c, uint32_t bits, uint32_t allowed, float (&x)[8]) {
-  if (bits) {
-    const u32x4_e4* cp = reinterpret_cast<const u32x4_e4*>(s.counts + 8 * c);
-    const f32x4_e4* bp = reinterpret_cast<const f32x4_e4*>(s.bias + 8 * c);
-    const u32x4 c0 = cp[0], c1 = cp[1];
-    const f32x4 b0 = bp[0], b1 = bp[1];
+// The largest of eight, a NaN above all.
+__device__ __forceinline__ float largest(const float (&x)[8]) {
+  float m = x[0];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (bits >> e & 1)
-        x[e] = penalised(x[e], e < 4 ? c0[e & 3] : c1[e & 3], e < 4 ? b0[e & 3] : b1[e & 3], s.rep, s.pres, s.freq,
-                         s.nd ? times_drafted(s, 8 * c + e) : 0);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (!(allowed >> e & 1)) x[e] = -__builtin_inff();
+  for (int e = 1; e < 8; ++e) m = __builtin_elementwise_maximum(m, x[e]);
+  return m;
 }
 
-// grid (rows, splits): one workgroup processes one slice of one row, and either
-// writes it (WRITE; INPLACE: only what changes) or reduces it to an argmax key.
+// A slice of a row: a lane has up to kTurns eights of it, 256 apart, whose loads are all in
+// flight at once.
+constexpr int kListed = 2048;  // known tokens of a slice that are shared out evenly
+template <typename T>
+constexpr int kTurns = sizeof(T) == 2 ? 4 : 2;
+template <typename T>
+constexpr int kSlice = 8 * kLThreads * kTurns<T>;
+
+// grid (rows, slices): one workgroup processes one slice of one row, and either writes it
+// (WRITE; INPLACE: only what changes) or reduces it to an argmax key.
+//
+// The slice streams by and is only masked: for the argmax a lane keeps the largest value and
+// where its eight lie (their order among each other is looked up once, at the end).  The
+// known tokens are few and lie unevenly; a lane that worked on one as it met it would have
+// its whole wave wait for two trips to memory, and nearly every wave meets one.  So a lane
+// leaves an eight with known tokens in LDS and their bits in a register, and then they are
+// listed and shared out over all lanes.  32 x 16 rows of 151936 in bf16 under masks after
+// 4000 tokens (167 MB), us, with the join of the keys: 112 as met; 67 listed from the bits
+// after the stream, whose logits then come a second time; 64 listed turn by turn, 100
+// instructions a turn of any wave that meets one; 44 so (masks alone 40).
 template <typename T, bool WRITE, bool INPLACE>
 __global__ __launch_bounds__(kLThreads) void process_kernel(const ProcessParams p) {
+  constexpr int U = kTurns<T>;
   __shared__ int32_t drafts[DFLASH_LOGITS_MAX_DRAFT];
-  __shared__ int nd_s;
+  __shared__ int nd_s, listed;
+  __shared__ __attribute__((aligned(16))) T held[kSlice<T>];
+  __shared__ uint16_t list[kListed];
   __shared__ uint64_t wbest[kLThreads / 64];
-  const int row = blockIdx.x, split = blockIdx.y;
+  const int row = blockIdx.x, split = blockIdx.y, tid = threadIdx.x;
   const int b = row / p.N, i = row - b * p.N;
-  const int start = split * p.chunk, end = min(p.V, start + p.chunk);  // chunk % 16 == 0
+  const int start = split * p.chunk, end = min(p.V, start + p.chunk);  // chunk % 16 == 0, <= kSlice
   const T* base = static_cast<const T*>(p.logits) + b * p.bs + i * p.rs;
   T* out = WRITE ? static_cast<T*>(p.out) + b * p.obs + i * p.ors : nullptr;
+
+  // Where there is no mask or state the row's own bytes stand for theirs: a branch here would
+  // have every load wait for the one before.
+  const uint8_t* known_row = p.counts == nullptr ? nullptr : reinterpret_cast<const uint8_t*>(p.known + (int64_t)b * ((p.V + 31) >> 5));
+  const uint8_t* mask_row = p.mask == nullptr ? nullptr : reinterpret_cast<const uint8_t*>(p.mask + b * p.mask_bs + i * p.mask_rs);
+  const uint8_t* mask_at = mask_row != nullptr ? mask_row : reinterpret_cast<const uint8_t*>(base);
+  const uint8_t* known_at = known_row != nullptr ? known_row : reinterpret_cast<const uint8_t*>(base);
+  const uint32_t mask_or = mask_row != nullptr ? 0 : 0xffu, known_and = known_row != nullptr ? 0xffu : 0;
+
+  // Eights tid, tid + 256, ... of the slice (the last one again where there is none).
+  const int c0 = start >> 3, eights = (end - start) >> 3;
+  float x[U][8];
+  uint32_t allowed[U], known[U];
+  if (eights > 0) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int c = c0 + min(tid + k * kLThreads, eights - 1);
+      allowed[k] = mask_at[c] | mask_or;
+      known[k] = known_at[c] & known_and;
+      if (!INPLACE) load8<T>(base + 8 * c, x[k]);
+    }
+  }
+
   RowState s{};
   const int n_before = p.counts != nullptr ? min(p.n_draft, i) : 0;
   if (p.counts != nullptr) {
     s.counts = p.counts + (int64_t)b * p.V;
-    s.known = reinterpret_cast<const uint8_t*>(p.known + (int64_t)b * ((p.V + 31) >> 5));
     s.bias = p.bias + (int64_t)b * p.V;
     s.rep = p.penalties[3 * b], s.pres = p.penalties[3 * b + 1], s.freq = p.penalties[3 * b + 2];
   }
-  if (p.mask != nullptr)
-    s.mask = reinterpret_cast<const uint8_t*>(p.mask + b * p.mask_bs + i * p.mask_rs);
-  if (n_before > 0) {  // wave 0 keeps the slice's drafts, in any order
-    if (threadIdx.x < 64) {
-      const int d = (int)threadIdx.x < n_before ? p.draft[b * p.dstride + threadIdx.x] : -1;
-      const bool in = d >= start && d < end;
-      const unsigned long long hit = __ballot(in);
-      if (in) drafts[__popcll(hit & ((1ull << threadIdx.x) - 1))] = d;
-      if (threadIdx.x == 0) nd_s = __popcll(hit);
-    }
-    __syncthreads();
-    s.drafts = drafts;
-    s.nd = nd_s;
+  if (tid == 0) listed = 0;
+  if (n_before > 0 && tid < 64) {  // wave 0 keeps the slice's drafts, in any order
+    const int d = tid < n_before ? p.draft[b * p.dstride + tid] : -1;
+    const bool in = d >= start && d < end;
+    const unsigned long long hit = __ballot(in);
+    if (in) drafts[__popcll(hit & ((1ull << tid) - 1))] = d;
+    if (tid == 0) nd_s = __popcll(hit);
   }
-  uint64_t best = 0;
-  const int c1 = start / 8 + (end - start) / 8;
-  for (int c = start / 8 + threadIdx.x; c < c1; c += kLThreads) {
-    const uint32_t allowed = s.mask != nullptr ? s.mask[c] : 0xffu;
-    const uint32_t bits = known_bits(s, c);
-    if (INPLACE && bits == 0 && allowed == 0xffu) continue;
-    float x[8];
-    load8<T>(base + 8 * c, x);
-    process8(s, c, bits, allowed, x);
-    if (WRITE) {
-      store8<T>(out + 8 * c, x);
-    } else {
+  __syncthreads();
+  s.drafts = drafts;
+  s.nd = n_before > 0 ? nd_s : 0;
+
+  uint64_t key = 0;
+  // A known and allowed token v of logit l, with its count and bias.
+  auto token = [&](int v, float l, int32_t count, float bias) {
+    l = penalised(l, (uint32_t)count, bias, s.rep, s.pres, s.freq, s.nd ? times_drafted(s, v) : 0);
+    if (WRITE)
+      out[v] = to_bits<T>(l);
+    else
+      key = u64_max(key, argmax_key(l, v));
+  };
+
+  uint32_t due = 0;  // 8 bits a turn: known and allowed
+  if (eights > 0) {
+    for (int k = 0; k < s.nd; ++k) {  // a draft is known to its lane
+      const int e = s.drafts[k] - start;
+      if ((e >> 3) % kLThreads == tid)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) best = u64_max(best, argmax_key(x[e], 8 * c + e));
+        for (int j = 0; j < U; ++j)
+          if ((e >> 3) / kLThreads == j) known[j] |= 1u << (e & 7);
+    }
+    float best = -__builtin_inff();
+    int best_k = -1;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int at = tid + k * kLThreads, c = c0 + at;
+      if (at >= eights) continue;
+      const uint32_t mine = known[k] & allowed[k];
+      if (INPLACE) {
+        if (mine == 0 && allowed[k] == 0xffu) continue;
+        load8<T>(base + 8 * c, x[k]);
+      }
+      due |= mine << (8 * k);
+      if (mine) store8<T>(held + 8 * at, x[k]);
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = x[k][e];
+      keep_bits(y, WRITE ? allowed[k] : allowed[k] & ~known[k]);
+      if (WRITE) {
+        if (!INPLACE || allowed[k] != 0xffu) store8<T>(out + 8 * c, y);
+      } else {
+        const float m = largest(y);
+        if (!(m <= best) && best == best) best = m, best_k = k;  // (the first NaN stays)
+      }
+    }
+    if (!WRITE) {
+      key = argmax_key(-__builtin_inff(), start);  // no value of the slice is below it
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (k != best_k) continue;
+        keep_bits(x[k], allowed[k] & ~known[k]);
+        int e = 7;
+#pragma unroll
+        for (int j = 6; j >= 0; --j) e = x[k][j] == best || (x[k][j] != x[k][j] && best != best) ? j : e;
+        key = u64_max(key, argmax_key(best, 8 * (c0 + tid + k * kLThreads) + e));
+      }
     }
   }
   // the row's last V % 8 entries, a lane each
-  const int v = 8 * c1 + threadIdx.x;
-  if (v < end) {
-    float x = load_logit<T>(base + v);
-    if (s.counts != nullptr && known_bits(s, v >> 3) >> (v & 7) & 1)
-      x = penalised(x, (uint32_t)s.counts[v], s.bias[v], s.rep, s.pres, s.freq, times_drafted(s, v));
-    if (s.mask != nullptr && !(s.mask[v >> 3] >> (v & 7) & 1)) x = -__builtin_inff();
-    if (WRITE)
-      out[v] = to_bits<T>(x);
+  if (const int v = 8 * (c0 + eights) + tid; v < end) {
+    const bool ok = mask_row == nullptr || (mask_row[v >> 3] >> (v & 7) & 1);
+    const bool special = known_row != nullptr && ((known_row[v >> 3] >> (v & 7) & 1) || times_drafted(s, v));
+    const float l = load_logit<T>(base + v);
+    if (WRITE && !ok) out[v] = to_bits<T>(-__builtin_inff());
+    if (WRITE && !INPLACE && ok && !special) out[v] = base[v];
+    if (ok && special)
+      token(v, l, s.counts[v], s.bias[v]);
     else
-      best = u64_max(best, argmax_key(x, v));
+      key = u64_max(key, argmax_key(ok ? l : -__builtin_inff(), v));
+  }
+
+  if (due) {
+    int at = atomicAdd(&listed, __popc(due));
+    while (due) {
+      const int bit = __builtin_ctz(due), e = 8 * (tid + (bit >> 3) * kLThreads) + (bit & 7);
+      due &= due - 1;
+      if (at < kListed)
+        list[at++] = (uint16_t)e;
+      else  // more than there is room for: at once (a lane's store of its own eight is behind it)
+        token(start + e, load_logit<T>(held + e), s.counts[start + e], s.bias[start + e]);
+    }
+  }
+  __syncthreads();  // (also: the stores of the listed tokens' eights are done)
+  const int n = min(listed, kListed);
+  for (int k = tid; k < n; k += 4 * kLThreads) {  // four trips to memory at a time
+    int e[4];
+    int32_t count[4];
+    float bias[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = list[min(k + j * kLThreads, n - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) count[j] = s.counts[start + e[j]], bias[j] = s.bias[start + e[j]];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (k + j * kLThreads < n) token(start + e[j], load_logit<T>(held + e[j]), count[j], bias[j]);
   }
   if (WRITE) return;
-  best = wave_max_u64(best);
-  if ((threadIdx.x & 63) == 0) wbest[threadIdx.x >> 6] = best;
+  key = wave_max_u64(key);
+  if ((tid & 63) == 0) wbest[tid >> 6] = key;
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
 #pragma unroll
-    for (int w = 1; w < kLThreads / 64; ++w) best = u64_max(best, wbest[w]);
-    p.keys[(int64_t)row * p.splits + split] = best;
+    for (int w = 1; w < kLThreads / 64; ++w) key = u64_max(key, wbest[w]);
+    p.keys[(int64_t)row * p.splits + split] = key;
   }
+}
+
+// A row's slices: as many as the greedy accept's, or as it takes of at most kSlice.
+Split plan_slices(int B, int N, int V, int dtype) {
+  const Split sp = plan_split(B, N, V);
+  const int chunk = std::min(sp.chunk, dtype == DFLASH_DTYPE_F32 ? kSlice<float> : kSlice<uint16_t>);
+  return Split{(int)ceil_div(V, chunk), chunk};
 }
 
 // Forget: only what a known bit is set for holds anything.
@@ -299,8 +399,8 @@ int check_state(const dflash_logits_state* s) {
 }
 
 template <bool WRITE, bool INPLACE>
-hipError_t launch_process(const ProcessParams& p, int dtype, int B, hipStream_t s) {
-  const dim3 grid((unsigned)(B * p.N), (unsigned)p.splits);
+hipError_t launch_process(const ProcessParams& p, int dtype, hipStream_t s) {
+  const dim3 grid(p.rows, p.splits);
   if (dtype == DFLASH_DTYPE_F32)
     hipLaunchKernelGGL((process_kernel<float, WRITE, INPLACE>), grid, dim3(kLThreads), 0, s, p);
   else if (dtype == DFLASH_DTYPE_BF16)
@@ -329,11 +429,13 @@ int make_params(ProcessParams& p, const void* logits, int dtype, int64_t bs, int
     if ((n_draft < N - 1 ? n_draft : N - 1) > DFLASH_LOGITS_MAX_DRAFT) return DFLASH_ERR_SHAPE;
     p.counts = state->counts, p.known = state->known, p.bias = state->bias, p.penalties = state->penalties;
   }
-  const Split sp = plan_split(B, N, V);
+  const Split sp = plan_slices(B, N, V, dtype);
+  if (sp.splits > 65535) return DFLASH_ERR_SHAPE;
   p.logits = logits, p.bs = bs, p.rs = rs;
   p.draft = draft, p.dstride = dstride, p.n_draft = n_draft;
   p.mask = mask, p.mask_bs = mask_bs, p.mask_rs = mask_rs;
   p.N = N, p.V = V, p.chunk = sp.chunk, p.splits = sp.splits;
+  p.rows = (unsigned)(B * N);
   return DFLASH_OK;
 }
 
@@ -392,8 +494,13 @@ extern "C" int dflash_logits_process(const void* logits, int logits_dtype, int64
   if (inplace && (out_batch_stride != batch_stride || out_row_stride != row_stride)) return DFLASH_ERR_SHAPE;
   p.out = out, p.obs = out_batch_stride, p.ors = out_row_stride;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return to_status(inplace ? launch_process<true, true>(p, logits_dtype, B, s)
-                           : launch_process<true, false>(p, logits_dtype, B, s));
+  return to_status(inplace ? launch_process<true, true>(p, logits_dtype, s)
+                           : launch_process<true, false>(p, logits_dtype, s));
+}
+
+extern "C" size_t dflash_greedy_accept_processed_workspace_bytes(int B, int N, int V) {
+  if (B <= 0 || N <= 0 || V <= 0) return 0;
+  return sizeof(uint64_t) * (size_t)B * N * plan_slices(B, N, V, DFLASH_DTYPE_F32).splits;
 }
 
 extern "C" int dflash_greedy_accept_processed(const void* logits, int logits_dtype, int64_t batch_stride,
@@ -407,11 +514,11 @@ extern "C" int dflash_greedy_accept_processed(const void* logits, int logits_dty
                             mask, mask_batch_stride, mask_row_stride, B, N, V);
   if (e || B == 0) return e;
   if (workspace == nullptr || (posterior == nullptr && matched == nullptr && bonus == nullptr)) return DFLASH_ERR_NULL;
-  if (workspace_bytes < dflash_greedy_accept_workspace_bytes(B, N, V)) return DFLASH_ERR_WORKSPACE;
+  if (workspace_bytes < sizeof(uint64_t) * (size_t)B * N * p.splits) return DFLASH_ERR_WORKSPACE;
   if ((uintptr_t)workspace % 8) return DFLASH_ERR_ALIGN;
   p.keys = static_cast<uint64_t*>(workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const hipError_t h = launch_process<false, false>(p, logits_dtype, B, s);
+  const hipError_t h = launch_process<false, false>(p, logits_dtype, s);
   if (h != hipSuccess) return (int)h;
   return to_status(launch_accept_finalize(p.keys, p.splits, B, N, draft, draft_stride, n_draft, posterior, matched,
                                           bonus, s));

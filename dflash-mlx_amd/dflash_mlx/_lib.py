@@ -146,6 +146,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dflash_logits_state_set_bias": (_I, [_VP, _VP, _I64, _VP, _I64, _I, _VP]),
     "dflash_logits_process": (
         _I, [_VP, _I, _I64, _I64, _VP, _VP, _I64, _I, _VP, _I64, _I64, _VP, _I64, _I64, _I, _I, _I, _VP]),
+    "dflash_greedy_accept_processed_workspace_bytes": (_SZ, [_I, _I, _I]),
     "dflash_greedy_accept_processed": (
         _I,
         [_VP, _I, _I64, _I64, _VP, _I64, _I, _VP, _VP, _I64, _I64, _VP, _VP, _VP, _I, _I, _I, _VP, _SZ, _VP],

@@ -130,8 +130,8 @@ def _greedy_accept_processed(lg, draft, want_posterior, state, mask):
         return post, matched, bonus
     if N == 0 or V == 0:
         raise ValueError(f"logits need at least one row and one vocabulary entry, got {tuple(lg.shape)}")
-    ws_bytes = int(_lib.load().dflash_greedy_accept_workspace_bytes(B, N, V))
-    ws = torch.empty((max(ws_bytes, 8),), dtype=torch.uint8, device=dev)
+    ws_bytes = int(_lib.load().dflash_greedy_accept_processed_workspace_bytes(B, N, V))
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
     _call("dflash_greedy_accept_processed", dev, lg.data_ptr(), _lib.dtype_tag(lg.dtype), lg.stride(0), lg.stride(1),
           _lib.ptr(d), d.stride(0) if d is not None else 0, d.shape[1] if d is not None else 0, sp, mp, mb, mr,
           _lib.ptr(post), matched.data_ptr(), bonus.data_ptr(), B, N, V, ws.data_ptr(), ws.numel())

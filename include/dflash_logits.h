@@ -80,7 +80,9 @@ int dflash_logits_process(const void* logits, int logits_dtype, int64_t batch_st
 
 /* dflash_greedy_accept of the processed logits, which are not stored: the greedy token of
  * a row is that of the largest fp32 value, the lowest on ties (a row that its mask leaves
- * nothing: token 0).  workspace: dflash_greedy_accept_workspace_bytes(B, N, V) bytes. */
+ * nothing: token 0).  workspace: dflash_greedy_accept_processed_workspace_bytes(B, N, V)
+ * bytes, 8-byte aligned. */
+size_t dflash_greedy_accept_processed_workspace_bytes(int B, int N, int V);
 int dflash_greedy_accept_processed(const void* logits, int logits_dtype, int64_t batch_stride,
                                    int64_t row_stride, const int32_t* draft, int64_t draft_stride,
                                    int n_draft, const dflash_logits_state* state, const uint32_t* mask,

@@ -63,7 +63,8 @@ def test_every_declared_entry_point_is_exported_and_bound(lib):
     text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "dflash_logits.h").read_text(), flags=re.S)
     names = set(re.findall(r"\b(dflash_[a-z0-9_]+)\s*\(", text))
     assert names == {"dflash_logits_state_reset", "dflash_logits_state_add", "dflash_logits_state_set_bias",
-                     "dflash_logits_process", "dflash_greedy_accept_processed"}
+                     "dflash_logits_process", "dflash_greedy_accept_processed",
+                     "dflash_greedy_accept_processed_workspace_bytes"}
     for name in names:
         assert hasattr(lib, name) and name in _lib.SIGNATURES
 
