@@ -329,43 +329,79 @@ Split plan_slices(int B, int N, int V, int dtype) {
   return Split{(int)ceil_div(V, chunk), chunk};
 }
 
-// Forget: only what a known bit is set for holds anything.
+// Forget: only what a known bit is set for holds anything.  A thread eight tokens' bits.
 __global__ __launch_bounds__(kLThreads) void state_reset_kernel(const dflash_logits_state s) {
   const int words = (s.V + 31) >> 5, b = blockIdx.y;
   const int w = blockIdx.x * kLThreads + threadIdx.x;
   if (w == 0) s.penalties[3 * b] = 1.f, s.penalties[3 * b + 1] = 0.f, s.penalties[3 * b + 2] = 0.f;
-  if (w >= words) return;
-  uint32_t* kp = s.known + (int64_t)b * words + w;
+  if (w >= 4 * words) return;
+  uint8_t* kp = reinterpret_cast<uint8_t*>(s.known + (int64_t)b * words) + w;
   uint32_t bits = *kp;
   if (bits == 0) return;
   *kp = 0;
-  while (bits) {
-    const int v = 32 * w + __builtin_ctz(bits);
-    bits &= bits - 1;
+  for (; bits; bits &= bits - 1) {
+    const int v = 8 * w + __builtin_ctz(bits);
     if (v >= s.V) break;
     s.counts[(int64_t)b * s.V + v] = 0;
     s.bias[(int64_t)b * s.V + v] = 0.f;
   }
 }
 
-// A thread a token.  Integer atomics: the result does not depend on their order.  A
-// stale bit only costs the atomic that would have been spared.
+// Four tokens a thread.  In text a few tokens come again and again, and atomics on one address
+// take turns (16 000 tokens of 32 sequences of which 5 % are one token: 50 us): a workgroup
+// first adds up equal tokens, and the known bits of a word, in tables in LDS, whose place a
+// token that finds it taken by another does without.  Integer sums and ORs: the result does
+// not depend on the order.
+constexpr int kAddTokens = 4 * kLThreads, kAddSlots = 1024;
 __global__ __launch_bounds__(kLThreads) void state_add_kernel(const dflash_logits_state s, const int32_t* tokens,
                                                              int64_t row_stride, int n, const int32_t* lens,
                                                              int prompt) {
+  __shared__ int32_t token_at[kAddSlots], times[kAddSlots], word_at[kAddSlots];
+  __shared__ uint32_t bits_at[kAddSlots];
   const int b = blockIdx.y;
-  const int j = blockIdx.x * kLThreads + threadIdx.x;
-  if (j >= (lens != nullptr ? min(n, lens[b]) : n)) return;
-  const int v = tokens[b * row_stride + j];
-  if ((uint32_t)v >= (uint32_t)s.V) return;
-  int32_t* count = s.counts + (int64_t)b * s.V + v;
-  if (!prompt)
-    atomicAdd(count, 1);
-  else if (*count >= 0)
-    atomicOr(reinterpret_cast<uint32_t*>(count), ~kCountMask);
-  uint32_t* word = s.known + (int64_t)b * ((s.V + 31) >> 5) + (v >> 5);
-  const uint32_t bit = 1u << (v & 31);
-  if (!(*word & bit)) atomicOr(word, bit);
+  const int end = lens != nullptr ? min(n, lens[b]) : n;
+  if ((int)blockIdx.x * kAddTokens >= end) return;
+  int32_t* counts = s.counts + (int64_t)b * s.V;
+  uint32_t* known = s.known + (int64_t)b * ((s.V + 31) >> 5);
+  int v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int j = blockIdx.x * kAddTokens + k * kLThreads + threadIdx.x;
+    v[k] = j < end ? tokens[b * row_stride + j] : -1;
+  }
+  for (int k = threadIdx.x; k < kAddSlots; k += kLThreads) token_at[k] = -1, times[k] = 0, word_at[k] = -1, bits_at[k] = 0;
+  __syncthreads();
+  auto add = [&](int t, int c) {
+    if (prompt)
+      atomicOr(reinterpret_cast<uint32_t*>(counts + t), ~kCountMask);
+    else
+      atomicAdd(counts + t, c);
+  };
+  auto learn = [&](int w, uint32_t bits) {
+    if ((known[w] & bits) != bits) atomicOr(known + w, bits);
+  };
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if ((uint32_t)v[k] >= (uint32_t)s.V) continue;
+    const int slot = ((uint32_t)v[k] * 2654435761u) >> 22;
+    const int was = atomicCAS(&token_at[slot], -1, v[k]);
+    if (was == -1 || was == v[k])
+      atomicAdd(&times[slot], 1);
+    else
+      add(v[k], 1);
+    if (was == v[k]) continue;  // its bit is on its way
+    const int w = v[k] >> 5, ws = w & (kAddSlots - 1);
+    const int had = atomicCAS(&word_at[ws], -1, w);
+    if (had == -1 || had == w)
+      atomicOr(&bits_at[ws], 1u << (v[k] & 31));
+    else
+      learn(w, 1u << (v[k] & 31));
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < kAddSlots; k += kLThreads) {
+    if (token_at[k] >= 0) add(token_at[k], times[k]);
+    if (word_at[k] >= 0) learn(word_at[k], bits_at[k]);
+  }
 }
 
 // A workgroup a sequence; of an id given twice the last stays.
@@ -447,7 +483,7 @@ using namespace dflash;
 extern "C" int dflash_logits_state_reset(const dflash_logits_state* state, void* stream) {
   const int e = check_state(state);
   if (e || state->B == 0) return e;
-  const dim3 grid((unsigned)ceil_div(ceil_div(state->V, 32), kLThreads), (unsigned)state->B);
+  const dim3 grid((unsigned)ceil_div(4 * ceil_div(state->V, 32), kLThreads), (unsigned)state->B);
   hipLaunchKernelGGL(state_reset_kernel, grid, dim3(kLThreads), 0, static_cast<hipStream_t>(stream), *state);
   return to_status(hipGetLastError());
 }
@@ -460,7 +496,7 @@ extern "C" int dflash_logits_state_add(const dflash_logits_state* state, const i
   if (n == 0 || state->B == 0) return DFLASH_OK;
   if (tokens == nullptr) return DFLASH_ERR_NULL;
   if ((uintptr_t)tokens % 4 || (uintptr_t)lens % 4) return DFLASH_ERR_ALIGN;
-  const dim3 grid((unsigned)ceil_div(n, kLThreads), (unsigned)state->B);
+  const dim3 grid((unsigned)ceil_div(n, kAddTokens), (unsigned)state->B);
   hipLaunchKernelGGL(state_add_kernel, grid, dim3(kLThreads), 0, static_cast<hipStream_t>(stream), *state, tokens,
                      row_stride, n, lens, prompt);
   return to_status(hipGetLastError());
