@@ -41,6 +41,7 @@ from .kv8 import (
 )
 from .logits import LogitsState, process_logits
 from .runtime import (
+    LogitsShaping,
     DFlashRuntimeEvent,
     dflash_generate,
     dflash_generate_stream,
@@ -73,6 +74,7 @@ __all__ = [
     "verify_block_stream",
     "Int8Weight",
     "KVCache",
+    "LogitsShaping",
     "LogitsState",
     "QuantizedKVCache",
     "Qwen35TargetAdapter",

@@ -11,7 +11,8 @@ by name; here both are passed in already built: ``target`` is a
 ``target.HybridTargetModel``, which is wrapped in one) and ``draft`` is any
 object with the drafter interface described in runtime.py.  Checkpoint
 loading, quantisation of the drafter and the MLX memory wiring are outside
-the verify hot path.
+the verify hot path.  ``shaping`` (a ``LogitsShaping``) puts penalties for
+repeated tokens, biases and a grammar on the tokens that are taken.
 """
 from __future__ import annotations
 
@@ -22,7 +23,7 @@ from typing import Any
 import torch
 
 from .adapters import LoadedTargetModel
-from .runtime import dflash_generate, dflash_generate_stream
+from .runtime import LogitsShaping, dflash_generate, dflash_generate_stream
 
 
 @dataclass
@@ -86,6 +87,7 @@ class DFlashGenerator:
         reset_peak_memory: bool = True,
         skip_special_tokens: bool = False,
         profile: bool = False,
+        shaping: LogitsShaping | None = None,
     ) -> DFlashResult:
         if reset_peak_memory and torch.cuda.is_available():
             torch.cuda.reset_peak_memory_stats()
@@ -101,6 +103,7 @@ class DFlashGenerator:
             verify_mode=verify_mode,
             verify_chunk_size=verify_chunk_size,
             profile=profile,
+            shaping=shaping,
         )
         generated_tokens = output_tokens[metrics["num_input_tokens"]:]
         return DFlashResult(
@@ -121,6 +124,7 @@ class DFlashGenerator:
         reset_peak_memory: bool = True,
         skip_special_tokens: bool = False,
         profile: bool = False,
+        shaping: LogitsShaping | None = None,
     ) -> Iterator[DFlashStreamEvent]:
         prompt_len = int(torch.as_tensor(prompt_tokens).reshape(-1).shape[0])
         decoded_text = ""
@@ -138,6 +142,7 @@ class DFlashGenerator:
             verify_mode=verify_mode,
             verify_chunk_size=verify_chunk_size,
             profile=profile,
+            shaping=shaping,
         ):
             generated_tokens = event.output_tokens[prompt_len:]
             text = self._decode(generated_tokens, skip_special_tokens)

@@ -44,7 +44,9 @@ import torch
 
 from . import _lib
 from .gdn_layer import QK_NORM_EPS, GatedDeltaConfig, GatedDeltaWeights
+from .int8 import Int8Weight, quantize_weight_i8
 from .kv8 import QuantizedKVCache, attn_verify_q8_workspace_bytes, kv_load_q8
+from .logits import LogitsState
 
 
 @dataclass(frozen=True)
@@ -109,6 +111,18 @@ class HybridWeights:
     # The LM head's fragment-tiled copy, made by the first runner that streams
     # it (tile_weight; V % 16 == 0).
     lm_head_tiled: torch.Tensor | None = None
+    # The LM head in 8-bit integers, made by the first target with weight_dtype int8
+    # (int8_weights; the layers' projections are in their dicts as "<name>_i8").
+    lm_head_i8: Int8Weight | None = None
+
+    def int8_weights(self, cfg: HybridConfig) -> None:
+        """Quantise every projection and the LM head by output channel (once)."""
+        for i, lw in enumerate(self.layers):
+            for name in ("w_gu", "w_down") + (("w_in", "w_out") if cfg.is_linear(i) else ("w_qkv", "w_o")):
+                if name + "_i8" not in lw:
+                    lw[name + "_i8"] = quantize_weight_i8(lw[name], gated=name == "w_gu")
+        if self.lm_head_i8 is None:
+            self.lm_head_i8 = quantize_weight_i8(self.lm_head)
 
     @staticmethod
     def random(cfg: HybridConfig, device, seed: int = 0, std: float = 0.02,
@@ -189,6 +203,7 @@ class _Plan:
     def __init__(self, T):
         self.T = T
         self.fwd: list = []
+        self.logits: list = []  # where the logits are stored for the accept
         self.lm = None
         self.commit: list = []
         self.conv_from = None
@@ -207,7 +222,9 @@ class HybridVerifyRunner:
 
     def __init__(self, cfg: HybridConfig, weights: HybridWeights, B: int, T: int, Smax: int,
                  device: torch.device, weight_layout: str = "tiled", fused_prologue: bool = True,
-                 fused_norms: bool = True, kv_dtype: torch.dtype = torch.bfloat16):
+                 fused_norms: bool = True, kv_dtype: torch.dtype = torch.bfloat16,
+                 weight_dtype: torch.dtype = torch.bfloat16, logits_state: LogitsState | None = None,
+                 masked: bool = False):
         """weight_layout: "tiled" streams weights re-laid out once as MFMA
         fragments (dflash_weight_tile_bf16, cached in the layer dicts as
         "<name>_tiled"; same sums bit for bit) wherever the row count is a
@@ -225,10 +242,23 @@ class HybridVerifyRunner:
         the faster form (fuses_norms(T) says whether a step of T tokens does);
         False: never.  The producing projections then split K inside a workgroup
         instead of across workgroups, so their sums (and what follows) differ
-        from the launch form in rounding."""
+        from the launch form in rounding.  weight_dtype: torch.int8 holds every
+        projection and the LM head in 8-bit integers, a scale a channel, and
+        quantises their rows by token (dflash_linear_i8).  logits_state: the
+        accept is of the logits under this state's penalties and biases (B
+        sequences), and a commit counts the tokens that it keeps (the caller
+        counts the prompt and the first block's first token).  masked: the accept
+        is under the bitmask self.mask, int32 [B, T, ceil(V / 32)], row t for
+        block token t's successor; all ones until the caller writes it."""
         if weight_layout not in ("tiled", "rowmajor"):
             raise ValueError(f"weight_layout must be 'tiled' or 'rowmajor', got {weight_layout!r}")
-        self.tiled = weight_layout == "tiled"
+        if weight_dtype not in (torch.bfloat16, torch.int8):
+            raise ValueError(f"weight_dtype must be bfloat16 or int8, got {weight_dtype}")
+        if logits_state is not None and (logits_state.B != B or logits_state.V != cfg.vocab_size):
+            raise ValueError(f"logits_state must be of {B} sequences and {cfg.vocab_size} tokens, got {logits_state}")
+        self.int8 = weight_dtype is torch.int8
+        self.logits_state = logits_state
+        self.tiled = weight_layout == "tiled" and not self.int8
         self.fused_norms = bool(fused_norms) and self.tiled
         if B < 1 or T < 1 or T > 16 or B * T > 64:
             raise ValueError("the verify step takes 1 <= T <= 16 block tokens and B*T <= 64 rows")
@@ -305,6 +335,11 @@ class HybridVerifyRunner:
         self.gemm_ws = z(int(lib.dflash_gemm_tail_workspace_bytes()), dt=torch.uint8)
         self.capture_layers: tuple[int, ...] = ()
         self.captured = None  # [B*T, len(capture_layers) * H] after set_capture
+        # logits stored for the accept: where something changes them, or of the 8-bit head
+        self.logits = (e(M, V, dt=f32 if self.int8 else bf)
+                       if self.int8 or logits_state is not None or masked else None)
+        self.mask = torch.full((B, T, -(-V // 32)), -1, dtype=i32, device=device) if masked else None
+        self.proc_ws = e(max(int(lib.dflash_greedy_accept_processed_workspace_bytes(B, T, V)), 8), dt=torch.uint8)
         self._plans: dict[int, _Plan] = {}
         self._prepare_weights()
         self.graph = None
@@ -340,6 +375,16 @@ class HybridVerifyRunner:
         cfg, M, H, I = self.cfg, self.B * self.T, self.cfg.hidden_size, self.cfg.intermediate_size
         dims = self._dims()
         lib = _lib.load()
+        if self.int8:
+            self.w.int8_weights(cfg)
+            self.splits = dict.fromkeys(dims, 0)  # every projection writes bf16
+            weights = [w for lw in self.w.layers for w in lw.values() if isinstance(w, Int8Weight)]
+            ws = max(int(lib.dflash_linear_i8_workspace_bytes(m, w.N, w.K, int(w.gated)))
+                     for w in weights + [self.w.lm_head_i8] for m in range(1, M + 1))
+            self.i8_ws = torch.empty(ws, dtype=torch.uint8, device=self.device)
+            self.part = torch.empty(1, dtype=torch.float32, device=self.device)
+            torch.cuda.synchronize(self.device)
+            return
         self.plan = self.TILED_PLAN if self.tiled else self.GEMM_PLAN
         self.splits = {k: int(lib.dflash_gemm_splits(dims[k][1], p[0])) if p[0] > 1 else 0
                        for k, p in self.plan.items()}
@@ -404,7 +449,15 @@ class HybridVerifyRunner:
             p = self._plans[T] = self._build_plan(T)
         return p
 
+    def _linear_i8_op(self, weight, x, out_ptr, out_dtype, out_stride, M):
+        return ("dflash_linear_i8",
+                (x.data_ptr(), _lib.DFLASH_DTYPE_BF16, x.stride(0), weight.codes.data_ptr(), weight.scales.data_ptr(),
+                 out_ptr, out_dtype, out_stride, M, weight.N, weight.K, int(weight.gated), self.i8_ws.data_ptr(),
+                 self.i8_ws.numel()))
+
     def _gemm_op(self, lw, name, x, out_ptr, out_stride, M):
+        if self.int8:
+            return self._linear_i8_op(lw[name + "_i8"], x, out_ptr, _lib.DFLASH_DTYPE_BF16, out_stride, M)
         n, k = self._dims()[name]
         ns, rpw, kw = self.plan[name]
         if self.tiled and name + "_tiled" in lw:
@@ -580,7 +633,9 @@ class HybridVerifyRunner:
                     fwd.append(self._residual_op("w_o", lw["ln_post"], M, None))
                 ai += 1
             gu_key = "w_gu_pairs_tiled" if self.tiled and "w_gu_pairs_tiled" in lw else None
-            if post:
+            if self.int8:
+                fwd.append(self._gemm_op(lw, "w_gu", self.xn, self.mlp_act.data_ptr(), I, M))
+            elif post:
                 fwd.append(("dflash_gemm_bf16_swiglu_tiled_normed",
                             self._norm_input(lw["ln_post"]) + (lw[gu_key].data_ptr(),
                                                                self.mlp_act.data_ptr(), I, M, 2 * I,
@@ -603,7 +658,25 @@ class HybridVerifyRunner:
         tail = (self.tokens.data_ptr() + 4, T, T - 1, self.posterior.data_ptr(),
                 self.matched.data_ptr(), self.bonus.data_ptr(), B, T, self.lm_ws.data_ptr(),
                 self.lm_ws.numel())
-        if self.w.lm_head_tiled is not None and self.tiled:
+        if self.logits is not None:
+            V, bf = cfg.vocab_size, _lib.DFLASH_DTYPE_BF16
+            lg, tag = self.logits.data_ptr(), _lib.dtype_tag(self.logits.dtype)
+            if self.int8:
+                pl.logits = [self._linear_i8_op(self.w.lm_head_i8, self.xn, lg, tag, V, M)]
+            elif self.w.lm_head_tiled is not None and self.tiled:
+                pl.logits = [("dflash_gemm_bf16_tiled", (self.xn.data_ptr(), H, self.w.lm_head_tiled.data_ptr(), lg, V,
+                                                         M, V, H, 1, 64, 4, None, 0))]
+            else:
+                pl.logits = [("dflash_gemm_bf16", (self.xn.data_ptr(), H, self.w.lm_head.data_ptr(), H, lg, V, M, V, H,
+                                                   1, 32, 4))]
+            drafts = (self.tokens.data_ptr() + 4, T, T - 1)
+            ends = (self.posterior.data_ptr(), self.matched.data_ptr(), self.bonus.data_ptr(), B, T, V,
+                    self.proc_ws.data_ptr(), self.proc_ws.numel())
+            W = -(-V // 32)
+            mask = (self.mask.data_ptr(), self.T * W, W) if self.mask is not None else (None, 0, 0)
+            state = self.logits_state._ptr if self.logits_state is not None else None
+            pl.lm = ("dflash_greedy_accept_processed", (lg, tag, T * V, V, *drafts, state, *mask, *ends))
+        elif self.w.lm_head_tiled is not None and self.tiled:
             pl.lm = ("dflash_lm_head_greedy_accept_tiled",
                      (self.xn.data_ptr(), H, self.w.lm_head_tiled.data_ptr(), H, cfg.vocab_size)
                      + tail)
@@ -621,6 +694,9 @@ class HybridVerifyRunner:
             ("dflash_conv_rollback", (cin, qkv, cin, self.keep.data_ptr(), cfg.n_linear, B, T, K1, C,
                                       T * rows, rows, 2)),
         ]
+        if self.logits_state is not None:  # posterior[:keep] are the accepted drafts and the bonus
+            pl.commit.append(("dflash_logits_state_add",
+                              (self.logits_state._ptr, self.posterior.data_ptr(), T, T, self.keep.data_ptr(), 0)))
         if self.conv_snap is not None:
             snap = _lib.ptr_array(list(self.conv_snap.unbind(0)))
             pl.keep_alive.append(snap)
@@ -721,7 +797,7 @@ class HybridVerifyRunner:
         p = self._plan(self.T if T is None else int(T))
         self._run(p.fwd)
         if lm_head:
-            self._run([p.lm])
+            self._run(p.logits + [p.lm])
 
     def forward_accept(self) -> None:
         """forward() of a full T-token block with the fused LM-head accept."""
@@ -738,7 +814,7 @@ class HybridVerifyRunner:
         the block's qkv rows, in place.  The KV lengths stay with the caller."""
         p = self._plan(int(T))
         self.keep.fill_(int(T))
-        self._run(p.commit[1:])
+        self._run(p.commit[1:2])
 
     def rollback_to(self, T: int) -> None:
         """Conv windows rebuilt from conv_snap and the block's qkv rows at the

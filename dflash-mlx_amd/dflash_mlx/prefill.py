@@ -48,6 +48,7 @@ import torch
 
 from . import _lib
 from .gdn_layer import QK_NORM_EPS
+from .int8 import Int8Weight
 
 
 MAX_SPLITS = 4
@@ -241,6 +242,7 @@ class HybridPrefill:
         self.max_rows = int(max_rows)
         self.rows_cap = 0
         self.kv_ws = torch.empty(0, dtype=torch.uint8, device=runner.device)  # attention over the 8-bit cache
+        self.i8_ws = torch.empty(0, dtype=torch.uint8, device=runner.device)  # projections in 8-bit integers
         self._lib = _lib.load()
         self.cus = torch.cuda.get_device_properties(runner.device).multi_processor_count
         self._weights()
@@ -273,6 +275,12 @@ class HybridPrefill:
         cfg = self.cfg
         self.w = []
         for i, lw in enumerate(self.run.w.layers):
+            if self.run.int8:  # row counts as in a tiled copy: a multiple of 16
+                names = {"w_gu_pairs": "w_gu", "w_down": "w_down"} | (
+                    {"w_in": "w_in", "w_out": "w_out"} if cfg.is_linear(i) else {"w_qkv": "w_qkv", "w_o": "w_o"})
+                ws = {n: lw[src + "_i8"] for n, src in names.items()}
+                self.w.append({n: (w, -(-w.N // 16) * 16) for n, w in ws.items()})
+                continue
             names = ["w_gu_pairs", "w_down"] + (["w_in", "w_out"] if cfg.is_linear(i)
                                                 else ["w_qkv", "w_o"])
             self.w.append({n: self._tiled(lw, n) for n in names})
@@ -305,6 +313,10 @@ class HybridPrefill:
         ws = int(self._lib.dflash_gdn_chunked_prefill_workspace_bytes(
             1, P, Hv, lc.linear_key_head_dim, Dv))
         self.chunk_ws = e(max(ws, 16), dt=torch.uint8)
+        if self.run.int8:
+            self.part = e(4, dt=f32)
+            self.rows_cap = P
+            return
         shapes = {(name in RESIDUAL, n, wt.numel() // n) for d in self.w for name, (wt, n) in d.items()}
         need = max((partial_floats(r, n, K, P, self.cus) for r, n, K in shapes), default=0)
         self.part = e(max(need, 4), dt=f32)
@@ -444,6 +456,9 @@ class HybridPrefill:
         the partials summed and cast by the reduce; or the rows of the whole
         rounds in one launch and the last n-tiles' rows split-K (tail_split)."""
         wt, n = weight
+        if isinstance(wt, Int8Weight):
+            self._linear_i8(wt, x_ptr, K, P, out_ptr, out_stride, stream)
+            return
         if P <= block_rows(False, n, K, self.cus):
             _lib.call("dflash_gemm_bf16_tiled_block", x_ptr, K, wt.data_ptr(), out_ptr, out_stride,
                       None, 0, P, n, K, int(swiglu), stream)
@@ -483,6 +498,9 @@ class HybridPrefill:
         """A projection whose output the residual stream adds: bf16 into r,
         or split-K fp32 partials into part; returns the split count (0: r)."""
         wt, n = weight
+        if isinstance(wt, Int8Weight):
+            self._linear_i8(wt, x_ptr, K, P, self.r.data_ptr(), self.cfg.hidden_size, stream)
+            return 0
         block = P <= block_rows(True, n, K, self.cus)
         ns = block_splits(n, self.cus, K) if block else residual_splits(n, P, self.cus, K)
         used = splits_used(K, ns) if ns > 1 else 0
@@ -497,6 +515,14 @@ class HybridPrefill:
             _lib.call("dflash_gemm_bf16_tiled_prefill", x_ptr, K, wt.data_ptr(), self.r.data_ptr(),
                       self.cfg.hidden_size, P, n, K, stream)
         return used
+
+    def _linear_i8(self, w, x_ptr, K, P, out_ptr, out_stride, stream) -> None:
+        bf = _lib.DFLASH_DTYPE_BF16
+        need = self._lib.dflash_linear_i8_workspace_bytes(P, w.N, w.K, int(w.gated))
+        if self.i8_ws.numel() < need:
+            self.i8_ws = torch.empty(need, dtype=torch.uint8, device=self.run.device)
+        _lib.call("dflash_linear_i8", x_ptr, bf, K, w.codes.data_ptr(), w.scales.data_ptr(), out_ptr, bf, out_stride, P,
+                  w.N, K, int(w.gated), self.i8_ws.data_ptr(), self.i8_ws.numel(), stream)
 
     def _kv_workspace(self, P: int) -> torch.Tensor:
         """The workspace of the attention over a cache in 8 bits (empty: no split)."""

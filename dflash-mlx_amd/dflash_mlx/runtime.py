@@ -30,7 +30,7 @@ here are far below 2**31).
 from __future__ import annotations
 
 import time
-from collections.abc import Iterator
+from collections.abc import Callable, Iterator
 from dataclasses import dataclass
 from typing import Any, Sequence
 
@@ -39,7 +39,7 @@ import torch
 from . import _lib
 from .gated_delta import _require_device
 from .kv8 import _call
-from .logits import LogitsState, check_draft, check_mask, check_state
+from .logits import MAX_BIAS, LogitsState, check_draft, check_mask, check_state, process_logits
 
 
 def _as_3d(logits: torch.Tensor) -> torch.Tensor:
@@ -316,9 +316,84 @@ def _target_device(target: Any):
     return getattr(model, "device", None) or getattr(target, "device", None) or "cuda"
 
 
-def _posterior(logits: torch.Tensor, temperature: float) -> list[int]:
-    """Posterior tokens of row 0 of [1, N, V] logits on the host."""
-    return sample_tokens(logits[:1], temperature)[0].cpu().tolist()
+class LogitsShaping:
+    """What a generation asks of its logits: a LogitsState of one sequence that counts
+    the prompt and every token taken, and a grammar.  token_mask(tokens) gives the
+    bitmask (int32 [ceil(V / 32)], any device) of what may follow the tokens, prompt
+    included, or None for anything."""
+
+    def __init__(self, repetition_penalty: float = 1.0, presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
+                 logit_bias: dict[int, float] | None = None,
+                 token_mask: Callable[[list[int]], torch.Tensor | None] | None = None):
+        if not repetition_penalty > 0:
+            raise ValueError(f"the repetition penalty must be positive, got {repetition_penalty}")
+        self.penalties = (float(repetition_penalty), float(presence_penalty), float(frequency_penalty))
+        self.logit_bias = dict(logit_bias or {})
+        if len(self.logit_bias) > MAX_BIAS:
+            raise ValueError(f"at most {MAX_BIAS} biases, got {len(self.logit_bias)}")
+        self.token_mask = token_mask
+        self.state: LogitsState | None = None
+        self.tokens: list[int] = []
+        self._waiting: list[tuple[list[int], bool]] = []
+
+    @property
+    def active(self) -> bool:
+        return self.penalties != (1.0, 0.0, 0.0) or bool(self.logit_bias) or self.token_mask is not None
+
+    def begin(self, prompt: list[int]) -> None:
+        self.state, self.tokens, self._waiting = None, [], []
+        self.commit(prompt, prompt=True)
+
+    def commit(self, tokens: list[int], prompt: bool = False) -> None:
+        """These tokens are taken."""
+        self.tokens += tokens
+        self._waiting.append((list(tokens), prompt))
+
+    def _ready(self, V: int, dev) -> LogitsState:
+        if self.state is None:  # the vocabulary is the first logits'
+            self.state = LogitsState.zeros(1, V, dev)
+            self.state.set_penalties(*self.penalties)
+            if self.logit_bias:
+                self.state.set_bias([list(self.logit_bias)], [[float(v) for v in self.logit_bias.values()]])
+            self._extra = LogitsState.zeros(1, V, dev)
+        for tokens, prompt in self._waiting:
+            if tokens:
+                self.state.add([tokens], prompt=prompt)
+        self._waiting = []
+        return self.state
+
+    def rows(self, n: int, V: int, dev, before: Sequence[int], drafts: Sequence[int]):
+        """(state, mask) of n rows, the first of which knows the drafts `before` too and row
+        i also drafts[:i]."""
+        state = self._ready(V, dev)
+        if before:
+            for name in ("counts", "known", "bias", "penalties"):
+                getattr(self._extra, name).copy_(getattr(state, name))
+            state = self._extra
+            state.add([list(before)])
+        if self.token_mask is None:
+            return state, None
+        mask = torch.full((1, n, -(-V // 32)), -1, dtype=torch.int32)
+        for i in range(n):
+            words = self.token_mask(self.tokens + list(before) + list(drafts[:i]))
+            if words is not None:
+                mask[0, i] = words
+        return state, mask.to(dev)
+
+
+def _posterior(logits: torch.Tensor, temperature: float, shaping: LogitsShaping | None = None,
+               before: Sequence[int] = (), drafts: Sequence[int] = ()) -> list[int]:
+    """Posterior tokens of row 0 of [1, N, V] logits on the host.  shaping: of the
+    processed logits; the rows know the drafts `before`, row i also drafts[:i]."""
+    logits = logits[:1]
+    if shaping is None:
+        return sample_tokens(logits, temperature)[0].cpu().tolist()
+    n, V = logits.shape[1:]
+    drafts = list(drafts[:n - 1])
+    state, mask = shaping.rows(n, V, logits.device, before, drafts)
+    if temperature < 1e-5:
+        return greedy_accept(logits, [drafts], state=state, mask=mask)[0][0].cpu().tolist()
+    return sample_tokens(process_logits(logits.float(), state, [drafts], mask=mask), temperature)[0].cpu().tolist()
 
 
 def _rollback(target, target_cache, rollback_records, draft_block_size, accepted_inputs,
@@ -338,6 +413,7 @@ def verify_block_stream(
     block_tokens: list[int],
     temperature: float,
     layer_ids: list[int],
+    shaping: LogitsShaping | None = None,
 ) -> tuple[int, int, torch.Tensor]:
     """runtime.py:86-114: verify token by token, stopping at the first
     mismatch (no rollback needed)."""
@@ -346,7 +422,7 @@ def verify_block_stream(
     for idx, token in enumerate(block_tokens):
         logits_step, hidden_step = target.forward_with_hidden_states(
             _block_tensor([token], dev), target_cache, layer_ids)
-        next_token = _posterior(logits_step[:, -1:, :], temperature)[0]
+        next_token = _posterior(logits_step[:, -1:, :], temperature, shaping, block_tokens[1:idx + 1])[0]
         verified_hidden_steps.append(hidden_step)
         if idx == len(block_tokens) - 1:
             return len(block_tokens), next_token, torch.cat(verified_hidden_steps, dim=1)
@@ -363,6 +439,7 @@ def verify_block_parallel_replay(
     temperature: float,
     layer_ids: list[int],
     profile: dict[str, float] | None = None,
+    shaping: LogitsShaping | None = None,
 ) -> tuple[int, int, torch.Tensor]:
     """One verify step (runtime.py:117-163): the whole block in one forward
     with rollback records, the posterior from its logits, the accept, and the
@@ -380,12 +457,14 @@ def verify_block_parallel_replay(
     if temperature < 1e-5:
         # draft = block[1:] against posterior rows 0..T-2; the bonus may come
         # from row `matched` <= T-1, so all T rows are argmax'ed (runtime.py:145-147).
+        shaped = {} if shaping is None else dict(zip(("state", "mask"), shaping.rows(
+            logits.shape[1], logits.shape[2], logits.device, (), block_tokens[1:])))
         _, matched_t, bonus_t = greedy_accept(logits[:1], block.to(logits.device)[:, 1:],
-                                              want_posterior=False)
+                                              want_posterior=False, **shaped)
         host = torch.stack([matched_t, bonus_t]).cpu()  # the one device->host sync
         matched, bonus = int(host[0, 0]), int(host[1, 0])
     else:
-        posterior = _posterior(logits, temperature)
+        posterior = _posterior(logits, temperature, shaping, (), block_tokens[1:])
         matched = longest_prefix_match(block_tokens[1:], posterior[:-1])
         bonus = posterior[matched]
     accepted_inputs = matched + 1
@@ -403,6 +482,7 @@ def verify_block_parallel_lazy_logits(
     layer_ids: list[int],
     logit_chunk_size: int,
     profile: dict[str, float] | None = None,
+    shaping: LogitsShaping | None = None,
 ) -> tuple[int, int, torch.Tensor]:
     """runtime.py:166-243: the verifier's normed hidden states first, then
     the LM head chunk by chunk until the first mismatch."""
@@ -419,7 +499,8 @@ def verify_block_parallel_lazy_logits(
         chunk_end = min(chunk_start + chunk_size, draft_block_size)
         logit_start = profile_start(profile)
         logits_chunk = target.lm_head_logits(norm_hidden_states[:, chunk_start:chunk_end, :])
-        posterior_chunk = _posterior(logits_chunk, temperature)
+        posterior_chunk = _posterior(logits_chunk, temperature, shaping, block_tokens[1:chunk_start + 1],
+                                     block_tokens[chunk_start + 1:])
         add_profile_elapsed(profile, "verify_lazy_logits_time_s", logit_start)
         prefix_start = profile_start(profile)
         for local_idx, token in enumerate(posterior_chunk):
@@ -451,6 +532,7 @@ def verify_block_parallel_greedy_argmax(
     temperature: float,
     layer_ids: list[int],
     profile: dict[str, float] | None = None,
+    shaping: LogitsShaping | None = None,
 ) -> tuple[int, int, torch.Tensor]:
     """runtime.py:246-292: the verifier's normed hidden states, then the
     target's lm_head_argmax hook (here the fused LM-head greedy kernel: no
@@ -463,7 +545,10 @@ def verify_block_parallel_greedy_argmax(
     add_profile_elapsed(profile, "verify_state_time_s", state_start)
 
     argmax_start = profile_start(profile)
-    posterior = target.lm_head_argmax(norm_hidden_states)[0].cpu().tolist()
+    if shaping is None:
+        posterior = target.lm_head_argmax(norm_hidden_states)[0].cpu().tolist()
+    else:  # the penalties need the logits
+        posterior = _posterior(target.lm_head_logits(norm_hidden_states), 0.0, shaping, (), block_tokens[1:])
     add_profile_elapsed(profile, "verify_argmax_time_s", argmax_start)
 
     prefix_start = profile_start(profile)
@@ -482,6 +567,7 @@ def verify_block_chunked(
     temperature: float,
     layer_ids: list[int],
     verify_chunk_size: int,
+    shaping: LogitsShaping | None = None,
 ) -> tuple[int, int, torch.Tensor]:
     """runtime.py:295-357: verify in chunks; on a mismatch restore the
     chunk's linear caches from a snapshot and re-run only its accepted
@@ -495,7 +581,8 @@ def verify_block_chunked(
         linear_snapshots = target.snapshot_linear_caches(target_cache)
         chunk_logits, chunk_hidden = target.forward_with_hidden_states(
             _block_tensor(chunk_tokens, dev), target_cache, layer_ids)
-        posterior_chunk = _posterior(chunk_logits, temperature)
+        posterior_chunk = _posterior(chunk_logits, temperature, shaping, block_tokens[1:cursor + 1],
+                                     block_tokens[cursor + 1:])
 
         max_compare = min(len(chunk_tokens), draft_block_size - cursor - 1)
         local_matches = 0
@@ -540,13 +627,15 @@ def dflash_generate_stream(
     verify_mode: str,
     verify_chunk_size: int,
     profile: bool = False,
+    shaping: LogitsShaping | None = None,
 ) -> Iterator[DFlashRuntimeEvent]:
     """The DFlash decode loop (runtime.py:360-555): prefill the prompt, then
     repeatedly draft a block [last token, drafts...] from the target hidden
     states, verify it, keep the accepted prefix plus the posterior's bonus
     token, and stop at max_new_tokens or a stop token.  Yields the new tokens
     after the prefill and after every block, then a final event with the
-    metrics."""
+    metrics.  shaping: every token is taken from the logits that it processes; the
+    drafts are proposed without it."""
     if verify_mode not in VERIFY_MODES:
         raise ValueError(f"unknown verify_mode {verify_mode!r}; one of {VERIFY_MODES}")
     prompt = torch.as_tensor(prompt_tokens).reshape(-1)
@@ -569,7 +658,14 @@ def dflash_generate_stream(
     # 4096-token prompt at the c4 shape), which nothing reads.
     logits, target_hidden = target.forward_accept_all_block(
         prompt.to(device=dev, dtype=torch.int32)[None], target_cache, layer_ids)
-    first_token = _posterior(logits[:, -1:, :], temperature)[0]
+    if shaping is not None:
+        if not shaping.active:
+            shaping = None
+        else:
+            shaping.begin(prompt.tolist())
+    first_token = _posterior(logits[:, -1:, :], temperature, shaping)[0]
+    if shaping is not None:
+        shaping.commit([first_token])
     prefill_time = time.perf_counter() - sync_start
 
     output_tokens = prompt.tolist() + [first_token]
@@ -598,23 +694,24 @@ def dflash_generate_stream(
         verify_start = profile_start(profile_times)
         if verify_mode == "stream":
             accepted_inputs, posterior_token, verifier_hidden = verify_block_stream(
-                target, target_cache, block_tokens, temperature, layer_ids)
+                target, target_cache, block_tokens, temperature, layer_ids, shaping)
         elif verify_mode == "chunked":
             accepted_inputs, posterior_token, verifier_hidden = verify_block_chunked(
                 target, target_cache, block_tokens, block_size, temperature, layer_ids,
-                verify_chunk_size)
+                verify_chunk_size, shaping)
         elif verify_mode == "parallel-lazy-logits":
             accepted_inputs, posterior_token, verifier_hidden = verify_block_parallel_lazy_logits(
                 target, target_cache, block_tokens, block_size, temperature, layer_ids,
-                verify_chunk_size, profile=profile_times)
+                verify_chunk_size, profile=profile_times, shaping=shaping)
         elif verify_mode == "parallel-greedy-argmax":
             accepted_inputs, posterior_token, verifier_hidden = \
                 verify_block_parallel_greedy_argmax(target, target_cache, block_tokens, block_size,
-                                                    temperature, layer_ids, profile=profile_times)
+                                                    temperature, layer_ids, profile=profile_times,
+                                                    shaping=shaping)
         else:
             accepted_inputs, posterior_token, verifier_hidden = verify_block_parallel_replay(
                 target, target_cache, block_tokens, block_size, temperature, layer_ids,
-                profile=profile_times)
+                profile=profile_times, shaping=shaping)
         acceptance_lengths.append(accepted_inputs)
         target_hidden = verifier_hidden[:, :accepted_inputs, :]
         add_profile_elapsed(profile_times, "verify_time_s", verify_start)
@@ -623,6 +720,8 @@ def dflash_generate_stream(
         output_tokens = output_tokens[:start]
         output_tokens.extend(block_tokens[:accepted_inputs])
         output_tokens.append(posterior_token)
+        if shaping is not None:
+            shaping.commit(output_tokens[start + 1:])
         start += accepted_inputs
         add_profile_elapsed(profile_times, "bookkeeping_time_s", bookkeeping_start)
 
@@ -683,6 +782,7 @@ def dflash_generate(
     verify_mode: str,
     verify_chunk_size: int,
     profile: bool = False,
+    shaping: LogitsShaping | None = None,
 ) -> tuple[list[int], dict[str, Any]]:
     """runtime.py:558-589: run the stream to the end; (output_tokens, metrics)."""
     final_event: DFlashRuntimeEvent | None = None
@@ -690,7 +790,7 @@ def dflash_generate(
         target=target, draft=draft, prompt_tokens=prompt_tokens, max_new_tokens=max_new_tokens,
         temperature=temperature, stop_token_ids=stop_token_ids, layer_ids=layer_ids,
         speculative_tokens=speculative_tokens, verify_mode=verify_mode,
-        verify_chunk_size=verify_chunk_size, profile=profile,
+        verify_chunk_size=verify_chunk_size, profile=profile, shaping=shaping,
     ):
         if event.finished:
             final_event = event

@@ -48,6 +48,7 @@ from . import _lib
 from .adapters import make_rollback_record
 from .cache import ArraysCache, KVCache
 from .hybrid_model import HybridConfig, HybridVerifyRunner, HybridWeights
+from .int8 import linear_i8
 from .kv8 import QuantizedKVCache, kv_read_q8, kv_rewind_q8
 from .prefill import HybridPrefill
 
@@ -142,12 +143,15 @@ class HybridTargetModel:
     def __init__(self, cfg: HybridConfig, weights: HybridWeights, device: torch.device,
                  max_seq_len: int = 4096, block_size: int = 16, weight_layout: str = "tiled",
                  eos_token_ids: set[int] | None = None, prompt_pass: str = "prefill",
-                 prefill_rows: int = 8192, kv_dtype: torch.dtype = torch.bfloat16):
+                 prefill_rows: int = 8192, kv_dtype: torch.dtype = torch.bfloat16,
+                 weight_dtype: torch.dtype = torch.bfloat16):
         """prompt_pass: "prefill" runs inputs longer than block_size in one
         pass (prefill.HybridPrefill, up to prefill_rows rows per pass);
         "blocks" runs them through the verify runner block_size tokens at a
         time.  kv_dtype: torch.int8 or torch.float8_e4m3fn hold the attention
-        layers' caches in 8 bits (kv8.QuantizedKVCache)."""
+        layers' caches in 8 bits (kv8.QuantizedKVCache).  weight_dtype: torch.int8
+        holds the projections and the LM head in 8-bit integers (int8.Int8Weight)
+        in the verify step and the prompt pass alike; logits are then fp32."""
         if prompt_pass not in ("prefill", "blocks"):
             raise ValueError(f"prompt_pass must be 'prefill' or 'blocks', got {prompt_pass!r}")
         self.cfg, self.weights, self.device = cfg, weights, torch.device(device)
@@ -157,6 +161,7 @@ class HybridTargetModel:
         self.prompt_pass = prompt_pass
         self.prefill_rows = int(prefill_rows)
         self.kv_dtype = kv_dtype
+        self.weight_dtype = weight_dtype
         self.eos_token_ids = set(eos_token_ids or ())
         self._smax = -(-(self.max_seq_len + self.block_size) // 64) * 64
 
@@ -167,7 +172,8 @@ class HybridTargetModel:
         runner."""
         cfg = self.cfg
         run = HybridVerifyRunner(cfg, self.weights, 1, self.block_size, self._smax, self.device,
-                                 weight_layout=self.weight_layout, kv_dtype=self.kv_dtype)
+                                 weight_layout=self.weight_layout, kv_dtype=self.kv_dtype,
+                                 weight_dtype=self.weight_dtype)
         run.snapshot_conv()
         cache = HybridCache()
         cache.runner = run
@@ -400,7 +406,11 @@ class HybridTargetModel:
         """lm_head(hidden) (custom_qwen35_model.py:1090-1097): bf16 logits
         [..., V] from this package's GEMMs: the prompt-sized GEMM over the
         fragment-tiled head for more than 64 rows, else the verify-sized
-        GEMM, 64 rows a launch."""
+        GEMM, 64 rows a launch.  fp32 logits of an 8-bit head."""
+        if self.weight_dtype is torch.int8:
+            if self.weights.lm_head_i8 is None:
+                self.weights.int8_weights(self.cfg)
+            return linear_i8(hidden.to(torch.bfloat16), self.weights.lm_head_i8, out_dtype=torch.float32)
         H, V = self.cfg.hidden_size, self.cfg.vocab_size
         lead = hidden.shape[:-1]
         x = hidden.reshape(-1, H).to(torch.bfloat16)
@@ -427,7 +437,9 @@ class HybridTargetModel:
     def lm_head_argmax(self, hidden: torch.Tensor) -> torch.Tensor:
         """The lm_head_argmax hook (adapters.py:267-271) as the fused LM-head
         greedy kernel: int32 argmax ids [..., N], no logits."""
-        from .runtime import lm_head_argmax
+        from .runtime import lm_head_argmax, sample_tokens
 
+        if self.weight_dtype is torch.int8:
+            return sample_tokens(self.lm_head_logits(hidden), 0.0)
         tiled = self.weights.lm_head_tiled if self.weight_layout == "tiled" else None
         return lm_head_argmax(hidden, self.weights.lm_head, weight_tiled=tiled)
