@@ -125,7 +125,10 @@ __global__ __launch_bounds__(256) void pack_kernel(const int8_t* codes, int64_t 
   const bool live = j < (gated ? half : N);
   const int k0 = 64 * ks + 16 * (lane >> 4);
   u32x4 v{0, 0, 0, 0};
-  if (live)
+  typedef u32x4 u32x4_e1 __attribute__((aligned(1)));
+  if (live && k0 + 16 <= K)
+    v = *reinterpret_cast<const u32x4_e1*>(codes + n * rs + k0);
+  else if (live)
     for (int e = 0; e < 16; ++e)
       if (k0 + e < K) v[e >> 2] |= (uint32_t)(uint8_t)codes[n * rs + k0 + e] << (8 * (e & 3));
   packed[((int64_t)ks * tiles + tile) * 64 + lane] = v;
@@ -284,7 +287,7 @@ PlanI8 plan_i8(int M, int tiles, int k_steps) {
 }
 
 bool bad_weight(int N, int K, int gated) {
-  return N <= 0 || K <= 0 || K > DFLASH_I8_MAX_K || N > INT32_MAX - 64 || (gated && N % 2);
+  return N <= 0 || K <= 0 || K > DFLASH_I8_MAX_K || N > DFLASH_I8_MAX_N || (gated && N % 2);
 }
 
 }  // namespace

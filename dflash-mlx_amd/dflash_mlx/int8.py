@@ -191,7 +191,8 @@ def matmul_i8(codes: torch.Tensor, scale: torch.Tensor, weight: Int8Weight, *, o
     M = rows.shape[0]
     # rows are read 16 bytes at a time, up to K rounded up to 16
     fits = rows.storage_offset() + (M - 1) * rows.stride(0) + Kp <= rows.untyped_storage().nbytes()
-    if not fits or rows.data_ptr() % 16 or M > 1 and (rows.stride(0) % 16 or rows.stride(0) < Kp):
+    s = rows.stride(0)
+    if not fits or rows.data_ptr() % 16 or M > 1 and (s % 16 or not Kp <= s <= 1 << 23):
         rows = torch.nn.functional.pad(rows, (0, Kp - K)) if Kp > K else rows.clone(memory_format=torch.contiguous_format)
     scale = scale.contiguous()
     n = _workspace_bytes("dflash_gemm_i8_workspace_bytes", M, weight)

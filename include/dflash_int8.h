@@ -34,9 +34,11 @@ extern "C" {
 
 /* Largest K: |sum| < 2^31. */
 #define DFLASH_I8_MAX_K 131072
+/* Largest N: offsets of channel scales fit 32 bits. */
+#define DFLASH_I8_MAX_N 268435456
 
 /* Bytes of a packed weight's codes, and the count of its scales; 0: a size is out of
- * range (N, K >= 1, K <= DFLASH_I8_MAX_K, N even if gated). */
+ * range (1 <= N <= DFLASH_I8_MAX_N, 1 <= K <= DFLASH_I8_MAX_K, N even if gated). */
 size_t dflash_weight_i8_bytes(int N, int K, int gated);
 size_t dflash_weight_i8_scales(int N, int gated);
 
@@ -51,8 +53,9 @@ int dflash_quantize_rows_i8(const void* x, int x_dtype, int64_t x_row_stride, vo
                             int64_t codes_row_stride, float* scale, int M, int K, void* stream);
 
 /* The product of codes x [M, K] (16-byte aligned, rows x_row_stride bytes apart, a multiple
- * of 16; rows are read up to K rounded up to 16, whatever is there) with a packed
- * weight.  out: bf16, fp16 or fp32, out_row_stride elements apart, at least N (gated: N / 2).
+ * of 16 and at most 2^23; rows are read up to K rounded up to 16, whatever is there) with a packed
+ * weight.  out: bf16, fp16 or fp32, out_row_stride elements apart, at least N
+ * (gated: N / 2) and at most 2^26.
  * workspace: dflash_gemm_i8_workspace_bytes(M, N, K, gated) bytes (for the current device; may be
  * 0), 16-byte aligned. */
 size_t dflash_gemm_i8_workspace_bytes(int M, int N, int K, int gated);

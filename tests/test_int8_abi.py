@@ -49,7 +49,7 @@ def test_sizes_of_packed_weights(lib):
     assert lib.dflash_weight_i8_bytes(33, 129, 0) == 3 * 4 * 1024
     assert lib.dflash_weight_i8_bytes(34, 128, 1) == 2 * 2 * 2 * 1024
     assert lib.dflash_weight_i8_scales(33, 0) == 48 and lib.dflash_weight_i8_scales(34, 1) == 64
-    for N, K, gated in ((0, 1, 0), (1, 0, 0), (1, 131073, 0), (3, 64, 1), (-2, 64, 1)):
+    for N, K, gated in ((0, 1, 0), (1, 0, 0), (1, 131073, 0), (3, 64, 1), (-2, 64, 1), (2 ** 28 + 1, 1, 0)):
         assert lib.dflash_weight_i8_bytes(N, K, gated) == 0
     assert lib.dflash_weight_i8_scales(3, 1) == 0
 
@@ -80,7 +80,7 @@ def test_rows_that_are_refused(lib):
 
 
 def test_products_that_are_refused(lib):
-    for kw in (dict(M=-1), dict(xs=192), dict(os=63)):
+    for kw in (dict(M=-1), dict(xs=192), dict(os=63), dict(xs=2 ** 23 + 16), dict(os=2 ** 26 + 1)):
         assert _gemm(lib, **kw) == SHAPE
     for name in ("x", "sx", "w", "sw", "out"):
         assert _gemm(lib, **{name: None}) == NULL
