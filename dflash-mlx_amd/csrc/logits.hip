@@ -161,7 +161,7 @@ constexpr int kSlice = 8 * kLThreads * kTurns<T>;
 // listed and shared out over all lanes.  32 x 16 rows of 151936 in bf16 under masks after
 // 4000 tokens (167 MB), us, with the join of the keys: 112 as met; 67 listed from the bits
 // after the stream, whose logits then come a second time; 64 listed turn by turn, 100
-// instructions a turn of any wave that meets one; 44 so (masks alone 40).
+// instructions a turn of any wave that meets one; 61 so (masks alone 39).
 template <typename T, bool WRITE, bool INPLACE>
 __global__ __launch_bounds__(kLThreads) void process_kernel(const ProcessParams p) {
   constexpr int U = kTurns<T>;
