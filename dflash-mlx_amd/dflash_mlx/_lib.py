@@ -138,6 +138,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dflash_quantize_rows_i8": (_I, [_VP, _I, _I64, _VP, _I64, _VP, _I, _I, _VP]),
     "dflash_gemm_i8_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "dflash_gemm_i8": (_I, [_VP, _I64, _VP, _VP, _VP, _VP, _I, _I64, _I, _I, _I, _I, _VP, _SZ, _VP]),
+    "dflash_add_rmsnorm_i8": (
+        _I, [_VP, _VP, _VP, _VP, _VP, _I64, _VP, _I64, _VP, _I, _I, ctypes.c_float, _VP]),
     "dflash_linear_i8_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "dflash_linear_i8": (
         _I, [_VP, _I, _I64, _VP, _VP, _VP, _I, _I64, _I, _I, _I, _I, _VP, _SZ, _VP]),

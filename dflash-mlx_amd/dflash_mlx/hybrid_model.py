@@ -383,6 +383,10 @@ class HybridVerifyRunner:
                      for w in weights + [self.w.lm_head_i8] for m in range(1, M + 1))
             self.i8_ws = torch.empty(ws, dtype=torch.uint8, device=self.device)
             self.part = torch.empty(1, dtype=torch.float32, device=self.device)
+            # the norms inside the layers leave their rows quantised
+            self.norm_codes = H % 16 == 0 and H <= 32768
+            self.i8_codes = torch.empty(M, H, dtype=torch.int8, device=self.device)
+            self.i8_scale = torch.empty(M, dtype=torch.float32, device=self.device)
             torch.cuda.synchronize(self.device)
             return
         self.plan = self.TILED_PLAN if self.tiled else self.GEMM_PLAN
@@ -457,7 +461,13 @@ class HybridVerifyRunner:
 
     def _gemm_op(self, lw, name, x, out_ptr, out_stride, M):
         if self.int8:
-            return self._linear_i8_op(lw[name + "_i8"], x, out_ptr, _lib.DFLASH_DTYPE_BF16, out_stride, M)
+            weight = lw[name + "_i8"]
+            if x is self.i8_codes:
+                return ("dflash_gemm_i8",
+                        (x.data_ptr(), x.stride(0), self.i8_scale.data_ptr(), weight.codes.data_ptr(),
+                         weight.scales.data_ptr(), out_ptr, _lib.DFLASH_DTYPE_BF16, out_stride, M, weight.N, weight.K,
+                         int(weight.gated), self.i8_ws.data_ptr(), self.i8_ws.numel()))
+            return self._linear_i8_op(weight, x, out_ptr, _lib.DFLASH_DTYPE_BF16, out_stride, M)
         n, k = self._dims()[name]
         ns, rpw, kw = self.plan[name]
         if self.tiled and name + "_tiled" in lw:
@@ -502,11 +512,16 @@ class HybridVerifyRunner:
         return (self.h.data_ptr(), self.h.stride(0), w_norm.data_ptr(), self.row_sumsq.data_ptr(),
                 H // 16, float(self.cfg.rms_norm_eps), None)
 
-    def _residual_op(self, name, w_norm, M, capture):
+    def _residual_op(self, name, w_norm, M, capture, codes=False):
         """h += the branch projection `name` just produced; xn = norm(h);
         capture = (pointer, row stride) also receives h."""
         H, eps = self.cfg.hidden_size, float(self.cfg.rms_norm_eps)
         h, xn, ns = self.h.data_ptr(), self.xn.data_ptr(), self.splits[name]
+        if codes:  # xn as its codes and scales instead
+            cap, cap_stride = capture if capture is not None else (None, 0)
+            return ("dflash_add_rmsnorm_i8",
+                    (h, self.r.data_ptr(), w_norm.data_ptr(), h, cap, cap_stride, self.i8_codes.data_ptr(), H,
+                     self.i8_scale.data_ptr(), M, H, eps))
         if capture is not None:
             rp = self.part.data_ptr() if ns else None
             r = None if ns else self.r.data_ptr()
@@ -552,11 +567,13 @@ class HybridVerifyRunner:
                      self.w.layers[0]["ln_in"].data_ptr(), self.h.data_ptr(), self.xn.data_ptr(),
                      M, H, eps)))
         L = cfg.num_hidden_layers
+        codes = self.int8 and self.norm_codes
         gi = ai = 0
         for i in range(L):
             lw = self.w.layers[i]
             if i > 0:
-                fwd.append(self._residual_op("w_down", lw["ln_in"], M, capture_of(i - 1)))
+                fwd.append(self._residual_op("w_down", lw["ln_in"], M, capture_of(i - 1), codes))
+            xn_in = self.i8_codes if codes and i > 0 else self.xn
             # the post-attention norm folds when this layer's output projection
             # and its gate|up GEMM both have tiled copies
             post = self.fuses_norms(T) and self._fusable(
@@ -564,7 +581,7 @@ class HybridVerifyRunner:
             if cfg.is_linear(i):
                 gw = lw["gdn"]
                 base = self.proj[gi].data_ptr()
-                fwd.append(self._gemm_op(lw, "w_in", self.xn, *dst("w_in", self.proj[gi]), M))
+                fwd.append(self._gemm_op(lw, "w_in", xn_in, *dst("w_in", self.proj[gi]), M))
                 conv = self.conv[gi].data_ptr()
                 a_ptr, b_ptr = base + 2 * (C + Hv * Dv + Hv), base + 2 * (C + Hv * Dv)
                 state, tape = self.state[gi].data_ptr(), self.tape[gi].data_ptr()
@@ -595,10 +612,10 @@ class HybridVerifyRunner:
                 else:
                     fwd.append(self._gemm_op(lw, "w_out", self.gnorm.view(-1, Hv * Dv),
                                              *dst("w_out", self.r), M))
-                    fwd.append(self._residual_op("w_out", lw["ln_post"], M, None))
+                    fwd.append(self._residual_op("w_out", lw["ln_post"], M, None, codes))
                 gi += 1
             else:
-                fwd.append(self._gemm_op(lw, "w_qkv", self.xn, *dst("w_qkv", self.aproj), M))
+                fwd.append(self._gemm_op(lw, "w_qkv", xn_in, *dst("w_qkv", self.aproj), M))
                 if self.splits["w_qkv"]:
                     fwd.append(("dflash_splitk_reduce", (pp, self.splits["w_qkv"], M, arows,
                                                          self.aproj.data_ptr(), arows)))
@@ -630,11 +647,11 @@ class HybridVerifyRunner:
                     fwd.append(self._residual_norm_op(lw, "w_o", self.attn_out, M, None))
                 else:
                     fwd.append(self._gemm_op(lw, "w_o", self.attn_out, *dst("w_o", self.r), M))
-                    fwd.append(self._residual_op("w_o", lw["ln_post"], M, None))
+                    fwd.append(self._residual_op("w_o", lw["ln_post"], M, None, codes))
                 ai += 1
             gu_key = "w_gu_pairs_tiled" if self.tiled and "w_gu_pairs_tiled" in lw else None
             if self.int8:
-                fwd.append(self._gemm_op(lw, "w_gu", self.xn, self.mlp_act.data_ptr(), I, M))
+                fwd.append(self._gemm_op(lw, "w_gu", self.i8_codes if codes else self.xn, self.mlp_act.data_ptr(), I, M))
             elif post:
                 fwd.append(("dflash_gemm_bf16_swiglu_tiled_normed",
                             self._norm_input(lw["ln_post"]) + (lw[gu_key].data_ptr(),

@@ -315,6 +315,7 @@ class HybridPrefill:
         self.chunk_ws = e(max(ws, 16), dt=torch.uint8)
         if self.run.int8:
             self.part = e(4, dt=f32)
+            self.i8_codes, self.i8_scale = e(P, H, dt=torch.int8), e(P, dt=f32)
             self.rows_cap = P
             return
         shapes = {(name in RESIDUAL, n, wt.numel() // n) for d in self.w for name, (wt, n) in d.items()}
@@ -383,6 +384,7 @@ class HybridPrefill:
         direct = _has_form(norm_out, self.xn[:P]) and norm_out.data_ptr() % 16 == 0
         last = norm_out if direct else self.xn
         layers = run.w.layers
+        self.coded = False  # the rows of the last norm: bf16, or codes
         call("dflash_embed_rmsnorm", run.w.embed.data_ptr(), tokens.data_ptr(), cfg.vocab_size,
              layers[0]["ln_in"].data_ptr(), h, xn, P, H, eps, stream)
         cap_ids = {layer: j for j, layer in enumerate(run.capture_layers)}
@@ -457,7 +459,7 @@ class HybridPrefill:
         rounds in one launch and the last n-tiles' rows split-K (tail_split)."""
         wt, n = weight
         if isinstance(wt, Int8Weight):
-            self._linear_i8(wt, x_ptr, K, P, out_ptr, out_stride, stream)
+            self._linear_i8(wt, x_ptr, K, P, out_ptr, out_stride, stream, self.coded)
             return
         if P <= block_rows(False, n, K, self.cus):
             _lib.call("dflash_gemm_bf16_tiled_block", x_ptr, K, wt.data_ptr(), out_ptr, out_stride,
@@ -516,11 +518,17 @@ class HybridPrefill:
                       self.cfg.hidden_size, P, n, K, stream)
         return used
 
-    def _linear_i8(self, w, x_ptr, K, P, out_ptr, out_stride, stream) -> None:
+    def _linear_i8(self, w, x_ptr, K, P, out_ptr, out_stride, stream, coded=False) -> None:
+        """coded: of the codes that the norm before it left."""
         bf = _lib.DFLASH_DTYPE_BF16
         need = self._lib.dflash_linear_i8_workspace_bytes(P, w.N, w.K, int(w.gated))
         if self.i8_ws.numel() < need:
             self.i8_ws = torch.empty(need, dtype=torch.uint8, device=self.run.device)
+        if coded:
+            _lib.call("dflash_gemm_i8", self.i8_codes.data_ptr(), K, self.i8_scale.data_ptr(), w.codes.data_ptr(),
+                      w.scales.data_ptr(), out_ptr, bf, out_stride, P, w.N, K, int(w.gated), self.i8_ws.data_ptr(),
+                      self.i8_ws.numel(), stream)
+            return
         _lib.call("dflash_linear_i8", x_ptr, bf, K, w.codes.data_ptr(), w.scales.data_ptr(), out_ptr, bf, out_stride, P,
                   w.N, K, int(w.gated), self.i8_ws.data_ptr(), self.i8_ws.numel(), stream)
 
@@ -544,6 +552,13 @@ class HybridPrefill:
         out) = RMSNorm(h) * weight; capture = (pointer, row stride) also receives h."""
         H, eps = self.cfg.hidden_size, float(self.cfg.rms_norm_eps)
         h, xn = self.h.data_ptr(), out or self.xn.data_ptr()
+        if self.run.int8 and self.run.norm_codes and out is None:  # xn as its codes and scales instead
+            cap, cap_stride = capture if capture is not None else (None, 0)
+            _lib.call("dflash_add_rmsnorm_i8", h, self.r.data_ptr(), weight.data_ptr(), h, cap, cap_stride,
+                      self.i8_codes.data_ptr(), H, self.i8_scale.data_ptr(), P, H, eps, stream)
+            self.coded = True
+            return
+        self.coded = False
         r = None if splits else self.r.data_ptr()
         part = self.part.data_ptr() if splits else None
         if capture is not None:

@@ -63,6 +63,16 @@ int dflash_gemm_i8(const void* x, int64_t x_row_stride, const float* x_scale, co
                    const float* packed_scale, void* out, int out_dtype, int64_t out_row_stride, int M, int N,
                    int K, int gated, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The residual add and RMSNorm before a projection, with the rows quantised for it
+ * (custom_qwen35_model.py:824-827, 841-845): h_out = bf16(h + r), row by row x = bf16(h_out *
+ * rsqrt(mean(h_out^2) + eps) * weight), codes and scales of x as dflash_quantize_rows_i8 gives
+ * them.  All of [M, H] bf16, contiguous; h_out may be h; r null: no add.  capture: null, or h_out
+ * again, capture_stride elements a row (a multiple of 8).  H a multiple of 16, at most 32768;
+ * every pointer 16-byte aligned. */
+int dflash_add_rmsnorm_i8(const void* h, const void* r, const void* weight, void* h_out, void* capture,
+                          int64_t capture_stride, void* codes, int64_t codes_row_stride, float* scale, int M,
+                          int H, float eps, void* stream);
+
 /* Both in one call: rows x (bf16 or fp16) quantised and multiplied, the same bits.  workspace:
  * dflash_linear_i8_workspace_bytes(M, N, K, gated) bytes (for the current device), 16-byte
  * aligned. */

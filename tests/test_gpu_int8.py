@@ -238,6 +238,43 @@ def test_captured_and_repeated(device, M):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("M,H", [(1, 16), (3, 256), (16, 2560), (5, 8192), (2, 20480), (600, 512), (513, 2576)])
+@pytest.mark.parametrize("add,capture", [(True, True), (False, False)])
+def test_add_rmsnorm(device, M, H, add, capture):
+    """h_out exactly; the codes and scales are those of a bf16 rounding of the norm, whose fp32
+    is off by at most 2^-19 of itself (sums of 20 + 10 + 16 terms at 2^-24 each, halved by the
+    root, and four steps more).  So a value within 2^-19 of a border, about one of 2^10, may
+    round the other way, by a whole step of 2^-7 of itself: its code moves by 127 * 2^-7 < 1,
+    and where the row's largest does, which the scale shows, by as much again."""
+    from dflash_mlx import _lib
+
+    g = torch.Generator().manual_seed(M + H)
+    h, r = (torch.randn(M, H, generator=g).bfloat16() for _ in range(2))
+    w = (1 + 0.1 * torch.randn(H, generator=g)).bfloat16()
+    hd, rd, wd = (t.to(device) for t in (h, r, w))
+    out, cap = torch.empty_like(hd), torch.full((M, 2 * H), 7.0, dtype=torch.bfloat16, device=device)
+    codes = torch.full((M, H + 16), 99, dtype=torch.int8, device=device)
+    scale = torch.empty(M, device=device)
+    _lib.call("dflash_add_rmsnorm_i8", hd.data_ptr(), rd.data_ptr() if add else None, wd.data_ptr(), out.data_ptr(),
+              cap.data_ptr() if capture else None, 2 * H, codes.data_ptr(), H + 16, scale.data_ptr(), M, H, 1e-6,
+              _lib.stream_handle(device))
+    want_h = (h.float() + r.float()).bfloat16() if add else h
+    assert torch.equal(out.cpu(), want_h)
+    assert (codes[:, H:] == 99).all()
+    if capture:
+        assert torch.equal(cap[:, :H].cpu(), want_h) and (cap[:, H:] == 7).all()
+    d = want_h.double()
+    x = (d / (d.square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()).bfloat16()
+    want, want_s = quantised(x)
+    moved = (codes[:, :H].cpu().long() - want).abs()
+    scale = scale.cpu().double()
+    assert moved.max() <= 2
+    assert ((scale - want_s).abs() <= 2.0 ** -7 * (1 + 2.0 ** -10) * want_s).all()
+    same = (scale - want_s).abs() <= 2.0 ** -22 * want_s
+    assert not same.any() or moved[same].max() <= 1
+    assert same.sum() >= M // 2 and (moved[same] > 0).sum() <= 1 + 0.004 * moved[same].numel()
+
+
 def test_rows_do_not_depend_on_their_number(device):
     """A row's output is the same bits whatever rows are beside it."""
     K, N = 640, 1100

@@ -39,7 +39,7 @@ def test_every_declared_entry_point_is_exported_and_bound(lib):
     names = set(re.findall(r"\b(dflash_[a-z0-9_]+)\s*\(", text))
     assert names == {"dflash_weight_i8_bytes", "dflash_weight_i8_scales", "dflash_weight_pack_i8",
                      "dflash_quantize_rows_i8", "dflash_gemm_i8", "dflash_gemm_i8_workspace_bytes",
-                     "dflash_linear_i8", "dflash_linear_i8_workspace_bytes"}
+                     "dflash_linear_i8", "dflash_linear_i8_workspace_bytes", "dflash_add_rmsnorm_i8"}
     for name in names:
         assert hasattr(lib, name) and name in _lib.SIGNATURES
 
@@ -107,6 +107,22 @@ def test_linears_that_are_refused(lib):
     assert _linear(lib, M=0, x=None) == 0
     assert lib.dflash_linear_i8_workspace_bytes(4, 64, 200, 0) == 4 * 208 + 16
     assert lib.dflash_linear_i8_workspace_bytes(0, 64, 200, 0) == 0
+
+
+def _norm(lib, h=P, r=P, w=P, out=P, cap=P, cap_stride=256, codes=P, cs=256, scale=P, M=4, H=256):
+    return lib.dflash_add_rmsnorm_i8(h, r, w, out, cap, cap_stride, codes, cs, scale, M, H, 1e-6, None)
+
+
+def test_norms_that_are_refused(lib):
+    for kw in (dict(M=-1), dict(H=0), dict(H=8), dict(H=32784), dict(cs=240), dict(cap_stride=248)):
+        assert _norm(lib, **kw) == SHAPE
+    for name in ("h", "w", "out", "codes", "scale"):
+        assert _norm(lib, **{name: None}) == NULL
+    for name in ("h", "r", "w", "out", "cap", "codes"):
+        assert _norm(lib, **{name: P + 8}) == ALIGN
+    for kw in (dict(cs=264), dict(cap_stride=260), dict(scale=P + 2)):
+        assert _norm(lib, **kw) == ALIGN
+    assert _norm(lib, M=0, h=None) == 0
 
 
 def test_python_refuses_host_tensors():
