@@ -29,6 +29,7 @@ here are far below 2**31).
 """
 from __future__ import annotations
 
+import copy
 import time
 from collections.abc import Callable, Iterator
 from dataclasses import dataclass
@@ -320,7 +321,8 @@ class LogitsShaping:
     """What a generation asks of its logits: a LogitsState of one sequence that counts
     the prompt and every token taken, and a grammar.  token_mask(tokens) gives the
     bitmask (int32 [ceil(V / 32)], any device) of what may follow the tokens, prompt
-    included, or None for anything."""
+    included, or None for anything.  Any number of generations may use one at a time:
+    each counts in its own (begin)."""
 
     def __init__(self, repetition_penalty: float = 1.0, presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
                  logit_bias: dict[int, float] | None = None,
@@ -340,9 +342,12 @@ class LogitsShaping:
     def active(self) -> bool:
         return self.penalties != (1.0, 0.0, 0.0) or bool(self.logit_bias) or self.token_mask is not None
 
-    def begin(self, prompt: list[int]) -> None:
-        self.state, self.tokens, self._waiting = None, [], []
-        self.commit(prompt, prompt=True)
+    def begin(self, prompt: list[int]) -> LogitsShaping:
+        """One generation's own, of the same wishes."""
+        run = copy.copy(self)
+        run.state, run.tokens, run._waiting = None, [], []
+        run.commit(prompt, prompt=True)
+        return run
 
     def commit(self, tokens: list[int], prompt: bool = False) -> None:
         """These tokens are taken."""
@@ -377,6 +382,8 @@ class LogitsShaping:
         for i in range(n):
             words = self.token_mask(self.tokens + list(before) + list(drafts[:i]))
             if words is not None:
+                if words.dtype is not torch.int32 or words.shape != mask.shape[2:]:
+                    raise ValueError(f"token_mask must give int32 [{mask.shape[2]}], got {words.dtype} {tuple(words.shape)}")
                 mask[0, i] = words
         return state, mask.to(dev)
 
@@ -662,7 +669,7 @@ def dflash_generate_stream(
         if not shaping.active:
             shaping = None
         else:
-            shaping.begin(prompt.tolist())
+            shaping = shaping.begin(prompt.tolist())
     first_token = _posterior(logits[:, -1:, :], temperature, shaping)[0]
     if shaping is not None:
         shaping.commit([first_token])

@@ -104,17 +104,20 @@ CASES = {"penalties": ((1.4, 0.6, 0.3), {}, None), "biases": ((1.0, 0.0, 0.0), B
 
 @pytest.mark.parametrize("mode", rt.VERIFY_MODES)
 @pytest.mark.parametrize("case", CASES)
-def test_every_mode_decodes_as_one_by_one(device, case, mode):
+def test_every_mode_decodes_as_one_by_one(device, case, mode, monkeypatch):
     penalties, bias, grammar = CASES[case]
     want = _reference(penalties, bias, grammar, N_NEW + 2 * BS)
     plain = _reference((1.0, 0.0, 0.0), {}, None, N_NEW)
     assert want[:N_NEW] != plain
+    runs, begin = [], LogitsShaping.begin
+    monkeypatch.setattr(LogitsShaping, "begin", lambda s, p: runs.append(begin(s, p)) or runs[-1])
     shaping = LogitsShaping(*penalties, logit_bias=bias, token_mask=grammar)
     drafter = Drafter(PROMPT + want, [3, None, 1, 5, 7])
     res = DFlashGenerator(Target(device), drafter).generate_from_tokens(
         torch.tensor(PROMPT), max_new_tokens=N_NEW, verify_mode=mode, verify_chunk_size=3, shaping=shaping)
     assert res.generated_tokens == want[:N_NEW]
     assert max(res.metrics["acceptance_lengths"]) == BS  # right drafts pass
+    shaping, = runs
     made, prompt = counts_of([PROMPT], [shaping.tokens[len(PROMPT):]], V)
     if shaping._waiting == []:
         counts = shaping.state.counts.cpu()[0].long()
@@ -137,6 +140,31 @@ def test_a_shaping_is_used_again_and_streams(device):
         events = list(DFlashGenerator(Target(device), Drafter(PROMPT + want, [4, None])).stream_from_tokens(
             torch.tensor(PROMPT), max_new_tokens=N_NEW, shaping=shaping))
         assert [t for e in events for t in e.token_ids] == want[:N_NEW]
+
+
+def test_two_generations_at_once(device):
+    want = _reference((1.4, 0.6, 0.3), {}, None, N_NEW + 2 * BS)
+    shaping = LogitsShaping(1.4, 0.6, 0.3)
+    streams = [DFlashGenerator(Target(device), Drafter(PROMPT + want, plan)).stream_from_tokens(
+        torch.tensor(PROMPT), max_new_tokens=N_NEW, shaping=shaping) for plan in ([4, None], [1, 6])]
+    got = [[], []]
+    live = [0, 1]
+    while live:  # an event of each in turn
+        for i in list(live):
+            event = next(streams[i], None)
+            if event is None:
+                live.remove(i)
+            else:
+                got[i] += event.token_ids
+    assert got == [want[:N_NEW]] * 2
+
+
+@pytest.mark.parametrize("bad", [torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int64),
+                                 torch.zeros(1, 2, dtype=torch.int32)])
+def test_a_grammar_of_another_form_is_refused(device, bad):
+    with pytest.raises(ValueError, match="token_mask"):
+        DFlashGenerator(Target(device), Drafter(PROMPT + [1] * 60, [None])).generate_from_tokens(
+            torch.tensor(PROMPT), max_new_tokens=4, shaping=LogitsShaping(token_mask=lambda t: bad))
 
 
 def test_sampling_keeps_to_the_grammar(device):
