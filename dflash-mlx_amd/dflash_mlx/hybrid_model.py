@@ -335,6 +335,8 @@ class HybridVerifyRunner:
         self.gemm_ws = z(int(lib.dflash_gemm_tail_workspace_bytes()), dt=torch.uint8)
         self.capture_layers: tuple[int, ...] = ()
         self.captured = None  # [B*T, len(capture_layers) * H] after set_capture
+        if logits_state is not None and logits_state.device != self.h.device:
+            raise ValueError(f"logits_state must be on {self.h.device}, got {logits_state}")
         # logits stored for the accept: where something changes them, or of the 8-bit head
         self.logits = (e(M, V, dt=f32 if self.int8 else bf)
                        if self.int8 or logits_state is not None or masked else None)

@@ -101,6 +101,24 @@ def _runner(weights, device, dtype, state, masked):
     return run
 
 
+def test_norms_that_leave_codes_and_norms_that_do_not(weights, device):
+    """Hidden sizes without whole 16s quantise in a launch of their own, as the codes' own
+    norm does: about one value in 2^10 lies near enough to a bf16 border that it rounds the
+    other way, by one code at most, where every code is off by 0.29 (rms) as it is.  So the
+    two differ by 2^-5 / 0.29, a ninth, of what either is off (0.15 at most, see above)."""
+    out = []
+    for codes in (True, False):
+        run = _runner(weights, device, torch.int8, None, False)
+        assert run.norm_codes
+        run.norm_codes = codes
+        run.tokens.copy_(_tokens(B, T, seed=4).int())
+        run.step()
+        out.append(run.xn.float())
+    err = (out[0] - out[1]).norm() / out[1].norm()
+    print(f"[int8 model] norms with and without codes: {err:.2e}", flush=True)
+    assert torch.isfinite(out[0]).all() and err <= 0.15 / 9
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int8])
 @pytest.mark.parametrize("masked", [False, True])
 def test_steps_under_a_state(weights, device, dtype, masked):
@@ -161,3 +179,7 @@ def test_refusals(weights, device):
         HybridVerifyRunner(CFG, weights, 1, 4, 64, device, weight_dtype=torch.float16)
     with pytest.raises(ValueError, match="logits_state"):
         HybridVerifyRunner(CFG, weights, 2, 4, 64, device, logits_state=LogitsState.zeros(1, V, device))
+    away = LogitsState.zeros(1, V, device)
+    away.device = torch.device("cuda", 7)
+    with pytest.raises(ValueError, match="logits_state"):
+        HybridVerifyRunner(CFG, weights, 1, 4, 64, device, logits_state=away)
