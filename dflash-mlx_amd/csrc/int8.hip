@@ -206,9 +206,18 @@ __global__ __launch_bounds__(256) void pack_kernel(const int8_t* codes, int64_t 
 // rows; its KW waves share K, each with a stretch of its own: no barrier while they
 // stream, weights D k-steps ahead in registers, rows (which every workgroup reads) from
 // the L2.  Their sums meet in LDS, integers, so their order does not matter.
-template <typename T, bool GATED, int MT, int VT, int KW, int D>
+//
+// RAW (1 bf16, 2 fp16): a single row comes as it is, and every workgroup quantises it for
+// itself into LDS while its first weights are on their way: 0.2 to 1.5 us where a launch
+// before takes 2.6 (1 x 2560 x 9216 7.6 us in all, 18432 x 2560 gated 10.2; a verify step of
+// one token 1.88 -> 1.78 ms).  Two rows take 2.1 to 2.8 so and four 2.3 to 4.7: no gain.
+template <typename T, bool GATED, int MT, int VT, int KW, int D, int RAW>
 __global__ __launch_bounds__(64 * KW) void stream_i8_kernel(const GemmI8 p) {
   __shared__ i32x4 sums[KW][VT * MT][64];
+  extern __shared__ __attribute__((aligned(16))) uint8_t codes_s[];
+  __shared__ uint32_t best_s[KW];
+  float raw_scale = 0.f;
+  static_assert(!RAW || MT == 1, "a single row");
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int t0 = VT * blockIdx.x;
@@ -217,24 +226,37 @@ __global__ __launch_bounds__(64 * KW) void stream_i8_kernel(const GemmI8 p) {
   const int last = (p.K - 1) >> 4;  // a row's last 16-byte piece; the weight is 0 behind K
   const u32x4* w[VT];
   const uint8_t* x[MT];
+  constexpr int kHeld = 3;
+  u32x4 held[kHeld] = {};
+  const int chunks = 2 * (last + 1);
+  if (RAW) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (const int c = threadIdx.x + i * 64 * KW; c < chunks) held[i] = load_row8(p.raw, c, p.K);
+  }
 #pragma unroll
   for (int v = 0; v < VT; ++v)
     w[v] = p.w + ((int64_t)k0 * p.tiles + min(t0 + v, p.tiles - 1)) * 64 + lane;
 #pragma unroll
-  for (int j = 0; j < MT; ++j) x[j] = p.x + (int64_t)min(16 * j + r16, p.M - 1) * p.xs;
+  for (int j = 0; j < MT; ++j)
+    x[j] = RAW ? codes_s : p.x + (int64_t)min(16 * j + r16, p.M - 1) * p.xs;
   struct Stage {
     i32x4 a[VT], b[MT];
   } ring[D];
-  auto load = [&](Stage& s, int i) __attribute__((always_inline)) {
-#pragma unroll
-    for (int v = 0; v < VT; ++v)
-      s.a[v] = __builtin_bit_cast(i32x4, __builtin_nontemporal_load(w[v] + (int64_t)i * p.tiles * 64));
+  auto load_rows = [&](Stage& s, int i) __attribute__((always_inline)) {
     const int piece = min(4 * (k0 + i) + g, last);
 #pragma unroll
     for (int j = 0; j < MT; ++j) s.b[j] = *reinterpret_cast<const i32x4*>(x[j] + 16 * piece);
   };
+  auto load = [&](Stage& s, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int v = 0; v < VT; ++v)
+      s.a[v] = __builtin_bit_cast(i32x4, __builtin_nontemporal_load(w[v] + (int64_t)i * p.tiles * 64));
+    if (!RAW) load_rows(s, i);
+  };
   i32x4 acc[VT][MT] = {};
-  auto multiply = [&](const Stage& s) __attribute__((always_inline)) {
+  auto multiply = [&](Stage& s, int i) __attribute__((always_inline)) {
+    if (RAW) load_rows(s, i);
 #pragma unroll
     for (int v = 0; v < VT; ++v)
 #pragma unroll
@@ -245,17 +267,40 @@ __global__ __launch_bounds__(64 * KW) void stream_i8_kernel(const GemmI8 p) {
   if (n > 0) {
 #pragma unroll
     for (int d = 0; d < D; ++d) load(ring[d], min(d, n - 1));
+  }
+  if (RAW) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) most = largest8(held[i], most);
+    for (int c = threadIdx.x + kHeld * 64 * KW; c < chunks; c += 64 * KW) most = largest8(load_row8(p.raw, c, p.K), most);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, off, 64));
+    if (lane == 0) best_s[wave] = most;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < KW; ++k) most = max(most, best_s[k]);
+    const RowScale r = row_scale<RAW == 1>(most);
+    raw_scale = r.scale;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (const int c = threadIdx.x + i * 64 * KW; c < chunks)
+        *reinterpret_cast<u32x2*>(codes_s + 8 * c) = codes8<RAW == 1>(held[i], r);
+    for (int c = threadIdx.x + kHeld * 64 * KW; c < chunks; c += 64 * KW)
+      *reinterpret_cast<u32x2*>(codes_s + 8 * c) = codes8<RAW == 1>(load_row8(p.raw, c, p.K), r);
+    __syncthreads();
+  }
+  if (n > 0) {
     int i = 0;
     for (; i + D <= n; i += D) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        multiply(ring[d]);
+        multiply(ring[d], i + d);
         load(ring[d], min(i + D + d, n - 1));
       }
     }
 #pragma unroll
     for (int d = 0; d < D; ++d)
-      if (i + d < n) multiply(ring[d]);
+      if (i + d < n) multiply(ring[d], i + d);
   }
   // Wave k adds up and stores the pairs (of channel tiles, by row tile) k, k + KW, ...
 #pragma unroll
@@ -275,7 +320,7 @@ __global__ __launch_bounds__(64 * KW) void stream_i8_kernel(const GemmI8 p) {
     if (t < p.tiles && m < p.M) {
       T* row = static_cast<T*>(p.out) + (int64_t)m * p.os;
       const f32x4 sa = tile_scales(p, t, g);
-      const float sx = p.sx[m];
+      const float sx = RAW ? raw_scale : p.sx[m];
       if (VT > 1) {
         store_pair<T, GATED>(p, t, g, row, 4 * g, a, b, sa, tile_scales(p, t + 1, g), sx);
       } else {
@@ -288,10 +333,10 @@ __global__ __launch_bounds__(64 * KW) void stream_i8_kernel(const GemmI8 p) {
   }
 }
 
-template <typename T, bool GATED, int MT, int VT, int KW, int D>
+template <typename T, bool GATED, int MT, int VT, int KW, int RAW>
 hipError_t launch_stream(const GemmI8& p, hipStream_t s) {
-  hipLaunchKernelGGL((stream_i8_kernel<T, GATED, MT, VT, KW, D>), dim3((unsigned)ceil_div(p.tiles, VT)), dim3(64 * KW),
-                     0, s, p);
+  hipLaunchKernelGGL((stream_i8_kernel<T, GATED, MT, VT, KW, 4, RAW>), dim3((unsigned)ceil_div(p.tiles, VT)),
+                     dim3(64 * KW), RAW ? 16 * (unsigned)ceil_div(p.K, 16) : 0, s, p);
   return hipGetLastError();
 }
 
@@ -299,12 +344,15 @@ hipError_t launch_stream(const GemmI8& p, hipStream_t s) {
 // launch's gap with it), 16 rows, one channel tile and 8 waves / two and 4 / four and 4:
 // 2560 x 9216 9.3 / 12.3 / 17.0, 2560 x 4096 6.1 / 7.0 / 9.3, 5120 x 2560 7.7 / 5.7 / 7.2,
 // 18432 x 2560 gated - / 13.2 / 13.4, 151936 x 2560 117 / 80 / 71.
-template <typename T, bool GATED, int MT>
+template <typename T, bool GATED, int MT, int RAW = 0>
 hipError_t launch_rows(const GemmI8& p, hipStream_t s) {
-  if (p.tiles <= 256) return launch_stream<T, GATED, MT, GATED ? 2 : 1, 8, 4>(p, s);
-  if (p.tiles <= 2048) return launch_stream<T, GATED, MT, 2, 4, 4>(p, s);
-  return launch_stream<T, GATED, MT, 4, 4, 4>(p, s);
+  if (p.tiles <= 256) return launch_stream<T, GATED, MT, GATED ? 2 : 1, 8, RAW>(p, s);
+  if (p.tiles <= 2048) return launch_stream<T, GATED, MT, 2, 4, RAW>(p, s);
+  return launch_stream<T, GATED, MT, 4, 4, RAW>(p, s);
 }
+
+// A row that the streaming workgroups quantise for themselves: their LDS holds its codes.
+constexpr int kRawK = 40960;
 
 template <typename T, bool GATED>
 hipError_t launch_gemm(const GemmI8& p, hipStream_t s) {
@@ -483,6 +531,24 @@ extern "C" int dflash_linear_i8(const void* x, int x_dtype, int64_t x_row_stride
       (uintptr_t)workspace % 16)
     return DFLASH_ERR_ALIGN;
   if (workspace_bytes < dflash_linear_i8_workspace_bytes(M, N, K, gated)) return DFLASH_ERR_WORKSPACE;
+  if (M == 1 && K <= kRawK) {
+    if (x == nullptr) return DFLASH_ERR_NULL;
+    if (x_dtype != DFLASH_DTYPE_BF16 && x_dtype != DFLASH_DTYPE_F16) return DFLASH_ERR_UNSUPPORTED;
+    if ((uintptr_t)x % 2) return DFLASH_ERR_ALIGN;
+    GemmI8 p{};
+    p.raw = static_cast<const uint16_t*>(x);
+    p.w = static_cast<const u32x4*>(packed_codes), p.sw = packed_scale;
+    p.out = out, p.os = out_row_stride, p.cols = cols;
+    p.M = M, p.K = K, p.k_steps = k_steps(K), p.tiles = channel_tiles(N, gated);
+    const bool bf = x_dtype == DFLASH_DTYPE_BF16;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto launch = [&](auto t) {
+      using T = decltype(t);
+      return gated ? (bf ? launch_rows<T, true, 1, 1>(p, s) : launch_rows<T, true, 1, 2>(p, s))
+                   : (bf ? launch_rows<T, false, 1, 1>(p, s) : launch_rows<T, false, 1, 2>(p, s));
+    };
+    return to_status(f32 ? launch(0.f) : out_dtype == DFLASH_DTYPE_BF16 ? launch(uint16_t{}) : launch(_Float16{}));
+  }
   char* ws = static_cast<char*>(workspace);
   const size_t cb = codes_bytes(M, K), sb = scales_bytes(M);
   float* scale = reinterpret_cast<float*>(ws + cb);

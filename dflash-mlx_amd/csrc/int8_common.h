@@ -40,6 +40,7 @@ struct GemmI8 {
   int K, k_steps, tiles;
   PlanI8 plan;
   void* workspace;  // where the splits' sums go
+  const uint16_t* raw;  // a single row that is not quantised yet (then not x and sx)
 };
 
 template <typename T>

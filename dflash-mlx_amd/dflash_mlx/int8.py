@@ -19,6 +19,7 @@ import torch
 from . import _lib
 from .gated_delta import _require_device
 from .kv8 import _call
+from .logits import _overlap
 
 MAX_K = 131072  # features: the sum of products of codes stays in 32 bits
 
@@ -161,6 +162,12 @@ def _output(out, out_dtype, lead, weight):
     return out, max(rows.stride(0), weight.cols)
 
 
+def _check_apart(out, name: str, x) -> None:
+    """Workgroups read x while others store."""
+    if out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and _overlap(out, x):
+        raise ValueError(f"out must lie apart from {name}")
+
+
 def _check_weight(weight, K: int, dev) -> None:
     if not isinstance(weight, Int8Weight):
         raise TypeError(f"weight must be an Int8Weight, got {type(weight).__name__}")
@@ -171,7 +178,7 @@ def _check_weight(weight, K: int, dev) -> None:
 def matmul_i8(codes: torch.Tensor, scale: torch.Tensor, weight: Int8Weight, *, out_dtype: torch.dtype = torch.bfloat16,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """(codes @ weight codes^T) * scale * weight scales, [..., N] (gated: silu(gate) * up,
-    [..., N / 2]) in out_dtype, or into out (whose type counts).
+    [..., N / 2]) in out_dtype, or into out (whose type counts, and which lies apart from codes).
 
     codes: int8 [..., K], scale: fp32 [...], as quantize_rows_i8 gives them."""
     _require_device("codes", codes)
@@ -184,9 +191,13 @@ def matmul_i8(codes: torch.Tensor, scale: torch.Tensor, weight: Int8Weight, *, o
     _require_device("scale", scale, dev)
     if scale.dtype is not torch.float32 or scale.shape != lead:
         raise ValueError(f"scale must be float32 {list(lead)}, got {scale.dtype} {list(scale.shape)}")
+    given = out is not None
     out, os = _output(out, out_dtype, lead, weight)
     if out.numel() == 0:
         return out
+    if given:
+        _check_apart(out, "codes", codes)
+        _check_apart(out, "scale", scale)
     rows, Kp = _rows_of(codes), -(-K // 16) * 16
     M = rows.shape[0]
     # rows are read 16 bytes at a time, up to K rounded up to 16
@@ -207,7 +218,7 @@ def linear_i8(x: torch.Tensor, weight: Int8Weight, *, out_dtype: torch.dtype | N
               out: torch.Tensor | None = None) -> torch.Tensor:
     """x @ weight^T with x's rows quantised on the way: matmul_i8(*quantize_rows_i8(x), weight).
 
-    x: bf16 or fp16 [..., K]; out_dtype: x's type by default."""
+    x: bf16 or fp16 [..., K]; out_dtype: x's type by default; out lies apart from x."""
     _require_device("x", x)
     if x.dtype not in _IN:
         raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
@@ -215,9 +226,12 @@ def linear_i8(x: torch.Tensor, weight: Int8Weight, *, out_dtype: torch.dtype | N
         raise ValueError("x must be [..., K]")
     lead, K, dev = x.shape[:-1], x.shape[-1], x.device
     _check_weight(weight, K, dev)
+    given = out is not None
     out, os = _output(out, x.dtype if out_dtype is None else out_dtype, lead, weight)
     if out.numel() == 0:
         return out
+    if given:
+        _check_apart(out, "x", x)
     rows = _rows_of(x)
     M = rows.shape[0]
     n = _workspace_bytes("dflash_linear_i8_workspace_bytes", M, weight)

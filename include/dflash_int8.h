@@ -75,7 +75,8 @@ int dflash_add_rmsnorm_i8(const void* h, const void* r, const void* weight, void
 
 /* Both in one call: rows x (bf16 or fp16) quantised and multiplied, the same bits.  workspace:
  * dflash_linear_i8_workspace_bytes(M, N, K, gated) bytes (for the current device), 16-byte
- * aligned. */
+ * aligned.  out lies apart from x (and from the codes, in the call above): a row may be read
+ * while outputs are stored. */
 size_t dflash_linear_i8_workspace_bytes(int M, int N, int K, int gated);
 int dflash_linear_i8(const void* x, int x_dtype, int64_t x_row_stride, const void* packed_codes,
                      const float* packed_scale, void* out, int out_dtype, int64_t out_row_stride, int M, int N,

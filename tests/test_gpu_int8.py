@@ -275,6 +275,44 @@ def test_add_rmsnorm(device, M, H, add, capture):
     assert same.sum() >= M // 2 and (moved[same] > 0).sum() <= 1 + 0.004 * moved[same].numel()
 
 
+@pytest.mark.parametrize("M", [1, 2, 3])
+@pytest.mark.parametrize("N,K,gated", [(40, 1, False), (2, 17, True), (5120, 2560, False), (5120, 2559, True), (4096, 9984, False),
+                                       (4100, 12300, False), (33024, 200, True), (48, 40960, False), (32784, 264, False),
+                                       (48, 40961, True)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_rows_quantised_on_the_way(device, M, N, K, gated, dtype):
+    """As by its two halves, to the bit: one row in LDS where it holds the codes, else by a launch before."""
+    g = torch.Generator().manual_seed(M * K + N)
+    x = torch.zeros(M, K + 3, dtype=dtype)
+    x[:, :K] = torch.randn(M, K, generator=g) * torch.logspace(-3, 3, M)[:, None]
+    x[:, K:] = torch.nan
+    if M > 2:
+        x[1, :K] = 0
+        x[2, K // 2] = torch.inf
+    x = x.to(device)[:, :K]
+    w = pack_weight_i8(torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8).to(device),
+                       torch.rand(N, generator=g).to(device) / K, gated=gated)
+    for out_dtype in (torch.float32, dtype):
+        got = linear_i8(x, w, out_dtype=out_dtype)
+        want = matmul_i8(*quantize_rows_i8(x), w, out_dtype=out_dtype)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+        if M > 2:
+            assert got[2].isnan().all()
+
+
+def test_outputs_over_their_inputs_are_refused(device):
+    w = pack_weight_i8(torch.ones(32, 32, dtype=torch.int8, device=device), torch.ones(32, device=device))
+    buf = torch.zeros(3, 32, dtype=torch.bfloat16, device=device)
+    with pytest.raises(ValueError, match="apart"):
+        linear_i8(buf, w, out=buf)
+    with pytest.raises(ValueError, match="apart"):
+        linear_i8(buf[:2], w, out=buf[1:])
+    linear_i8(buf[:1], w, out=buf[1:2])
+    codes, scale = quantize_rows_i8(buf)
+    with pytest.raises(ValueError, match="apart"):
+        matmul_i8(codes[:1], scale[:1], w, out=codes.view(torch.bfloat16).view(-1)[:32].view(1, 32))
+
+
 def test_rows_do_not_depend_on_their_number(device):
     """A row's output is the same bits whatever rows are beside it."""
     K, N = 640, 1100
