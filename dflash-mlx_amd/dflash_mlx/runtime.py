@@ -30,6 +30,7 @@ here are far below 2**31).
 from __future__ import annotations
 
 import copy
+import functools
 import time
 from collections.abc import Callable, Iterator
 from dataclasses import dataclass
@@ -125,18 +126,22 @@ def _greedy_accept_processed(lg, draft, want_posterior, state, mask):
     d = check_draft(draft, B, N, dev, state is not None)
     mp, mb, mr = check_mask(mask, B, N, V, dev) if mask is not None else (None, 0, 0)
     post = torch.empty((B, N), dtype=torch.int32, device=dev) if want_posterior else None
-    ends = torch.empty((2, B), dtype=torch.int32, device=dev)
-    matched, bonus = ends[0], ends[1]
+    matched, bonus = torch.empty((2, B), dtype=torch.int32, device=dev).unbind()
     if B == 0:
         return post, matched, bonus
     if N == 0 or V == 0:
         raise ValueError(f"logits need at least one row and one vocabulary entry, got {tuple(lg.shape)}")
-    ws_bytes = int(_lib.load().dflash_greedy_accept_processed_workspace_bytes(B, N, V))
-    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+    ws_bytes = _processed_workspace(B, N, V)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     _call("dflash_greedy_accept_processed", dev, lg.data_ptr(), _lib.dtype_tag(lg.dtype), lg.stride(0), lg.stride(1),
           _lib.ptr(d), d.stride(0) if d is not None else 0, d.shape[1] if d is not None else 0, sp, mp, mb, mr,
-          _lib.ptr(post), matched.data_ptr(), bonus.data_ptr(), B, N, V, ws.data_ptr(), ws.numel())
+          _lib.ptr(post), matched.data_ptr(), bonus.data_ptr(), B, N, V, ws.data_ptr(), ws_bytes)
     return post, matched, bonus
+
+
+@functools.lru_cache(maxsize=1024)
+def _processed_workspace(B: int, N: int, V: int) -> int:
+    return int(_lib.load().dflash_greedy_accept_processed_workspace_bytes(B, N, V))
 
 
 def lm_head_greedy_accept(
