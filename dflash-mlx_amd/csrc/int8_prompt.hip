@@ -70,6 +70,13 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
+// The compute waves': their LDS reads are done, since behind it the loaders refill the slots.
+// (The products that use them are no memory operations, so the compiler may place these, and
+// its own wait for the reads, on either side.)
+__device__ __forceinline__ void read_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // Wait until at most n groups of LPL loads of this wave are outstanding (n <= 6).
 template <int LPL>
 __device__ __forceinline__ void wait_groups(int n) {
@@ -271,7 +278,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void prompt_i8_kerne
 #pragma unroll
       for (int j = 0; j < RT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
     if (t0 >= p.tiles) {  // the wave's sums would never be stored
-      for (int i = 0; i < steps; ++i) barrier();
+      for (int i = 0; i < steps; ++i) read_barrier();
       ws = (ws + steps) % S::WS;
       xs = (xs + steps / 2) % S::RS;
       ++tile;
@@ -279,10 +286,10 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void prompt_i8_kerne
     } else {
       for (int i = 0; i < steps; i += 2) {
         const i32x4* xst = lds + S::kRowBase / 16 + xs * (S::kRowSlot / 16);
-        barrier();
+        read_barrier();
         whole_step(wfrag + ws * (S::kWeightSlot / 16), xst + boff0, acc);
         ws = ws == S::WS - 1 ? 0 : ws + 1;
-        barrier();
+        read_barrier();
         whole_step(wfrag + ws * (S::kWeightSlot / 16), xst + boff1, acc);
         ws = ws == S::WS - 1 ? 0 : ws + 1;
         xs = xs == S::RS - 1 ? 0 : xs + 1;
