@@ -70,13 +70,6 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
-// The compute waves': their LDS reads are done, since behind it the loaders refill the slots.
-// (The products that use them are no memory operations, so the compiler may place these, and
-// its own wait for the reads, on either side.)
-__device__ __forceinline__ void read_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 // Wait until at most n groups of LPL loads of this wave are outstanding (n <= 6).
 template <int LPL>
 __device__ __forceinline__ void wait_groups(int n) {

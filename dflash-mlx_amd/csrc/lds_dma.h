@@ -39,5 +39,12 @@ __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// The barrier of waves that read slots which loader waves refill behind it: their LDS
+// reads are done.  (The products that use them are no memory operations, so the compiler
+// may place these, and its own wait for the reads, on either side.)
+__device__ __forceinline__ void read_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 }  // namespace
 }  // namespace dflash

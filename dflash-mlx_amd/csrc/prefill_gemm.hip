@@ -443,11 +443,10 @@ __global__ __launch_bounds__(kWThreads, 1) void prefill_gemm_wide_kernel(const P
   // Half k-step i multiplies weight slot i % 3 and activation slot
   // (i / 2) % 3.  Before it each loader's loads of what it needs must be
   // done and every wave must have passed the barrier, which also frees the
-  // slots read at half k-step i - 1 for what the loaders issue next (a
-  // compute wave reaches the barrier only after the MFMAs that consumed its
-  // reads).  The barrier is the bare instruction: its waits are explicit
-  // (the loads by count, the fragment reads by the MFMAs that consumed
-  // them), where a workgroup fence would also wait for the later loads.
+  // slots read at half k-step i - 1 for what the loaders issue next.  The
+  // barrier is the bare instruction with explicit waits (the loads by
+  // count, a compute wave's fragment reads all), where a workgroup fence
+  // would also wait for the later loads.
   // Every wave runs nhs barriers; the loaders then exit and the compute
   // waves store their sums (no barrier after the loop).
   if (wave >= 10) {
@@ -529,9 +528,7 @@ __global__ __launch_bounds__(kWThreads, 1) void prefill_gemm_wide_kernel(const P
   auto pipeline = [&](auto MMA) {
     int ws = 0;  // the weight slot of stage i
     for (int i = 0; i < nhs; ++i) {
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
+      read_barrier();
       const u32x4* ast = lds + (kWActBase + ((i >> 1) % 3) * kWActSlot) / 16;
       if (decltype(MMA)::value)
         wide_mma(lds + ws * (kWWeightSlot / 16), ast, wr, wc, lane, (i & 1) ? boff1 : boff0, acc);

@@ -94,3 +94,7 @@ def test_the_reading_of_waits():
 
 def test_int8_prompt_products(library, tmp_path):
     _check(tmp_path, "prompt_i8_kernel", 12)
+
+
+def test_bf16_prompt_products(library, tmp_path):
+    _check(tmp_path, "prefill_gemm_wide_kernel", 2)
