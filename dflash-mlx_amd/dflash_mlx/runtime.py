@@ -326,8 +326,9 @@ class LogitsShaping:
     """What a generation asks of its logits: a LogitsState of one sequence that counts
     the prompt and every token taken, and a grammar.  token_mask(tokens) gives the
     bitmask (int32 [ceil(V / 32)], any device) of what may follow the tokens, prompt
-    included, or None for anything.  Any number of generations may use one at a time:
-    each counts in its own (begin)."""
+    included, or None for anything; it is asked about texts only that it allows itself
+    (drafts that it rules out end their block).
+    Any number of generations may use one at a time: each counts in its own (begin)."""
 
     def __init__(self, repetition_penalty: float = 1.0, presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
                  logit_bias: dict[int, float] | None = None,
@@ -386,11 +387,23 @@ class LogitsShaping:
         mask = torch.full((1, n, -(-V // 32)), -1, dtype=torch.int32)
         for i in range(n):
             words = self.token_mask(self.tokens + list(before) + list(drafts[:i]))
-            if words is not None:
-                if words.dtype is not torch.int32 or words.shape != mask.shape[2:]:
-                    raise ValueError(f"token_mask must give int32 [{mask.shape[2]}], got {words.dtype} {tuple(words.shape)}")
-                mask[0, i] = words
+            if words is None:
+                continue
+            if words.dtype is not torch.int32 or words.shape != mask.shape[2:]:
+                raise ValueError(f"token_mask must give int32 [{mask.shape[2]}], got {words.dtype} {tuple(words.shape)}")
+            mask[0, i] = words
+            # a draft that cannot be taken ends the block: the rows behind it are not looked at
+            if i < len(drafts) and not self._allowed(mask[0, i], drafts[i], V):
+                break
         return state, mask.to(dev)
+
+    @staticmethod
+    def _allowed(words: torch.Tensor, token: int, V: int) -> bool:
+        """The token is one that a row under these words may give (a row without any gives 0)."""
+        bits = words if V % 32 == 0 else torch.cat((words[:-1], words[-1:] & ((1 << V % 32) - 1)))
+        if not bool(bits.any()):
+            return token == 0
+        return 0 <= token < V and bool(words[token // 32] >> token % 32 & 1)
 
 
 def _posterior(logits: torch.Tensor, temperature: float, shaping: LogitsShaping | None = None,
