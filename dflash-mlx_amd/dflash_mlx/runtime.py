@@ -327,7 +327,7 @@ class LogitsShaping:
     the prompt and every token taken, and a grammar.  token_mask(tokens) gives the
     bitmask (int32 [ceil(V / 32)], any device) of what may follow the tokens, prompt
     included, or None for anything; it is asked about texts only that it allows itself
-    (drafts that it rules out end their block).
+    (drafts that it rules out end their block).  Where it leaves nothing, the token is 0.
     Any number of generations may use one at a time: each counts in its own (begin)."""
 
     def __init__(self, repetition_penalty: float = 1.0, presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
@@ -418,7 +418,10 @@ def _posterior(logits: torch.Tensor, temperature: float, shaping: LogitsShaping 
     state, mask = shaping.rows(n, V, logits.device, before, drafts)
     if temperature < 1e-5:
         return greedy_accept(logits, [drafts], state=state, mask=mask)[0][0].cpu().tolist()
-    return sample_tokens(process_logits(logits.float(), state, [drafts], mask=mask), temperature)[0].cpu().tolist()
+    shaped = process_logits(logits.float(), state, [drafts], mask=mask)
+    nothing = torch.isneginf(shaped).all(-1)  # token 0, as the greedy accept has it
+    tokens = sample_tokens(shaped.masked_fill_(nothing[..., None], 0.0), temperature)
+    return tokens.masked_fill_(nothing, 0)[0].cpu().tolist()
 
 
 def _rollback(target, target_cache, rollback_records, draft_block_size, accepted_inputs,

@@ -61,7 +61,7 @@ def test_greedy(device, grammar, mode):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("mode", SAMPLED)
-@pytest.mark.parametrize("grammar", ["alternating"])
+@pytest.mark.parametrize("grammar", GRAMMARS)
 def test_sampled(device, grammar, mode):
     """Near the greedy tokens, so that drafts pass, and far from them."""
     want = _reference((1.0, 0.0, 0.0), {}, GRAMMARS[grammar], N_NEW + 2 * BS)
