@@ -375,9 +375,10 @@ class LogitsShaping:
 
     def rows(self, n: int, V: int, dev, before: Sequence[int], drafts: Sequence[int]):
         """(state, mask) of n rows, the first of which knows the drafts `before` too and row
-        i also drafts[:i]."""
-        state = self._ready(V, dev)
-        if before:
+        i also drafts[:i].  No state where the grammar is all that is asked for: blocks are
+        then of any length (a state counts MAX_DRAFT drafts)."""
+        state = self._ready(V, dev) if self.penalties != (1.0, 0.0, 0.0) or self.logit_bias else None
+        if before and state is not None:
             for name in ("counts", "known", "bias", "penalties"):
                 getattr(self._extra, name).copy_(getattr(state, name))
             state = self._extra

@@ -75,6 +75,28 @@ def test_sampled(device, grammar, mode):
         strict(PROMPT + res.generated_tokens)  # every token is one that may follow
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", rt.VERIFY_MODES)
+def test_long_blocks(device, mode):
+    """A state counts 64 drafts; a grammar alone needs no state."""
+    block = 70
+    want = _reference((1.0, 0.0, 0.0), {}, _grammar, 100 + 2 * block)
+
+    def drafter():
+        d = Drafter(PROMPT + want, [None, 66])
+        d.block_size = block
+        return d
+
+    args = dict(max_new_tokens=100, verify_mode=mode, verify_chunk_size=block)
+    res = DFlashGenerator(Target(device), drafter()).generate_from_tokens(
+        torch.tensor(PROMPT), shaping=LogitsShaping(token_mask=_grammar), **args)
+    assert res.generated_tokens == want[:100] and max(res.metrics["acceptance_lengths"]) == block
+    if mode not in ("stream", "chunked"):
+        with pytest.raises(ValueError, match="at most 64 drafts"):
+            DFlashGenerator(Target(device), drafter()).generate_from_tokens(
+                torch.tensor(PROMPT), shaping=LogitsShaping(1.1, token_mask=_grammar), **args)
+
+
 def test_rows_behind_a_forbidden_draft(monkeypatch):
     """The grammar is asked about the rows up to the first draft that it rules out (no GPU)."""
     state = SimpleNamespace(**dict.fromkeys(("counts", "known", "bias", "penalties"), torch.zeros(1)), add=lambda t: None)
@@ -90,7 +112,7 @@ def test_rows_behind_a_forbidden_draft(monkeypatch):
 
     def masks(grammar, drafts, n=4, before=()):
         asked = []
-        shaping = LogitsShaping(token_mask=lambda t: asked.append(t) or grammar(t)).begin([7])
+        shaping = LogitsShaping(1.5, token_mask=lambda t: asked.append(t) or grammar(t)).begin([7])
         mask = shaping.rows(n, V, "cpu", before, drafts)[1]
         assert mask.shape == (1, n, W) and mask.dtype is torch.int32
         return mask[0], asked
