@@ -28,12 +28,15 @@
 //     (order-preserving value bits << 32 | ~index); the workgroup's best per
 //     hidden row goes to keys[row, workgroup], and the accept's finalize
 //     kernel merges them, compares the draft and picks the bonus.
+//   - LOGITS instantiations store the accumulators as fp32 logits instead, for
+//     an accept of processed logits: the sums that the fused accept compares.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "accept_common.h"
 #include "block_gemm.h"
 #include "dflash_gdn.h"
+#include "dflash_lm_logits.h"
 #include "device_common.h"
 #include "host_common.h"
 
@@ -59,7 +62,22 @@ struct LmParams {
   int M, H, V;
   int nwg;         // workgroups (= gridDim.x)
   uint64_t* keys;  // [M, nwg]
+  float* logits;   // LOGITS: [M] rows of stride ls, and no keys
+  int64_t ls;
 };
+
+// Logits v .. v + 3 of hidden row m, those below V.
+__device__ __forceinline__ void store_logits(const LmParams& p, int m, int v, const f32x4& x) {
+  typedef f32x4 f32x4_e4 __attribute__((aligned(4)));  // rows of odd length begin at any element
+  if (m >= p.M) return;
+  float* dst = p.logits + (int64_t)m * p.ls + v;
+  if (v + 4 <= p.V) {
+    *reinterpret_cast<f32x4_e4*>(dst) = x;
+  } else {
+    for (int i = 0; i < 4; ++i)
+      if (v + i < p.V) dst[i] = x[i];
+  }
+}
 
 __device__ __forceinline__ bf16x8 as_bf16x8(u32x4 x) { return __builtin_bit_cast(bf16x8, x); }
 
@@ -70,7 +88,7 @@ struct LmStage {
   u32x4 b[MT][2];   // hidden fragments, two 8-element halves per M tile
 };
 
-template <int MT, int VT, int D>
+template <int MT, int VT, int D, bool LOGITS>
 __global__ __launch_bounds__(kLmThreads) void lm_head_argmax_kernel(const LmParams p) {
   __shared__ uint64_t wkeys[kLmThreads / 64][MT * 16];
   __shared__ __attribute__((aligned(16))) unsigned char
@@ -150,6 +168,13 @@ __global__ __launch_bounds__(kLmThreads) void lm_head_argmax_kernel(const LmPara
     }
   }
 
+  if (LOGITS) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int vt = 0; vt < VT; ++vt) store_logits(p, mt * 16 + r16, vwave + vt * 16 + g * 4, acc[vt][mt]);
+    return;
+  }
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     uint64_t best = 0;
@@ -195,7 +220,7 @@ constexpr int kLmTiledVT = 4;
 static_assert(kLmTiledRG * kLmTiledVT * 16 == kVocabRowsPerBlock,
               "both layouts give a workgroup the same vocab rows (one workspace size)");
 
-template <int MT, int VT, int D, int KW>
+template <int MT, int VT, int D, int KW, bool LOGITS>
 __global__ __launch_bounds__(kLmThreads) void lm_head_argmax_tiled_kernel(const LmParams p) {
   constexpr int RG = (kLmThreads / 64) / KW;
   __shared__ uint64_t wkeys[RG][MT * 16];
@@ -286,6 +311,13 @@ __global__ __launch_bounds__(kLmThreads) void lm_head_argmax_tiled_kernel(const 
       for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) acc[vt][mt] += red[rg][q][vt * MT + mt][lane];
+    if (LOGITS) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int vt = 0; vt < VT; ++vt) store_logits(p, mt * 16 + r16, vwave + vt * 16 + g * 4, acc[vt][mt]);
+      return;
+    }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       uint64_t best = 0;
@@ -307,6 +339,7 @@ __global__ __launch_bounds__(kLmThreads) void lm_head_argmax_tiled_kernel(const 
       if (g == 0) wkeys[rg][mt * 16 + r16] = best;
     }
   }
+  if (LOGITS) return;
   __syncthreads();
   if (threadIdx.x < MT * 16 && (int)threadIdx.x < p.M) {
     uint64_t m = wkeys[0][threadIdx.x];
@@ -330,6 +363,7 @@ __global__ __launch_bounds__(kLmThreads) void lm_head_argmax_tiled_kernel(const 
 // Wave q finishes hidden rows 16q .. 16q+15.
 constexpr int kLmBlockMT = kMaxLmRows / 16;
 
+template <bool LOGITS>
 __global__ __launch_bounds__(kBlockThreads, 1) void lm_head_argmax_block_kernel(const LmParams p) {
   constexpr int MT = kLmBlockMT, VT = kVocabRowsPerBlock / 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[block_lds_bytes<MT>()];
@@ -352,6 +386,11 @@ __global__ __launch_bounds__(kBlockThreads, 1) void lm_head_argmax_block_kernel(
 #pragma unroll
   for (int v0 = 0; v0 < VT; v0 += 2)
     block_merge<MT, VT>(red, acc, wave, lane, v0, [&](int, const f32x4 (&s)[2]) {
+      if (LOGITS) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) store_logits(p, wave * 16 + r16, (rt0 + v0 + j) * 16 + g * 4, s[j]);
+        return;
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -360,6 +399,7 @@ __global__ __launch_bounds__(kBlockThreads, 1) void lm_head_argmax_block_kernel(
           if (v < p.V) best = u64_max(best, argmax_key(s[j][i], v));
         }
     });
+  if (LOGITS) return;
 #pragma unroll
   for (int off = 16; off <= 32; off <<= 1) {  // the 4 lane groups of a hidden row
     const uint32_t lo = __shfl_xor((unsigned)(best & 0xffffffffu), off, 64);
@@ -377,19 +417,20 @@ int lm_blocks(int V) { return (int)ceil_div(V, kVocabRowsPerBlock); }
 template <int MT>
 constexpr int lm_tiled_depth() { return MT == 1 ? 4 : (MT == 2 ? 3 : 2); }
 
-template <int MT>
+template <int MT, bool LOGITS>
 hipError_t launch_tiled_mt(const LmParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((lm_head_argmax_tiled_kernel<MT, kLmTiledVT, lm_tiled_depth<MT>(), kLmTiledKW>),
+  hipLaunchKernelGGL((lm_head_argmax_tiled_kernel<MT, kLmTiledVT, lm_tiled_depth<MT>(), kLmTiledKW, LOGITS>),
                      dim3(p.nwg), dim3(kLmThreads), 0, s, p);
   return hipGetLastError();
 }
 
+template <bool LOGITS>
 hipError_t launch_tiled(const LmParams& p, hipStream_t s) {
-  if (p.M <= 16) return launch_tiled_mt<1>(p, s);
-  if (p.M <= 32) return launch_tiled_mt<2>(p, s);
-  if (p.M <= 48) return launch_tiled_mt<3>(p, s);
+  if (p.M <= 16) return launch_tiled_mt<1, LOGITS>(p, s);
+  if (p.M <= 32) return launch_tiled_mt<2, LOGITS>(p, s);
+  if (p.M <= 48) return launch_tiled_mt<3, LOGITS>(p, s);
   if (p.hs <= kBlockMaxRowStride && p.V <= kBlockMaxN) {
-    hipLaunchKernelGGL(lm_head_argmax_block_kernel, dim3(p.nwg), dim3(kBlockThreads), 0, s, p);
+    hipLaunchKernelGGL(lm_head_argmax_block_kernel<LOGITS>, dim3(p.nwg), dim3(kBlockThreads), 0, s, p);
     return hipGetLastError();
   }
   // past the block kernel's 32-bit offsets: 48 rows, then the others
@@ -397,20 +438,34 @@ hipError_t launch_tiled(const LmParams& p, hipStream_t s) {
   head.M = 48;
   rest.M = p.M - 48;
   rest.hidden = p.hidden + 48 * p.hs;
-  rest.keys = p.keys + (int64_t)48 * p.nwg;
-  const hipError_t e = launch_tiled_mt<3>(head, s);
-  return e != hipSuccess ? e : launch_tiled_mt<1>(rest, s);
+  if (LOGITS)
+    rest.logits = p.logits + 48 * p.ls;
+  else
+    rest.keys = p.keys + (int64_t)48 * p.nwg;
+  const hipError_t e = launch_tiled_mt<3, LOGITS>(head, s);
+  return e != hipSuccess ? e : launch_tiled_mt<1, LOGITS>(rest, s);
 }
 
 // Prefetch depth per M-tile count (operand ring of ~100 VGPRs per lane).
 template <int MT>
 constexpr int lm_depth() { return MT == 1 ? 6 : (MT == 2 ? 4 : 2); }
 
-template <int MT>
+template <int MT, bool LOGITS>
 hipError_t launch_mt(const LmParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((lm_head_argmax_kernel<MT, kVT, lm_depth<MT>()>), dim3(p.nwg),
+  hipLaunchKernelGGL((lm_head_argmax_kernel<MT, kVT, lm_depth<MT>(), LOGITS>), dim3(p.nwg),
                      dim3(kLmThreads), 0, s, p);
   return hipGetLastError();
+}
+
+template <bool LOGITS>
+hipError_t launch_lm_head(const LmParams& p, bool tiled, hipStream_t s) {
+  if (tiled) return launch_tiled<LOGITS>(p, s);
+  switch ((int)ceil_div(p.M, 16)) {
+    case 1: return launch_mt<1, LOGITS>(p, s);
+    case 2: return launch_mt<2, LOGITS>(p, s);
+    case 3: return launch_mt<3, LOGITS>(p, s);
+    default: return launch_mt<4, LOGITS>(p, s);
+  }
 }
 
 }  // namespace
@@ -456,20 +511,36 @@ int lm_head_impl(const void* hidden, int64_t hidden_row_stride, const void* weig
   p.nwg = lm_blocks(V);
   p.keys = static_cast<uint64_t*>(workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipError_t e;
-  if (tiled) {
-    e = launch_tiled(p, s);
-  } else {
-    switch ((int)ceil_div(p.M, 16)) {
-      case 1: e = launch_mt<1>(p, s); break;
-      case 2: e = launch_mt<2>(p, s); break;
-      case 3: e = launch_mt<3>(p, s); break;
-      default: e = launch_mt<4>(p, s); break;
-    }
-  }
+  const hipError_t e = launch_lm_head<false>(p, tiled, s);
   if (e != hipSuccess) return (int)e;
   return to_status(launch_accept_finalize(p.keys, p.nwg, B, N, draft, draft_stride, n_draft,
                                           posterior, matched, bonus, s));
+}
+
+int lm_logits_impl(const void* hidden, int64_t hidden_row_stride, const void* weight,
+                   int64_t weight_row_stride, int H, int V, float* logits, int64_t logits_row_stride,
+                   int M, void* stream) {
+  const bool tiled = weight_row_stride < 0;
+  if (M < 0 || H <= 0 || V <= 0) return DFLASH_ERR_SHAPE;
+  if (M > kMaxLmRows || H % kKStep != 0 || (tiled && V % 16 != 0)) return DFLASH_ERR_UNSUPPORTED;
+  if (hidden_row_stride < H || (!tiled && weight_row_stride < H) || logits_row_stride < V) return DFLASH_ERR_SHAPE;
+  if (M == 0) return DFLASH_OK;
+  if (hidden == nullptr || weight == nullptr || logits == nullptr) return DFLASH_ERR_NULL;
+  if (((uintptr_t)hidden & 15) || ((uintptr_t)weight & 15) || (hidden_row_stride % 8) ||
+      (!tiled && (weight_row_stride % 8)) || ((uintptr_t)logits & 3))
+    return DFLASH_ERR_ALIGN;
+  LmParams p{};
+  p.hidden = static_cast<const uint16_t*>(hidden);
+  p.hs = hidden_row_stride;
+  p.weight = static_cast<const uint16_t*>(weight);
+  p.ws = tiled ? 0 : weight_row_stride;
+  p.M = M;
+  p.H = H;
+  p.V = V;
+  p.nwg = lm_blocks(V);
+  p.logits = logits;
+  p.ls = logits_row_stride;
+  return to_status(launch_lm_head<true>(p, tiled, static_cast<hipStream_t>(stream)));
 }
 
 }  // namespace
@@ -498,4 +569,19 @@ extern "C" int dflash_lm_head_greedy_accept_tiled(const void* hidden, int64_t hi
   return dflash::lm_head_impl(hidden, hidden_row_stride, weight_tiled, -1, H, V, draft,
                               draft_stride, n_draft, posterior, matched, bonus, B, N, workspace,
                               workspace_bytes, stream);
+}
+
+extern "C" int dflash_lm_head_logits(const void* hidden, int64_t hidden_row_stride, const void* weight,
+                                     int64_t weight_row_stride, int H, int V, float* logits,
+                                     int64_t logits_row_stride, int M, void* stream) {
+  if (weight_row_stride < 0) return DFLASH_ERR_SHAPE;
+  return dflash::lm_logits_impl(hidden, hidden_row_stride, weight, weight_row_stride, H, V, logits,
+                                logits_row_stride, M, stream);
+}
+
+extern "C" int dflash_lm_head_logits_tiled(const void* hidden, int64_t hidden_row_stride,
+                                           const void* weight_tiled, int H, int V, float* logits,
+                                           int64_t logits_row_stride, int M, void* stream) {
+  return dflash::lm_logits_impl(hidden, hidden_row_stride, weight_tiled, -1, H, V, logits,
+                                logits_row_stride, M, stream);
 }

@@ -1,5 +1,6 @@
 """ctypes binding of libdflash_gfx950.so (declared in include/dflash_gdn.h,
-include/dflash_kv8.h, include/dflash_int8.h and include/dflash_logits.h).
+include/dflash_kv8.h, include/dflash_int8.h, include/dflash_logits.h and
+include/dflash_lm_logits.h).
 
 The library is loaded after ``import torch`` so that it binds to the HIP
 runtime torch already loaded (both use the soname libamdhip64.so.7); loading
@@ -175,6 +176,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I,
         [_VP, _I64, _VP, _I, _I, _VP, _I64, _I, _VP, _VP, _VP, _I, _I, _VP, _SZ, _VP],
     ),
+    "dflash_lm_head_logits": (_I, [_VP, _I64, _VP, _I64, _I, _I, _VP, _I64, _I, _VP]),
+    "dflash_lm_head_logits_tiled": (_I, [_VP, _I64, _VP, _I, _I, _VP, _I64, _I, _VP]),
     "dflash_greedy_accept_conv_rollback": (
         _I,
         [_VP, _I, _I64, _I64, _VP, _I64, _I, _VP, _VP, _VP, _I, _I, _I, _VP, _SZ,  # accept

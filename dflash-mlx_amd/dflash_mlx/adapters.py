@@ -119,6 +119,11 @@ class Qwen35TargetAdapter:
     def lm_head_logits(self, model, hidden_states):
         return model.lm_head_logits(hidden_states)
 
+    def lm_head_logits_fp32(self, model, hidden_states):
+        """The logits that lm_head_argmax compares, where the model has them apart
+        from lm_head_logits."""
+        return getattr(model, "lm_head_logits_fp32", model.lm_head_logits)(hidden_states)
+
     def lm_head_argmax(self, model, hidden_states):
         """The hook of adapters.py:267-271, served by the fused LM-head
         greedy kernel (no logits)."""
@@ -204,6 +209,10 @@ class LoadedTargetModel:
 
     def lm_head_logits(self, hidden_states):
         return self.adapter.lm_head_logits(self.model, hidden_states)
+
+    def lm_head_logits_fp32(self, hidden_states):
+        hook = getattr(self.adapter, "lm_head_logits_fp32", self.adapter.lm_head_logits)
+        return hook(self.model, hidden_states)
 
     def lm_head_argmax(self, hidden_states):
         return self.adapter.lm_head_argmax(self.model, hidden_states)

@@ -245,7 +245,7 @@ class HybridVerifyRunner:
         from the launch form in rounding.  weight_dtype: torch.int8 holds every
         projection and the LM head in 8-bit integers, a scale a channel, and
         quantises their rows by token (dflash_linear_i8).  logits_state: the
-        accept is of the logits under this state's penalties and biases (B
+        accept is of the fp32 logits under this state's penalties and biases (B
         sequences), and a commit counts the tokens that it keeps (the caller
         counts the prompt and the first block's first token).  masked: the accept
         is under the bitmask self.mask, int32 [B, T, ceil(V / 32)], row t for
@@ -337,9 +337,9 @@ class HybridVerifyRunner:
         self.captured = None  # [B*T, len(capture_layers) * H] after set_capture
         if logits_state is not None and logits_state.device != self.h.device:
             raise ValueError(f"logits_state must be on {self.h.device}, got {logits_state}")
-        # logits stored for the accept: where something changes them, or of the 8-bit head
-        self.logits = (e(M, V, dt=f32 if self.int8 else bf)
-                       if self.int8 or logits_state is not None or masked else None)
+        # logits stored for the accept: where something changes them, or of the 8-bit head; in
+        # fp32, so that their greedy tokens are those of the accept that stores none
+        self.logits = e(M, V, dt=f32) if self.int8 or logits_state is not None or masked else None
         self.mask = torch.full((B, T, -(-V // 32)), -1, dtype=i32, device=device) if masked else None
         self.proc_ws = e(max(int(lib.dflash_greedy_accept_processed_workspace_bytes(B, T, V)), 8), dt=torch.uint8)
         self._plans: dict[int, _Plan] = {}
@@ -678,16 +678,16 @@ class HybridVerifyRunner:
                 self.matched.data_ptr(), self.bonus.data_ptr(), B, T, self.lm_ws.data_ptr(),
                 self.lm_ws.numel())
         if self.logits is not None:
-            V, bf = cfg.vocab_size, _lib.DFLASH_DTYPE_BF16
+            V = cfg.vocab_size
             lg, tag = self.logits.data_ptr(), _lib.dtype_tag(self.logits.dtype)
             if self.int8:
                 pl.logits = [self._linear_i8_op(self.w.lm_head_i8, self.xn, lg, tag, V, M)]
             elif self.w.lm_head_tiled is not None and self.tiled:
-                pl.logits = [("dflash_gemm_bf16_tiled", (self.xn.data_ptr(), H, self.w.lm_head_tiled.data_ptr(), lg, V,
-                                                         M, V, H, 1, 64, 4, None, 0))]
+                pl.logits = [("dflash_lm_head_logits_tiled",
+                              (self.xn.data_ptr(), H, self.w.lm_head_tiled.data_ptr(), H, V, lg, V, M))]
             else:
-                pl.logits = [("dflash_gemm_bf16", (self.xn.data_ptr(), H, self.w.lm_head.data_ptr(), H, lg, V, M, V, H,
-                                                   1, 32, 4))]
+                pl.logits = [("dflash_lm_head_logits",
+                              (self.xn.data_ptr(), H, self.w.lm_head.data_ptr(), H, H, V, lg, V, M))]
             drafts = (self.tokens.data_ptr() + 4, T, T - 1)
             ends = (self.posterior.data_ptr(), self.matched.data_ptr(), self.bonus.data_ptr(), B, T, V,
                     self.proc_ws.data_ptr(), self.proc_ws.numel())

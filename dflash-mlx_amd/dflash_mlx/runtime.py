@@ -576,8 +576,9 @@ def verify_block_parallel_greedy_argmax(
     argmax_start = profile_start(profile)
     if shaping is None:
         posterior = target.lm_head_argmax(norm_hidden_states)[0].cpu().tolist()
-    else:  # the penalties need the logits
-        posterior = _posterior(target.lm_head_logits(norm_hidden_states), 0.0, shaping, (), block_tokens[1:])
+    else:  # the penalties need the logits, those that the argmax compares
+        logits = getattr(target, "lm_head_logits_fp32", target.lm_head_logits)(norm_hidden_states)
+        posterior = _posterior(logits, 0.0, shaping, (), block_tokens[1:])
     add_profile_elapsed(profile, "verify_argmax_time_s", argmax_start)
 
     prefix_start = profile_start(profile)

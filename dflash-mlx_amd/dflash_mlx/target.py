@@ -434,6 +434,28 @@ class HybridTargetModel:
                           H, 1, 32, 4, stream)
         return out.view(*lead, V)
 
+    def lm_head_logits_fp32(self, hidden: torch.Tensor) -> torch.Tensor:
+        """fp32 logits [..., V], the sums that lm_head_argmax compares: what
+        penalties and masks are applied to where it would take the tokens."""
+        if self.weight_dtype is torch.int8:
+            return self.lm_head_logits(hidden)
+        H, V = self.cfg.hidden_size, self.cfg.vocab_size
+        lead = hidden.shape[:-1]
+        x = hidden.reshape(-1, H).to(torch.bfloat16)
+        if x.stride(-1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+            x = x.contiguous()
+        out = torch.empty((x.shape[0], V), dtype=torch.float32, device=self.device)
+        w, stream = self.weights, _lib.stream_handle(self.device)
+        for m0 in range(0, x.shape[0], 64):
+            m = min(64, x.shape[0] - m0)
+            xp, op = x[m0:].data_ptr(), out[m0:].data_ptr()
+            if w.lm_head_tiled is not None and self.weight_layout == "tiled":
+                _lib.call("dflash_lm_head_logits_tiled", xp, x.stride(0), w.lm_head_tiled.data_ptr(), H, V, op, V, m,
+                          stream)
+            else:
+                _lib.call("dflash_lm_head_logits", xp, x.stride(0), w.lm_head.data_ptr(), H, H, V, op, V, m, stream)
+        return out.view(*lead, V)
+
     def lm_head_argmax(self, hidden: torch.Tensor) -> torch.Tensor:
         """The lm_head_argmax hook (adapters.py:267-271) as the fused LM-head
         greedy kernel: int32 argmax ids [..., N], no logits."""
