@@ -66,7 +66,8 @@ def _matrix(name: str, t, dtypes) -> None:
 
 
 def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor, *, gated: bool = False) -> Int8Weight:
-    """int8 codes [N, K] and fp32 scales [N] as a packed weight.  gated: the rows are [gate; up]."""
+    """int8 codes [N, K] and fp32 scales [N] as a packed weight.  gated: the rows are [gate; up].
+    Codes of the largest K are at least -127: a sum of -128 * -128 would leave 32 bits."""
     _matrix("codes", codes, (torch.int8,))
     N, K = codes.shape
     dev = codes.device
@@ -80,6 +81,8 @@ def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor, *, gated: bool = Fa
                          "an even number of channels if gated)")
     if K > 1 and codes.stride(1) != 1 or N > 1 and codes.stride(0) < K:
         codes = codes.contiguous()
+    if K == MAX_K and bool((codes == -128).any()):
+        raise ValueError(f"codes of {K} features must be at least -127")
     scale = scale.contiguous()
     packed = torch.empty(nbytes, dtype=torch.int8, device=dev)
     scales = torch.empty(int(lib.dflash_weight_i8_scales(N, int(gated))), dtype=torch.float32, device=dev)

@@ -32,7 +32,8 @@
 extern "C" {
 #endif
 
-/* Largest K: |sum| < 2^31. */
+/* Largest K: |sum| < 2^31, for any codes below it, and at it if no code of the weight is -128
+ * (quantised ones are -127 to 127). */
 #define DFLASH_I8_MAX_K 131072
 /* Largest N: offsets of channel scales fit 32 bits. */
 #define DFLASH_I8_MAX_N 268435456
