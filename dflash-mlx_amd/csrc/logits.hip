@@ -151,7 +151,9 @@ template <typename T>
 constexpr int kSlice = 8 * kLThreads * kTurns<T>;
 
 // grid (rows, slices): one workgroup processes one slice of one row, and either writes it
-// (WRITE; INPLACE: only what changes) or reduces it to an argmax key.
+// (WRITE; INPLACE: only the eights in which something changes, whole where a token of one is
+// masked: storing the masked entries alone took 185 us where this takes 113, 32 x 16 rows of
+// 151936 in fp32 of which 3 % are allowed) or reduces it to an argmax key.
 //
 // The slice streams by and is only masked: for the argmax a lane keeps the largest value and
 // where its eight lie (their order among each other is looked up once, at the end).  The

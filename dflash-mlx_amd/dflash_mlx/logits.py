@@ -216,7 +216,8 @@ def process_logits(logits: torch.Tensor, state: LogitsState | None = None, draft
     draft: [B, n] token ids, draft i known to the rows from i + 1 on (the block's tokens
     after its first, which is counted already).  mask: int32 words [B, N, ceil(V / 32)],
     or [N, ceil(V / 32)] for B = 1.  out: a tensor like the logits, or the logits
-    themselves: then only the entries that change are touched."""
+    themselves: then the entries that nothing changes keep their values, and eights of a
+    row without a masked or known token are not touched."""
     _require_device("logits", logits, None)
     if logits.dtype not in _FLOATS:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")

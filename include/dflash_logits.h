@@ -69,8 +69,9 @@ int dflash_logits_state_set_bias(const dflash_logits_state* state, const int32_t
 
 /* Processed logits [B, N, V] to out, rounded once to the logits' type (logits_dtype: a
  * dflash_gdn.h tag).  Strides in elements; a row's V entries are contiguous.  out may be
- * the logits themselves with the same strides: entries that nothing changes are then not
- * touched.  state null: only the mask.  draft [B, n_draft]: draft token i is known to the
+ * the logits themselves with the same strides: entries that nothing changes then keep their
+ * values, and eights of a row (from a multiple of 8 on) that hold no masked and no known token
+ * are not touched.  state null: only the mask.  draft [B, n_draft]: draft token i is known to the
  * rows from i + 1 on.  mask: words, batch and row stride in words (0: shared), or null. */
 int dflash_logits_process(const void* logits, int logits_dtype, int64_t batch_stride, int64_t row_stride,
                           const dflash_logits_state* state, const int32_t* draft, int64_t draft_stride,
