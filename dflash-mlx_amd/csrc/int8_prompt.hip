@@ -28,11 +28,12 @@ namespace {
 constexpr int kBandChannels = 4096;  // channels per band of the tile walk
 
 // A tile's shape and what follows from it.
-template <int WR_, int WC_, int RT_, int WS_, int RS_, int LPL_>
+template <int WR_, int WC_, int RT_, int WS_, int RS_, int LPL_, bool SPLITS_>
 struct Shape {
   // RT: row tiles of 16 a wave; WS, RS: slots of weights and rows
   static constexpr int WR = WR_, WC = WC_, RT = RT_, WS = WS_, RS = RS_;
   static constexpr int LPL = LPL_;  // loads a loader wave and step
+  static constexpr bool kSplits = SPLITS_;  // may K be split over workgroups
   static constexpr int kRows = 16 * RT * WC, kChannels = 64 * WR, kBand = kBandChannels / kChannels;
   static constexpr int kCompute = WR * WC, kWeightLoaders = 4 * WR / LPL, kRowLoaders = kRows / 16 / LPL;
   static constexpr int kGroup = kCompute + kWeightLoaders + kRowLoaders;  // waves
@@ -51,11 +52,13 @@ struct Shape {
   static constexpr int kLdsU4 = (kScaleBase + kScaleSlots * kScaleSlot) / 16;
 };
 
-// 256 x 256: half the bytes per product.  128 x 128: two workgroups a compute unit, one's
+// 256 x 256: half the bytes per product; 128 of its 168 registers are sums, and 6 that the
+// outputs need wait in scratch (written once, read once a tile).
+// 128 x 128: two workgroups a compute unit, one's
 // products beside the other's waits; four loads a loader wave, whose issue the small tile's
 // k-step waited for (40 against 48 us for a step chain of 144).
-using Wide = Shape<4, 2, 8, 3, 3, 8>;
-using Narrow = Shape<2, 2, 4, 3, 3, 4>;
+using Wide = Shape<4, 2, 8, 3, 3, 8, false>;
+using Narrow = Shape<2, 2, 4, 3, 3, 4, true>;
 
 struct PromptI8 {
   GemmI8 g;
@@ -368,12 +371,16 @@ hipError_t launch_shape(const GemmI8& p, int splits, hipStream_t s) {
   splits = (int)ceil_div(p.k_steps, q.split_steps);
   q.total = q.tiles * splits;
   q.per_xcd = (int)ceil_div(q.total, 8);
-  if (splits > 1) {
-    q.part = static_cast<int32_t*>(p.workspace);
-    hipLaunchKernelGGL((prompt_i8_kernel<float, false, true, S>), dim3((unsigned)(8 * q.per_xcd)), dim3(S::kThreads), 0, s, q);
-    const int64_t threads = (int64_t)p.M * (GATED ? p.tiles / 2 : p.tiles) * 4;
-    hipLaunchKernelGGL((join_i8_kernel<T, GATED>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, s, p, q.part, splits);
-    return hipGetLastError();
+  if constexpr (S::kSplits) {
+    if (splits > 1) {
+      q.part = static_cast<int32_t*>(p.workspace);
+      hipLaunchKernelGGL((prompt_i8_kernel<float, false, true, S>), dim3((unsigned)(8 * q.per_xcd)), dim3(S::kThreads), 0,
+                         s, q);
+      const int64_t threads = (int64_t)p.M * (GATED ? p.tiles / 2 : p.tiles) * 4;
+      hipLaunchKernelGGL((join_i8_kernel<T, GATED>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, s, p, q.part,
+                         splits);
+      return hipGetLastError();
+    }
   }
   // as many workgroups as the compute units' LDS holds walk the tiles
   const int slots = std::max(device_cus() * (160 * 1024 / (16 * S::kLdsU4)) / 8, 1);
@@ -384,7 +391,7 @@ hipError_t launch_shape(const GemmI8& p, int splits, hipStream_t s) {
 
 template <typename T, bool GATED>
 hipError_t launch_prompt_i8(const GemmI8& p, hipStream_t s) {
-  if (p.plan.kind == PlanI8::kWide) return launch_shape<Wide, T, GATED>(p, p.plan.splits, s);
+  if (p.plan.kind == PlanI8::kWide) return launch_shape<Wide, T, GATED>(p, 1, s);
   return launch_shape<Narrow, T, GATED>(p, p.plan.splits, s);
 }
 
