@@ -189,6 +189,8 @@ def check_draft(draft, B: int, N: int, dev, counted: bool):
         return None
     if isinstance(draft, torch.Tensor):
         _require_device("draft", draft, dev)
+        if draft.dtype is torch.int64:  # ids that 32 bits would wrap stay outside the vocabulary
+            draft = draft.clamp(-1, 2 ** 31 - 1)
         draft = draft.to(torch.int32)
     else:
         draft = torch.tensor(draft, dtype=torch.int32).to(dev)
