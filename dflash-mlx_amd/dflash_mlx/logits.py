@@ -102,12 +102,13 @@ class LogitsState:
         _call("dflash_logits_state_reset", self.device, self._ptr)
 
     def set_penalties(self, repetition=1.0, presence=0.0, frequency=0.0) -> None:
-        """Numbers, or a tensor or list of one a sequence."""
+        """Numbers, or a tensor or list of one a sequence.  Repetition penalties are positive (not
+        looked at in a tensor on the device)."""
         for j, (name, p) in enumerate((("repetition", repetition), ("presence", presence), ("frequency", frequency))):
             if not isinstance(p, torch.Tensor):
                 p = torch.tensor(p, dtype=torch.float32)
-                if j == 0 and not bool((p > 0).all()):
-                    raise ValueError(f"the repetition penalty must be positive, got {repetition}")
+            if j == 0 and p.device.type == "cpu" and not bool((p > 0).all()):
+                raise ValueError(f"the repetition penalty must be positive, got {repetition}")
             if p.dim() and tuple(p.shape) != (self.B,):
                 raise ValueError(f"{name} must be a number or [{self.B}], got {tuple(p.shape)}")
             self.penalties[:, j].copy_(p)
