@@ -247,7 +247,8 @@ class HybridVerifyRunner:
         quantises their rows by token (dflash_linear_i8).  logits_state: the
         accept is of the fp32 logits under this state's penalties and biases (B
         sequences), and a commit counts the tokens that it keeps (the caller
-        counts the prompt and the first block's first token).  masked: the accept
+        counts the prompt, the first block's first token and the tokens of blocks
+        that accept_all keeps).  masked: the accept
         is under the bitmask self.mask, int32 [B, T, ceil(V / 32)], row t for
         block token t's successor; all ones until the caller writes it."""
         if weight_layout not in ("tiled", "rowmajor"):
@@ -830,7 +831,8 @@ class HybridVerifyRunner:
     def accept_all(self, T: int) -> None:
         """Keep every token of the last T-token block: keep = T (the states
         follow tape[T-1] on the next load) and the conv windows advanced by
-        the block's qkv rows, in place.  The KV lengths stay with the caller."""
+        the block's qkv rows, in place.  The KV lengths stay with the caller, and
+        so do the block's tokens where a logits_state counts: they may be a prompt's."""
         p = self._plan(int(T))
         self.keep.fill_(int(T))
         self._run(p.commit[1:2])

@@ -120,3 +120,23 @@ def test_a_grammar_that_allows_everything_changes_nothing(device):
     for m0 in range(0, 140, 64):
         assert torch.equal(m.lm_head_argmax(rows[m0:m0 + 64]).cpu().long(),
                            argmax_lowest(logits.view(140, V)[m0:m0 + 64].cpu()))
+
+
+def test_blocks_that_are_kept_whole_are_the_callers_to_count(device):
+    """accept_all leaves a state alone; the next commit counts as ever."""
+    V = 1024
+    cfg, w = _weights(device, V)
+    state = LogitsState.zeros(1, V, device)
+    run = HybridVerifyRunner(cfg, w, 1, 8, 256, device, logits_state=state)
+    run.set_state([0])
+    run.tokens.copy_(torch.arange(8, dtype=torch.int32)[None])
+    run.forward()
+    run.accept_all(8)
+    run.lens.add_(8)
+    assert state.counts.abs().sum() == 0 and state.known.abs().sum() == 0
+    state.add([list(range(9))], prompt=True)
+    run.tokens.copy_(torch.arange(8, 16, dtype=torch.int32)[None])
+    run.step()
+    counts = state.counts[0].cpu().long()
+    made = torch.where(counts < 0, counts + 2 ** 31, counts)
+    assert made.sum() == run.matched.item() + 1 and (counts[:9] < 0).all() and run.lens.item() == 8 + run.keep.item()
