@@ -373,8 +373,11 @@ hipError_t launch_gemm(const GemmI8& p, int gated, hipStream_t s) {
 //   wide: 0.62 a k-step of 64 and 8 a tile's outputs, a round of the compute units;
 //   narrow: 0.45 a k-step where two workgroups share a unit, 0.27 alone, and 4 a tile; the
 //     splits' sums are written and read at 4 TB/s by a launch of 2.5.
-// Within 15 % of the measured times of 64 to 4096 rows, 2560 to 151936 channels and 1001 to
-// 9216 features; it picked the fastest or one within 7 % of it.
+// Of the measured times of 23 products of 17 to 4096 rows, 2560 to 151936 channels and 1001 to
+// 9216 features, weights not in the cache, the estimate is 0.95 to 1.1 for streams and 256 x 256
+// tiles and 0.9 to 1.25 for 128 x 128 tiles of whole K; 1.25 to 1.4 where K is split (64 x 2560 x
+// 9216 in 12: 17.7 for 13.5); and too short where a narrow launch waits for its weight: 63 for 78
+// to 95 us of 17 and 64 x 151936 x 2560, 12.3 for 16.5 of 700 x 5003 x 1001.
 PlanI8 plan_i8(int M, int tiles, int k_steps) {
   PlanI8 best{PlanI8::kStream, 1};
   if (M <= 16) return best;

@@ -145,8 +145,8 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void prompt_i8_kerne
 
   // K-steps are counted through all of a workgroup's tiles.  Step i multiplies weight slot
   // i % WS and row slot (i / 2) % RS.  Before it each loader's loads of what it needs are done
-  // and every wave has passed the barrier, which also frees the slots read at step i - 1
-  // for what the loaders issue next: while a tile's outputs are stored, the next tile's
+  // and every wave has passed the barrier, a compute wave with its reads done (read_barrier), which
+  // frees the slots read at step i - 1 for what the loaders issue next: while a tile's outputs are stored, the next tile's
   // first steps are on their way.  A tile's scales are loaded before its first step; the
   // waits count steps' loads alone, so that these only make them wait for more.
   if (wave >= S::kCompute + S::kWeightLoaders) {
